@@ -32,6 +32,8 @@ EXT = HERE / ("gpuos_ext" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 DEV_HEADERS = [CSRC / "gpuos_abi.h", CSRC / "ops.cuh", CSRC / "executor.cuh", CSRC / "batch.cuh",
                CSRC / "lean.cuh"]
+# one object each: gpuos_rotary, gpuos_cache_*, gpuos_route*, gpuos_logprobs*
+ROWOPS = ["rotary", "cache", "route", "logprobs"]
 HOST_HEADERS = [CSRC / "gpuos_abi.h", CSRC / "runtime.h", CSRC / "jit.h", ROOT / "include" / "gpuos_b200.h"]
 
 
@@ -63,6 +65,19 @@ def build_lib(force=False, verbose=False) -> Path:
     if force or _stale(nobj, [CSRC / "noalloc.cu", ROOT / "include" / "gpuos_b200.h", *DEV_HEADERS]):
         _run([NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
               "-c", CSRC / "noalloc.cu", "-o", nobj], verbose)
+    # the row operators
+    robj2 = BUILD / "rowops.o"
+    if force or _stale(robj2, [CSRC / "rowops.cpp"]):
+        _run(["g++", "-std=c++17", "-O2", "-fPIC", "-Wall", f"-I{CUDA_HOME / 'include'}",
+              "-c", CSRC / "rowops.cpp", "-o", robj2], verbose)
+    rowobjs = [robj2]
+    for name in ROWOPS:
+        obj = BUILD / f"{name}.o"
+        rowobjs.append(obj)
+        if force or _stale(obj, [CSRC / f"{name}.cu", CSRC / "rowops.cuh", CSRC / "rowops.h",
+                                 ROOT / "include" / "gpuos_b200.h"]):
+            _run([NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
+                  "-c", CSRC / f"{name}.cu", "-o", obj], verbose)
     # the relocatable batch kernel for custom expressions, embedded as bytes
     jcubin = BUILD / "jit_kernel.cubin"
     jblob = BUILD / "jit_blob.cpp"
@@ -91,9 +106,9 @@ def build_lib(force=False, verbose=False) -> Path:
     if force or _stale(iobj, [CSRC / "ipc.cpp", *HOST_HEADERS]):
         _run(["g++", "-std=c++17", "-O2", "-fPIC", "-Wall", "-Wno-unused-parameter",
               f"-I{CUDA_HOME / 'include'}", "-c", CSRC / "ipc.cpp", "-o", iobj], verbose)
-    if force or _stale(LIB, [kobj, robj, nobj, jobj, jbobj, iobj]):
+    if force or _stale(LIB, [kobj, robj, nobj, jobj, jbobj, iobj, *rowobjs]):
         _run([NVCC, *ARCH, "-shared", "-cudart", "static", "-o", LIB, kobj, robj, nobj, jobj, jbobj,
-              iobj, "-Xlinker", "--no-undefined", "-lpthread", "-ldl", "-lrt"], verbose)
+              iobj, *rowobjs, "-Xlinker", "--no-undefined", "-lpthread", "-ldl", "-lrt"], verbose)
     return LIB
 
 
@@ -102,14 +117,15 @@ def build_ext(force=False, verbose=False) -> Path:
     from torch.utils import cpp_extension
 
     lib = build_lib(force, verbose)
-    if not (force or _stale(EXT, [CSRC / "ext.cpp", lib, *HOST_HEADERS])):
+    if not (force or _stale(EXT, [CSRC / "ext.cpp", CSRC / "rowops_ext.cpp", lib, *HOST_HEADERS])):
         return EXT
     inc = [f"-I{p}" for p in cpp_extension.include_paths()]
     inc += [f"-I{sysconfig.get_paths()['include']}", f"-I{CUDA_HOME / 'include'}"]
     tlib = cpp_extension.library_paths()[0]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-          "-DTORCH_EXTENSION_NAME=gpuos_ext", *inc, CSRC / "ext.cpp", "-o", EXT,
+          "-DTORCH_EXTENSION_NAME=gpuos_ext", *inc, CSRC / "ext.cpp", CSRC / "rowops_ext.cpp",
+          "-o", EXT,
           f"-L{HERE}", "-lgpuos_b200", f"-L{tlib}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
           "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}"], verbose)
     return EXT

@@ -15,6 +15,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libgpuos_b200.so"
 
 OK, EINVAL, ECUDA, ETIMEOUT, ESTATE, EUNSUPPORTED, EDEVICE, ENVRTC = 0, -1, -2, -3, -4, -5, -6, -7
 F32, F16, BF16 = 0, 1, 2
+I32, F64, I64, U8, I8, E4M3 = 3, 4, 5, 6, 7, 8  # the row operators' other tensors
 MODE_PERSISTENT, MODE_STREAM = 0, 1
 OP_ADD, OP_MUL, OP_SUB, OP_DIV = 0, 1, 2, 3
 
@@ -89,6 +90,17 @@ SIGNATURES = {
     "gpuos_reduce_rows_noalloc": (ctypes.c_int32, [ctypes.c_int32, _VP, ctypes.c_int32,
                                                    ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                                    _VP, ctypes.c_int32, _VP]),
+    "gpuos_rotary": (ctypes.c_int32, [ctypes.c_int32, P(Tensor), P(Tensor), P(Tensor), P(Tensor),
+                                      ctypes.c_float, ctypes.c_int32, _VP]),
+    "gpuos_cache_write": (ctypes.c_int32, [ctypes.c_int32, P(Tensor), P(Tensor), P(Tensor),
+                                           P(Tensor), _VP]),
+    "gpuos_cache_read": (ctypes.c_int32, [ctypes.c_int32, P(Tensor), P(Tensor), P(Tensor),
+                                          P(Tensor), _VP]),
+    "gpuos_route": (ctypes.c_int32, [P(Tensor)] * 4 + [ctypes.c_int32] * 5 + [ctypes.c_float, _VP]),
+    "gpuos_route_grad": (ctypes.c_int32, [P(Tensor)] * 4 + [ctypes.c_int32] * 2 +
+                         [ctypes.c_float, _VP]),
+    "gpuos_logprobs": (ctypes.c_int32, [P(Tensor)] * 7 + [ctypes.c_float, _VP]),
+    "gpuos_logprobs_grad": (ctypes.c_int32, [P(Tensor)] * 7 + [ctypes.c_float, _VP]),
     "gpuos_match_expression": (ctypes.c_int32, [ctypes.c_char_p, ctypes.c_int32,
                                                 P(ctypes.c_int32), P(ctypes.c_float),
                                                 P(ctypes.c_float)]),
@@ -152,7 +164,9 @@ def tensor(t) -> Tensor:
     global _DT
     if _DT is None:
         import torch
-        _DT = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+        _DT = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int32: I32,
+               torch.float64: F64, torch.int64: I64, torch.uint8: U8, torch.int8: I8,
+               torch.float8_e4m3fn: E4M3}
     d = Tensor()
     d.data = t.data_ptr() if t.numel() else None
     d.dtype = _DT[t.dtype]

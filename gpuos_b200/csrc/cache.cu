@@ -1,0 +1,518 @@
+// gpuos_cache_write / gpuos_cache_read: a paged cache of keys and values held
+// in 8 or 4 bits, one scale for each group of G elements of a head's row.
+//
+//   a     = max |x| over the group's finite elements
+//   scale = a * fl(1/Q)            Q = 127 (int8), 448 (e4m3), 7 (int4)
+//   inv   = fl(1/a) * Q
+//   code  = x * inv rounded to the format, nearest even
+//   x'    = code * scale, rounded once to the output type
+//
+// all in 32-bit arithmetic with a rounding after each step, so the codes are a
+// function of the inputs alone: no step may be contracted or reordered.
+// Groups below 2^-100 are stored as zeros (their reciprocal leaves the normal
+// range), an infinity as the largest code of its sign, NaN as code 0 (int8,
+// int4) or NaN (e4m3).
+//
+// Both kernels move every byte once and hold a group in the registers of
+// neighbouring lanes: 8 elements a lane, the maximum joined by shuffles.
+#include <cuda_fp8.h>
+
+#include "rowops.cuh"
+
+namespace gpuos {
+namespace rowops {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kUnit = 8;  // elements a lane moves at once
+
+enum Format { kInt8, kE4M3, kInt4 };
+
+struct CacheTensor {
+  const void* x;   // write: the rows; read: unused
+  void* o;         // read: the rows
+  void* codes;
+  float* scales;
+  int64_t rs, rh;              // row tensor: strides of token and head (elements)
+  int64_t cp, cr, ch;          // codes: strides of page, row, head (bytes)
+  int64_t sp, sr, sh, sg;      // scales: strides of page, row, head, group
+  uint32_t items;              // per token: groups (write) or units (read)
+  FastDiv per_head;            // groups or units of a head
+  uint32_t group;              // elements
+  uint32_t head;               // elements
+  FastDiv group_div;
+};
+
+struct CacheArgs {
+  CacheTensor t[2];
+  const void* slots;
+  int64_t ss;
+  int64_t rows;       // pages * page
+  FastDiv page;
+  uint32_t tokens;
+  FastDiv token_items[2];
+  uint32_t lanes_log; // write: lanes that share a group
+  int slot_wide;
+};
+
+__device__ __forceinline__ float q_max(int f) { return f == kInt8 ? 127.f : f == kE4M3 ? 448.f : 7.f; }
+
+// Nearest-even rounding of |y| < 2^22 to an integer, left in the low bits: one
+// addition at full rate where a conversion runs at a quarter of it.
+__device__ __forceinline__ uint32_t round_bits(float y) { return __float_as_uint(__fadd_rn(y, 12582912.f)); }
+
+// 8 values to the codes of their format, in order from the lowest bits.
+template <int F>
+__device__ __forceinline__ uint2 encode(const float (&y)[kUnit]) {
+  uint2 r = make_uint2(0, 0);
+  if constexpr (F == kInt8) {
+    uint32_t b[kUnit];
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) b[i] = round_bits(y[i]);
+    r.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+    r.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
+  } else if constexpr (F == kE4M3) {
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      h[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * i], y[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+    r.x = h[0] | (h[1] << 16);
+    r.y = h[2] | (h[3] << 16);
+  } else {
+    // code + 8 in the low 4 bits: the magic sum's low bits are the code's two's complement
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) r.x |= ((round_bits(y[i]) + 8u) & 15u) << (4 * i);
+  }
+  return r;
+}
+
+// The values of 8 codes.  An integer k in the low bits of a float near 2^23
+// makes it 2^23 + k exactly; a subtraction gives k back at full rate.
+template <int F>
+__device__ __forceinline__ void decode(uint2 r, float (&y)[kUnit]) {
+  if constexpr (F == kInt8) {
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) {
+      const uint32_t w = (i < 4 ? r.x : r.y) ^ 0x80808080u;  // code + 128
+      y[i] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 | (i & 3))) - 8388736.f;
+    }
+  } else if constexpr (F == kE4M3) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = i < 2 ? r.x : r.y;
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * (i & 1))), __NV_E4M3);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      y[2 * i] = f.x;
+      y[2 * i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i)
+      y[i] = __uint_as_float(0x4b000000u | ((r.x >> (4 * i)) & 15u)) - 8388616.f;
+  }
+}
+
+template <int F> constexpr int kCodeBits = F == kInt4 ? 4 : 8;
+
+// Codes of the first n of 8 elements.
+template <int F, bool VEC>
+__device__ __forceinline__ void store_codes(uint8_t* p, uint2 r, int n) {
+  if constexpr (VEC) {
+    if constexpr (F == kInt4) *reinterpret_cast<uint32_t*>(p) = r.x;
+    else *reinterpret_cast<uint2*>(p) = r;
+  } else {
+    const int bytes = n * kCodeBits<F> / 8;
+    for (int i = 0; i < bytes; ++i) p[i] = (uint8_t)((i < 4 ? r.x : r.y) >> (8 * (i & 3)));
+  }
+}
+
+template <int F, bool VEC>
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p, int n) {
+  uint2 r = make_uint2(0, 0);
+  if constexpr (VEC) {
+    if constexpr (F == kInt4) r.x = __ldcs(reinterpret_cast<const uint32_t*>(p));
+    else r = __ldcs(reinterpret_cast<const uint2*>(p));
+  } else {
+    const int bytes = n * kCodeBits<F> / 8;
+    for (int i = 0; i < bytes; ++i) {
+      if (i < 4) r.x |= (uint32_t)p[i] << (8 * i);
+      else r.y |= (uint32_t)p[i] << (8 * (i - 4));
+    }
+  }
+  return r;
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_unit(const T* p, int n, float (&x)[kUnit]) {
+  if constexpr (VEC) {
+    constexpr int W = 16 / sizeof(T);
+#pragma unroll
+    for (int k = 0; k < kUnit; k += W) {
+      const Pack<T, W> q = load_pack<T, W>(p + k);
+#pragma unroll
+      for (int i = 0; i < W; ++i) x[k + i] = to_f(q.v[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) x[i] = i < n ? to_f(p[i]) : 0.f;
+  }
+}
+
+// max that keeps a NaN: a group with one, or with an infinity, shows it in its
+// maximum and takes the careful path below.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// NU units a lane: groups of up to 32 * 8 * NU elements.  IT groups of a lane
+// are in flight.
+template <typename T, int F, bool VEC, int NU, int IT>
+__global__ void __launch_bounds__(kThreads)
+gpuos_cache_write_kernel(const __grid_constant__ CacheArgs a) {
+  const CacheTensor& t = a.t[blockIdx.y];
+  const uint32_t lanes = 1u << a.lanes_log;
+  const uint32_t lane = threadIdx.x & (lanes - 1);
+  const uint32_t per_pass = kThreads >> a.lanes_log;  // groups a CTA handles at once
+  const uint32_t all = a.tokens * t.items;
+  const uint32_t base = blockIdx.x * per_pass * IT + (threadIdx.x >> a.lanes_log);
+  if (base - (threadIdx.x >> a.lanes_log) >= all) return;  // the whole CTA
+
+  float x[IT][NU][kUnit];
+  int64_t co[IT], so[IT];
+  bool has[IT];
+#pragma unroll
+  for (int u = 0; u < IT; ++u) {
+    const uint32_t gi = base + u * per_pass;
+    has[u] = false;
+#pragma unroll
+    for (int k = 0; k < NU; ++k)
+#pragma unroll
+      for (int i = 0; i < kUnit; ++i) x[u][k][i] = 0.f;
+    if (gi >= all) continue;
+    const uint32_t token = a.token_items[blockIdx.y].div(gi);
+    const uint32_t m = gi - token * t.items;
+    const uint32_t head = t.per_head.div(m), g = m - head * t.per_head.d;
+    const int64_t slot = load_index(a.slots, a.slot_wide, token * a.ss);
+    has[u] = slot >= 0 && slot < a.rows;  // rows < 2^31
+    const T* p = static_cast<const T*>(t.x) + token * t.rs + head * t.rh + (int64_t)g * t.group;
+#pragma unroll
+    for (int k = 0; k < NU; ++k) {
+      const int e = (lane + k * lanes) * kUnit;
+      if (has[u] && e < (int)t.group) load_unit<T, VEC>(p + e, (int)t.group - e, x[u][k]);
+    }
+    const uint32_t page = a.page.div((uint32_t)slot), row = (uint32_t)slot - page * a.page.d;
+    co[u] = page * t.cp + row * t.cr + head * t.ch + ((int64_t)g * t.group) * kCodeBits<F> / 8;
+    so[u] = page * t.sp + row * t.sr + head * t.sh + g * t.sg;
+  }
+#pragma unroll
+  for (int u = 0; u < IT; ++u) {
+    float m = 0.f;
+#pragma unroll
+    for (int k = 0; k < NU; ++k)
+#pragma unroll
+      for (int i = 0; i < kUnit; ++i) m = max_nan(m, fabsf(x[u][k][i]));
+    for (uint32_t d = lanes >> 1; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(~0u, m, d));
+    const bool plain = m < __int_as_float(0x7f800000);  // all elements finite
+    if (!__all_sync(~0u, plain)) {
+      float f = 0.f;
+#pragma unroll
+      for (int k = 0; k < NU; ++k)
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i) {
+          const float v = fabsf(x[u][k][i]);
+          if (v < __int_as_float(0x7f800000)) f = fmaxf(f, v);
+        }
+      for (uint32_t d = lanes >> 1; d; d >>= 1) f = fmaxf(f, __shfl_xor_sync(~0u, f, d));
+      m = f;
+    }
+    if (!has[u]) continue;
+    const float q = q_max(F);
+    const bool fits = m >= 0x1p-100f;
+    const float inv = fits ? __fmul_rn(__frcp_rn(m), q) : 0.f;
+    if (lane == 0) t.scales[so[u]] = fits ? __fmul_rn(m, 1.f / q) : 0.f;
+#pragma unroll
+    for (int k = 0; k < NU; ++k) {
+      const int e = (lane + k * lanes) * kUnit;
+      if (e >= (int)t.group) continue;
+      float y[kUnit];
+#pragma unroll
+      for (int i = 0; i < kUnit; ++i) y[i] = __fmul_rn(x[u][k][i], inv);
+      if (!plain) {
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i) {
+          const float v = x[u][k][i];
+          if (fabsf(v) == __int_as_float(0x7f800000)) y[i] = copysignf(q, v);
+          else if (v != v) y[i] = F == kE4M3 ? v : 0.f;
+        }
+      }
+      store_codes<F, VEC>(static_cast<uint8_t*>(t.codes) + co[u] + e * kCodeBits<F> / 8, encode<F>(y),
+                          min((int)t.group - e, kUnit));
+    }
+  }
+}
+
+template <typename T, int F, bool VEC, int IT>
+__global__ void __launch_bounds__(kThreads)
+gpuos_cache_read_kernel(const __grid_constant__ CacheArgs a) {
+  const CacheTensor& t = a.t[blockIdx.y];
+  const uint32_t all = a.tokens * t.items;
+  const uint32_t base = blockIdx.x * kThreads * IT + threadIdx.x;
+  uint2 code[IT];
+  float scale[IT][VEC ? 1 : kUnit];
+  T* o[IT];
+  int n[IT];
+#pragma unroll
+  for (int u = 0; u < IT; ++u) {
+    const uint32_t it = base + u * kThreads;
+    n[u] = 0;
+    if (it >= all) continue;
+    const uint32_t token = a.token_items[blockIdx.y].div(it);
+    const uint32_t m = it - token * t.items;
+    const uint32_t head = t.per_head.div(m), e = (m - head * t.per_head.d) * kUnit;
+    const int64_t slot = load_index(a.slots, a.slot_wide, token * a.ss);
+    o[u] = static_cast<T*>(t.o) + token * t.rs + head * t.rh + e;
+    n[u] = min((int)(t.head - e), kUnit);
+    code[u] = make_uint2(0, 0);
+#pragma unroll
+    for (int i = 0; i < (VEC ? 1 : kUnit); ++i) scale[u][i] = 0.f;
+    if (slot < 0 || slot >= a.rows) {  // no row: zeros
+      if (F == kInt4) code[u].x = 0x88888888u;
+      continue;
+    }
+    const uint32_t page = a.page.div((uint32_t)slot), row = (uint32_t)slot - page * a.page.d;
+    code[u] = load_codes<F, VEC>(static_cast<const uint8_t*>(t.codes) + page * t.cp + row * t.cr +
+                                     head * t.ch + e * kCodeBits<F> / 8, n[u]);
+    const float* s = t.scales + page * t.sp + row * t.sr + head * t.sh;
+    if constexpr (VEC) {
+      scale[u][0] = __ldg(s + t.group_div.div(e) * t.sg);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kUnit; ++i)
+        if (i < n[u]) scale[u][i] = __ldg(s + t.group_div.div(e + i) * t.sg);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < IT; ++u) {
+    if (n[u] == 0) continue;
+    float y[kUnit];
+    decode<F>(code[u], y);
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) y[i] = __fmul_rn(y[i], scale[u][VEC ? 0 : i]);
+    if constexpr (VEC) {
+      constexpr int W = 16 / sizeof(T);
+#pragma unroll
+      for (int k = 0; k < kUnit; k += W) {
+        Pack<T, W> q;
+#pragma unroll
+        for (int i = 0; i < W; ++i) q.v[i] = from_f<T>(y[k + i]);
+        store_pack<T, W>(o[u] + k, q);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kUnit; ++i)
+        if (i < n[u]) o[u][i] = from_f<T>(y[i]);
+    }
+  }
+}
+
+int format_of(int32_t dt) {
+  switch (dt) {
+    case GPUOS_I8: return kInt8;
+    case GPUOS_E4M3: return kE4M3;
+    case GPUOS_U8: return kInt4;
+    default: invalid("codes must be int8, float8_e4m3fn or uint8 (two 4-bit codes a byte)");
+  }
+}
+
+// The checks both directions share.  `rows` are the tensors of rows (x or out).
+CacheArgs prepare(int32_t n, const gpuos_tensor* rows, const char* name, const gpuos_tensor* slots,
+                  const gpuos_tensor* codes, const gpuos_tensor* scales, bool write, bool* vec) {
+  need(n == 1 || n == 2, "takes one or two tensors");
+  need(rows && slots && codes && scales, "NULL tensor");
+  check_tensor(slots, 1, "slots");
+  need(is_index(slots->dtype), "slots must be int32 or int64");
+  CacheArgs a{};
+  *vec = true;
+  const int64_t tokens = slots->sizes[0];
+  need(tokens < (1ll << 31), "too many tokens");
+  for (int i = 0; i < n; ++i) {
+    const gpuos_tensor &x = rows[i], &c = codes[i], &s = scales[i];
+    check_tensor(&x, 3, name);
+    check_tensor(&c, 4, "codes");
+    check_tensor(&s, 4, "scales");
+    need(is_real(x.dtype), write ? "x must be float32, float16 or bfloat16" : "out must be float32, float16 or bfloat16");
+    need(x.dtype == rows[0].dtype, "the tensors of rows must have one dtype");
+    const int f = format_of(c.dtype);
+    need(c.dtype == codes[0].dtype, "the caches must have one format");
+    need(s.dtype == GPUOS_F32, "scales must be float32");
+    const int64_t head = x.sizes[2], bits = f == kInt4 ? 4 : 8;
+    need(x.sizes[0] == tokens, "slots must name one row for each token");
+    need(head > 0 && head < (1 << 20) && x.sizes[1] < (1 << 20), "heads or elements out of range");
+    need(head * bits % 8 == 0, "4-bit codes need an even head size");
+    need(c.sizes[2] == x.sizes[1] && c.sizes[3] == head * bits / 8,
+         "codes must be (page, row, head, codes of a head)");
+    for (int d = 0; d < 3; ++d) need(s.sizes[d] == c.sizes[d], "scales must have the pages, rows and heads of codes");
+    need(c.sizes[0] == codes[0].sizes[0] && c.sizes[1] == codes[0].sizes[1], "the caches must have the same pages");
+    need(s.sizes[3] > 0 && head % s.sizes[3] == 0, "the groups of scales must divide the head");
+    const int64_t group = head / s.sizes[3];
+    need(group <= 1024, "a group has at most 1024 elements");
+    need(group * bits % 8 == 0, "a group of 4-bit codes must fill whole bytes");
+    if (numel(x)) need(x.strides[2] == 1 || head == 1, "the last dim of the rows must be contiguous");
+    if (numel(c)) need(c.strides[3] == 1 || c.sizes[3] == 1, "the last dim of codes must be contiguous");
+    need((__int128)tokens * x.sizes[1] * std::max(s.sizes[3], (head + kUnit - 1) / kUnit) < (1ll << 31),
+         "too many elements in one call");
+    const bool fits = rows_aligned(x, 16 / esize(x.dtype)) && rows_aligned(c, f == kInt4 ? 4 : 8) &&
+                      group % kUnit == 0;
+    if (!fits) *vec = false;
+    CacheTensor& t = a.t[i];
+    t.x = x.data;
+    t.o = x.data;
+    t.codes = c.data;
+    t.scales = static_cast<float*>(s.data);
+    t.rs = x.strides[0];
+    t.rh = x.strides[1];
+    t.cp = c.strides[0];
+    t.cr = c.strides[1];
+    t.ch = c.strides[2];
+    t.sp = s.strides[0];
+    t.sr = s.strides[1];
+    t.sh = s.strides[2];
+    t.sg = s.strides[3];
+    t.head = (uint32_t)head;
+    t.group = (uint32_t)group;
+    t.group_div = FastDiv(t.group);
+    const uint32_t per_head = write ? (uint32_t)s.sizes[3] : (uint32_t)((head + kUnit - 1) / kUnit);
+    t.per_head = FastDiv(per_head);
+    t.items = (uint32_t)x.sizes[1] * per_head;
+    a.token_items[i] = FastDiv(std::max(t.items, 1u));
+  }
+  const __int128 cache_rows = (__int128)codes[0].sizes[0] * codes[0].sizes[1];
+  need(cache_rows < ((__int128)1 << 31), "the cache has too many rows");
+  a.rows = (int64_t)cache_rows;
+  a.page = FastDiv((uint32_t)std::max<int64_t>(1, codes[0].sizes[1]));
+  a.slots = slots->data;
+  a.ss = slots->strides[0];
+  a.slot_wide = slots->dtype == GPUOS_I64;
+  a.tokens = (uint32_t)tokens;
+  return a;
+}
+
+template <typename T, int F>
+void launch_write(const CacheArgs& a, bool vec, int n, uint32_t most_group, uint64_t most, cudaStream_t s) {
+  const uint32_t lanes = 1u << a.lanes_log;
+  const int units = (int)((most_group + kUnit * lanes - 1) / (kUnit * lanes));
+  const uint64_t per_pass = kThreads >> a.lanes_log;
+  // few groups: one a lane, so that they start on many SMs at once
+  const int it = units == 1 && most > per_pass * 4 * (uint64_t)sm_count() ? 4 : 1;
+  const dim3 grid((unsigned)((most + per_pass * it - 1) / (per_pass * it)), n);
+#define GPUOS_CW(VEC, NU, IT) gpuos_cache_write_kernel<T, F, VEC, NU, IT><<<grid, kThreads, 0, s>>>(a)
+  if (vec) {
+    if (units == 1 && it == 4) GPUOS_CW(true, 1, 4);
+    else if (units == 1) GPUOS_CW(true, 1, 1);
+    else GPUOS_CW(true, 4, 1);
+  } else {
+    if (units == 1 && it == 4) GPUOS_CW(false, 1, 4);
+    else if (units == 1) GPUOS_CW(false, 1, 1);
+    else GPUOS_CW(false, 4, 1);
+  }
+#undef GPUOS_CW
+}
+
+template <typename T, int F>
+void launch_read(const CacheArgs& a, bool vec, int n, uint64_t most, cudaStream_t s) {
+  const int it = vec && most > kThreads * 4 * (uint64_t)sm_count() ? 4 : 1;
+  const dim3 grid((unsigned)((most + kThreads * it - 1) / (kThreads * it)), n);
+  if (vec && it == 4) gpuos_cache_read_kernel<T, F, true, 4><<<grid, kThreads, 0, s>>>(a);
+  else if (vec) gpuos_cache_read_kernel<T, F, true, 1><<<grid, kThreads, 0, s>>>(a);
+  else gpuos_cache_read_kernel<T, F, false, 1><<<grid, kThreads, 0, s>>>(a);
+}
+
+template <typename L>
+void by_type(int32_t dt, int32_t codes, L&& launch) {
+  auto with = [&](auto type) {
+    using T = decltype(type);
+    switch (format_of(codes)) {
+      case kInt8: launch(type, std::integral_constant<int, kInt8>()); break;
+      case kE4M3: launch(type, std::integral_constant<int, kE4M3>()); break;
+      default: launch(type, std::integral_constant<int, kInt4>()); break;
+    }
+    (void)sizeof(T);
+  };
+  if (dt == GPUOS_F32) with(float());
+  else if (dt == GPUOS_F16) with(__half());
+  else with(__nv_bfloat16());
+}
+
+void cache_write(int32_t n, const gpuos_tensor* x, const gpuos_tensor* slots, const gpuos_tensor* codes,
+                 const gpuos_tensor* scales, cudaStream_t stream) {
+  bool vec;
+  CacheArgs a = prepare(n, x, "x", slots, codes, scales, true, &vec);
+  uint32_t group = 1;
+  uint64_t most = 0;
+  for (int i = 0; i < n; ++i) {
+    check_output(codes[i], "codes");
+    check_output(scales[i], "scales");
+    no_overlap(codes[i], scales[i], "codes overlap scales");
+    for (int k = 0; k < n; ++k) {
+      no_overlap(codes[i], x[k], "codes overlap x");
+      no_overlap(scales[i], x[k], "scales overlap x");
+      if (k == i) continue;
+      no_overlap(codes[i], codes[k], "the caches overlap");
+      no_overlap(scales[i], scales[k], "the caches overlap");
+      no_overlap(codes[i], scales[k], "the caches overlap");
+    }
+    no_overlap(codes[i], *slots, "codes overlap slots");
+    no_overlap(scales[i], *slots, "scales overlap slots");
+    group = std::max(group, a.t[i].group);
+    most = std::max(most, (uint64_t)a.tokens * a.t[i].items);
+  }
+  if (most == 0 || a.rows == 0) return;
+  a.lanes_log = 0;
+  while (a.lanes_log < 5 && (uint32_t)(kUnit << a.lanes_log) < group) ++a.lanes_log;
+  by_type(x[0].dtype, codes[0].dtype, [&](auto type, auto f) {
+    launch_write<decltype(type), decltype(f)::value>(a, vec, n, group, most, stream);
+  });
+  cuda_ok(cudaGetLastError(), "launch");
+}
+
+void cache_read(int32_t n, const gpuos_tensor* slots, const gpuos_tensor* codes, const gpuos_tensor* scales,
+                const gpuos_tensor* out, cudaStream_t stream) {
+  bool vec;
+  const CacheArgs a = prepare(n, out, "out", slots, codes, scales, false, &vec);
+  uint64_t most = 0;
+  for (int i = 0; i < n; ++i) {
+    check_output(out[i], "out");
+    no_overlap(out[i], *slots, "out overlaps slots");
+    for (int k = 0; k < n; ++k) {
+      no_overlap(out[i], codes[k], "out overlaps codes");
+      no_overlap(out[i], scales[k], "out overlaps scales");
+      if (k != i) no_overlap(out[i], out[k], "the outputs overlap");
+    }
+    most = std::max(most, (uint64_t)a.tokens * a.t[i].items);
+  }
+  if (most == 0) return;
+  by_type(out[0].dtype, codes[0].dtype, [&](auto type, auto f) {
+    launch_read<decltype(type), decltype(f)::value>(a, vec, n, most, stream);
+  });
+  cuda_ok(cudaGetLastError(), "launch");
+}
+
+}  // namespace
+}  // namespace rowops
+}  // namespace gpuos
+
+extern "C" int32_t gpuos_cache_write(int32_t n, const gpuos_tensor* x, const gpuos_tensor* slots,
+                                     const gpuos_tensor* codes, const gpuos_tensor* scales, void* stream) {
+  return gpuos::rowops::entry("gpuos_cache_write", [&] {
+    gpuos::rowops::cache_write(n, x, slots, codes, scales, static_cast<cudaStream_t>(stream));
+  });
+}
+
+extern "C" int32_t gpuos_cache_read(int32_t n, const gpuos_tensor* slots, const gpuos_tensor* codes,
+                                    const gpuos_tensor* scales, const gpuos_tensor* out, void* stream) {
+  return gpuos::rowops::entry("gpuos_cache_read", [&] {
+    gpuos::rowops::cache_read(n, slots, codes, scales, out, static_cast<cudaStream_t>(stream));
+  });
+}

@@ -635,4 +635,13 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "gpuos_ext",
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_gpuos_ext(void) { return PyModule_Create(&kModule); }
+PyMethodDef* gpuos_rowops_methods();  // rowops_ext.cpp
+
+PyMODINIT_FUNC PyInit_gpuos_ext(void) {
+  PyObject* m = PyModule_Create(&kModule);
+  if (m && PyModule_AddFunctions(m, gpuos_rowops_methods()) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -1,0 +1,278 @@
+"""Row operators of a language model's step, beside the executor's elementwise
+requests and reductions: rotary positions, a quantised cache, routing to
+experts, and log probabilities of given tokens.
+
+Each call runs one kernel at once on torch's current stream of its tensors'
+device; it allocates its outputs (where `out` gives none) and nothing else, so it
+may be captured into a CUDA graph.  As with an op of torch's own, requests
+submitted to an executor are seen once they are flushed; inside a
+``scheduler_context`` of the calling thread, pending requests on the call's
+tensors are flushed first.  Tensors are CUDA tensors of one device.  A call that
+breaks a rule raises ``ValueError`` (``TypeError`` for a dtype, ``RuntimeError``
+for a device) and launches nothing.
+
+``rotary``, ``route`` and ``logprobs`` take part in autograd; their gradients
+are also there as calls of their own (``rotary(..., inverse=True)``,
+``route_grad``, ``logprobs_grad``), for steps that are captured or keep no graph.
+include/gpuos_b200.h states each operator's formula and its edge cases.
+"""
+from __future__ import annotations
+
+import math
+from typing import NamedTuple, Optional, Tuple, Union
+
+import torch
+
+from . import load as _load
+from . import scheduler as _scheduler
+
+_ext = _load()
+_entered = _scheduler._entered
+
+_SCORE = {"softmax": 0, "sigmoid": 1}
+_GROUP_SCORE = {"max": 0, "top2": 1}
+_ROW_DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+CACHE_FORMATS = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn, "int4": torch.uint8}
+
+Tensors = Union[torch.Tensor, Tuple[torch.Tensor, ...]]
+
+
+def _tuple(x) -> tuple:
+    return (x,) if isinstance(x, torch.Tensor) else tuple(x)
+
+
+def _order(reads, writes=()):
+    if getattr(_entered, "modes", None):
+        _scheduler.order_after_pending([t for t in reads if t is not None], writes)
+
+
+def _choice(table, value, name):
+    try:
+        return table[value]
+    except (KeyError, TypeError):
+        raise ValueError(f"{name} must be one of {', '.join(map(repr, table))}, not {value!r}") from None
+
+
+def _row(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """A gradient as the kernels read it: elements of a row side by side."""
+    if g is None or g.dim() == 0 or g.stride(-1) == 1 or g.size(-1) == 1:
+        return g
+    return g.contiguous()
+
+
+# ---- rotary positions ----------------------------------------------------------
+def rotary_frequencies(rot_dim: int, *, base: float = 10000.0, scaling: str = "none",
+                       factor: float = 1.0, low: float = 1.0, high: float = 32.0,
+                       length: Optional[int] = None, device=None) -> torch.Tensor:
+    """``inv_freq`` of ``rotary``: float64 [rot_dim / 2], radians a position turns
+    each pair by, ``base ** (-2 i / rot_dim)`` scaled for contexts `factor` times
+    the trained one:
+
+    * ``"none"``; ``"linear"``: all divided by `factor` (positions interpolated);
+    * ``"ntk"``: the base grows so that the slowest pair is divided by `factor`;
+    * ``"ramp"``: pairs that turn more than `high` times within the trained
+      `length` stay, those that turn less than `low` times are divided by `factor`, the others are
+      mixed linearly in their number of turns.
+    """
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError("rot_dim must be even and at least 2")
+    if not (base > 1 and math.isfinite(base) and factor > 0 and math.isfinite(factor)):
+        raise ValueError("base must be above 1 and factor above 0, both finite")
+    if scaling == "ntk":
+        if rot_dim > 2:
+            base = base * factor ** (rot_dim / (rot_dim - 2))
+    elif scaling not in ("none", "linear", "ramp"):
+        raise ValueError(f"scaling must be 'none', 'linear', 'ntk' or 'ramp', not {scaling!r}")
+    f = base ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    if scaling == "linear":
+        f = f / factor
+    if scaling == "ramp":
+        if length is None or not high > low:
+            raise ValueError("ramp needs length, and low below high")
+        keep = ((length * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        f = f / factor * (1 - keep) + f * keep
+    return f if device is None else f.to(device)
+
+
+def rotary(x: Tensors, positions: torch.Tensor, inv_freq: torch.Tensor, *, scale: float = 1.0,
+           interleaved: bool = False, inverse: bool = False, out: Optional[Tensors] = None) -> Tensors:
+    """Rotary positions on `x`, a tensor or a pair of tensors (queries and keys) of
+    the same tokens: (token, head, element) or (batch, token, head, element), any
+    strides but the last, which is 1.  `positions` (int32 or int64) has the token
+    dims.  The first ``2 * len(inv_freq)`` elements of each head are rotated by
+    ``position * inv_freq`` (in 64 bits) and multiplied by `scale`, in pairs (i, i + half),
+    or (2i, 2i + 1) if `interleaved`; the others are copied.  `inverse` rotates back
+    (the transposed map, also the gradient).  `out` may be `x`.  Returns tensors as `x` is given."""
+    xs = _tuple(x)
+    outs = None if out is None else _tuple(out)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in xs):
+        if outs is not None:
+            raise ValueError("out cannot be given where a gradient is needed")
+        got = _Rotary.apply(positions, inv_freq, scale, interleaved, inverse, *xs)
+    else:
+        _order((*xs, positions, inv_freq), outs or ())
+        got = _ext.rotary(xs, outs, positions, inv_freq, scale, interleaved, inverse)
+    return got[0] if isinstance(x, torch.Tensor) else got
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, positions, inv_freq, scale, interleaved, inverse, *xs):
+        _order((*xs, positions, inv_freq))
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.how = dict(scale=scale, interleaved=interleaved, inverse=not inverse)
+        ctx.set_materialize_grads(False)
+        return _ext.rotary(xs, None, positions, inv_freq, scale, interleaved, inverse)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        positions, inv_freq = ctx.saved_tensors
+        need = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[5 + i]]
+        got = [None] * len(grads)
+        if need:
+            for i, g in zip(need, rotary(tuple(_row(grads[i]) for i in need), positions, inv_freq, **ctx.how)):
+                got[i] = g
+        return (None,) * 5 + tuple(got)
+
+
+# ---- quantised cache -------------------------------------------------------------
+def cache_alloc(pages: int, page_size: int, heads: int, head_dim: int, *, format: str = "int8",
+                group: Optional[int] = None, device=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """An empty cache: (codes, scales), zeros.  codes is (page, row, head, code) in
+    the format's dtype (int8; float8_e4m3fn; uint8 with two 4-bit codes a byte);
+    scales is float32 (page, row, head, group) with a scale for each `group`
+    elements (default: the whole head)."""
+    dtype = _choice(CACHE_FORMATS, format, "format")
+    group = head_dim if group is None else group
+    if group < 1 or head_dim % group or (format == "int4" and group % 2):
+        raise ValueError("group must divide head_dim (and be even for int4)")
+    width = head_dim // 2 if format == "int4" else head_dim
+    device = "cuda" if device is None else device
+    codes = torch.zeros(pages, page_size, heads, width, dtype=torch.uint8, device=device)
+    scales = torch.zeros(pages, page_size, heads, head_dim // group, device=device)
+    return codes.view(dtype), scales
+
+
+def cache_write(x: Tensors, slots: torch.Tensor, codes: Tensors, scales: Tensors) -> None:
+    """Quantise rows into a paged cache: `x` is a tensor or a pair (keys and
+    values), (token, head, element); token t goes to row ``slots[t]`` of the cache, counted
+    through its pages.  A slot outside the cache (-1: padding) writes nothing; the
+    slots inside it must differ.  `codes` and `scales` as from ``cache_alloc``, one of each
+    for each of `x`; any strides but the last (a page may hold its heads before its rows)."""
+    xs, cs, ss = _tuple(x), _tuple(codes), _tuple(scales)
+    _order((*xs, slots), (*cs, *ss))
+    _ext.cache_write(xs, slots, cs, ss)
+
+
+def cache_read(slots: torch.Tensor, codes: Tensors, scales: Tensors, *, dtype: torch.dtype = torch.bfloat16,
+               out: Optional[Tensors] = None) -> Tensors:
+    """The rows of a cache at `slots` (token, head, element) in `dtype`, or written
+    to `out`; zeros for a slot outside the cache.  Returns tensors as `codes` is given."""
+    cs, ss = _tuple(codes), _tuple(scales)
+    outs = None if out is None else _tuple(out)
+    _order((slots, *cs, *ss), outs or ())
+    if dtype not in _ROW_DTYPE:
+        raise TypeError("dtype must be float32, float16 or bfloat16")
+    got = _ext.cache_read(slots, cs, ss, outs, _ROW_DTYPE[dtype])
+    return got[0] if isinstance(codes, torch.Tensor) else got
+
+
+# ---- routing -----------------------------------------------------------------------
+def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Optional[torch.Tensor] = None,
+          groups: int = 1, top_groups: int = 1, group_score: str = "max", renormalize: bool = False,
+          scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(weights float32, experts int64), both (token, top_k), of logits (token,
+    expert): the `top_k` experts with the largest score (+ `bias`, float32 [expert], for balance:
+    it chooses and does not weigh), in falling order, of equal ones the lowest index
+    first.  With `groups`, only experts of the best `top_groups` groups are chosen from; a group is
+    worth its largest key, or with ``group_score="top2"`` the sum of its two
+    largest.  Weights are the scores, divided by their sum if `renormalize`, times `scale`.
+    The choice is that of exact arithmetic."""
+    how = (_choice(_SCORE, score, "score"), groups, top_groups, _choice(_GROUP_SCORE, group_score, "group_score"),
+           renormalize, scale)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _Route.apply(logits, bias, top_k, how)
+    _order((logits, bias))
+    return _ext.route(logits, bias, top_k, *how)
+
+
+def route_grad(logits: torch.Tensor, experts: torch.Tensor, grad_weights: torch.Tensor, *, score: str = "softmax",
+               renormalize: bool = False, scale: float = 1.0) -> torch.Tensor:
+    """The gradient of the logits from that of ``route``'s weights (float32)."""
+    _order((logits, experts, grad_weights))
+    return _ext.route_grad(logits, experts, grad_weights, _choice(_SCORE, score, "score"), renormalize, scale)
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, top_k, how):
+        _order((logits, bias))
+        weights, experts = _ext.route(logits, bias, top_k, *how)
+        ctx.save_for_backward(logits, experts)
+        ctx.how = (how[0], how[4], how[5])
+        ctx.mark_non_differentiable(experts)
+        return weights, experts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_weights, _):
+        logits, experts = ctx.saved_tensors
+        _order((logits, experts, grad_weights))
+        return _ext.route_grad(logits, experts, grad_weights, *ctx.how), None, None, None
+
+
+# ---- log probabilities ---------------------------------------------------------------
+class LogProbs(NamedTuple):
+    logprob: torch.Tensor                  # float32 [row]
+    entropy: Optional[torch.Tensor]        # float32 [row], nats
+    top_logprobs: Optional[torch.Tensor]   # float32 (row, top)
+    top_tokens: Optional[torch.Tensor]     # int64 (row, top)
+    stats: Optional[torch.Tensor]          # float32 (row, 2), for logprobs_grad
+
+
+def logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0, entropy: bool = False,
+             temperature: float = 1.0, stats: bool = False) -> LogProbs:
+    """Log probabilities of `targets` (int32 or int64 [row]) under
+    ``softmax(logits / temperature)``, logits (row, token); with `entropy` the
+    distribution's entropy, with `top` the likeliest tokens and their log probabilities (at
+    most 64; of equal logits the lowest index first), with `stats` what
+    ``logprobs_grad`` needs.  A negative target is padding (0).  Gradients flow to
+    the logits from ``logprob`` and ``entropy``."""
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return LogProbs(*_LogProbs.apply(logits, targets, top, entropy, temperature))
+    _order((logits, targets))
+    return LogProbs(*_ext.logprobs(logits, targets, top, entropy, temperature, stats))
+
+
+def logprobs_grad(logits: torch.Tensor, targets: torch.Tensor, result: LogProbs,
+                  grad_logprob: Optional[torch.Tensor], grad_entropy: Optional[torch.Tensor] = None, *,
+                  temperature: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The gradient of the logits from those of ``logprobs``'s logprob and entropy
+    (float32 [row]); `result` is what ``logprobs(..., stats=True)`` gave for the same
+    arguments.  `out` may be `logits`."""
+    if result.stats is None:
+        raise ValueError("result has no stats: call logprobs(..., stats=True)")
+    _order((logits, targets, result.stats, result.entropy, grad_logprob, grad_entropy), () if out is None else (out,))
+    return _ext.logprobs_grad(logits, targets, result.stats, result.entropy, grad_logprob, grad_entropy, temperature, out)
+
+
+class _LogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, top, entropy, temperature):
+        _order((logits, targets))
+        got = _ext.logprobs(logits, targets, top, entropy, temperature, True)
+        ctx.save_for_backward(logits, targets, got[1], got[4])
+        ctx.temperature = temperature
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*(t for t in got[2:] if t is not None))
+        return got
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_logprob, grad_entropy, *_):
+        if grad_logprob is None and grad_entropy is None:
+            return (None,) * 5
+        logits, targets, entropy, stats = ctx.saved_tensors
+        _order((logits, targets, stats, entropy, grad_logprob, grad_entropy))
+        return (_ext.logprobs_grad(logits, targets, stats, entropy, grad_logprob, grad_entropy, ctx.temperature,
+                                   None),) + (None,) * 4

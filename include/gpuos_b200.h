@@ -35,6 +35,13 @@ extern "C" {
 #define GPUOS_F32 0
 #define GPUOS_F16 1
 #define GPUOS_BF16 2
+/* codes of the row operators' other tensors; requests take the three above only */
+#define GPUOS_I32 3
+#define GPUOS_F64 4
+#define GPUOS_I64 5
+#define GPUOS_U8 6
+#define GPUOS_I8 7
+#define GPUOS_E4M3 8 /* 8-bit floating point: 4 exponent and 3 mantissa bits, no infinities */
 
 /* execution modes */
 #define GPUOS_MODE_PERSISTENT 0 /* resident worker grid fed through a mapped doorbell */
@@ -328,6 +335,108 @@ int32_t gpuos_get_stats(gpuos_executor* ex, gpuos_stats* out);
 int32_t gpuos_reduce_rows_noalloc(int32_t variant, const void* x, int32_t x_dtype, int64_t rows,
                                   int64_t cols, int64_t row_stride, void* out, int32_t out_dtype,
                                   void* stream);
+
+/* ---- row operators of a language model's step ------------------------------
+ * No counterpart in the reference.  They stand beside gpuos_reduce_rows_noalloc:
+ * each runs at once on `stream` (a cudaStream_t of the current device; NULL =
+ * the legacy stream), needs no executor, allocates nothing and keeps nothing
+ * between calls, so calls may overlap, run on several streams and be captured
+ * into CUDA graphs.  Requests queued on an executor are not seen before they are
+ * flushed.  Strides are in elements and not negative; an output must not
+ * overlap itself, an input (but for the in-place forms below) or another
+ * output; a call that breaks a rule returns GPUOS_EINVAL and launches nothing.
+ * Sums, softmax statistics and scores are held in 32 bits or more; a result
+ * is rounded once, when it is stored. */
+
+/* Rotary positions on n = 1 or 2 tensors (queries and keys) of the same tokens.
+ * x[i], out[i]: f32, f16 or bf16, (token, head, element) or (batch, token, head,
+ * element), last stride 1; heads and elements may differ between the two.
+ * positions: i32 or i64, x's token dims; any value.  inv_freq: f64 or f32
+ * [pairs], radians a position turns pair i by, at most 2048 pairs.  With
+ * a = position * inv_freq[i] (in 64 bits), pair (x1, x2) of the head's first
+ * 2 * pairs elements becomes scale * (x1 cos a - x2 sin a, x2 cos a + x1 sin a);
+ * the other elements are copied unscaled.  Pair i is elements (i, i + pairs), or
+ * (2i, 2i + 1) with GPUOS_ROTARY_INTERLEAVED.  GPUOS_ROTARY_INVERSE takes -a:
+ * the transposed map, which is also the gradient.  out[i] may be x[i]. */
+#define GPUOS_ROTARY_INTERLEAVED 1
+#define GPUOS_ROTARY_INVERSE 2
+int32_t gpuos_rotary(int32_t n, const gpuos_tensor* x, const gpuos_tensor* out,
+                     const gpuos_tensor* positions, const gpuos_tensor* inv_freq, float scale,
+                     int32_t flags, void* stream);
+
+/* Write the rows of n = 1 or 2 tensors (keys and values) into a paged cache
+ * held in 8 or 4 bits.  x[i]: f32, f16 or bf16 (token, head, element), last
+ * stride 1.  slots: i32 or i64 [token]: token t goes to row slots[t] % page of page
+ * slots[t] / page; a slot outside the cache (-1: padding) writes nothing; the
+ * slots of one call that are in the cache must differ (a row named twice holds a
+ * mixture).  codes[i]: (page, row, head, code) with last stride 1; the dtype is the format: GPUOS_I8,
+ * GPUOS_E4M3, or GPUOS_U8 for two 4-bit codes a byte (the even element in the
+ * low half, 8 added to the code).  scales[i]: f32 (page, row, head, group), the
+ * head's elements in groups of at most 1024 neighbours.  Over a group with the largest magnitude a, in
+ * 32 bits with each step rounded: scale = a * (1/Q), code = x * ((1/a) * Q)
+ * rounded to the format, nearest even; Q = 127, 448, 7.  Where a < 2^-100
+ * scale and codes are 0.  An infinity takes the largest code and does not count
+ * for a, nor does NaN, which takes code 0 (E4M3: NaN). */
+int32_t gpuos_cache_write(int32_t n, const gpuos_tensor* x, const gpuos_tensor* slots,
+                          const gpuos_tensor* codes, const gpuos_tensor* scales, void* stream);
+
+/* Read rows back: out[i][t] = code * scale of row slots[t], rounded to out's
+ * dtype (f32, f16 or bf16); zeros for a slot outside the cache.  Arguments as
+ * in gpuos_cache_write; slots may repeat. */
+int32_t gpuos_cache_read(int32_t n, const gpuos_tensor* slots, const gpuos_tensor* codes,
+                         const gpuos_tensor* scales, const gpuos_tensor* out, void* stream);
+
+/* Route tokens to experts.  logits: f32, f16 or bf16 (token, expert), last
+ * stride 1, at most 1024 experts.  Scores s are the softmax or the sigmoid of a
+ * row, keys are s + bias (bias: f32 [expert] or NULL; without one experts are
+ * ordered by their logits).  The experts form `groups` (at most 64) groups of neighbours;
+ * a group is worth its largest key or the sum of its two largest, and the best
+ * `top_groups` stay open.  experts (i32 or i64, (token, top_k), top_k at most 64)
+ * gets the largest keys of the open groups in falling order, weights (f32) their
+ * scores without bias, divided by their sum with `renormalize`, times `scale`.
+ * The choice is that of exact arithmetic; of equal keys, and of equal groups, the
+ * lowest index comes first.  A NaN logit counts as -inf in the choice; a row of
+ * -inf has scores 0 (softmax), and where the chosen scores sum to 0 the
+ * renormalised weights are 0. */
+#define GPUOS_SCORE_SOFTMAX 0
+#define GPUOS_SCORE_SIGMOID 1
+#define GPUOS_GROUP_MAX 0
+#define GPUOS_GROUP_TOP2 1
+int32_t gpuos_route(const gpuos_tensor* logits, const gpuos_tensor* bias,
+                    const gpuos_tensor* weights, const gpuos_tensor* experts, int32_t score,
+                    int32_t groups, int32_t top_groups, int32_t group_score, int32_t renormalize,
+                    float scale, void* stream);
+
+/* The gradient of gpuos_route's weights: grad_logits (logits' sizes and dtype)
+ * from grad_weights (f32, (token, top_k)) and the experts chosen.  An expert
+ * outside the row counts as not chosen. */
+int32_t gpuos_route_grad(const gpuos_tensor* logits, const gpuos_tensor* experts,
+                         const gpuos_tensor* grad_weights, const gpuos_tensor* grad_logits,
+                         int32_t score, int32_t renormalize, float scale, void* stream);
+
+/* Log probabilities of given tokens under softmax(logits / temperature).
+ * logits: f32, f16 or bf16 (row, token), last stride 1, fewer than 2^30 tokens;
+ * targets: i32 or i64 [row].  logprob: f32 [row], 0 where the target is negative
+ * (padding), NaN where it is past the row.  Optional (NULL: not wanted):
+ * entropy, f32 [row], in nats; top_logprobs (f32) and top_tokens (i32 or i64),
+ * both (row, k) with k at most 64: the likeliest tokens in falling order, of equal ones
+ * the lowest index; stats, f32 (row, 2): the row's maximum and the sum of
+ * exp((x - maximum) / temperature), for the gradient.  A -inf logit is a masked
+ * token.  A row of -inf has log probabilities -inf and entropy 0; one with NaN
+ * or +inf has NaN, and alternatives that are some tokens of the row. */
+int32_t gpuos_logprobs(const gpuos_tensor* logits, const gpuos_tensor* targets,
+                       const gpuos_tensor* logprob, const gpuos_tensor* entropy,
+                       const gpuos_tensor* top_logprobs, const gpuos_tensor* top_tokens,
+                       const gpuos_tensor* stats, float temperature, void* stream);
+
+/* The gradient of gpuos_logprobs' logprob and entropy (one of grad_logprob and
+ * grad_entropy may be NULL; grad_entropy needs entropy): grad_logits has logits'
+ * sizes and dtype and may be logits itself.  Padding rows take no gradient of
+ * logprob; a row of -inf has gradient 0. */
+int32_t gpuos_logprobs_grad(const gpuos_tensor* logits, const gpuos_tensor* targets,
+                            const gpuos_tensor* stats, const gpuos_tensor* entropy,
+                            const gpuos_tensor* grad_logprob, const gpuos_tensor* grad_entropy,
+                            const gpuos_tensor* grad_logits, float temperature, void* stream);
 
 #ifdef __cplusplus
 }
