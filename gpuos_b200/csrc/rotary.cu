@@ -11,10 +11,12 @@
 // where a 32-bit product is off by whole radians.  What is left, at most half
 // a turn, is rounded to 32 bits (2^-25 turns) for sincospif.
 //
-// One CTA takes whole tokens: it computes the tokens' (c, d) once into shared
-// memory and every head reads them there, so the sines cost R/2 evaluations a
-// token, not R/2 a head, and the kernel is left with its bytes: x once in, once
-// out.  The first items' loads are in flight while the sines are computed.
+// A thread belongs to one token and one group of V elements (16 bytes where
+// alignment allows) and walks over the heads in steps: its pairs' (c, d) stay in
+// registers, and a head costs its loads, the arithmetic and its stores.  The
+// CTA computes the (c, d) of its tokens once, into shared memory, while the first
+// heads' loads are in flight: R/2 sines a token, not R/2 a head.  What is left are the
+// bytes: x once in, once out.
 #include "rowops.cuh"
 
 namespace gpuos {
@@ -22,16 +24,15 @@ namespace rowops {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kItems = 4;           // items a thread has in flight
+constexpr int kHeads = 4;           // heads a thread has in flight
 constexpr int kTablePairs = 2048;   // (c, d) pairs a CTA holds: 16 KB
 
 struct RotTensor {
   const void* x;
   void* o;
   int64_t xs0, xs1, xh, os0, os1, oh;  // element strides: outer token, inner token, head
-  uint32_t items;                      // per token: heads * per_head
-  FastDiv per_head;
-  uint32_t copies;                     // items of a head from `turned` on are copied
+  uint32_t heads;
+  uint32_t copies;                     // groups of V elements behind the rotated ones
 };
 
 struct RotArgs {
@@ -39,14 +40,14 @@ struct RotArgs {
   const void* pos;
   const void* freq;
   int64_t ps0, ps1, fs;
-  int64_t tokens;
-  int64_t inner;        // tokens of the inner token dim
-  uint32_t half;        // pairs
-  uint32_t turned;      // items of a head that are rotated
+  uint32_t tokens;
+  FastDiv inner;        // tokens of the inner token dim
+  FastDiv half;         // pairs
+  uint32_t units;       // groups of V elements (of x1 in the half layout) that are rotated
+  FastDiv lanes;        // threads side by side over a head's groups
+  FastDiv per_token;    // threads of a token: lanes * head groups
+  uint32_t head_step;   // head groups of all CTAs that share a token
   uint32_t tile;        // tokens a CTA takes
-  uint32_t split;       // CTAs that share a tile's items
-  FastDiv token_items;
-  FastDiv half_div;
   float scale;
   int pos_wide, freq_wide;
 };
@@ -74,39 +75,6 @@ __device__ __forceinline__ void put(T* p, const Pack<T, V>& r) {
   }
 }
 
-struct Item {
-  uint32_t token;  // of the tile
-  uint32_t j;      // of the head
-  int64_t xo, oo;  // element offsets of the item's first element
-  int which;
-  bool turn;
-};
-
-template <int V, bool INTER>
-__device__ __forceinline__ Item locate(const RotArgs& a, uint32_t it, int64_t tok0) {
-  Item r;
-  r.token = a.token_items.div(it);
-  uint32_t m = it - r.token * a.token_items.d;
-  r.which = m >= a.t[0].items;
-  if (r.which) m -= a.t[0].items;
-  const RotTensor& t = a.t[r.which];
-  const uint32_t head = t.per_head.div(m);
-  r.j = m - head * t.per_head.d;
-  r.turn = r.j < a.turned;
-  const int64_t token = tok0 + r.token;
-  int64_t outer = 0, inner = token;
-  if (a.inner != a.tokens) {
-    outer = token / a.inner;
-    inner = token - outer * a.inner;
-  }
-  // rotated items step by V; the copied part starts behind all R elements
-  const int64_t e = r.turn ? (int64_t)r.j * V
-                           : 2 * (int64_t)a.half + (int64_t)(r.j - a.turned) * V;
-  r.xo = outer * t.xs0 + inner * t.xs1 + head * t.xh + e;
-  r.oo = outer * t.os0 + inner * t.os1 + head * t.oh + e;
-  return r;
-}
-
 // The table holds for item j of a head the V (half layout) or V/2 pairs it
 // needs, chunk k of two pairs at [k][j], so that neighbouring lanes read
 // neighbouring 16 bytes.
@@ -120,101 +88,129 @@ __device__ __forceinline__ uint32_t table_at(uint32_t token, uint32_t pair, uint
 template <typename T, int V, int VL, bool INTER>
 __global__ void __launch_bounds__(kThreads)
 gpuos_rotary_kernel(const __grid_constant__ RotArgs a) {
-  constexpr int P = INTER ? V / 2 : V;  // pairs an item rotates
+  constexpr int P = INTER ? V / 2 : V;  // pairs of a group
   __shared__ __align__(16) float2 table[kTablePairs];
-  const uint32_t tile = blockIdx.x / a.split, part = blockIdx.x - tile * a.split;
-  const int64_t tok0 = (int64_t)tile * a.tile;
-  const uint32_t ntok = (uint32_t)min((int64_t)a.tile, a.tokens - tok0);
-  const uint32_t all = ntok * a.token_items.d;
-  const uint32_t lo = (uint32_t)((uint64_t)all * part / a.split);
-  const uint32_t hi = (uint32_t)((uint64_t)all * (part + 1) / a.split);
+  const uint32_t half = a.half.d;
+  const uint32_t tok0 = blockIdx.x * a.tile;
+  const uint32_t ntok = min(a.tile, a.tokens - tok0);
+  const uint32_t mine = a.per_token.div(threadIdx.x);  // token of the tile
+  const uint32_t rest = threadIdx.x - mine * a.per_token.d;
+  const uint32_t group = a.lanes.div(rest), j0 = rest - group * a.lanes.d;
+  const uint32_t h0 = group + blockIdx.y * (a.per_token.d / a.lanes.d);
+  const bool live = mine < ntok;
+  const uint32_t heads = a.t[0].heads + a.t[1].heads;
 
-  Item item[kItems];
-  Pack<T, V> x1[kItems], x2[kItems];
-  auto load = [&](uint32_t base) {
+  // the token's rows
+  const T *x0 = nullptr, *x1 = nullptr;
+  T *o0 = nullptr, *o1 = nullptr;
+  if (live) {
+    const uint32_t outer = a.inner.div(tok0 + mine), in = tok0 + mine - outer * a.inner.d;
+    x0 = static_cast<const T*>(a.t[0].x) + outer * a.t[0].xs0 + in * a.t[0].xs1;
+    x1 = static_cast<const T*>(a.t[1].x) + outer * a.t[1].xs0 + in * a.t[1].xs1;
+    o0 = static_cast<T*>(a.t[0].o) + outer * a.t[0].os0 + in * a.t[0].os1;
+    o1 = static_cast<T*>(a.t[1].o) + outer * a.t[1].os0 + in * a.t[1].os1;
+  }
+  auto from = [&](uint32_t h) {
+    return h < a.t[0].heads ? x0 + h * a.t[0].xh : x1 + (h - a.t[0].heads) * a.t[1].xh;
+  };
+  auto to = [&](uint32_t h) {
+    return h < a.t[0].heads ? o0 + h * a.t[0].oh : o1 + (h - a.t[0].heads) * a.t[1].oh;
+  };
+
+  Pack<T, V> p[kHeads], q[kHeads];
+  auto load = [&](uint32_t h, uint32_t j) {
 #pragma unroll
-    for (int u = 0; u < kItems; ++u) {
-      const uint32_t it = base + u * kThreads + threadIdx.x;
-      if (it >= hi) break;
-      item[u] = locate<V, INTER>(a, it, tok0);
-      const T* p = static_cast<const T*>(a.t[item[u].which].x) + item[u].xo;
-      fetch<T, V, VL>(p, x1[u]);
-      if (!INTER && item[u].turn) fetch<T, V, VL>(p + a.half, x2[u]);
+    for (int u = 0; u < kHeads; ++u) {
+      const uint32_t hu = h + u * a.head_step;
+      if (hu >= heads) break;
+      const T* x = from(hu) + j * V;
+      fetch<T, V, VL>(x, p[u]);
+      if (!INTER) fetch<T, V, VL>(x + half, q[u]);
     }
   };
-  load(lo);
+  if (live && j0 < a.units) load(h0, j0);
 
-  for (uint32_t k = threadIdx.x; k < ntok * a.half; k += kThreads) {
-    const uint32_t tok = a.half_div.div(k), pair = k - tok * a.half;
-    const int64_t token = tok0 + tok;
-    int64_t outer = 0, inner = token;
-    if (a.inner != a.tokens) {
-      outer = token / a.inner;
-      inner = token - outer * a.inner;
-    }
-    const int64_t p = load_index(a.pos, a.pos_wide, outer * a.ps0 + inner * a.ps1);
+  for (uint32_t k = threadIdx.x; k < ntok * half; k += kThreads) {
+    const uint32_t tok = a.half.div(k), pair = k - tok * half;
+    const uint32_t outer = a.inner.div(tok0 + tok), in = tok0 + tok - outer * a.inner.d;
+    const int64_t at = load_index(a.pos, a.pos_wide, outer * a.ps0 + in * a.ps1);
     const double f = a.freq_wide ? static_cast<const double*>(a.freq)[pair * a.fs]
                                  : (double)static_cast<const float*>(a.freq)[pair * a.fs];
-    const double turns = (double)p * f * 0.15915494309189533577;  // 1 / (2 pi)
+    const double turns = (double)at * f * 0.15915494309189533577;  // 1 / (2 pi)
     float s, c;
     sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-    table[table_at<P>(tok, pair, a.half)] = make_float2(c * fabsf(a.scale), s * a.scale);
+    table[table_at<P>(tok, pair, half)] = make_float2(c * fabsf(a.scale), s * a.scale);
   }
   __syncthreads();
+  if (!live) return;
 
-  for (uint32_t base = lo; base < hi; base += kItems * kThreads) {
-    if (base != lo) load(base);
+  for (uint32_t j = j0; j < a.units; j += a.lanes.d) {
+    const float2* tab = table + mine * half;
+    float2 cd[P];
+    if constexpr (P == 1) {
+      cd[0] = tab[j];
+    } else {
 #pragma unroll
-    for (int u = 0; u < kItems; ++u) {
-      const uint32_t it = base + u * kThreads + threadIdx.x;
-      if (it >= hi) break;
-      T* o = static_cast<T*>(a.t[item[u].which].o) + item[u].oo;
-      if (!item[u].turn) {
-        put<T, V, VL>(o, x1[u]);
-        continue;
+      for (int k = 0; k < P / 2; ++k) {
+        const float4 w = *reinterpret_cast<const float4*>(tab + (k * a.units + j) * 2);
+        cd[2 * k] = make_float2(w.x, w.y);
+        cd[2 * k + 1] = make_float2(w.z, w.w);
       }
-      const float2* tab = table + item[u].token * a.half;
-      float2 cd[P];
-      if constexpr (P == 1) {
-        cd[0] = tab[item[u].j];
-      } else {
+    }
+    for (uint32_t h = h0; h < heads; h += kHeads * a.head_step) {
+      if (j != j0 || h != h0) load(h, j);
 #pragma unroll
-        for (int k = 0; k < P / 2; ++k) {
-          const float4 q = *reinterpret_cast<const float4*>(tab + (k * (a.half / P) + item[u].j) * 2);
-          cd[2 * k] = make_float2(q.x, q.y);
-          cd[2 * k + 1] = make_float2(q.z, q.w);
+      for (int u = 0; u < kHeads; ++u) {
+        const uint32_t hu = h + u * a.head_step;
+        if (hu >= heads) break;
+        T* o = to(hu) + j * V;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          T& first = p[u].v[INTER ? 2 * i : i];
+          T& second = INTER ? p[u].v[2 * i + 1] : q[u].v[i];
+          const float v = to_f(first), w = to_f(second);
+          first = from_f<T>(v * cd[i].x - w * cd[i].y);
+          second = from_f<T>(w * cd[i].x + v * cd[i].y);
+        }
+        put<T, V, VL>(o, p[u]);
+        if (!INTER) put<T, V, VL>(o + half, q[u]);
+      }
+    }
+  }
+  // the elements that are not rotated
+  if (a.t[0].copies | a.t[1].copies) {
+    for (uint32_t h = h0; h < heads; h += kHeads * a.head_step) {
+      const uint32_t most = max(a.t[0].copies, a.t[1].copies);
+      for (uint32_t j = j0; j < most; j += a.lanes.d) {
+#pragma unroll
+        for (int u = 0; u < kHeads; ++u) {
+          const uint32_t hu = h + u * a.head_step;
+          if (hu >= heads) break;
+          if (j < a.t[hu >= a.t[0].heads].copies) fetch<T, V, VL>(from(hu) + 2 * half + j * V, p[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kHeads; ++u) {
+          const uint32_t hu = h + u * a.head_step;
+          if (hu >= heads) break;
+          if (j < a.t[hu >= a.t[0].heads].copies) put<T, V, VL>(to(hu) + 2 * half + j * V, p[u]);
         }
       }
-      Pack<T, V> y1, y2;
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const float p = to_f(INTER ? x1[u].v[2 * i] : x1[u].v[i]);
-        const float q = to_f(INTER ? x1[u].v[2 * i + 1] : x2[u].v[i]);
-        const T r = from_f<T>(p * cd[i].x - q * cd[i].y), w = from_f<T>(q * cd[i].x + p * cd[i].y);
-        if (INTER) {
-          y1.v[2 * i] = r;
-          y1.v[2 * i + 1] = w;
-        } else {
-          y1.v[i] = r;
-          y2.v[i] = w;
-        }
-      }
-      put<T, V, VL>(o, y1);
-      if (!INTER) put<T, V, VL>(o + a.half, y2);
     }
   }
 }
 
 template <typename T>
-void launch(const RotArgs& a, int v, int vl, bool inter, unsigned grid, cudaStream_t s) {
+void launch(const RotArgs& a, int v, int vl, bool inter, dim3 grid, cudaStream_t s) {
   constexpr int W = 16 / sizeof(T);
 #define GPUOS_ROT(V, VL, I) gpuos_rotary_kernel<T, V, VL, I><<<grid, kThreads, 0, s>>>(a)
   if (inter) {
     if (v == W) GPUOS_ROT(W, W, true);
+    else if (v == W / 2 && vl == W / 2) GPUOS_ROT(W / 2, W / 2, true);
     else if (vl == 2) GPUOS_ROT(2, 2, true);
     else GPUOS_ROT(2, 1, true);
   } else {
     if (v == W) GPUOS_ROT(W, W, false);
+    else if (v == W / 2) GPUOS_ROT(W / 2, W / 2, false);
     else if (v == 2) GPUOS_ROT(2, 2, false);
     else GPUOS_ROT(1, 1, false);
   }
@@ -236,7 +232,6 @@ void rotary(int32_t n, const gpuos_tensor* x, const gpuos_tensor* out, const gpu
   need(nd == 3 || nd == 4, "x must have 3 dims (token, head, element) or 4 (batch, token, head, element)");
   check_tensor(positions, nd - 2, "positions");
   RotArgs a{};
-  int W = 16 / esize(x[0].dtype), vec = W, pair = 2;
   for (int i = 0; i < n; ++i) {
     check_tensor(&x[i], nd, "x");
     check_tensor(&out[i], nd, "out");
@@ -265,34 +260,27 @@ void rotary(int32_t n, const gpuos_tensor* x, const gpuos_tensor* out, const gpu
         need(!overlap(out[i], out[k]), "the outputs overlap");
       }
   }
-  // 16-byte items where pointers, strides, the rotated and the copied part
-  // allow it, else two elements at a time, else one
+  // groups of 16 bytes where pointers, strides, the rotated and the copied
+  // part allow it, else of 8, else of two elements, else single ones
+  const int W = 16 / esize(x[0].dtype);
+  int vl = W;
   for (int i = 0; i < n; ++i) {
     if (numel(x[i]) == 0) continue;
     const int64_t rest = x[i].sizes[nd - 1] - 2 * half;
-    auto fits = [&](int v) {
-      return rows_aligned(x[i], v) && rows_aligned(out[i], v) && rest % v == 0 &&
-             (inter ? 2 * half : half) % v == 0;
-    };
-    if (vec > 2 && !fits(vec)) vec = 2;
-    if (!fits(2)) pair = 1;
+    while (vl > 1 && !(rows_aligned(x[i], vl) && rows_aligned(out[i], vl) && rest % vl == 0 &&
+                       (inter ? 2 * half : half) % vl == 0))
+      vl = vl > 2 ? std::max(vl / 2, 2) : 1;
   }
-  int v = vec, vl = vec;
-  if (vec == 2) {
-    vl = pair;
-    v = inter ? 2 : pair;
-  }
-  if (inter && v == 2 && vl == 1)  // scalar accesses still move two elements at a time
-    for (int i = 0; i < n; ++i) need((x[i].sizes[nd - 1] - 2 * half) % 2 == 0, "interleaved pairs need an even head size");
+  const int v = inter && vl == 1 ? 2 : vl;  // interleaved: single accesses still move a pair
+  if (v != vl)
+    for (int i = 0; i < n; ++i)
+      need((x[i].sizes[nd - 1] - 2 * half) % 2 == 0, "interleaved pairs need an even head size");
 
-  uint64_t per_token = 0;
-  a.half = (uint32_t)half;
-  a.turned = (uint32_t)(inter ? 2 * half / v : half / v);
-  a.inner = x[0].sizes[nd - 3];
-  a.tokens = nd == 4 ? x[0].sizes[0] * a.inner : a.inner;
+  const bool four = nd == 4;
+  const __int128 tokens = four ? (__int128)x[0].sizes[0] * x[0].sizes[1] : x[0].sizes[0];
+  uint32_t heads = 0, copies = 0;
   for (int i = 0; i < n; ++i) {
     RotTensor& t = a.t[i];
-    const bool four = nd == 4;
     t.x = x[i].data;
     t.o = out[i].data;
     t.xs0 = four ? x[i].strides[0] : 0;
@@ -301,44 +289,34 @@ void rotary(int32_t n, const gpuos_tensor* x, const gpuos_tensor* out, const gpu
     t.os1 = out[i].strides[nd - 3];
     t.xh = x[i].strides[nd - 2];
     t.oh = out[i].strides[nd - 2];
-    const int64_t rest = x[i].sizes[nd - 1] - 2 * half;
+    t.heads = (uint32_t)x[i].sizes[nd - 2];
     // in place the part that is not rotated is there already
-    const uint32_t per_head = a.turned + (same_view(x[i], out[i]) ? 0 : (uint32_t)(rest / v));
-    t.per_head = FastDiv(std::max(per_head, 1u));
-    t.items = (uint32_t)x[i].sizes[nd - 2] * per_head;
-    per_token += (uint64_t)x[i].sizes[nd - 2] * per_head;
+    t.copies = same_view(x[i], out[i]) ? 0 : (uint32_t)((x[i].sizes[nd - 1] - 2 * half) / v);
+    heads += t.heads;
+    copies = std::max(copies, t.copies);
   }
-  if (a.tokens == 0 || per_token == 0) return;
-  need(per_token < (1u << 24), "a token has too many elements");
+  a.units = (uint32_t)((inter ? 2 * half : half) / v);
+  if (tokens == 0 || heads == 0 || (a.units == 0 && copies == 0)) return;
+  need(tokens < (__int128)0x7fffffff, "too many tokens");
+  a.tokens = (uint32_t)tokens;
+  a.inner = FastDiv((uint32_t)x[0].sizes[nd - 3]);
+  a.half = FastDiv((uint32_t)half);
   a.pos = positions->data;
-  a.ps0 = nd == 4 ? positions->strides[0] : 0;
+  a.ps0 = four ? positions->strides[0] : 0;
   a.ps1 = positions->strides[nd - 3];
   a.pos_wide = positions->dtype == GPUOS_I64;
   a.freq = inv_freq->data;
   a.fs = half ? inv_freq->strides[0] : 0;
   a.freq_wide = inv_freq->dtype == GPUOS_F64;
   a.scale = (flags & GPUOS_ROTARY_INVERSE) ? -scale : scale;
-  a.token_items = FastDiv((uint32_t)per_token);
-  a.half_div = FastDiv(std::max<uint32_t>(a.half, 1));
 
-  // A CTA takes the tokens that give each thread its items; few tokens are
-  // split over more CTAs, one item a thread, so that a decode step's loads
-  // start on many SMs at once.
-  const int sms = sm_count();
-  const uint64_t full = kItems * kThreads;
-  uint64_t tile = std::max<uint64_t>(1, full / per_token);
-  if (half) tile = std::min<uint64_t>(tile, kTablePairs / half);
-  const uint64_t spread = std::max<uint64_t>(1, (uint64_t)a.tokens / (2 * sms));
-  tile = std::min(tile, spread);
-  const uint64_t tiles = ((uint64_t)a.tokens + tile - 1) / tile;
-  uint64_t split = 1;
-  if (tiles < (uint64_t)sms)
-    split = std::max<uint64_t>(1, std::min<uint64_t>((tile * per_token + kThreads - 1) / kThreads,
-                                                     2 * sms / tiles));
-  need(tiles * split < 0x7fffffffull, "too many tokens");
-  a.tile = (uint32_t)tile;
-  a.split = (uint32_t)split;
-  const unsigned grid = (unsigned)(tiles * split);
+  const Spread sp = spread(a.tokens, a.units ? a.units : copies, heads, kThreads,
+                           half ? kTablePairs / (uint32_t)half : kThreads);
+  a.lanes = FastDiv(sp.lanes);
+  a.per_token = FastDiv(sp.lanes * sp.groups);
+  a.head_step = sp.groups * sp.split;
+  a.tile = sp.tile;
+  const dim3 grid(sp.tiles, sp.split);
   if (x[0].dtype == GPUOS_F32) launch<float>(a, v, vl, inter, grid, stream);
   else if (x[0].dtype == GPUOS_F16) launch<__half>(a, v, vl, inter, grid, stream);
   else launch<__nv_bfloat16>(a, v, vl, inter, grid, stream);

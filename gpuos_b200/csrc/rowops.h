@@ -194,5 +194,32 @@ inline int sm_count() {
   return known[dev];
 }
 
+// How tokens of `heads` rows of `units` groups are spread over CTAs: a thread
+// belongs to one token and one group and walks over about 8 heads in steps of
+// groups * split; with few tokens the heads are spread over more threads, then
+// over more CTAs, so that their loads start at once on many SMs.
+struct Spread {
+  uint32_t lanes;   // threads side by side over a head's groups
+  uint32_t groups;  // heads a CTA takes at once
+  uint32_t tile;    // tokens a CTA takes
+  uint32_t tiles;   // CTAs over the tokens
+  uint32_t split;   // CTAs over the heads
+};
+
+inline Spread spread(uint32_t tokens, uint32_t units, uint32_t heads, uint32_t threads, uint32_t most_tile) {
+  const uint32_t sms = (uint32_t)sm_count();
+  Spread s;
+  s.lanes = std::min(std::max(units, 1u), threads);
+  s.groups = 1;
+  while (s.lanes * s.groups * 2 <= threads && s.groups * 2 <= heads &&
+         (s.groups * 16 <= heads || (uint64_t)tokens * s.lanes * s.groups < (uint64_t)threads * 4 * sms))
+    s.groups *= 2;
+  s.tile = std::min(threads / (s.lanes * s.groups), most_tile);
+  s.tiles = (tokens + s.tile - 1) / s.tile;
+  s.split = 1;
+  while (s.tiles * s.split < sms && s.groups * s.split < heads) s.split *= 2;
+  return s;
+}
+
 }  // namespace rowops
 }  // namespace gpuos
