@@ -13,8 +13,10 @@
 // range), an infinity as the largest code of its sign, NaN as code 0 (int8,
 // int4) or NaN (e4m3).
 //
-// Both kernels move every byte once and hold a group in the registers of
-// neighbouring lanes: 8 elements a lane, the maximum joined by shuffles.
+// Both kernels move every byte once, 8 elements a lane.  What could bound them
+// above that are instructions, so each token's row of the cache is found once by the lanes that
+// share the token, which then walk over its heads; a write holds a group in the
+// registers of neighbouring lanes and joins its maximum by shuffles.
 #include <cuda_fp8.h>
 
 #include "rowops.cuh"
@@ -29,29 +31,32 @@ constexpr int kUnit = 8;  // elements a lane moves at once
 enum Format { kInt8, kE4M3, kInt4 };
 
 struct CacheTensor {
-  const void* x;   // write: the rows; read: unused
-  void* o;         // read: the rows
+  void* rows;                  // what is written (read only) or read into
   void* codes;
   float* scales;
-  int64_t rs, rh;              // row tensor: strides of token and head (elements)
+  int64_t rs, rh;              // rows: strides of token and head (elements)
   int64_t cp, cr, ch;          // codes: strides of page, row, head (bytes)
   int64_t sp, sr, sh, sg;      // scales: strides of page, row, head, group
-  uint32_t items;              // per token: groups (write) or units (read)
-  FastDiv per_head;            // groups or units of a head
-  uint32_t group;              // elements
+  uint32_t heads;
   uint32_t head;               // elements
-  FastDiv group_div;
+  uint32_t group;              // elements
+  uint32_t items;              // write: groups of a token
+  FastDiv groups;              // of a head
+  FastDiv group_div;           // by `group`
+  uint32_t lanes_log;          // write: lanes that share a group
 };
 
 struct CacheArgs {
   CacheTensor t[2];
   const void* slots;
   int64_t ss;
-  int64_t rows;       // pages * page
+  int64_t rows;        // pages * page
   FastDiv page;
   uint32_t tokens;
-  FastDiv token_items[2];
-  uint32_t lanes_log; // write: lanes that share a group
+  uint32_t token_log;  // write: lanes that share a token
+  // read: how the threads are spread
+  uint32_t tile, head_step;
+  FastDiv lanes, per_token;
   int slot_wide;
 };
 
@@ -142,19 +147,20 @@ __device__ __forceinline__ uint2 load_codes(const uint8_t* p, int n) {
   return r;
 }
 
+// 8 elements as they are stored.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_unit(const T* p, int n, float (&x)[kUnit]) {
+__device__ __forceinline__ void load_unit(const T* p, int n, Pack<T, kUnit>& x) {
   if constexpr (VEC) {
     constexpr int W = 16 / sizeof(T);
 #pragma unroll
     for (int k = 0; k < kUnit; k += W) {
       const Pack<T, W> q = load_pack<T, W>(p + k);
 #pragma unroll
-      for (int i = 0; i < W; ++i) x[k + i] = to_f(q.v[i]);
+      for (int i = 0; i < W; ++i) x.v[k + i] = q.v[i];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i) x[i] = i < n ? to_f(p[i]) : 0.f;
+    for (int i = 0; i < kUnit; ++i) x.v[i] = i < n ? p[i] : from_f<T>(0.f);
   }
 }
 
@@ -166,153 +172,181 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// NU units a lane: groups of up to 32 * 8 * NU elements.  IT groups of a lane
-// are in flight.
+// max |x| of 8 elements (16-bit types two at a time).
+template <typename T>
+__device__ __forceinline__ float max_abs(const Pack<T, kUnit>& x) {
+  if constexpr (sizeof(T) == 2) {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    const T2* h = reinterpret_cast<const T2*>(&x);
+    const T2 m = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+    return max_nan(to_f(m.x), to_f(m.y));
+  } else {
+    float m = fabsf(x.v[0]);
+#pragma unroll
+    for (int i = 1; i < kUnit; ++i) m = max_nan(m, fabsf(x.v[i]));
+    return m;
+  }
+}
+
+// NU units a lane: groups of up to 32 * 8 * NU elements.  A lane has IT groups in flight.
 template <typename T, int F, bool VEC, int NU, int IT>
 __global__ void __launch_bounds__(kThreads)
 gpuos_cache_write_kernel(const __grid_constant__ CacheArgs a) {
   const CacheTensor& t = a.t[blockIdx.y];
-  const uint32_t lanes = 1u << a.lanes_log;
-  const uint32_t lane = threadIdx.x & (lanes - 1);
-  const uint32_t per_pass = kThreads >> a.lanes_log;  // groups a CTA handles at once
-  const uint32_t all = a.tokens * t.items;
-  const uint32_t base = blockIdx.x * per_pass * IT + (threadIdx.x >> a.lanes_log);
-  if (base - (threadIdx.x >> a.lanes_log) >= all) return;  // the whole CTA
+  const uint32_t token = blockIdx.x * (kThreads >> a.token_log) + (threadIdx.x >> a.token_log);
+  const uint32_t of_token = threadIdx.x & ((1u << a.token_log) - 1);
+  const uint32_t lane = of_token & ((1u << t.lanes_log) - 1);
+  const uint32_t step = 1u << (a.token_log - t.lanes_log);
+  const float inf = __int_as_float(0x7f800000), q = q_max(F);
 
-  float x[IT][NU][kUnit];
-  int64_t co[IT], so[IT];
-  bool has[IT];
-#pragma unroll
-  for (int u = 0; u < IT; ++u) {
-    const uint32_t gi = base + u * per_pass;
-    has[u] = false;
-#pragma unroll
-    for (int k = 0; k < NU; ++k)
-#pragma unroll
-      for (int i = 0; i < kUnit; ++i) x[u][k][i] = 0.f;
-    if (gi >= all) continue;
-    const uint32_t token = a.token_items[blockIdx.y].div(gi);
-    const uint32_t m = gi - token * t.items;
-    const uint32_t head = t.per_head.div(m), g = m - head * t.per_head.d;
+  bool has = false;
+  const T* x0 = nullptr;
+  uint8_t* codes = nullptr;
+  float* scales = nullptr;
+  if (token < a.tokens) {
     const int64_t slot = load_index(a.slots, a.slot_wide, token * a.ss);
-    has[u] = slot >= 0 && slot < a.rows;  // rows < 2^31
-    const T* p = static_cast<const T*>(t.x) + token * t.rs + head * t.rh + (int64_t)g * t.group;
-#pragma unroll
-    for (int k = 0; k < NU; ++k) {
-      const int e = (lane + k * lanes) * kUnit;
-      if (has[u] && e < (int)t.group) load_unit<T, VEC>(p + e, (int)t.group - e, x[u][k]);
-    }
+    has = slot >= 0 && slot < a.rows;  // rows < 2^31
     const uint32_t page = a.page.div((uint32_t)slot), row = (uint32_t)slot - page * a.page.d;
-    co[u] = page * t.cp + row * t.cr + head * t.ch + ((int64_t)g * t.group) * kCodeBits<F> / 8;
-    so[u] = page * t.sp + row * t.sr + head * t.sh + g * t.sg;
+    x0 = static_cast<const T*>(t.rows) + token * t.rs;
+    codes = static_cast<uint8_t*>(t.codes) + page * t.cp + row * t.cr;
+    scales = t.scales + page * t.sp + row * t.sr;
   }
+  if (!__any_sync(~0u, has)) return;  // a warp of padding
+
+  for (uint32_t g0 = of_token >> t.lanes_log; __any_sync(~0u, g0 < t.items); g0 += step * IT) {
+    Pack<T, kUnit> x[IT][NU];
+    uint32_t head[IT], g[IT];
 #pragma unroll
-  for (int u = 0; u < IT; ++u) {
-    float m = 0.f;
+    for (int u = 0; u < IT; ++u) {
+      const uint32_t gi = g0 + u * step;
+      head[u] = t.groups.div(gi);
+      g[u] = gi - head[u] * t.groups.d;
+      const T* p = x0 + head[u] * t.rh + g[u] * t.group;
 #pragma unroll
-    for (int k = 0; k < NU; ++k)
+      for (int k = 0; k < NU; ++k) {
+        const uint32_t e = (lane + (k << t.lanes_log)) * kUnit;
 #pragma unroll
-      for (int i = 0; i < kUnit; ++i) m = max_nan(m, fabsf(x[u][k][i]));
-    for (uint32_t d = lanes >> 1; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(~0u, m, d));
-    const bool plain = m < __int_as_float(0x7f800000);  // all elements finite
-    if (!__all_sync(~0u, plain)) {
-      float f = 0.f;
-#pragma unroll
-      for (int k = 0; k < NU; ++k)
-#pragma unroll
-        for (int i = 0; i < kUnit; ++i) {
-          const float v = fabsf(x[u][k][i]);
-          if (v < __int_as_float(0x7f800000)) f = fmaxf(f, v);
-        }
-      for (uint32_t d = lanes >> 1; d; d >>= 1) f = fmaxf(f, __shfl_xor_sync(~0u, f, d));
-      m = f;
-    }
-    if (!has[u]) continue;
-    const float q = q_max(F);
-    const bool fits = m >= 0x1p-100f;
-    const float inv = fits ? __fmul_rn(__frcp_rn(m), q) : 0.f;
-    if (lane == 0) t.scales[so[u]] = fits ? __fmul_rn(m, 1.f / q) : 0.f;
-#pragma unroll
-    for (int k = 0; k < NU; ++k) {
-      const int e = (lane + k * lanes) * kUnit;
-      if (e >= (int)t.group) continue;
-      float y[kUnit];
-#pragma unroll
-      for (int i = 0; i < kUnit; ++i) y[i] = __fmul_rn(x[u][k][i], inv);
-      if (!plain) {
-#pragma unroll
-        for (int i = 0; i < kUnit; ++i) {
-          const float v = x[u][k][i];
-          if (fabsf(v) == __int_as_float(0x7f800000)) y[i] = copysignf(q, v);
-          else if (v != v) y[i] = F == kE4M3 ? v : 0.f;
-        }
+        for (int i = 0; i < kUnit; ++i) x[u][k].v[i] = from_f<T>(0.f);
+        if (has && gi < t.items && e < t.group) load_unit<T, VEC>(p + e, (int)(t.group - e), x[u][k]);
       }
-      store_codes<F, VEC>(static_cast<uint8_t*>(t.codes) + co[u] + e * kCodeBits<F> / 8, encode<F>(y),
-                          min((int)t.group - e, kUnit));
+    }
+#pragma unroll
+    for (int u = 0; u < IT; ++u) {
+      float m = max_abs(x[u][0]);
+#pragma unroll
+      for (int k = 1; k < NU; ++k) m = max_nan(m, max_abs(x[u][k]));
+      for (uint32_t d = (1u << t.lanes_log) >> 1; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(~0u, m, d));
+      const bool plain = m < inf;  // all elements finite
+      if (!__all_sync(~0u, plain)) {
+        float f = 0.f;
+#pragma unroll
+        for (int k = 0; k < NU; ++k)
+#pragma unroll
+          for (int i = 0; i < kUnit; ++i) {
+            const float v = fabsf(to_f(x[u][k].v[i]));
+            if (v < inf) f = fmaxf(f, v);
+          }
+        for (uint32_t d = (1u << t.lanes_log) >> 1; d; d >>= 1) f = fmaxf(f, __shfl_xor_sync(~0u, f, d));
+        m = f;
+      }
+      if (!has || g0 + u * step >= t.items) continue;
+      const bool fits = m >= 0x1p-100f;
+      const float inv = fits ? __fmul_rn(__frcp_rn(m), q) : 0.f;
+      if (lane == 0) scales[head[u] * t.sh + g[u] * t.sg] = fits ? __fmul_rn(m, 1.f / q) : 0.f;
+      uint8_t* c = codes + head[u] * t.ch + g[u] * t.group * kCodeBits<F> / 8;
+#pragma unroll
+      for (int k = 0; k < NU; ++k) {
+        const uint32_t e = (lane + (k << t.lanes_log)) * kUnit;
+        if (e >= t.group) continue;
+        float y[kUnit];
+#pragma unroll
+        for (int i = 0; i < kUnit; i += 2) {
+          const float2 r = mul2(make_float2(to_f(x[u][k].v[i]), to_f(x[u][k].v[i + 1])), both(inv));
+          y[i] = r.x;
+          y[i + 1] = r.y;
+        }
+        if (!plain) {
+#pragma unroll
+          for (int i = 0; i < kUnit; ++i) {
+            const float v = to_f(x[u][k].v[i]);
+            if (fabsf(v) == inf) y[i] = copysignf(q, v);
+            else if (v != v) y[i] = F == kE4M3 ? v : 0.f;
+          }
+        }
+        store_codes<F, VEC>(c + e * kCodeBits<F> / 8, encode<F>(y), (int)min(t.group - e, (uint32_t)kUnit));
+      }
     }
   }
 }
 
-template <typename T, int F, bool VEC, int IT>
+template <typename T, int F, bool VEC>
 __global__ void __launch_bounds__(kThreads)
 gpuos_cache_read_kernel(const __grid_constant__ CacheArgs a) {
-  const CacheTensor& t = a.t[blockIdx.y];
-  const uint32_t all = a.tokens * t.items;
-  const uint32_t base = blockIdx.x * kThreads * IT + threadIdx.x;
-  uint2 code[IT];
-  float scale[IT][VEC ? 1 : kUnit];
-  T* o[IT];
-  int n[IT];
+  constexpr int IT = VEC ? 4 : 1;  // heads a thread has in flight
+  constexpr int S = VEC ? 1 : kUnit;
+  const CacheTensor& t = a.t[blockIdx.z];
+  const uint32_t mine = a.per_token.div(threadIdx.x);
+  const uint32_t token = blockIdx.x * a.tile + mine;
+  if (mine >= a.tile || token >= a.tokens) return;
+  const uint32_t rest = threadIdx.x - mine * a.per_token.d;
+  const uint32_t group = a.lanes.div(rest), j0 = rest - group * a.lanes.d;
+  const uint32_t h0 = group + blockIdx.y * (a.per_token.d / a.lanes.d);
+  const int64_t slot = load_index(a.slots, a.slot_wide, token * a.ss);
+  const bool has = slot >= 0 && slot < a.rows;
+  const uint32_t page = a.page.div((uint32_t)slot), row = (uint32_t)slot - page * a.page.d;
+  const uint8_t* codes = static_cast<const uint8_t*>(t.codes) + page * t.cp + row * t.cr;
+  const float* scales = t.scales + page * t.sp + row * t.sr;
+  T* o0 = static_cast<T*>(t.rows) + token * t.rs;
+
+  for (uint32_t j = j0; j * kUnit < t.head; j += a.lanes.d) {
+    const uint32_t e = j * kUnit;
+    const int n = (int)min(t.head - e, (uint32_t)kUnit);
+    int64_t sg[S];
 #pragma unroll
-  for (int u = 0; u < IT; ++u) {
-    const uint32_t it = base + u * kThreads;
-    n[u] = 0;
-    if (it >= all) continue;
-    const uint32_t token = a.token_items[blockIdx.y].div(it);
-    const uint32_t m = it - token * t.items;
-    const uint32_t head = t.per_head.div(m), e = (m - head * t.per_head.d) * kUnit;
-    const int64_t slot = load_index(a.slots, a.slot_wide, token * a.ss);
-    o[u] = static_cast<T*>(t.o) + token * t.rs + head * t.rh + e;
-    n[u] = min((int)(t.head - e), kUnit);
-    code[u] = make_uint2(0, 0);
+    for (int i = 0; i < S; ++i) sg[i] = t.group_div.div(e + i) * t.sg;
+    for (uint32_t h = h0; h < t.heads; h += IT * a.head_step) {
+      uint2 code[IT];
+      float scale[IT][S];
 #pragma unroll
-    for (int i = 0; i < (VEC ? 1 : kUnit); ++i) scale[u][i] = 0.f;
-    if (slot < 0 || slot >= a.rows) {  // no row: zeros
-      if (F == kInt4) code[u].x = 0x88888888u;
-      continue;
-    }
-    const uint32_t page = a.page.div((uint32_t)slot), row = (uint32_t)slot - page * a.page.d;
-    code[u] = load_codes<F, VEC>(static_cast<const uint8_t*>(t.codes) + page * t.cp + row * t.cr +
-                                     head * t.ch + e * kCodeBits<F> / 8, n[u]);
-    const float* s = t.scales + page * t.sp + row * t.sr + head * t.sh;
-    if constexpr (VEC) {
-      scale[u][0] = __ldg(s + t.group_div.div(e) * t.sg);
-    } else {
+      for (int u = 0; u < IT; ++u) {
+        const uint32_t hu = h + u * a.head_step;
+        if (hu >= t.heads) break;
+        code[u] = make_uint2(F == kInt4 ? 0x88888888u : 0u, 0u);  // no row: zeros
 #pragma unroll
-      for (int i = 0; i < kUnit; ++i)
-        if (i < n[u]) scale[u][i] = __ldg(s + t.group_div.div(e + i) * t.sg);
-    }
-  }
+        for (int i = 0; i < S; ++i) scale[u][i] = 0.f;
+        if (has) {
+          code[u] = load_codes<F, VEC>(codes + hu * t.ch + e * kCodeBits<F> / 8, n);
 #pragma unroll
-  for (int u = 0; u < IT; ++u) {
-    if (n[u] == 0) continue;
-    float y[kUnit];
-    decode<F>(code[u], y);
-#pragma unroll
-    for (int i = 0; i < kUnit; ++i) y[i] = __fmul_rn(y[i], scale[u][VEC ? 0 : i]);
-    if constexpr (VEC) {
-      constexpr int W = 16 / sizeof(T);
-#pragma unroll
-      for (int k = 0; k < kUnit; k += W) {
-        Pack<T, W> q;
-#pragma unroll
-        for (int i = 0; i < W; ++i) q.v[i] = from_f<T>(y[k + i]);
-        store_pack<T, W>(o[u] + k, q);
+          for (int i = 0; i < S; ++i)
+            if (VEC || i < n) scale[u][i] = __ldg(scales + hu * t.sh + sg[i]);
+        }
       }
-    } else {
 #pragma unroll
-      for (int i = 0; i < kUnit; ++i)
-        if (i < n[u]) o[u][i] = from_f<T>(y[i]);
+      for (int u = 0; u < IT; ++u) {
+        const uint32_t hu = h + u * a.head_step;
+        if (hu >= t.heads) break;
+        T* o = o0 + hu * t.rh + e;
+        float y[kUnit];
+        decode<F>(code[u], y);
+        if constexpr (VEC) {
+          constexpr int W = 16 / sizeof(T);
+#pragma unroll
+          for (int k = 0; k < kUnit; k += W) {
+            Pack<T, W> w;
+#pragma unroll
+            for (int i = 0; i < W; i += 2) {
+              const float2 r = mul2(make_float2(y[k + i], y[k + i + 1]), both(scale[u][0]));
+              w.v[i] = from_f<T>(r.x);
+              w.v[i + 1] = from_f<T>(r.y);
+            }
+            store_pack<T, W>(o + k, w);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kUnit; ++i)
+            if (i < n) o[i] = from_f<T>(__fmul_rn(y[i], scale[u][i]));
+        }
+      }
     }
   }
 }
@@ -367,8 +401,7 @@ CacheArgs prepare(int32_t n, const gpuos_tensor* rows, const char* name, const g
                       group % kUnit == 0;
     if (!fits) *vec = false;
     CacheTensor& t = a.t[i];
-    t.x = x.data;
-    t.o = x.data;
+    t.rows = x.data;
     t.codes = c.data;
     t.scales = static_cast<float*>(s.data);
     t.rs = x.strides[0];
@@ -380,13 +413,13 @@ CacheArgs prepare(int32_t n, const gpuos_tensor* rows, const char* name, const g
     t.sr = s.strides[1];
     t.sh = s.strides[2];
     t.sg = s.strides[3];
+    t.heads = (uint32_t)x.sizes[1];
     t.head = (uint32_t)head;
     t.group = (uint32_t)group;
     t.group_div = FastDiv(t.group);
-    const uint32_t per_head = write ? (uint32_t)s.sizes[3] : (uint32_t)((head + kUnit - 1) / kUnit);
-    t.per_head = FastDiv(per_head);
-    t.items = (uint32_t)x.sizes[1] * per_head;
-    a.token_items[i] = FastDiv(std::max(t.items, 1u));
+    t.groups = FastDiv((uint32_t)s.sizes[3]);
+    t.items = t.heads * t.groups.d;
+    while (t.lanes_log < 5 && (uint32_t)(kUnit << t.lanes_log) < t.group) ++t.lanes_log;
   }
   const __int128 cache_rows = (__int128)codes[0].sizes[0] * codes[0].sizes[1];
   need(cache_rows < ((__int128)1 << 31), "the cache has too many rows");
@@ -400,33 +433,21 @@ CacheArgs prepare(int32_t n, const gpuos_tensor* rows, const char* name, const g
 }
 
 template <typename T, int F>
-void launch_write(const CacheArgs& a, bool vec, int n, uint32_t most_group, uint64_t most, cudaStream_t s) {
-  const uint32_t lanes = 1u << a.lanes_log;
-  const int units = (int)((most_group + kUnit * lanes - 1) / (kUnit * lanes));
-  const uint64_t per_pass = kThreads >> a.lanes_log;
-  // few groups: one a lane, so that they start on many SMs at once
-  const int it = units == 1 && most > per_pass * 4 * (uint64_t)sm_count() ? 4 : 1;
-  const dim3 grid((unsigned)((most + per_pass * it - 1) / (per_pass * it)), n);
+void launch_write(const CacheArgs& a, bool vec, bool large, int n, cudaStream_t s) {
+  const uint32_t per_cta = kThreads >> a.token_log;
+  const dim3 grid((a.tokens + per_cta - 1) / per_cta, n);
 #define GPUOS_CW(VEC, NU, IT) gpuos_cache_write_kernel<T, F, VEC, NU, IT><<<grid, kThreads, 0, s>>>(a)
-  if (vec) {
-    if (units == 1 && it == 4) GPUOS_CW(true, 1, 4);
-    else if (units == 1) GPUOS_CW(true, 1, 1);
-    else GPUOS_CW(true, 4, 1);
-  } else {
-    if (units == 1 && it == 4) GPUOS_CW(false, 1, 4);
-    else if (units == 1) GPUOS_CW(false, 1, 1);
-    else GPUOS_CW(false, 4, 1);
-  }
+  if (vec && !large) GPUOS_CW(true, 1, 4);
+  else if (vec) GPUOS_CW(true, 4, 1);
+  else if (!large) GPUOS_CW(false, 1, 2);
+  else GPUOS_CW(false, 4, 1);
 #undef GPUOS_CW
 }
 
 template <typename T, int F>
-void launch_read(const CacheArgs& a, bool vec, int n, uint64_t most, cudaStream_t s) {
-  const int it = vec && most > kThreads * 4 * (uint64_t)sm_count() ? 4 : 1;
-  const dim3 grid((unsigned)((most + kThreads * it - 1) / (kThreads * it)), n);
-  if (vec && it == 4) gpuos_cache_read_kernel<T, F, true, 4><<<grid, kThreads, 0, s>>>(a);
-  else if (vec) gpuos_cache_read_kernel<T, F, true, 1><<<grid, kThreads, 0, s>>>(a);
-  else gpuos_cache_read_kernel<T, F, false, 1><<<grid, kThreads, 0, s>>>(a);
+void launch_read(const CacheArgs& a, bool vec, dim3 grid, cudaStream_t s) {
+  if (vec) gpuos_cache_read_kernel<T, F, true><<<grid, kThreads, 0, s>>>(a);
+  else gpuos_cache_read_kernel<T, F, false><<<grid, kThreads, 0, s>>>(a);
 }
 
 template <typename L>
@@ -449,8 +470,6 @@ void cache_write(int32_t n, const gpuos_tensor* x, const gpuos_tensor* slots, co
                  const gpuos_tensor* scales, cudaStream_t stream) {
   bool vec;
   CacheArgs a = prepare(n, x, "x", slots, codes, scales, true, &vec);
-  uint32_t group = 1;
-  uint64_t most = 0;
   for (int i = 0; i < n; ++i) {
     check_output(codes[i], "codes");
     check_output(scales[i], "scales");
@@ -465,14 +484,20 @@ void cache_write(int32_t n, const gpuos_tensor* x, const gpuos_tensor* slots, co
     }
     no_overlap(codes[i], *slots, "codes overlap slots");
     no_overlap(scales[i], *slots, "scales overlap slots");
-    group = std::max(group, a.t[i].group);
-    most = std::max(most, (uint64_t)a.tokens * a.t[i].items);
   }
-  if (most == 0 || a.rows == 0) return;
-  a.lanes_log = 0;
-  while (a.lanes_log < 5 && (uint32_t)(kUnit << a.lanes_log) < group) ++a.lanes_log;
+  if (a.tokens == 0 || a.rows == 0 || a.t[0].items + a.t[1].items == 0) return;
+  // a warp serves a token, or several whose groups do not fill it
+  uint32_t wanted = 1;
+  bool large = false;
+  for (int i = 0; i < n; ++i) {
+    const CacheTensor& t = a.t[i];
+    wanted = std::max(wanted, std::max(t.items, 1u) << t.lanes_log);
+    large = large || t.group > 32 * kUnit;
+    a.token_log = std::max(a.token_log, t.lanes_log);
+  }
+  while (a.token_log < 5 && (1u << a.token_log) < wanted) ++a.token_log;
   by_type(x[0].dtype, codes[0].dtype, [&](auto type, auto f) {
-    launch_write<decltype(type), decltype(f)::value>(a, vec, n, group, most, stream);
+    launch_write<decltype(type), decltype(f)::value>(a, vec, large, n, stream);
   });
   cuda_ok(cudaGetLastError(), "launch");
 }
@@ -480,8 +505,8 @@ void cache_write(int32_t n, const gpuos_tensor* x, const gpuos_tensor* slots, co
 void cache_read(int32_t n, const gpuos_tensor* slots, const gpuos_tensor* codes, const gpuos_tensor* scales,
                 const gpuos_tensor* out, cudaStream_t stream) {
   bool vec;
-  const CacheArgs a = prepare(n, out, "out", slots, codes, scales, false, &vec);
-  uint64_t most = 0;
+  CacheArgs a = prepare(n, out, "out", slots, codes, scales, false, &vec);
+  uint32_t heads = 0, head = 0;
   for (int i = 0; i < n; ++i) {
     check_output(out[i], "out");
     no_overlap(out[i], *slots, "out overlaps slots");
@@ -490,11 +515,18 @@ void cache_read(int32_t n, const gpuos_tensor* slots, const gpuos_tensor* codes,
       no_overlap(out[i], scales[k], "out overlaps scales");
       if (k != i) no_overlap(out[i], out[k], "the outputs overlap");
     }
-    most = std::max(most, (uint64_t)a.tokens * a.t[i].items);
+    heads = std::max(heads, a.t[i].heads);
+    head = std::max(head, a.t[i].head);
   }
-  if (most == 0) return;
+  if (a.tokens == 0 || heads == 0) return;
+  const Spread sp = spread(a.tokens, (head + kUnit - 1) / kUnit, heads, kThreads, kThreads);
+  a.lanes = FastDiv(sp.lanes);
+  a.per_token = FastDiv(sp.lanes * sp.groups);
+  a.head_step = sp.groups * sp.split;
+  a.tile = sp.tile;
+  const dim3 grid(sp.tiles, sp.split, n);
   by_type(out[0].dtype, codes[0].dtype, [&](auto type, auto f) {
-    launch_read<decltype(type), decltype(f)::value>(a, vec, n, most, stream);
+    launch_read<decltype(type), decltype(f)::value>(a, vec, grid, stream);
   });
   cuda_ok(cudaGetLastError(), "launch");
 }

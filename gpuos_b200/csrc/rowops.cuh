@@ -60,6 +60,21 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& r) {
   *reinterpret_cast<Pack<T, N>*>(p) = r;
 }
 
+// Two 32-bit products or sums in one instruction, each rounded on its own.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
 // `n` of the index tensor, 32 or 64 bit.
 __device__ __forceinline__ int64_t load_index(const void* p, bool wide, int64_t n) {
   return wide ? __ldg(static_cast<const long long*>(p) + n) : (int64_t)__ldg(static_cast<const int*>(p) + n);
