@@ -24,7 +24,6 @@ namespace rowops {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kHeads = 4;           // heads a thread has in flight
 constexpr int kTablePairs = 2048;   // (c, d) pairs a CTA holds: 16 KB
 
 struct RotTensor {
@@ -117,18 +116,15 @@ gpuos_rotary_kernel(const __grid_constant__ RotArgs a) {
     return h < a.t[0].heads ? o0 + h * a.t[0].oh : o1 + (h - a.t[0].heads) * a.t[1].oh;
   };
 
-  Pack<T, V> p[kHeads], q[kHeads];
+  // a rotated group (both halves), and the group of the copied part with its number
+  Pack<T, V> p, q, r;
   auto load = [&](uint32_t h, uint32_t j) {
-#pragma unroll
-    for (int u = 0; u < kHeads; ++u) {
-      const uint32_t hu = h + u * a.head_step;
-      if (hu >= heads) break;
-      const T* x = from(hu) + j * V;
-      fetch<T, V, VL>(x, p[u]);
-      if (!INTER) fetch<T, V, VL>(x + half, q[u]);
-    }
+    const T* x = from(h) + j * V;
+    fetch<T, V, VL>(x, p);
+    if (!INTER) fetch<T, V, VL>(x + half, q);
+    if (j < a.t[h >= a.t[0].heads].copies) fetch<T, V, VL>(x + 2 * half, r);
   };
-  if (live && j0 < a.units) load(h0, j0);
+  if (live && j0 < a.units && h0 < heads) load(h0, j0);
 
   for (uint32_t k = threadIdx.x; k < ntok * half; k += kThreads) {
     const uint32_t tok = a.half.div(k), pair = k - tok * half;
@@ -157,43 +153,31 @@ gpuos_rotary_kernel(const __grid_constant__ RotArgs a) {
         cd[2 * k + 1] = make_float2(w.z, w.w);
       }
     }
-    for (uint32_t h = h0; h < heads; h += kHeads * a.head_step) {
+    for (uint32_t h = h0; h < heads; h += a.head_step) {
       if (j != j0 || h != h0) load(h, j);
+      T* o = to(h) + j * V;
 #pragma unroll
-      for (int u = 0; u < kHeads; ++u) {
-        const uint32_t hu = h + u * a.head_step;
-        if (hu >= heads) break;
-        T* o = to(hu) + j * V;
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-          T& first = p[u].v[INTER ? 2 * i : i];
-          T& second = INTER ? p[u].v[2 * i + 1] : q[u].v[i];
-          const float v = to_f(first), w = to_f(second);
-          first = from_f<T>(v * cd[i].x - w * cd[i].y);
-          second = from_f<T>(w * cd[i].x + v * cd[i].y);
-        }
-        put<T, V, VL>(o, p[u]);
-        if (!INTER) put<T, V, VL>(o + half, q[u]);
+      for (int i = 0; i < P; ++i) {
+        T& first = p.v[INTER ? 2 * i : i];
+        T& second = INTER ? p.v[2 * i + 1] : q.v[i];
+        const float v = to_f(first), w = to_f(second);
+        first = from_f<T>(v * cd[i].x - w * cd[i].y);
+        second = from_f<T>(w * cd[i].x + v * cd[i].y);
       }
+      put<T, V, VL>(o, p);
+      if (!INTER) put<T, V, VL>(o + half, q);
+      if (j < a.t[h >= a.t[0].heads].copies) put<T, V, VL>(o + 2 * half, r);
     }
   }
-  // the elements that are not rotated
-  if (a.t[0].copies | a.t[1].copies) {
-    for (uint32_t h = h0; h < heads; h += kHeads * a.head_step) {
-      const uint32_t most = max(a.t[0].copies, a.t[1].copies);
-      for (uint32_t j = j0; j < most; j += a.lanes.d) {
-#pragma unroll
-        for (int u = 0; u < kHeads; ++u) {
-          const uint32_t hu = h + u * a.head_step;
-          if (hu >= heads) break;
-          if (j < a.t[hu >= a.t[0].heads].copies) fetch<T, V, VL>(from(hu) + 2 * half + j * V, p[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < kHeads; ++u) {
-          const uint32_t hu = h + u * a.head_step;
-          if (hu >= heads) break;
-          if (j < a.t[hu >= a.t[0].heads].copies) put<T, V, VL>(to(hu) + 2 * half + j * V, p[u]);
-        }
+  // where more is copied than rotated
+  if (a.t[0].copies > a.units || a.t[1].copies > a.units) {
+    uint32_t from_j = j0;
+    while (from_j < a.units) from_j += a.lanes.d;
+    for (uint32_t h = h0; h < heads; h += a.head_step) {
+      const uint32_t copies = a.t[h >= a.t[0].heads].copies;
+      for (uint32_t j = from_j; j < copies; j += a.lanes.d) {
+        fetch<T, V, VL>(from(h) + 2 * half + j * V, r);
+        put<T, V, VL>(to(h) + 2 * half + j * V, r);
       }
     }
   }
