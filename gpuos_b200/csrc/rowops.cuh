@@ -42,12 +42,13 @@ struct alignas(sizeof(T) * N) Pack {
   T v[N];
 };
 
-// The loads bypass no cache but mark streamed data: it is not read again.
-template <typename T, int N>
+// STREAM marks data that is not read again.
+template <typename T, int N, bool STREAM = true>
 __device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
   Pack<T, N> r;
   constexpr int B = sizeof(T) * N;
-  if constexpr (B == 16) *reinterpret_cast<uint4*>(&r) = __ldcs(reinterpret_cast<const uint4*>(p));
+  if constexpr (!STREAM) r = *reinterpret_cast<const Pack<T, N>*>(p);
+  else if constexpr (B == 16) *reinterpret_cast<uint4*>(&r) = __ldcs(reinterpret_cast<const uint4*>(p));
   else if constexpr (B == 8) *reinterpret_cast<uint2*>(&r) = __ldcs(reinterpret_cast<const uint2*>(p));
   else if constexpr (B == 4) *reinterpret_cast<uint32_t*>(&r) = __ldcs(reinterpret_cast<const uint32_t*>(p));
   else if constexpr (B == 2) *reinterpret_cast<uint16_t*>(&r) = __ldcs(reinterpret_cast<const unsigned short*>(p));
@@ -71,6 +72,13 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   unsigned long long r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r)
       : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
+        "l"(*reinterpret_cast<unsigned long long*>(&c)));
   return *reinterpret_cast<float2*>(&r);
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
