@@ -11,13 +11,20 @@
 // for the gradients g of log p(y) and h of H.
 //
 // Forward reads the row once.  A thread keeps its own running maximum, sum and
-// weighted sum (rescaled when a pack of 16 bytes raises the maximum) in 32 bits; they
-// are joined at the row's end.  For the alternatives every warp keeps a list of
-// candidates no smaller than a bound that the whole row shares: the k-th
-// largest of 64 maxima taken from the row's first packs, raised whenever a list fills up
-// and is cut back to its k largest.  Elements below the bound cost one comparison a pack.
-// Few long rows are split over a cluster of up to 8 CTAs, which join through
+// weighted sum in 32 bits, rescaled when a step of U 16-byte packs raises the
+// maximum; they are joined at the row's end.  The alternatives cost nothing
+// while the row streams but a maximum that each thread leaves behind now and
+// then.  At the row's end the k-th largest of 64 maxima over threads is a bound
+// that k elements reach, and only packs under a maximum that reaches it are read
+// again (a few KB).  Rows of many equal or masked logits make more candidates than that:
+// they are read again whole, through lists of a warp each, cut back when full
+// to the k largest, which raises the bound.  Few or
+// long rows are split over a cluster of up to 8 CTAs, which join through
 // distributed shared memory: no workspace, and the same order of sums each time.
+//
+// At 16 bits an SM's share of the memory rate is about 12 elements a cycle,
+// its exponentials 16, its instructions 128 lanes: the loop is kept to about 5
+// instructions an element (maxima of two elements at once, packed 32-bit sums and products).
 #include <cooperative_groups.h>
 
 #include "rowops.cuh"
@@ -29,9 +36,11 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kMaxTop = 64;
+constexpr int kRowThreads = 256;  // of a CTA; short rows take 128
 constexpr int kList = 128;    // candidates a warp holds
 constexpr int kSeeds = 64;    // maxima that give the first bound
 constexpr float kLn2 = 0.693147180559945309f;
+constexpr float kLowest = -3.402823466e38f;  // the lowest finite number: where a maximum starts
 
 struct LogArgs {
   const void* x;
@@ -51,6 +60,7 @@ struct LogArgs {
   float k2;       // log2(e) / t
   float t, inv_t;
   uint32_t top_k;
+  uint32_t parts;   // gradient: CTAs of a row
   int target_wide, token_wide, vec;
 };
 
@@ -76,7 +86,9 @@ __device__ __forceinline__ float value_of(unsigned long long key) {
 // Running maximum m, s = sum 2^y and w = sum y 2^y with y = (x - m) log2(e) / t.
 // m starts at the lowest finite number, so a masked (-inf) element is just a zero term.
 struct Running {
-  float m = -3.402823466e38f, s = 0.f, w = 0.f;
+  float m = kLowest, s = 0.f, w = 0.f;
+  __device__ Running() {}
+  __device__ Running(float m_, float s_, float w_) : m(m_), s(s_), w(w_) {}
 };
 
 template <bool ENT>
@@ -90,32 +102,94 @@ __device__ __forceinline__ void join(Running& a, float m, float s, float w, floa
   a.m = top;
 }
 
-template <bool ENT, int N>
-__device__ __forceinline__ void add_pack(Running& r, const float (&x)[N], float cm, float k2) {
-  if (cm > r.m) {
-    const float d = fmaxf((r.m - cm) * k2, -1e4f), f = ex2(d);
-    if (ENT) r.w = f * (r.w + d * r.s);
-    r.s *= f;
-    r.m = cm;
-  }
+// Joins the first LANES lanes of a warp.
+template <int LANES, bool ENT>
+__device__ __forceinline__ Running join_lanes(Running t, float k2) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float y = (x[i] - r.m) * k2;
-    const float e = ex2(y);
-    r.s += e;
-    if (ENT) r.w = fmaf(fmaxf(y, -1e4f), e, r.w);
+  for (int d = LANES / 2; d; d >>= 1) {
+    const float m = __shfl_xor_sync(~0u, t.m, d), s = __shfl_xor_sync(~0u, t.s, d), w = __shfl_xor_sync(~0u, t.w, d);
+    join<ENT>(t, m, s, w, k2);
+  }
+  return t;
+}
+
+// The maximum of a pack's elements; a NaN does not count.
+template <typename T, int N>
+__device__ __forceinline__ float max_of(const Pack<T, N>& x) {
+  if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    const T2* h = reinterpret_cast<const T2*>(&x);
+    T2 m = h[0];
+#pragma unroll
+    for (int i = 1; i < N / 2; ++i) m = __hmax2(m, h[i]);
+    return fmaxf(to_f(m.x), to_f(m.y));
+  } else {
+    float m = to_f(x.v[0]);
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = fmaxf(m, to_f(x.v[i]));
+    return m;
   }
 }
 
+// Running sums of a thread: s and w in two parts each, for packed arithmetic.
+struct Sums {
+  float m = kLowest;
+  float2 s = {0.f, 0.f}, w = {0.f, 0.f};
+};
+
+// Raises the maximum to cm (a NaN or anything smaller does nothing).
+template <bool ENT>
+__device__ __forceinline__ void raise(Sums& r, float cm, float k2) {
+  if (cm > r.m) {
+    const float d = fmaxf((r.m - cm) * k2, -1e4f), f = ex2(d);
+    if (ENT) r.w = mul2(both(f), fma2(both(d), r.s, r.w));
+    r.s = mul2(both(f), r.s);
+    r.m = cm;
+  }
+}
+
+template <bool ENT>
+__device__ __forceinline__ void add_two(Sums& r, float2 x, float k2) {
+  const float2 y = mul2(add2(x, both(-r.m)), both(k2));
+  const float2 e = make_float2(ex2(y.x), ex2(y.y));
+  r.s = add2(r.s, e);
+  // a masked element's y is -inf: its term is 0, not inf * 0
+  if (ENT) r.w = fma2(make_float2(fmaxf(y.x, -1e4f), fmaxf(y.y, -1e4f)), e, r.w);
+}
+
+constexpr uint32_t kMarks = 16;    // maxima a thread leaves on its way along a row
+constexpr uint32_t kReach = 512;   // of them that may reach the bound, and
+constexpr uint32_t kFew = 4;       // packs a thread then reads again, before the lists are used
+
+// Kept small: what the CTAs of an SM do not take of its memory holds their loads
+// in flight (at 45 KB a CTA the loop ran a third slower than at 15).
+template <typename T, int THREADS>
+struct TopShared {
+  static constexpr uint32_t kWarps = THREADS / 32;
+  static constexpr uint32_t kPool = std::max<uint32_t>(kMarks * THREADS * sizeof(T) / 8, kWarps * (kList + kMaxTop));
+  static constexpr uint32_t kAll = std::min<uint32_t>(kPool, 1024);
+  unsigned long long bound;          // no candidate below it is needed
+  uint32_t count;                    // of the candidates
+  uint32_t reached;                  // of `reach`
+  float seeds[kSeeds];
+  uint32_t reach[kReach];            // (mark, thread) whose maximum reaches the bound
+  unsigned long long last[kMaxTop];  // the top_k, sorted
+  // one after the other: the marks; the candidates; where those are too many, each
+  // warp's list, and behind them the lists joined
+  unsigned long long pool[kPool];
+  unsigned long long best[];         // of a cluster's first CTA: each part's top_k
+  __device__ T* marks() { return reinterpret_cast<T*>(pool); }
+  __device__ unsigned long long* list(uint32_t warp) { return pool + warp * kList; }
+  __device__ unsigned long long* joined() { return pool + kWarps * kList; }
+};
+
+template <int THREADS> struct RowShared;
+template <int THREADS> constexpr size_t kTopAt = (sizeof(RowShared<THREADS>) + 15) / 16 * 16;
+
 template <int THREADS>
-struct LogShared {
-  unsigned long long bound;                       // no candidate below it is needed
-  uint32_t count;
-  unsigned long long lists[THREADS / 32][kList];
-  unsigned long long all[THREADS / 32 * kList];   // the lists joined; seeds before that
+struct RowShared {
   float m[THREADS / 32], s[THREADS / 32], w[THREADS / 32];
-  unsigned long long best[kMaxTop];               // this CTA's top_k, sorted
-  float part[3];                                  // this CTA's m, s, w
+  Running part[8];                   // each part's m, s, w
 };
 
 // Cuts a warp's list of n keys to its k largest, sorted, and raises the bound.
@@ -144,27 +218,25 @@ __device__ __forceinline__ uint32_t cut(unsigned long long* list, uint32_t n, ui
   return n < k ? n : k;
 }
 
-// The whole warp offers N elements a lane from index `at` on (valid ones: n).
-template <int N>
-__device__ __forceinline__ void offer(const float (&x)[N], uint32_t at, int n, uint32_t k, unsigned long long* list,
-                                      uint32_t& count, volatile unsigned long long* bound) {
+// The whole warp offers N elements a lane from index `at` on; `open` says which.
+template <typename T, int N>
+__device__ __forceinline__ void offer(const Pack<T, N>& x, uint32_t open, uint32_t at, uint32_t k,
+                                      unsigned long long* list, uint32_t& count, unsigned long long* bound) {
   const uint32_t lane = threadIdx.x & 31;
-  unsigned long long b = *bound;
-  uint32_t open = 0;
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (i < n && key_of(x[i], at + i) >= b) open |= 1u << i;
+  unsigned long long b = *(volatile unsigned long long*)bound;
   while (__any_sync(~0u, open)) {
     if (count > kList - 32) {
-      count = cut(list, count, k, const_cast<unsigned long long*>(bound));
-      b = *bound;
+      count = cut(list, count, k, bound);
+      b = *(volatile unsigned long long*)bound;
     }
-    unsigned long long key = 0;
+    const int first = __ffs(open) - 1;
+    float v = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (__ffs(open) - 1 == i) key = key_of(x[i], at + i);
+      if (first == i) v = to_f(x.v[i]);
+    const unsigned long long key = key_of(v, at + first);
+    const bool take = open != 0 && key >= b;
     open &= open - 1;
-    const bool take = key != 0 && key >= b;
     const uint32_t who = __ballot_sync(~0u, take);
     if (take) list[count + __popc(who & ((1u << lane) - 1))] = key;
     count += __popc(who);
@@ -172,24 +244,47 @@ __device__ __forceinline__ void offer(const float (&x)[N], uint32_t at, int n, u
   }
 }
 
-// Ranks n unique keys by counting; those below k go to out, sorted.
+// Which of the elements of a pack at index `at` have a key of at least `bound` (a NaN
+// stands for -inf in the order).
+template <typename T, int N>
+__device__ __forceinline__ uint32_t candidates(const Pack<T, N>& x, uint32_t at, unsigned long long bound) {
+  const float least = value_of(bound);
+  const uint32_t last = ~(uint32_t)bound;  // of elements equal to it, those up to its index
+  uint32_t open = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float v = to_f(x.v[i]);
+    if (v > least || (!(v < least) && (v == least || least == -INFINITY) && at + i <= last)) open |= 1u << i;
+  }
+  return open;
+}
+
+// Ranks n unique keys by counting the larger ones, 8 lanes to a key; those
+// below k go to out, sorted.
 template <int THREADS>
 __device__ __forceinline__ void rank_into(const unsigned long long* keys, uint32_t n, uint32_t k, unsigned long long* out) {
-  for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-    const unsigned long long mine = keys[i];
+  for (uint32_t i0 = 0; i0 < n; i0 += THREADS / 8) {
+    const uint32_t i = i0 + threadIdx.x / 8;
+    const unsigned long long mine = i < n ? keys[i] : 0;
     uint32_t rank = 0;
-    for (uint32_t j = 0; j < n; ++j) rank += keys[j] > mine;
-    if (rank < k) out[rank] = mine;
+    for (uint32_t j = threadIdx.x & 7; j < n; j += 8) rank += keys[j] > mine;
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) rank += __shfl_xor_sync(~0u, rank, d);
+    if ((threadIdx.x & 7) == 0 && i < n && rank < k) out[rank] = mine;
   }
 }
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
 template <typename T, int THREADS, bool ENT, bool TOP>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, THREADS == kRowThreads ? 6 : 1)
 gpuos_logprobs_kernel(const __grid_constant__ LogArgs a) {
   constexpr int W = 16 / sizeof(T);
   constexpr int U = 4;  // packs a thread has in flight
   extern __shared__ __align__(16) uint8_t smem[];
-  LogShared<THREADS>& sh = *reinterpret_cast<LogShared<THREADS>*>(smem);
+  RowShared<THREADS>& sh = *reinterpret_cast<RowShared<THREADS>*>(smem);
+  TopShared<T, THREADS>& top = *reinterpret_cast<TopShared<T, THREADS>*>(smem + kTopAt<THREADS>);
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t parts = cluster.num_blocks(), part = cluster.block_rank();
   const int64_t row = blockIdx.x / parts;
@@ -205,161 +300,241 @@ gpuos_logprobs_kernel(const __grid_constant__ LogArgs a) {
   const uint32_t tail = head + packs * W;
   const T* body = x + head;
 
-  Running r;
-  uint32_t count = 0;
+  // read ahead: the row's last step needs it
+  int64_t target = -1;
+  float target_x = 0.f;
+  if (part == 0 && threadIdx.x == 0) {
+    target = load_index(a.targets, a.target_wide, row * a.ts);
+    if (target >= 0 && target < a.cols) target_x = to_f(x[target]);
+  }
+  if (parts > 1) cluster_arrive();
+
+  Sums r;
   if (TOP && threadIdx.x == 0) {
-    sh.bound = 0;
-    sh.count = 0;
+    top.bound = 0;
+    top.count = 0;
+    top.reached = 0;
   }
 
   // the loose elements, at most 2 (W - 1), go to the last part's first warp
-  float loose = -INFINITY;
+  Pack<T, 1> loose;
   uint32_t loose_at = 0;
   bool has_loose = false;
   if (part == parts - 1 && warp == 0) {
-    const uint32_t nl = head + (cols - tail);
-    has_loose = lane < nl;
+    has_loose = lane < head + (cols - tail);
     if (has_loose) {
       loose_at = lane < head ? lane : tail + (lane - head);
-      loose = to_f(x[loose_at]);
+      loose.v[0] = x[loose_at];
     }
   }
 
+  const uint32_t steps = (p1 - p0 + THREADS * U - 1) / (THREADS * U);
+  const uint32_t stretch = (steps + kMarks - 1) / kMarks;  // steps a mark covers
+  uint32_t mark = 0, left = stretch;
+  float marked = -INFINITY;
   for (uint32_t base = p0; base < p1; base += THREADS * U) {
+    // a step: U packs a thread, all of them or (the last step) those below p1
     Pack<T, W> q[U];
+    const uint32_t mine = base + threadIdx.x;
+    const bool whole = base + THREADS * U <= p1;
+    if (whole) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t p = base + u * THREADS + threadIdx.x;
-      if (p < p1) q[u] = load_pack<T, W>(body + (uint64_t)p * W);
-    }
-    if (TOP && base == p0) {
-      // the first bound: the k-th largest of 64 maxima, each over its own lanes' first packs
-      unsigned long long best = 0;
-      if (p0 + threadIdx.x < p1) {
-        const uint32_t at = head + (p0 + threadIdx.x) * W;
+      for (int u = 0; u < U; ++u) q[u] = load_pack<T, W>(body + (uint64_t)(mine + u * THREADS) * W);
+    } else {
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-          const unsigned long long key = key_of(to_f(q[0].v[i]), at + i);
-          best = key > best ? key : best;
+      for (int u = 0; u < U; ++u) {
+        if (mine + u * THREADS < p1) {
+          q[u] = load_pack<T, W>(body + (uint64_t)(mine + u * THREADS) * W);
+        } else {
+#pragma unroll
+          for (int i = 0; i < W; ++i) q[u].v[i] = from_f<T>(-INFINITY);
         }
       }
-#pragma unroll
-      for (int d = 1; d < THREADS / kSeeds; d <<= 1) {
-        const unsigned long long o = __shfl_xor_sync(~0u, best, d);
-        best = o > best ? o : best;
-      }
-      if (threadIdx.x % (THREADS / kSeeds) == 0) sh.all[threadIdx.x / (THREADS / kSeeds)] = best;
-      __syncthreads();
-      if (threadIdx.x < kSeeds) {
-        const unsigned long long mine = sh.all[threadIdx.x];
-        uint32_t rank = 0;
-        for (int j = 0; j < kSeeds; ++j) rank += sh.all[j] > mine;
-        if (mine != 0 && rank == a.top_k - 1) sh.bound = mine;
-      }
-      __syncthreads();
     }
+    float cm = max_of(q[0]);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t first = base + u * THREADS + warp * 32;  // the warp's first pack
-      if (first >= p1) break;
-      const uint32_t p = first + lane;
-      float v[W];
-      float cm = -INFINITY;
-      const bool in = p < p1;
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        v[i] = in ? to_f(q[u].v[i]) : -INFINITY;
-        cm = fmaxf(cm, v[i]);
-      }
-      add_pack<ENT, W>(r, v, cm, a.k2);
-      if (TOP) {
-        const float least = value_of(*(volatile unsigned long long*)&sh.bound);
-        if (__any_sync(~0u, in && cm >= least))
-          offer<W>(v, head + p * W, in ? W : 0, a.top_k, sh.lists[warp], count, &sh.bound);
+    for (int u = 1; u < U; ++u) cm = fmaxf(cm, max_of(q[u]));
+    raise<ENT>(r, cm, a.k2);
+    if (TOP) {
+      marked = fmaxf(marked, cm);
+      if (--left == 0 || base + THREADS * U >= p1) {
+        top.marks()[mark++ * THREADS + threadIdx.x] = from_f<T>(marked);
+        marked = -INFINITY;
+        left = stretch;
       }
     }
+    // a last step's missing packs are -inf: terms of 0
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < W; i += 2) add_two<ENT>(r, make_float2(to_f(q[u].v[i]), to_f(q[u].v[i + 1])), a.k2);
   }
-  if (TOP && p0 >= p1) __syncthreads();  // the bound's start is set
-  if (part == parts - 1 && warp == 0) {
-    const float v[1] = {loose};
-    if (has_loose) add_pack<ENT, 1>(r, v, fmaxf(loose, -INFINITY), a.k2);
-    if (TOP) offer<1>(v, loose_at, has_loose ? 1 : 0, a.top_k, sh.lists[warp], count, &sh.bound);
+  if (has_loose) {
+    const float v = to_f(loose.v[0]);
+    raise<ENT>(r, v, a.k2);
+    add_two<ENT>(r, make_float2(v, -INFINITY), a.k2);
   }
 
   // join: lanes, warps, then the cluster's CTAs, always in the same order
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    const float m = __shfl_xor_sync(~0u, r.m, d), s = __shfl_xor_sync(~0u, r.s, d), w = __shfl_xor_sync(~0u, r.w, d);
-    join<ENT>(r, m, s, w, a.k2);
-  }
+  const Running t = join_lanes<32, ENT>(Running{r.m, r.s.x + r.s.y, r.w.x + r.w.y}, a.k2);
   if (lane == 0) {
-    sh.m[warp] = r.m;
-    sh.s[warp] = r.s;
-    sh.w[warp] = r.w;
+    sh.m[warp] = t.m;
+    sh.s[warp] = t.s;
+    sh.w[warp] = t.w;
+  }
+  constexpr int L = THREADS / kSeeds;  // lanes to a seed
+  if (TOP) {
+    float m = r.m;
+#pragma unroll
+    for (int d = 1; d < L; d <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+    if (threadIdx.x % L == 0) top.seeds[threadIdx.x / L] = m;
   }
   __syncthreads();
   if (TOP) {
-    const unsigned long long b = *(volatile unsigned long long*)&sh.bound;
-    for (uint32_t i = lane; i < count; i += 32) {
-      const unsigned long long key = sh.lists[warp][i];
-      if (key >= b) sh.all[atomicAdd(&sh.count, 1u)] = key;
+    const int seed = threadIdx.x / L;
+    const float me = top.seeds[seed];
+    uint32_t rank = 0;
+#pragma unroll
+    for (int j = threadIdx.x % L; j < kSeeds; j += L) {
+      const float o = top.seeds[j];
+      rank += o > me || (o == me && j < seed);
     }
-    for (uint32_t i = threadIdx.x; i < a.top_k; i += THREADS) sh.best[i] = 0;
+#pragma unroll
+    for (int d = 1; d < L; d <<= 1) rank += __shfl_xor_sync(~0u, rank, d);
+    // A maximum that is still where it started was reached by nothing: no bound.
+    // Otherwise every element of this value and above counts, whatever its index.
+    if (threadIdx.x % L == 0 && rank == a.top_k - 1 && me > kLowest) top.bound = key_of(me, 0) & ~0xffffffffull;
+    for (uint32_t i = threadIdx.x; i < a.top_k; i += THREADS) top.last[i] = 0;
     __syncthreads();
-    rank_into<THREADS>(sh.all, sh.count, a.top_k, sh.best);
-  }
-  if (threadIdx.x == 0) {
-    Running c;
-    for (int i = 0; i < THREADS / 32; ++i) join<ENT>(c, sh.m[i], sh.s[i], sh.w[i], a.k2);
-    sh.part[0] = c.m;
-    sh.part[1] = c.s;
-    sh.part[2] = c.w;
-  }
-  if (parts > 1) cluster.sync();
-  else __syncthreads();
-  if (part == 0) {
-    Running c;
-    for (uint32_t i = 0; i < parts; ++i) {
-      const float* o = parts > 1 ? cluster.map_shared_rank(sh.part, i) : sh.part;
-      join<ENT>(c, o[0], o[1], o[2], a.k2);
-    }
-    const float ln_s = logf(c.s);
-    const bool none = c.s == 0.f;  // every logit is -inf
-    if (threadIdx.x == 0) {
-      const int64_t y = load_index(a.targets, a.target_wide, row * a.ts);
-      float lp;
-      if (y < 0) lp = 0.f;
-      else if (y >= a.cols) lp = NAN;
-      else lp = none ? -INFINITY : (to_f(x[y]) - c.m) / a.t - ln_s;
-      a.logprob[row * a.ls] = lp;
-      if (ENT) a.entropy[row * a.es] = none ? 0.f : ln_s - kLn2 * c.w / c.s;
-      if (a.stats) {
-        a.stats[row * a.ss] = c.m;
-        a.stats[row * a.ss + a.sk] = c.s;
+    const unsigned long long bound = top.bound;
+    if (r.m >= value_of(bound))
+      for (uint32_t i = 0; i < mark; ++i)
+        if (to_f(top.marks()[i * THREADS + threadIdx.x]) >= value_of(bound)) {
+          const uint32_t n = atomicAdd(&top.reached, 1u);
+          if (n < kReach) top.reach[n] = i << 16 | threadIdx.x;
+        }
+    __syncthreads();
+    // the packs under those marks, a lane each
+    const uint32_t each = stretch * U;
+    const bool few = top.reached <= kReach && (uint64_t)top.reached * each <= kFew * THREADS;
+    if (few) {
+      const uint32_t items = top.reached * each;
+      Pack<T, W> q[kFew];
+      uint32_t at[kFew];
+#pragma unroll
+      for (int u = 0; u < kFew; ++u) {
+        const uint32_t it = u * THREADS + threadIdx.x;
+        at[u] = p1;
+        if (it < items) {
+          const uint32_t i = it / each, to = top.reach[i];
+          at[u] = p0 + ((to >> 16) * each + (it - i * each)) * THREADS + (to & 0xffff);
+        }
+        if (at[u] < p1) q[u] = load_pack<T, W>(body + (uint64_t)at[u] * W);
+      }
+#pragma unroll
+      for (int u = 0; u < kFew; ++u) {
+        if (at[u] >= p1) continue;
+        uint32_t open = candidates<T, W>(q[u], head + at[u] * W, bound);
+        while (open) {
+          const int e = __ffs(open) - 1;
+          open &= open - 1;
+          float v = 0.f;
+#pragma unroll
+          for (int i = 0; i < W; ++i)
+            if (e == i) v = to_f(q[u].v[i]);
+          const uint32_t n = atomicAdd(&top.count, 1u);
+          if (n < top.kAll) top.pool[n] = key_of(v, head + at[u] * W + e);
+        }
+      }
+      if (has_loose && candidates<T, 1>(loose, loose_at, bound)) {
+        const uint32_t n = atomicAdd(&top.count, 1u);
+        if (n < top.kAll) top.pool[n] = key_of(to_f(loose.v[0]), loose_at);
       }
     }
+    __syncthreads();
+    if (!few || top.count > top.kAll) {
+      // many equal or masked logits: the row again, through lists that are cut
+      __syncthreads();
+      if (threadIdx.x == 0) top.count = 0;
+      uint32_t count = 0;  // of this warp's list
+      for (uint32_t p = p0 + threadIdx.x; __any_sync(~0u, p < p1); p += THREADS) {
+        Pack<T, W> q;
+        uint32_t open = 0;
+        if (p < p1) {
+          q = load_pack<T, W>(body + (uint64_t)p * W);
+          open = candidates<T, W>(q, head + p * W, *(volatile unsigned long long*)&top.bound);
+        }
+        offer<T, W>(q, open, head + p * W, a.top_k, top.list(warp), count, &top.bound);
+      }
+      if (part == parts - 1 && warp == 0)
+        offer<T, 1>(loose, has_loose ? candidates<T, 1>(loose, loose_at, *(volatile unsigned long long*)&top.bound) : 0u,
+                    loose_at, a.top_k, top.list(warp), count, &top.bound);
+      if (count > a.top_k) count = cut(top.list(warp), count, a.top_k, &top.bound);
+      __syncthreads();
+      const unsigned long long b = *(volatile unsigned long long*)&top.bound;
+      for (uint32_t i = lane; i < count; i += 32) {
+        const unsigned long long key = top.list(warp)[i];
+        if (key >= b) top.joined()[atomicAdd(&top.count, 1u)] = key;
+      }
+      __syncthreads();
+      rank_into<THREADS>(top.joined(), top.count, a.top_k, top.last);
+    } else {
+      rank_into<THREADS>(top.pool, top.count, a.top_k, top.last);
+    }
+    if (parts > 1) __syncthreads();
+  }
+  // every part writes its results into the shared memory of the row's first CTA,
+  // which has started (the barrier above) and waits for them (the one below)
+  Running* to = &sh.part[part];
+  if (parts > 1) {
+    cluster_wait();
+    to = cluster.map_shared_rank(to, 0);
     if (TOP) {
-      const unsigned long long* best = sh.best;
-      if (parts > 1) {
-        // the parts' lists, joined and ranked again
-        for (uint32_t i = threadIdx.x; i < parts * a.top_k; i += THREADS)
-          sh.all[i] = cluster.map_shared_rank(sh.best, i / a.top_k)[i % a.top_k];
-        __syncthreads();
-        unsigned long long* out = sh.lists[0];
-        rank_into<THREADS>(sh.all, parts * a.top_k, a.top_k, out);
-        __syncthreads();
-        best = out;
-      }
-      for (uint32_t i = threadIdx.x; i < a.top_k; i += THREADS) {
-        const float v = value_of(best[i]);
-        a.top[row * a.tps + i * a.tpk] = none ? -INFINITY : (v - c.m) / a.t - ln_s;
-        const uint32_t token = ~(uint32_t)best[i];
-        if (a.token_wide) static_cast<int64_t*>(a.tokens)[row * a.tks + i * a.tkk] = token;
-        else static_cast<int32_t*>(a.tokens)[row * a.tks + i * a.tkk] = (int32_t)token;
-      }
+      unsigned long long* best = cluster.map_shared_rank(top.best, 0) + part * a.top_k;
+      for (uint32_t i = threadIdx.x; i < a.top_k; i += THREADS) best[i] = top.last[i];
     }
   }
-  if (parts > 1) cluster.sync();  // the other CTAs' shared memory is read above
+  if (warp == THREADS / 32 - 1) {
+    Running c;
+    if (lane < THREADS / 32) c = Running{sh.m[lane], sh.s[lane], sh.w[lane]};
+    c = join_lanes<THREADS / 32, ENT>(c, a.k2);
+    if (lane == 0) *to = c;
+  }
+  if (parts > 1) {
+    cluster_arrive();
+    if (part != 0) return;
+    cluster_wait();
+    if (TOP) rank_into<THREADS>(top.best, parts * a.top_k, a.top_k, top.last);
+  }
+  __syncthreads();
+  if (warp != 0) return;
+  Running c;
+  if (lane < parts) c = sh.part[lane];
+  c = join_lanes<8, ENT>(c, a.k2);
+  c = Running{__shfl_sync(~0u, c.m, 0), __shfl_sync(~0u, c.s, 0), __shfl_sync(~0u, c.w, 0)};
+  const float ln_s = logf(c.s);
+  const bool none = c.s == 0.f;  // every logit is -inf
+  if (lane == 0) {
+    float lp;
+    if (target < 0) lp = 0.f;
+    else if (target >= a.cols) lp = NAN;
+    else lp = none ? -INFINITY : (target_x - c.m) / a.t - ln_s;
+    a.logprob[row * a.ls] = lp;
+    if (ENT) a.entropy[row * a.es] = none ? 0.f : ln_s - kLn2 * c.w / c.s;
+    if (a.stats) {
+      a.stats[row * a.ss] = c.m;
+      a.stats[row * a.ss + a.sk] = c.s;
+    }
+  }
+  if (TOP) {
+    for (uint32_t i = lane; i < a.top_k; i += 32) {
+      const unsigned long long key = top.last[i];
+      a.top[row * a.tps + i * a.tpk] = none ? -INFINITY : (value_of(key) - c.m) / a.t - ln_s;
+      const uint32_t token = ~(uint32_t)key;
+      if (a.token_wide) static_cast<int64_t*>(a.tokens)[row * a.tks + i * a.tkk] = token;
+      else static_cast<int32_t*>(a.tokens)[row * a.tks + i * a.tkk] = (int32_t)token;
+    }
+  }
 }
 
 constexpr int kGradThreads = 256;
@@ -371,7 +546,9 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kGradThreads)
 gpuos_logprobs_grad_kernel(const __grid_constant__ LogArgs a) {
   constexpr int W = VEC ? 16 / sizeof(T) : 1;
-  const int64_t row = blockIdx.x;
+  // from the last row on: forward read it last, so that it may still be in L2
+  const uint32_t from_end = blockIdx.x / a.parts, part = blockIdx.x - from_end * a.parts;
+  const int64_t row = a.rows - 1 - from_end;
   const T* x = static_cast<const T*>(a.x) + row * a.xs;
   T* o = static_cast<T*>(a.gx) + row * a.gs;
   const int64_t y = load_index(a.targets, a.target_wide, row * a.ts);
@@ -398,8 +575,8 @@ gpuos_logprobs_grad_kernel(const __grid_constant__ LogArgs a) {
     head = min(cols, off ? W - off : 0u);
   }
   const uint32_t packs = (cols - head) / W, tail = head + packs * W;
-  const uint32_t base = blockIdx.y * (kGradThreads * kGradPacks) + threadIdx.x;
-  if (VEC && blockIdx.y == 0) {
+  const uint32_t base = part * (kGradThreads * kGradPacks) + threadIdx.x;
+  if (VEC && part == 0) {
     for (uint32_t i = threadIdx.x; i < head; i += kGradThreads) o[i] = from_f<T>(value(to_f(x[i]), i));
     for (uint32_t i = tail + threadIdx.x; i < cols; i += kGradThreads) o[i] = from_f<T>(value(to_f(x[i]), i));
   }
@@ -422,7 +599,7 @@ gpuos_logprobs_grad_kernel(const __grid_constant__ LogArgs a) {
 
 template <typename T, int THREADS, bool ENT, bool TOP>
 void launch(const LogArgs& a, uint32_t parts, cudaStream_t s) {
-  const size_t smem = sizeof(LogShared<THREADS>);
+  const size_t smem = kTopAt<THREADS> + (TOP ? sizeof(TopShared<T, THREADS>) + (parts > 1 ? parts * a.top_k * 8 : 0) : 0);
   auto kernel = gpuos_logprobs_kernel<T, THREADS, ENT, TOP>;
   if (smem > 48 * 1024)
     cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory");
@@ -450,12 +627,12 @@ void by_outputs(const LogArgs& a, uint32_t parts, cudaStream_t s) {
 
 template <typename T>
 void forward(const LogArgs& a, cudaStream_t s) {
-  constexpr int64_t kStep = 512 * 16 / sizeof(T);  // elements a CTA reads at once
+  constexpr int64_t kStep = kRowThreads * 16 / sizeof(T);  // elements a CTA reads at once
   uint32_t parts = 1;
   while (parts < 8 && a.rows * parts < 2 * sm_count() && a.cols >= kStep * parts * 2) parts *= 2;
-  // a row of one step of 128 threads leaves most of a larger CTA idle
+  // a row of one pack for each of 128 threads leaves most of a larger CTA idle
   if (parts == 1 && a.cols <= kStep / 2) by_outputs<T, 128>(a, parts, s);
-  else by_outputs<T, 512>(a, parts, s);
+  else by_outputs<T, kRowThreads>(a, parts, s);
 }
 
 LogArgs prepare(const gpuos_tensor* x, const gpuos_tensor* targets, float temperature) {
@@ -546,11 +723,12 @@ void logprobs(const gpuos_tensor* x, const gpuos_tensor* targets, const gpuos_te
 }
 
 template <typename T>
-void backward(const LogArgs& a, cudaStream_t s) {
+void backward(LogArgs a, cudaStream_t s) {
   const int64_t per = (int64_t)kGradThreads * kGradPacks * (a.vec ? 16 / (int)sizeof(T) : 1);
   const int64_t parts = (a.cols + per - 1) / per;
-  need(parts < 65536, "too many tokens");
-  const dim3 grid((unsigned)a.rows, (unsigned)parts);
+  need(a.rows * parts < 0x7fffffffll, "too many logits");
+  a.parts = (uint32_t)parts;
+  const unsigned grid = (unsigned)(a.rows * parts);
   if (a.vec) gpuos_logprobs_grad_kernel<T, true><<<grid, kGradThreads, 0, s>>>(a);
   else gpuos_logprobs_grad_kernel<T, false><<<grid, kGradThreads, 0, s>>>(a);
   cuda_ok(cudaGetLastError(), "launch");
