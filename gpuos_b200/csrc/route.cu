@@ -7,15 +7,21 @@
 //   top_k largest keys of the open groups; of equal ones the lowest index
 //   w    = s of the chosen (/ their sum) * scale
 //
-// The chosen experts are those of exact arithmetic.  Keys are computed in 32
-// bits with a known error bound; where two keys whose order matters are closer
-// than the bound (and not of equal inputs), the token is done again in 64 bits.
+// The chosen experts are those of exact arithmetic, at the price of a fast
+// selection: every key becomes one unsigned integer, the key's place in the
+// row's range above the expert's slot, so that a maximum over lanes gives key and
+// expert at once and of equal keys the lowest index.  16-bit logits without a
+// bias fit whole; other keys are computed in 32 bits, with a known error bound, and rounded
+// to 22 to 24 bits of the range that the largest ones span.  Where two keys whose
+// order matters come out closer than the error, the token is done again in 64 bits
+// (about one in a thousand of random logits).
 //
 // A token belongs to LPT lanes of a warp, each holding NPL neighbouring experts
-// in registers: up to 256 experts take 8 a lane and as many lanes as needed, so
-// that one warp serves up to 8 tokens of few experts.  Rounds of maximum over
-// the lanes pick the experts; a lane's experts are neighbours, so the first
-// lane that holds the maximum holds the lowest index.
+// of one group in registers: up to 256 experts take 8 a lane and as many lanes as
+// needed, so that one warp serves up to 8 tokens of few experts.  A lane sorts its
+// keys once; a round of the selection is then a maximum over the lanes' first ones.
+// Few experts make the kernel a matter of instructions, not of bytes: 16384
+// tokens of 256 take 18 MB, 2.8 us.
 #include "rowops.cuh"
 
 namespace gpuos {
@@ -37,35 +43,27 @@ struct RouteArgs {
   int64_t tokens;
   uint32_t n;          // experts
   uint32_t top_k, groups, top_groups;
-  FastDiv per_group;
+  uint32_t per_group;  // experts of a group
+  // How a token's experts are seated: by groups, so that no lane has experts of two, or, where
+  // the groups are too many for the lanes of a warp, all in a row.
+  uint32_t seat_groups, seat_per_group;
+  FastDiv lanes;       // lanes of a group
   float scale;
   int sigmoid, renorm, top2, wide, vec;
 };
 
 template <typename R> struct Num;
 template <> struct Num<float> {
-  using Key = uint32_t;
   static __device__ __forceinline__ float exp_(float x) { return expf(x); }
-  // An unsigned integer that orders as x does; NaN as -inf; never 0.
-  static __device__ __forceinline__ Key key(float x) {
-    if (x != x) x = -INFINITY;
-    const uint32_t b = __float_as_uint(x + 0.f);
-    return (b >> 31) ? ~b : b | 0x80000000u;
-  }
-  static __device__ __forceinline__ float value(Key k) {
-    return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
-  }
 };
 template <> struct Num<double> {
   using Key = unsigned long long;
   static __device__ __forceinline__ double exp_(double x) { return exp(x); }
+  // An unsigned integer that orders as x does; NaN as -inf; never 0.
   static __device__ __forceinline__ Key key(double x) {
     if (x != x) x = -INFINITY;
     const Key b = (Key)__double_as_longlong(x + 0.0);
     return (b >> 63) ? ~b : b | (1ull << 63);
-  }
-  static __device__ __forceinline__ double value(Key k) {
-    return __longlong_as_double((long long)((k >> 63) ? k & ~(1ull << 63) : ~k));
   }
 };
 
@@ -86,7 +84,7 @@ __device__ __forceinline__ V lanes_sum(V v) {
   return v;
 }
 
-// A lane's NPL logits from `at` on; those from n on are -inf.
+// A lane's n of NPL logits from `at` on; the others are -inf.
 template <typename T, int NPL>
 __device__ __forceinline__ void load_logits(const T* row, uint32_t at, uint32_t n, bool vec, bool live,
                                             float (&x)[NPL]) {
@@ -95,25 +93,25 @@ __device__ __forceinline__ void load_logits(const T* row, uint32_t at, uint32_t 
 #pragma unroll
     for (int k = 0; k < NPL; k += W) {
       Pack<T, W> q;
-      const bool in = live && at + k < n;
-      if (in) q = load_pack<T, W>(row + at + k);
+      const bool in = live && k < (int)n;
+      if (in) q = load_pack<T, W, false>(row + at + k);
 #pragma unroll
       for (int i = 0; i < W; ++i) x[k + i] = in ? to_f(q.v[i]) : -INFINITY;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) x[i] = live && at + i < n ? to_f(row[at + i]) : -INFINITY;
+    for (int i = 0; i < NPL; ++i) x[i] = live && i < (int)n ? to_f(row[at + i]) : -INFINITY;
   }
 }
 
-// Scores of a lane's experts in R; a row without a finite maximum below NaN
-// has scores 0 (nothing is left by its mask).
+// Scores of a lane's n of NPL experts in R; a row of -inf has softmax scores 0
+// (nothing is left by its mask).  NaN stays: one makes the whole row's scores NaN.
 template <typename R, int NPL, int LPT>
-__device__ __forceinline__ void score(const float (&x)[NPL], uint32_t at, uint32_t n, bool sigmoid, R (&s)[NPL],
-                                      float* top, R* total) {
+__device__ __forceinline__ void score(const float (&x)[NPL], uint32_t n, bool sigmoid, R (&s)[NPL],
+                                      float* top = nullptr, R* total = nullptr) {
   if (sigmoid) {
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) s[i] = at + i < n ? R(1) / (R(1) + Num<R>::exp_(-(R)x[i])) : R(0);
+    for (int i = 0; i < NPL; ++i) s[i] = i < (int)n ? R(1) / (R(1) + Num<R>::exp_(-(R)x[i])) : R(0);
     return;
   }
   float m = -INFINITY;
@@ -123,7 +121,6 @@ __device__ __forceinline__ void score(const float (&x)[NPL], uint32_t at, uint32
   R sum = 0;
 #pragma unroll
   for (int i = 0; i < NPL; ++i) {
-    // NaN stays: one makes the whole row's scores NaN
     s[i] = (m == -INFINITY && x[i] == -INFINITY) ? R(0) : Num<R>::exp_((R)x[i] - (R)m);
     sum += s[i];
   }
@@ -131,155 +128,146 @@ __device__ __forceinline__ void score(const float (&x)[NPL], uint32_t at, uint32
   const R inv = sum == R(0) ? R(0) : R(1) / sum;
 #pragma unroll
   for (int i = 0; i < NPL; ++i) s[i] *= inv;
-  *top = m;
-  *total = sum;
+  if (top) *top = m;
+  if (total) *total = sum;
+}
+
+// The 16 bits of a value that came from T, -0 as 0.
+template <typename T>
+__device__ __forceinline__ uint32_t half_bits(float x) {
+  x += 0.f;
+  if constexpr (std::is_same_v<T, __half>) return __half_as_ushort(__float2half_rn(x));
+  else return __float_as_uint(x) >> 16;
 }
 
 template <int LPT> constexpr uint32_t kLanes = LPT == 32 ? ~0u : (1u << (LPT & 31)) - 1;
 
-struct Chosen {
-  float score;
-  uint32_t expert;
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2e = 1.44269504088896341f;
+
+template <int LPT>
+__device__ __forceinline__ uint32_t lanes_max_u32(uint32_t v) {
+  if constexpr (LPT == 32) return __reduce_max_sync(~0u, v);
+  else return lanes_max<LPT>(v);
+}
+
+// Where a lane's experts are.
+struct Seat {
+  uint32_t lane, base;  // in the token; of the token in the warp
+  uint32_t group, first_lane;  // the lane's group, and that group's first lane in the token
+  uint32_t at, n;       // first expert and how many of the lane's NPL
 };
 
-// One token's selection in R.  Returns whether 32-bit keys leave the order in
-// doubt (always false in 64 bits).
-template <typename R, int NPL, int LPT>
-__device__ __forceinline__ bool select(const RouteArgs& a, const float (&x)[NPL], const float (&bias)[NPL],
-                                       uint32_t lane, uint32_t base_lane, R (&s)[NPL], double* worth,
-                                       Chosen* chosen) {
-  using Key = typename Num<R>::Key;
-  constexpr bool kWide = sizeof(R) == 8;
-  const uint32_t at = lane * NPL;
-  float m = 0.f;
-  R total = 0;
-  score<R, NPL, LPT>(x, at, a.n, a.sigmoid, s, &m, &total);
+// The expert of slot lane * NPL + i.
+template <int NPL>
+__device__ __forceinline__ uint32_t expert_of(const RouteArgs& a, uint32_t slot) {
+  const uint32_t lane = slot / NPL, g = a.lanes.div(lane);
+  return g * a.seat_per_group + (lane - g * a.lanes.d) * NPL + slot % NPL;
+}
+
+// One token's selection in 64 bits: chosen[r] is the slot of rank r.
+template <int NPL, int LPT>
+__device__ __noinline__ void select_exact(const RouteArgs& a, const float (&x)[NPL], const float (&bias)[NPL],
+                                          const Seat seat, bool keyed, double* worth, uint16_t* chosen) {
+  using Key = Num<double>::Key;
+  double s[NPL];
+  score<double, NPL, LPT>(x, seat.n, a.sigmoid, s);
   Key key[NPL];
-  const bool keyed = a.bias != nullptr;
 #pragma unroll
   for (int i = 0; i < NPL; ++i)
-    key[i] = at + i < a.n ? Num<R>::key(keyed ? s[i] + (R)bias[i] : (R)x[i]) : Key(0);
-  bool doubt = false;
-
+    key[i] = i < (int)seat.n ? Num<double>::key(keyed ? s[i] + (double)bias[i] : (double)x[i]) : Key(0);
   if (a.groups > 1) {
-    // with the sum of two the scores themselves count, not the logits
+    // what counts for a group: the keys, or the scores where two of them add up
+    double v[NPL];
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+      v[i] = keyed ? s[i] + (double)bias[i] : a.top2 ? s[i] : (double)x[i];
+      if (!(v[i] >= -INFINITY)) v[i] = -INFINITY;  // NaN
+    }
     for (uint32_t g = 0; g < a.groups; ++g) {
-      const uint32_t lo = g * a.per_group.d, hi = lo + a.per_group.d;
-      Key k1 = 0;
-      uint32_t first = ~0u;
+      const uint32_t lo = g * a.per_group, hi = lo + a.per_group;
+      double w1 = -INFINITY, w2 = -INFINITY;
 #pragma unroll
       for (int i = 0; i < NPL; ++i)
-        if (at + i >= lo && at + i < hi && key[i] > k1) {
-          k1 = key[i];
-          first = i;
+        if (i < (int)seat.n && seat.at + i >= lo && seat.at + i < hi) {
+          w2 = fmax(w2, fmin(w1, v[i]));
+          w1 = fmax(w1, v[i]);
         }
-      const Key best = lanes_max<LPT>(k1);
-      R v = keyed || !a.top2 ? Num<R>::value(best) : R(0);
-      if (a.top2) {
-        const uint32_t has = __ballot_sync(~0u, k1 == best && first != ~0u) >> base_lane;
-        const uint32_t owner = __ffs(has & kLanes<LPT>) - 1;
-        Key k2 = 0;
-        R s1 = 0, s2 = 0;
 #pragma unroll
-        for (int i = 0; i < NPL; ++i)
-          if (at + i >= lo && at + i < hi) {
-            if (lane == owner && i == (int)first) s1 = s[i];
-            else if (key[i] > k2) {
-              k2 = key[i];
-              s2 = s[i];
-            }
-          }
-        const Key second = lanes_max<LPT>(k2);
-        if (keyed) {
-          v += second ? Num<R>::value(second) : R(0);
-        } else {
-          // the scores of the two (equal keys have equal scores)
-          s2 = second && k2 == second ? s2 : R(0);
-          v = lanes_max<LPT>(s1) + lanes_max<LPT>(s2);
-        }
+      for (int d = LPT / 2; d; d >>= 1) {
+        const double o1 = __shfl_xor_sync(~0u, w1, d), o2 = __shfl_xor_sync(~0u, w2, d);
+        w2 = fmax(fmin(w1, o1), fmax(w2, o2));
+        w1 = fmax(w1, o1);
       }
-      if (lane == 0) worth[g] = (double)v;
+      if (seat.lane == 0) worth[g] = a.top2 && a.per_group > 1 ? w1 + w2 : w1;
     }
     __syncwarp();
     // a group stays open where fewer than top_groups are better, or as good and before it
-    double in = INFINITY, out = -INFINITY;  // the worst open one and the best closed one
     unsigned long long open = 0;
-    for (uint32_t g = lane; g < a.groups; g += LPT) {
-      const auto mine = Num<double>::key(worth[g]);
+    for (uint32_t g = seat.lane; g < a.groups; g += LPT) {
+      const Key mine = Num<double>::key(worth[g]);
       uint32_t before = 0;
       for (uint32_t h = 0; h < a.groups; ++h) {
-        const auto other = Num<double>::key(worth[h]);
+        const Key other = Num<double>::key(worth[h]);
         before += other > mine || (other == mine && h < g);
       }
-      if (before < a.top_groups) {
-        open |= 1ull << g;
-        in = fmin(in, worth[g]);
-      } else {
-        out = fmax(out, worth[g]);
-      }
+      if (before < a.top_groups) open |= 1ull << g;
     }
 #pragma unroll
     for (int d = LPT / 2; d; d >>= 1) open |= __shfl_xor_sync(~0u, open, d);
-    if (!kWide && (keyed || a.top2)) {
-      in = -lanes_max<LPT>(-in);
-      out = lanes_max<LPT>(out);
-      // each worth is off by at most 20 * 2^-24 of its scores (at most 2) and 2 * 2^-24 of itself
-      if (!(in - out > 5e-6 + 5e-7 * fabs(in))) doubt = true;
-    }
 #pragma unroll
     for (int i = 0; i < NPL; ++i)
-      if (!((open >> a.per_group.div(at + i)) & 1)) key[i] = 0;
-    __syncwarp();
+      if (i < (int)seat.n && !((open >> ((seat.at + i) / a.per_group)) & 1)) key[i] = 0;
   }
-
   Key mine = 0;
 #pragma unroll
   for (int i = 0; i < NPL; ++i) mine = key[i] > mine ? key[i] : mine;
-  float before_key = INFINITY, before_s = 0.f, before_x = 0.f, before_b = 0.f;
-  const bool check = !kWide && keyed;
-  for (uint32_t r = 0; r <= a.top_k; ++r) {
-    if (r == a.top_k && !check) break;
+  for (uint32_t r = 0; r < a.top_k; ++r) {
     const Key best = lanes_max<LPT>(mine);
-    const uint32_t has = __ballot_sync(~0u, mine == best) >> base_lane;
-    const uint32_t owner = __ffs(has & kLanes<LPT>) - 1;
-    float sc = 0.f, xx = 0.f, bb = 0.f;
-    uint32_t e = 0;
-    if (lane == owner) {
+    const uint32_t has = __ballot_sync(~0u, mine == best) >> seat.base;
+    if (seat.lane == (uint32_t)(__ffs(has & kLanes<LPT>) - 1)) {
       bool found = false;
       Key next = 0;
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
         if (!found && key[i] == best) {
           found = true;
-          sc = (float)s[i];
-          xx = x[i];
-          bb = bias[i];
-          e = at + i;
+          chosen[r] = (uint16_t)(seat.lane * NPL + i);
           key[i] = 0;
         }
         next = key[i] > next ? key[i] : next;
       }
       mine = next;
-      if (r < a.top_k) chosen[r] = Chosen{sc, e};
-    }
-    if (check) {
-      const uint32_t from = base_lane + owner;
-      sc = __shfl_sync(~0u, sc, from);
-      xx = __shfl_sync(~0u, xx, from);
-      bb = __shfl_sync(~0u, bb, from);
-      const float k = Num<float>::value((uint32_t)best);
-      // each key is off by at most 10 * 2^-24 of its score and 2^-24 of itself; equal inputs tie exactly
-      if (best != 0 && r > 0 && !(before_key - k > 1.25e-6f * fmaxf(sc, before_s) + 2.5e-7f * fabsf(k)) &&
-          !(xx == before_x && bb == before_b))
-        doubt = true;
-      before_key = k;
-      before_s = sc;
-      before_x = xx;
-      before_b = bb;
     }
   }
   __syncwarp();
-  return doubt;
+}
+
+// Sorts a lane's keys, the largest first (compare-exchanges of Batcher's merge).
+template <int N>
+__device__ __forceinline__ void sort_down(uint32_t (&k)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+      for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const uint32_t hi = max(k[i + j], k[i + j + q]), lo = min(k[i + j], k[i + j + q]);
+            k[i + j] = hi;
+            k[i + j + q] = lo;
+          }
 }
 
 template <typename T, int NPL, int LPT>
@@ -287,43 +275,225 @@ __global__ void __launch_bounds__(kThreads)
 gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   constexpr uint32_t kTokens = kThreads / LPT;  // tokens a CTA handles at once
-  const uint32_t sub = threadIdx.x / LPT, lane = threadIdx.x % LPT, base_lane = (threadIdx.x & 31) - lane;
+  constexpr uint32_t kSlots = LPT * NPL;
+  constexpr int kBits = kSlots <= 256 ? 24 : 22;  // of a key, above the slot's
+  constexpr bool kHalf = sizeof(T) == 2;
+  const uint32_t sub = threadIdx.x / LPT;
   double* worth = reinterpret_cast<double*>(smem) + sub * (a.groups > 1 ? a.groups : 0);
-  Chosen* chosen = reinterpret_cast<Chosen*>(reinterpret_cast<double*>(smem) +
-                                             kTokens * (a.groups > 1 ? a.groups : 0)) + sub * a.top_k;
-  const uint32_t at = lane * NPL;
+  uint16_t* chosen = reinterpret_cast<uint16_t*>(reinterpret_cast<double*>(smem) +
+                                                 kTokens * (a.groups > 1 ? a.groups : 0)) + sub * a.top_k;
+  Seat seat;
+  seat.lane = threadIdx.x % LPT;
+  seat.base = (threadIdx.x & 31) - seat.lane;
+  seat.group = a.lanes.div(seat.lane);
+  seat.first_lane = seat.group * a.lanes.d;
+  const uint32_t in_group = (seat.lane - seat.first_lane) * NPL;
+  seat.at = seat.group * a.seat_per_group + in_group;
+  seat.n = seat.group < a.seat_groups && in_group < a.seat_per_group
+               ? min((uint32_t)NPL, a.seat_per_group - in_group) : 0;
   float bias[NPL];
+  bool keyed = a.bias != nullptr;
+  if (keyed) {
+    // a bias that is the same for all does not change the order
+    const float b0 = __ldg(a.bias);
+    bool same = b0 - b0 == 0.f;
 #pragma unroll
-  for (int i = 0; i < NPL; ++i) bias[i] = a.bias && at + i < a.n ? __ldg(a.bias + (at + i) * a.bs) : 0.f;
+    for (int i = 0; i < NPL; ++i) {
+      bias[i] = i < (int)seat.n ? __ldg(a.bias + (seat.at + i) * a.bs) : b0;
+      same = same && bias[i] == b0;
+    }
+    keyed = !__syncthreads_and(same);
+  }
+
   for (int64_t t0 = (int64_t)blockIdx.x * kTokens; t0 < a.tokens; t0 += (int64_t)gridDim.x * kTokens) {
     const int64_t t = t0 + sub;
     const bool live = t < a.tokens;
+    const T* row = static_cast<const T*>(a.x) + (live ? t * a.xs : 0);
     float x[NPL];
-    load_logits<T, NPL>(static_cast<const T*>(a.x) + (live ? t * a.xs : 0), at, a.n, a.vec, live, x);
-    bool doubt;
-    {
-      float s[NPL];
-      doubt = select<float, NPL, LPT>(a, x, bias, lane, base_lane, s, worth, chosen);
-    }
-    if (__any_sync(~0u, doubt)) {
-      double s[NPL];
-      select<double, NPL, LPT>(a, x, bias, lane, base_lane, s, worth, chosen);
-    }
-    float total = 1.f;
-    if (a.renorm) {
+    load_logits<T, NPL>(row, seat.at, seat.n, a.vec, live, x);
+    // scores, as far as the order or the weights need all of them
+    float s[NPL], m = 0.f, total = 1.f;
+    const bool scored = keyed || (a.groups > 1 && a.top2);
+    if (!a.sigmoid) {
+      m = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) m = fmaxf(m, x[i]);
+      m = lanes_max<LPT>(m);
       total = 0.f;
-      for (uint32_t r = 0; r < a.top_k; ++r) total += chosen[r].score;
-    }
-    const float by = total == 0.f ? 0.f : a.scale / total;
-    if (live)
-      for (uint32_t r = lane; r < a.top_k; r += LPT) {
-        a.weights[t * a.ws + r * a.wk] = a.renorm ? chosen[r].score * by : chosen[r].score * a.scale;
-        if (a.wide) static_cast<int64_t*>(a.experts)[t * a.es + r * a.ek] = chosen[r].expert;
-        else static_cast<int32_t*>(a.experts)[t * a.es + r * a.ek] = (int32_t)chosen[r].expert;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) {
+        s[i] = m == -INFINITY && x[i] == -INFINITY ? 0.f : ex2((x[i] - m) * kLog2e);
+        total += s[i];
       }
+      total = lanes_sum<LPT>(total);
+      const float by = total == 0.f ? 0.f : rcp(total);
+      if (scored) {
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) s[i] *= by;
+      }
+    } else if (scored) {
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) s[i] = rcp(1.f + ex2(x[i] * -kLog2e));
+    }
+    // A score is off by at most 10 * 2^-24 of the largest one (1 for a sigmoid), a
+    // key by 2^-24 of itself more; two of them by twice that.
+    const float s_max = a.sigmoid ? 1.f : rcp(total);
+    bool doubt = a.top_k > LPT || a.groups != a.seat_groups;
+    bool open = seat.n > 0;
+    if (a.groups > 1 && a.groups == a.seat_groups) {
+      float v1 = -INFINITY, v2 = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i)
+        if (i < (int)seat.n) {
+          const float v = keyed ? s[i] + bias[i] : a.top2 ? s[i] : x[i];
+          if (v != v) doubt = true;
+          v2 = fmaxf(v2, fminf(v1, v));
+          v1 = fmaxf(v1, v);
+        }
+      float w1 = v1, w2 = v2;
+      for (uint32_t i = 1; i < a.lanes.d; ++i) {
+        uint32_t from = seat.lane + i;
+        if (from >= seat.first_lane + a.lanes.d) from -= a.lanes.d;
+        const float o1 = __shfl_sync(~0u, v1, seat.base + from), o2 = __shfl_sync(~0u, v2, seat.base + from);
+        w2 = fmaxf(fminf(w1, o1), fmaxf(w2, o2));
+        w1 = fmaxf(w1, o1);
+      }
+      const bool two = a.top2 && a.per_group > 1;
+      const float w = two ? w1 + w2 : w1;
+      // two keys: twice the error; without scores the largest logits are exact
+      const float error = keyed || a.top2 ? (two ? 2.f : 1.f) * 1.25e-6f * s_max + 5e-7f * fabsf(w) : 0.f;
+      uint32_t before = 0, maybe = 0;
+      for (uint32_t h = 0; h < a.groups; ++h) {
+        const float o = __shfl_sync(~0u, w, seat.base + h * a.lanes.d);
+        before += o > w || (o == w && h < seat.group);
+        // Another group within the error: its order is in doubt.  A NaN or two infinities too.
+        maybe += h != seat.group && error > 0.f && !(fabsf(o - w) > error);
+      }
+      open = open && before < a.top_groups;
+      // it matters where it could open this group or close it
+      if (seat.n && maybe && before < a.top_groups + maybe && before + maybe >= a.top_groups) doubt = true;
+    }
+
+    uint32_t key[NPL];
+    bool exact = false;
+    uint32_t slack = 0;  // keys this close are in doubt
+    if (kHalf && !keyed) {
+      exact = true;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) {
+        const uint32_t b = half_bits<T>(x[i]);
+        key[i] = (((b & 0x8000u) ? ~b & 0xffffu : b | 0x8000u) << 16) | (kSlots - 1 - (seat.lane * NPL + i));
+        if (x[i] != x[i]) doubt = true;
+      }
+    } else {
+      // the range from the largest key down to one that top_k + 1 others reach
+      float k[NPL], hi = -INFINITY, lo = INFINITY;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) {
+        k[i] = keyed ? s[i] + bias[i] : x[i];
+        if (i < (int)seat.n) {
+          hi = fmaxf(hi, k[i]);
+          lo = fminf(lo, k[i]);
+        }
+      }
+      const uint32_t lanes = __popc(__ballot_sync(~0u, open) >> seat.base & kLanes<LPT>);
+      const float top = lanes_max<LPT>(open ? hi : -INFINITY);
+      lo = -lanes_max<LPT>(open ? -(a.top_k < lanes ? hi : lo) : -INFINITY);
+      lo = fmaxf(lo, top - 64.f);
+      const float range = fmaxf(top - lo, 1e-30f);
+      const float by = (float)((1 << kBits) - 64) / range;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) {
+        const uint32_t f = (uint32_t)fminf(fmaxf(fmaf(k[i] - lo, by, 16.f), 1.f), (float)((1 << kBits) - 1));
+        key[i] = f << (32 - kBits) | (kSlots - 1 - (seat.lane * NPL + i));
+      }
+      // Rounding to places keeps the order of exact keys, or makes them equal; for the others
+      // their error counts, and the roundings of the difference, below 4 places.
+      if (keyed) {
+        const float error = 1.25e-6f * s_max + 2.5e-7f * fmaxf(fabsf(top), fabsf(lo));
+        slack = 4 + (uint32_t)fminf(error * by, 4e9f);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NPL; ++i)
+      if (!open || i >= (int)seat.n) key[i] = 0;
+
+    uint32_t won = 0;  // of rank `lane`
+    if (NPL <= 8) {
+      sort_down<NPL>(key);
+    } else {
+#pragma unroll
+      for (int i = 1; i < NPL; ++i) {  // the largest first
+        const uint32_t hi = max(key[0], key[i]);
+        key[i] = min(key[0], key[i]);
+        key[0] = hi;
+      }
+    }
+    uint32_t last = ~0u;
+    for (uint32_t r = 0; r < a.top_k + (exact ? 0 : 1); ++r) {
+      const uint32_t best = lanes_max_u32<LPT>(key[0]);
+      if (!exact) {
+        const uint32_t f = best >> (32 - kBits);
+        if (best != 0 && (last - f <= slack || (r < a.top_k && f < 8))) doubt = true;
+        last = f;
+      }
+      if (seat.lane == r) won = best;
+      if (key[0] == best) {
+        if (NPL <= 8) {
+#pragma unroll
+          for (int i = 0; i + 1 < NPL; ++i) key[i] = key[i + 1];
+          key[NPL - 1] = 0;
+        } else {
+          key[0] = 0;
+#pragma unroll
+          for (int i = 1; i < NPL; ++i) {
+            const uint32_t hi = max(key[0], key[i]);
+            key[i] = min(key[0], key[i]);
+            key[0] = hi;
+          }
+        }
+      }
+    }
+    const bool redo = __any_sync(~0u, doubt && live);
+    if (redo) select_exact<NPL, LPT>(a, x, bias, seat, keyed, worth, chosen);
+
+    // weights from the chosen logits, a lane each
+    float sum = 0.f;
+    for (uint32_t r = seat.lane; r < a.top_k; r += LPT) {
+      const uint32_t slot = redo ? chosen[r] : kSlots - 1 - (won & ((1u << (exact ? 16 : 32 - kBits)) - 1));
+      const uint32_t e = expert_of<NPL>(a, slot);
+      const float v = live ? to_f(row[e]) : 0.f;
+      float sc;
+      if (a.sigmoid) sc = 1.f / (1.f + expf(-v));
+      else sc = total == 0.f ? 0.f : expf(v - m) / total;
+      sum += sc;
+      if (live) {
+        if (!a.renorm) a.weights[t * a.ws + r * a.wk] = sc * a.scale;
+        if (a.wide) static_cast<int64_t*>(a.experts)[t * a.es + r * a.ek] = e;
+        else static_cast<int32_t*>(a.experts)[t * a.es + r * a.ek] = (int32_t)e;
+      }
+      won = __float_as_uint(sc);  // the only one of a lane where it is needed below
+    }
+    if (a.renorm) {
+      sum = lanes_sum<LPT>(sum);
+      const float by = sum == 0.f ? 0.f : a.scale / sum;
+      for (uint32_t r = seat.lane; r < a.top_k; r += LPT) {
+        float sc = __uint_as_float(won);
+        if (a.top_k > LPT) {  // several ranks a lane: again
+          const float v = live ? to_f(row[expert_of<NPL>(a, chosen[r])]) : 0.f;
+          sc = a.sigmoid ? 1.f / (1.f + expf(-v)) : total == 0.f ? 0.f : expf(v - m) / total;
+        }
+        if (live) a.weights[t * a.ws + r * a.wk] = sc * by;
+      }
+    }
     __syncwarp();
   }
 }
+
+struct Chosen {
+  float score;
+  uint32_t expert;
+};
 
 // The gradient of the weights through the chosen scores:
 //   renormalised, S the sum of the chosen:  ds_j = scale (g_j - sum_i g_i s_i / S) / S,  else scale g_j
@@ -343,9 +513,9 @@ gpuos_route_grad_kernel(const __grid_constant__ RouteArgs a) {
     const bool live = t < a.tokens;
     const T* row = static_cast<const T*>(a.x) + (live ? t * a.xs : 0);
     float x[NPL], s[NPL];
-    load_logits<T, NPL>(row, at, a.n, a.vec, live, x);
+    load_logits<T, NPL>(row, at, at < a.n ? min((uint32_t)NPL, a.n - at) : 0u, a.vec, live, x);
     float m = 0.f, total = 1.f;
-    score<float, NPL, LPT>(x, at, a.n, a.sigmoid, s, &m, &total);
+    score<float, NPL, LPT>(x, at < a.n ? min((uint32_t)NPL, a.n - at) : 0u, a.sigmoid, s, &m, &total);
     // the chosen ones' scores and gradients, a lane each
     float sum = 0.f, dot = 0.f;
     for (uint32_t r = lane; r < a.top_k; r += LPT) {
@@ -411,10 +581,17 @@ gpuos_route_grad_kernel(const __grid_constant__ RouteArgs a) {
 }
 
 template <typename T, int NPL, int LPT>
-void launch(const RouteArgs& a, bool grad, cudaStream_t s) {
+void launch(RouteArgs a, bool grad, cudaStream_t s) {
   constexpr uint32_t kTokens = kThreads / LPT;
   const uint64_t ctas = ((uint64_t)a.tokens + kTokens - 1) / kTokens;
   const unsigned grid = (unsigned)std::min<uint64_t>(ctas, (uint64_t)sm_count() * 8);
+  a.seat_groups = a.groups;
+  a.seat_per_group = a.per_group;
+  if (a.groups * ((a.per_group + NPL - 1) / NPL) > LPT) {
+    a.seat_groups = 1;
+    a.seat_per_group = a.n;
+  }
+  a.lanes = FastDiv((a.seat_per_group + NPL - 1) / NPL);
   if (grad) {
     const size_t smem = kThreads * NPL * sizeof(float) + kTokens * a.top_k * sizeof(Chosen);
     if (smem > 48 * 1024)
@@ -422,22 +599,23 @@ void launch(const RouteArgs& a, bool grad, cudaStream_t s) {
                                    cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory");
     gpuos_route_grad_kernel<T, NPL, LPT><<<grid, kThreads, smem, s>>>(a);
   } else {
-    const size_t smem = kTokens * ((a.groups > 1 ? a.groups : 0) * sizeof(double) + a.top_k * sizeof(Chosen));
-    if (smem > 48 * 1024)
-      cuda_ok(cudaFuncSetAttribute(gpuos_route_kernel<T, NPL, LPT>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory");
+    const size_t smem = kTokens * ((a.groups > 1 ? a.groups : 0) * sizeof(double) + a.top_k * sizeof(uint16_t));
     gpuos_route_kernel<T, NPL, LPT><<<grid, kThreads, smem, s>>>(a);
   }
   cuda_ok(cudaGetLastError(), "launch");
 }
 
+// Lanes a token needs with NPL experts a lane, none of two groups.
+uint32_t lanes_for(const RouteArgs& a, uint32_t npl) { return a.groups * ((a.per_group + npl - 1) / npl); }
+
 template <typename T>
 void by_size(const RouteArgs& a, bool grad, cudaStream_t s) {
-  if (a.n <= 32) launch<T, 8, 4>(a, grad, s);
-  else if (a.n <= 64) launch<T, 8, 8>(a, grad, s);
-  else if (a.n <= 128) launch<T, 8, 16>(a, grad, s);
-  else if (a.n <= 256) launch<T, 8, 32>(a, grad, s);
-  else if (a.n <= 512) launch<T, 16, 32>(a, grad, s);
+  const uint32_t lanes = lanes_for(a, 8);
+  if (lanes <= 4) launch<T, 8, 4>(a, grad, s);
+  else if (lanes <= 8) launch<T, 8, 8>(a, grad, s);
+  else if (lanes <= 16) launch<T, 8, 16>(a, grad, s);
+  else if (lanes <= 32) launch<T, 8, 32>(a, grad, s);
+  else if (lanes_for(a, 16) <= 32) launch<T, 16, 32>(a, grad, s);
   else launch<T, 32, 32>(a, grad, s);
 }
 
@@ -481,7 +659,7 @@ RouteArgs prepare(const gpuos_tensor* x, const gpuos_tensor* weights, const char
   a.renorm = renorm != 0;
   a.wide = experts->dtype == GPUOS_I64;
   a.groups = a.top_groups = 1;
-  a.per_group = FastDiv((uint32_t)n);
+  a.per_group = (uint32_t)n;
   const int w = 16 / esize(x->dtype);
   a.vec = n % w == 0 && rows_aligned(*x, w);
   return a;
@@ -500,7 +678,7 @@ void route(const gpuos_tensor* x, const gpuos_tensor* bias, const gpuos_tensor* 
   a.wk = weights->strides[1];
   a.groups = (uint32_t)groups;
   a.top_groups = (uint32_t)top_groups;
-  a.per_group = FastDiv(a.n / groups);
+  a.per_group = a.n / groups;
   a.top2 = group_score == GPUOS_GROUP_TOP2;
   if (bias) {
     check_tensor(bias, 1, "bias");
@@ -510,7 +688,11 @@ void route(const gpuos_tensor* x, const gpuos_tensor* bias, const gpuos_tensor* 
     no_overlap(*weights, *bias, "weights overlap bias");
     no_overlap(*experts, *bias, "experts overlap bias");
   }
-  if (groups == top_groups) a.groups = 1;  // every group is open
+  if (groups == top_groups) {  // every group is open
+    a.groups = 1;
+    a.per_group = a.n;
+  }
+  a.vec = a.vec && a.per_group % (16 / esize(x->dtype)) == 0;
   check_output(*weights, "weights");
   check_output(*experts, "experts");
   no_overlap(*weights, *experts, "weights overlap experts");
