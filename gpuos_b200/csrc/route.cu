@@ -13,8 +13,10 @@
 // expert at once and of equal keys the lowest index.  16-bit logits without a
 // bias fit whole; other keys are computed in 32 bits, with a known error bound, and rounded
 // to 22 to 24 bits of the range that the largest ones span.  Where two keys whose
-// order matters come out closer than the error, the token is done again in 64 bits
-// (about one in a thousand of random logits).
+// order matters come out closer than the error, about one token in two thousand of random
+// logits, its lanes do it again in 64 bits.  What that does not settle (keys
+// within 2^-38, NaN, more ranks than lanes, groups that fit no seats) is left for the
+// CTA's second part, a warp to a token.
 //
 // A token belongs to LPT lanes of a warp, each holding NPL neighbouring experts
 // of one group in registers: up to 256 experts take 8 a lane and as many lanes as
@@ -30,6 +32,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTop = 64;
+constexpr uint32_t kCtaTokens = 1024;  // a CTA takes at most
 constexpr int kMaxGroups = 64;
 
 struct RouteArgs {
@@ -48,33 +51,58 @@ struct RouteArgs {
   // the groups are too many for the lanes of a warp, all in a row.
   uint32_t seat_groups, seat_per_group;
   FastDiv lanes;       // lanes of a group
+  uint32_t exact_warps;  // of a CTA, that do tokens in doubt
   float scale;
   int sigmoid, renorm, top2, wide, vec;
 };
 
-template <typename R> struct Num;
-template <> struct Num<float> {
-  static __device__ __forceinline__ float exp_(float x) { return expf(x); }
-};
-template <> struct Num<double> {
-  using Key = unsigned long long;
-  static __device__ __forceinline__ double exp_(double x) { return exp(x); }
-  // An unsigned integer that orders as x does; NaN as -inf; never 0.
-  static __device__ __forceinline__ Key key(double x) {
-    if (x != x) x = -INFINITY;
-    const Key b = (Key)__double_as_longlong(x + 0.0);
-    return (b >> 63) ? ~b : b | (1ull << 63);
-  }
-};
+using Key64 = unsigned long long;
 
-template <int LPT, typename V>
-__device__ __forceinline__ V lanes_max(V v) {
+// An unsigned integer that orders as x does; NaN as -inf; never 0.
+__device__ __forceinline__ Key64 key64(double x) {
+  if (x != x) x = -INFINITY;
+  const Key64 b = (Key64)__double_as_longlong(x + 0.0);
+  return (b >> 63) ? ~b : b | (1ull << 63);
+}
+
+// Maxima over a token's lanes; over a whole warp in one instruction.
+template <int LPT>
+__device__ __forceinline__ uint32_t lanes_top(uint32_t v) {
+  if constexpr (LPT == 32) {
+    return __reduce_max_sync(~0u, v);
+  } else {
 #pragma unroll
-  for (int d = LPT / 2; d; d >>= 1) {
-    const V o = __shfl_xor_sync(~0u, v, d);
-    v = o > v ? o : v;
+    for (int d = LPT / 2; d; d >>= 1) v = max(v, __shfl_xor_sync(~0u, v, d));
+    return v;
   }
-  return v;
+}
+template <int LPT>
+__device__ __forceinline__ Key64 lanes_top(Key64 v) {
+  if constexpr (LPT == 32) {
+    const uint32_t hi = __reduce_max_sync(~0u, (uint32_t)(v >> 32));
+    const uint32_t lo = __reduce_max_sync(~0u, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+    return (Key64)hi << 32 | lo;
+  } else {
+#pragma unroll
+    for (int d = LPT / 2; d; d >>= 1) v = max(v, __shfl_xor_sync(~0u, v, d));
+    return v;
+  }
+}
+template <int LPT>
+__device__ __forceinline__ float lanes_top(float v) {
+  if constexpr (LPT == 32) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+  } else {
+#pragma unroll
+    for (int d = LPT / 2; d; d >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, d));
+    return v;
+  }
+}
+
+__device__ __forceinline__ double value64(Key64 k) {
+  return __longlong_as_double((long long)((k >> 63) ? k & ~(1ull << 63) : ~k));
 }
 
 template <int LPT, typename V>
@@ -104,34 +132,6 @@ __device__ __forceinline__ void load_logits(const T* row, uint32_t at, uint32_t 
   }
 }
 
-// Scores of a lane's n of NPL experts in R; a row of -inf has softmax scores 0
-// (nothing is left by its mask).  NaN stays: one makes the whole row's scores NaN.
-template <typename R, int NPL, int LPT>
-__device__ __forceinline__ void score(const float (&x)[NPL], uint32_t n, bool sigmoid, R (&s)[NPL],
-                                      float* top = nullptr, R* total = nullptr) {
-  if (sigmoid) {
-#pragma unroll
-    for (int i = 0; i < NPL; ++i) s[i] = i < (int)n ? R(1) / (R(1) + Num<R>::exp_(-(R)x[i])) : R(0);
-    return;
-  }
-  float m = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < NPL; ++i) m = fmaxf(m, x[i]);
-  m = lanes_max<LPT>(m);
-  R sum = 0;
-#pragma unroll
-  for (int i = 0; i < NPL; ++i) {
-    s[i] = (m == -INFINITY && x[i] == -INFINITY) ? R(0) : Num<R>::exp_((R)x[i] - (R)m);
-    sum += s[i];
-  }
-  sum = lanes_sum<LPT>(sum);
-  const R inv = sum == R(0) ? R(0) : R(1) / sum;
-#pragma unroll
-  for (int i = 0; i < NPL; ++i) s[i] *= inv;
-  if (top) *top = m;
-  if (total) *total = sum;
-}
-
 // The 16 bits of a value that came from T, -0 as 0.
 template <typename T>
 __device__ __forceinline__ uint32_t half_bits(float x) {
@@ -154,12 +154,6 @@ __device__ __forceinline__ float rcp(float x) {
 }
 constexpr float kLog2e = 1.44269504088896341f;
 
-template <int LPT>
-__device__ __forceinline__ uint32_t lanes_max_u32(uint32_t v) {
-  if constexpr (LPT == 32) return __reduce_max_sync(~0u, v);
-  else return lanes_max<LPT>(v);
-}
-
 // Where a lane's experts are.
 struct Seat {
   uint32_t lane, base;  // in the token; of the token in the warp
@@ -174,82 +168,235 @@ __device__ __forceinline__ uint32_t expert_of(const RouteArgs& a, uint32_t slot)
   return g * a.seat_per_group + (lane - g * a.lanes.d) * NPL + slot % NPL;
 }
 
-// One token's selection in 64 bits: chosen[r] is the slot of rank r.
-template <int NPL, int LPT>
-__device__ __noinline__ void select_exact(const RouteArgs& a, const float (&x)[NPL], const float (&bias)[NPL],
-                                          const Seat seat, bool keyed, double* worth, uint16_t* chosen) {
-  using Key = Num<double>::Key;
-  double s[NPL];
-  score<double, NPL, LPT>(x, seat.n, a.sigmoid, s);
-  Key key[NPL];
-#pragma unroll
-  for (int i = 0; i < NPL; ++i)
-    key[i] = i < (int)seat.n ? Num<double>::key(keyed ? s[i] + (double)bias[i] : (double)x[i]) : Key(0);
-  if (a.groups > 1) {
-    // what counts for a group: the keys, or the scores where two of them add up
-    double v[NPL];
-#pragma unroll
-    for (int i = 0; i < NPL; ++i) {
-      v[i] = keyed ? s[i] + (double)bias[i] : a.top2 ? s[i] : (double)x[i];
-      if (!(v[i] >= -INFINITY)) v[i] = -INFINITY;  // NaN
+// One token's selection in 64 bits, by a warp: keys are held as ordered integers in
+// `key` (a.n of them, 0 for those of closed groups), the groups' worths in `worth`.
+template <typename T>
+__device__ __forceinline__ void route_exact(const RouteArgs& a, bool keyed, int64_t t, Key64* key, Key64* worth) {
+  const uint32_t lane = threadIdx.x & 31;
+  const T* row = static_cast<const T*>(a.x) + t * a.xs;
+  float m = -INFINITY;
+  double total = 0;
+  if (!a.sigmoid) {
+    for (uint32_t e = lane; e < a.n; e += 32) m = fmaxf(m, to_f(row[e]));
+    m = lanes_top<32>(m);
+#pragma unroll 1
+    for (uint32_t e = lane; e < a.n; e += 32) {
+      const float v = to_f(row[e]);
+      if (v != -INFINITY || m != -INFINITY) total += exp((double)v - (double)m);
     }
-    for (uint32_t g = 0; g < a.groups; ++g) {
-      const uint32_t lo = g * a.per_group, hi = lo + a.per_group;
-      double w1 = -INFINITY, w2 = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < NPL; ++i)
-        if (i < (int)seat.n && seat.at + i >= lo && seat.at + i < hi) {
-          w2 = fmax(w2, fmin(w1, v[i]));
-          w1 = fmax(w1, v[i]);
-        }
-#pragma unroll
-      for (int d = LPT / 2; d; d >>= 1) {
-        const double o1 = __shfl_xor_sync(~0u, w1, d), o2 = __shfl_xor_sync(~0u, w2, d);
-        w2 = fmax(fmin(w1, o1), fmax(w2, o2));
-        w1 = fmax(w1, o1);
+    total = lanes_sum<32>(total);
+  }
+  auto score = [&](float v) {
+    if (a.sigmoid) return 1.0 / (1.0 + exp(-(double)v));
+    return total == 0.0 ? 0.0 : exp((double)v - (double)m) / total;
+  };
+#pragma unroll 1
+  for (uint32_t e = lane; e < a.n; e += 32) {
+    // without a bias the order is the logits', but of two scores that add up
+    const float v = to_f(row[e]);
+    key[e] = key64(keyed ? score(v) + (double)a.bias[e * a.bs] : a.groups > 1 && a.top2 ? score(v) : (double)v);
+  }
+  __syncwarp();
+  if (a.groups > 1) {
+    const bool two = a.top2 && a.per_group > 1;
+#pragma unroll 1
+    for (uint32_t g = lane; g < a.groups; g += 32) {
+      Key64 k1 = 0, k2 = 0;
+#pragma unroll 4
+      for (uint32_t i = 0; i < a.per_group; ++i) {
+        const Key64 k = key[g * a.per_group + i];
+        k2 = max(k2, min(k1, k));
+        k1 = max(k1, k);
       }
-      if (seat.lane == 0) worth[g] = a.top2 && a.per_group > 1 ? w1 + w2 : w1;
+      worth[g] = two ? key64(value64(k1) + value64(k2)) : k1;
     }
     __syncwarp();
-    // a group stays open where fewer than top_groups are better, or as good and before it
     unsigned long long open = 0;
-    for (uint32_t g = seat.lane; g < a.groups; g += LPT) {
-      const Key mine = Num<double>::key(worth[g]);
+#pragma unroll 1
+    for (uint32_t g = lane; g < a.groups; g += 32) {
+      const Key64 w = worth[g];
       uint32_t before = 0;
-      for (uint32_t h = 0; h < a.groups; ++h) {
-        const Key other = Num<double>::key(worth[h]);
-        before += other > mine || (other == mine && h < g);
-      }
+#pragma unroll 4
+      for (uint32_t h = 0; h < a.groups; ++h) before += worth[h] > w || (worth[h] == w && h < g);
       if (before < a.top_groups) open |= 1ull << g;
     }
+    open = (unsigned long long)__reduce_or_sync(~0u, (uint32_t)(open >> 32)) << 32 | __reduce_or_sync(~0u, (uint32_t)open);
+#pragma unroll 1
+    for (uint32_t e = lane; e < a.n; e += 32) {
+      if (!((open >> (e / a.per_group)) & 1)) key[e] = 0;
+      else if (!keyed) key[e] = key64(to_f(row[e]));
+    }
+    __syncwarp();
+  }
+  // rounds: the largest key, of equal ones the lowest index
+  Key64 mine = 0;
+  uint32_t at = 0;
+  auto again = [&] {
+    mine = 0;
+#pragma unroll 8
+    for (uint32_t e = lane; e < a.n; e += 32)
+      if (key[e] > mine) {
+        mine = key[e];
+        at = e;
+      }
+  };
+  again();
+  float sum = 0.f;
+#pragma unroll 1
+  for (uint32_t r = 0; r < a.top_k; ++r) {
+    const Key64 best = lanes_top<32>(mine);
+    const uint32_t e = __reduce_min_sync(~0u, mine == best ? at : ~0u);
+    if (mine == best && at == e) {
+      key[e] = 0;
+      again();
+    }
+    const float s = (float)score(to_f(row[e]));
+    sum += s;
+    if (lane == 0) {
+      a.weights[t * a.ws + r * a.wk] = a.renorm ? s : s * a.scale;
+      if (a.wide) static_cast<int64_t*>(a.experts)[t * a.es + r * a.ek] = e;
+      else static_cast<int32_t*>(a.experts)[t * a.es + r * a.ek] = (int32_t)e;
+    }
+  }
+  if (a.renorm) {
+    const float by = sum == 0.f ? 0.f : a.scale / sum;
+    if (lane == 0)
+#pragma unroll 1
+      for (uint32_t r = 0; r < a.top_k; ++r) a.weights[t * a.ws + r * a.wk] *= by;
+  }
+  __syncwarp();
+}
+
+// 2^y to 2^-41, |y| at most 1000: the exponential series of the fraction, to t^10 (the rest is
+// below 0.35^11 / 11!).
+__device__ __forceinline__ double exp2_series(double y) {
+  y = fmin(fmax(y, -1000.0), 1000.0);
+  const int n = __double2int_rn(y);
+  const double t = (y - (double)n) * 0.69314718055994530942;
+  double p = 1.0 / 3628800.0;
+  p = fma(p, t, 1.0 / 362880.0);
+  p = fma(p, t, 1.0 / 40320.0);
+  p = fma(p, t, 1.0 / 5040.0);
+  p = fma(p, t, 1.0 / 720.0);
+  p = fma(p, t, 1.0 / 120.0);
+  p = fma(p, t, 1.0 / 24.0);
+  p = fma(p, t, 1.0 / 6.0);
+  p = fma(p, t, 0.5);
+  p = fma(p, t, 1.0);
+  p = fma(p, t, 1.0);
+  return __longlong_as_double(__double_as_longlong(p) + ((long long)n << 52));
+}
+
+// 1 / d by one Newton step from 23 bits; 0 where that is below 2^-126.
+__device__ __forceinline__ double inverse(double d) {
+  const double r = (double)rcp((float)d);
+  return r * fma(-d, r, 2.0);
+}
+
+// One token's selection in 64 bits by its own lanes: lane r gets the slot of rank r.
+// Returns whether two keys whose order matters are still too close.
+template <typename T, int NPL, int LPT, bool GROUPED>
+__device__ __forceinline__ bool resolve(const RouteArgs& a, const T* row, bool live, const Seat& seat, bool keyed,
+                                        uint32_t* slot) {
+  constexpr double kClose = 0x1p-38, kLog2eD = 1.44269504088896340736;
+  float x[NPL];
+  load_logits<T, NPL>(row, seat.at, seat.n, a.vec, live, x);
+  double v[NPL];
+  if (!keyed && !(GROUPED && a.top2)) {
 #pragma unroll
-    for (int d = LPT / 2; d; d >>= 1) open |= __shfl_xor_sync(~0u, open, d);
+    for (int i = 0; i < NPL; ++i) v[i] = (double)x[i];
+  } else if (a.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) v[i] = inverse(1.0 + exp2_series((double)x[i] * -kLog2eD));
+  } else {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < NPL; ++i) m = fmaxf(m, x[i]);
+    m = lanes_top<LPT>(m);
+    double total = 0;
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+      v[i] = x[i] == -INFINITY ? 0.0 : exp2_series(((double)x[i] - (double)m) * kLog2eD);
+      total += v[i];
+    }
+    total = lanes_sum<LPT>(total);
+    const double by = total == 0.0 ? 0.0 : inverse(total);  // nothing is left of a row of -inf
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) v[i] *= by;
+  }
+  if (keyed) {
 #pragma unroll
     for (int i = 0; i < NPL; ++i)
-      if (i < (int)seat.n && !((open >> ((seat.at + i) / a.per_group)) & 1)) key[i] = 0;
+      if (i < (int)seat.n) v[i] += (double)__ldg(a.bias + (seat.at + i) * a.bs);
   }
-  Key mine = 0;
+  bool close = false, open = seat.n > 0;
+  if (GROUPED) {
+    double l1 = -INFINITY, l2 = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < NPL; ++i) mine = key[i] > mine ? key[i] : mine;
-  for (uint32_t r = 0; r < a.top_k; ++r) {
-    const Key best = lanes_max<LPT>(mine);
+    for (int i = 0; i < NPL; ++i)
+      if (i < (int)seat.n) {
+        l2 = fmax(l2, fmin(l1, v[i]));
+        l1 = fmax(l1, v[i]);
+      }
+    double w1 = l1, w2 = l2;
+#pragma unroll 1
+    for (uint32_t i = 1; i < a.lanes.d; ++i) {
+      uint32_t from = seat.lane + i;
+      if (from >= seat.first_lane + a.lanes.d) from -= a.lanes.d;
+      const double o1 = __shfl_sync(~0u, l1, seat.base + from), o2 = __shfl_sync(~0u, l2, seat.base + from);
+      w2 = fmax(fmin(w1, o1), fmax(w2, o2));
+      w1 = fmax(w1, o1);
+    }
+    const double w = a.top2 && a.per_group > 1 ? w1 + w2 : w1;
+    uint32_t before = 0, near = 0;
+#pragma unroll 1
+    for (uint32_t h = 0; h < a.groups; ++h) {
+      const double o = __shfl_sync(~0u, w, seat.base + h * a.lanes.d);
+      before += o > w || (o == w && h < seat.group);
+      near += o != w && fabs(o - w) < kClose;
+    }
+    close = seat.n && near != 0;
+    open = open && before < a.top_groups;
+    if (!keyed && a.top2) {
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) v[i] = (double)x[i];
+    }
+  }
+  Key64 key[NPL], mine = 0;
+#pragma unroll
+  for (int i = 0; i < NPL; ++i) {
+    key[i] = open && i < (int)seat.n ? key64(v[i]) : Key64(0);
+    mine = max(mine, key[i]);
+  }
+  double last = INFINITY;
+#pragma unroll 1
+  for (uint32_t r = 0; r <= a.top_k; ++r) {
+    const Key64 best = lanes_top<LPT>(mine);
     const uint32_t has = __ballot_sync(~0u, mine == best) >> seat.base;
-    if (seat.lane == (uint32_t)(__ffs(has & kLanes<LPT>) - 1)) {
+    const uint32_t owner = __ffs(has & kLanes<LPT>) - 1;
+    uint32_t at = 0;
+    if (seat.lane == owner) {
       bool found = false;
-      Key next = 0;
+      mine = 0;
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
         if (!found && key[i] == best) {
           found = true;
-          chosen[r] = (uint16_t)(seat.lane * NPL + i);
+          at = seat.lane * NPL + i;
           key[i] = 0;
         }
-        next = key[i] > next ? key[i] : next;
+        mine = max(mine, key[i]);
       }
-      mine = next;
+    }
+    at = __shfl_sync(~0u, at, seat.base + owner);
+    if (seat.lane == r) *slot = at;
+    if (best != 0) {
+      const double k = value64(best);
+      if (keyed && k != last && last - k < kClose) close = true;
+      last = k;
     }
   }
-  __syncwarp();
+  return close;
 }
 
 // Sorts a lane's keys, the largest first (compare-exchanges of Batcher's merge).
@@ -270,18 +417,20 @@ __device__ __forceinline__ void sort_down(uint32_t (&k)[N]) {
           }
 }
 
-template <typename T, int NPL, int LPT>
-__global__ void __launch_bounds__(kThreads)
+template <typename T, int NPL, int LPT, bool GROUPED>
+__global__ void __launch_bounds__(kThreads, NPL <= 8 ? 4 : 1)
 gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   constexpr uint32_t kTokens = kThreads / LPT;  // tokens a CTA handles at once
   constexpr uint32_t kSlots = LPT * NPL;
-  constexpr int kBits = kSlots <= 256 ? 24 : 22;  // of a key, above the slot's
+  constexpr int kShift = kSlots <= 256 ? 8 : 10;  // bits of a slot, below the key's
+  constexpr float kPlaces = (float)((1u << (32 - kShift)) - 1);
   constexpr bool kHalf = sizeof(T) == 2;
+  __shared__ uint32_t left;              // tokens in doubt,
+  __shared__ uint16_t which[kCtaTokens];  // and which of this CTA's
   const uint32_t sub = threadIdx.x / LPT;
-  double* worth = reinterpret_cast<double*>(smem) + sub * (a.groups > 1 ? a.groups : 0);
-  uint16_t* chosen = reinterpret_cast<uint16_t*>(reinterpret_cast<double*>(smem) +
-                                                 kTokens * (a.groups > 1 ? a.groups : 0)) + sub * a.top_k;
+  if (threadIdx.x == 0) left = 0;
+  __syncthreads();
   Seat seat;
   seat.lane = threadIdx.x % LPT;
   seat.base = (threadIdx.x & 31) - seat.lane;
@@ -304,30 +453,41 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
     }
     keyed = !__syncthreads_and(same);
   }
+  const bool scored = keyed || (GROUPED && a.top2);
 
-  for (int64_t t0 = (int64_t)blockIdx.x * kTokens; t0 < a.tokens; t0 += (int64_t)gridDim.x * kTokens) {
+  for (uint32_t step = 0;; ++step) {
+    const int64_t t0 = ((int64_t)step * gridDim.x + blockIdx.x) * kTokens;
+    if (t0 >= a.tokens) break;
     const int64_t t = t0 + sub;
     const bool live = t < a.tokens;
     const T* row = static_cast<const T*>(a.x) + (live ? t * a.xs : 0);
     float x[NPL];
     load_logits<T, NPL>(row, seat.at, seat.n, a.vec, live, x);
+    // a NaN (or infinities of both signs) shows in the sum and goes the exact way
+    float check = x[0];
+#pragma unroll
+    for (int i = 1; i < NPL; ++i) check += x[i];
+    const bool odd = check != check;
+    bool later = a.top_k >= LPT || (GROUPED && a.groups != a.seat_groups), doubt = false;
+
     // scores, as far as the order or the weights need all of them
     float s[NPL], m = 0.f, total = 1.f;
-    const bool scored = keyed || (a.groups > 1 && a.top2);
     if (!a.sigmoid) {
-      m = -INFINITY;
+      m = x[0];
 #pragma unroll
-      for (int i = 0; i < NPL; ++i) m = fmaxf(m, x[i]);
-      m = lanes_max<LPT>(m);
+      for (int i = 1; i < NPL; ++i) m = fmaxf(m, x[i]);
+      m = lanes_top<LPT>(m);
+      // a row of -inf: every difference is -inf, not NaN
+      const float shift = m == -INFINITY ? 0.f : m;
       total = 0.f;
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
-        s[i] = m == -INFINITY && x[i] == -INFINITY ? 0.f : ex2((x[i] - m) * kLog2e);
+        s[i] = ex2((x[i] - shift) * kLog2e);
         total += s[i];
       }
       total = lanes_sum<LPT>(total);
-      const float by = total == 0.f ? 0.f : rcp(total);
       if (scored) {
+        const float by = total == 0.f ? 0.f : rcp(total);
 #pragma unroll
         for (int i = 0; i < NPL; ++i) s[i] *= by;
       }
@@ -335,21 +495,21 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
 #pragma unroll
       for (int i = 0; i < NPL; ++i) s[i] = rcp(1.f + ex2(x[i] * -kLog2e));
     }
-    // A score is off by at most 10 * 2^-24 of the largest one (1 for a sigmoid), a
-    // key by 2^-24 of itself more; two of them by twice that.
-    const float s_max = a.sigmoid ? 1.f : rcp(total);
-    bool doubt = a.top_k > LPT || a.groups != a.seat_groups;
+    // A sigmoid is off by at most 2e-7: (1 - s) s times the exponential's 2^-22 and 2^-24 |x| log2 e,
+    // the sum's and the reciprocal's roundings.  A softmax by 6.2e-7 of the row's largest:
+    // the exponential's error, at most 1.1 * 2^-24 of it from its argument, the sum's, the products'.
+    // Two keys by twice that, and by 2^-24 of themselves each.
+    const float s_error = a.sigmoid ? 4.2e-7f : 1.25e-6f * rcp(total);
     bool open = seat.n > 0;
-    if (a.groups > 1 && a.groups == a.seat_groups) {
+    if (GROUPED && a.groups == a.seat_groups) {
       float v1 = -INFINITY, v2 = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < NPL; ++i)
-        if (i < (int)seat.n) {
-          const float v = keyed ? s[i] + bias[i] : a.top2 ? s[i] : x[i];
-          if (v != v) doubt = true;
-          v2 = fmaxf(v2, fminf(v1, v));
-          v1 = fmaxf(v1, v);
-        }
+      for (int i = 0; i < NPL; ++i) {
+        float v = keyed ? s[i] + bias[i] : a.top2 ? s[i] : x[i];
+        if (i >= (int)seat.n) v = -INFINITY;
+        v2 = fmaxf(v2, fminf(v1, v));
+        v1 = fmaxf(v1, v);
+      }
       float w1 = v1, w2 = v2;
       for (uint32_t i = 1; i < a.lanes.d; ++i) {
         uint32_t from = seat.lane + i;
@@ -360,65 +520,60 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
       }
       const bool two = a.top2 && a.per_group > 1;
       const float w = two ? w1 + w2 : w1;
-      // two keys: twice the error; without scores the largest logits are exact
-      const float error = keyed || a.top2 ? (two ? 2.f : 1.f) * 1.25e-6f * s_max + 5e-7f * fabsf(w) : 0.f;
-      uint32_t before = 0, maybe = 0;
+      // Without scores the largest logits are exact.  With them, how many other groups are
+      // clearly better, and how many may be: their order is within the error.
+      const float error = scored ? (two ? 2.f : 1.f) * s_error + 5e-7f * fabsf(w) : 0.f;
+      uint32_t better = 0, before = 0, worse = 0;
       for (uint32_t h = 0; h < a.groups; ++h) {
         const float o = __shfl_sync(~0u, w, seat.base + h * a.lanes.d);
         before += o > w || (o == w && h < seat.group);
-        // Another group within the error: its order is in doubt.  A NaN or two infinities too.
-        maybe += h != seat.group && error > 0.f && !(fabsf(o - w) > error);
+        better += o - w > error;
+        worse += w - o > error;
       }
       open = open && before < a.top_groups;
       // it matters where it could open this group or close it
-      if (seat.n && maybe && before < a.top_groups + maybe && before + maybe >= a.top_groups) doubt = true;
+      if (seat.n && error > 0.f && (better < a.top_groups) != (worse >= a.groups - a.top_groups)) doubt = true;
     }
 
     uint32_t key[NPL];
-    bool exact = false;
+    const bool exact = kHalf && !keyed;
     uint32_t slack = 0;  // keys this close are in doubt
-    if (kHalf && !keyed) {
-      exact = true;
+    if (exact) {
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
         const uint32_t b = half_bits<T>(x[i]);
         key[i] = (((b & 0x8000u) ? ~b & 0xffffu : b | 0x8000u) << 16) | (kSlots - 1 - (seat.lane * NPL + i));
-        if (x[i] != x[i]) doubt = true;
       }
     } else {
       // the range from the largest key down to one that top_k + 1 others reach
-      float k[NPL], hi = -INFINITY, lo = INFINITY;
+      float hi = -INFINITY, lo = INFINITY;
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
-        k[i] = keyed ? s[i] + bias[i] : x[i];
+        s[i] = keyed ? s[i] + bias[i] : x[i];
         if (i < (int)seat.n) {
-          hi = fmaxf(hi, k[i]);
-          lo = fminf(lo, k[i]);
+          hi = fmaxf(hi, s[i]);
+          lo = fminf(lo, s[i]);
         }
       }
       const uint32_t lanes = __popc(__ballot_sync(~0u, open) >> seat.base & kLanes<LPT>);
-      const float top = lanes_max<LPT>(open ? hi : -INFINITY);
-      lo = -lanes_max<LPT>(open ? -(a.top_k < lanes ? hi : lo) : -INFINITY);
+      const float top = lanes_top<LPT>(open ? hi : -INFINITY);
+      lo = -lanes_top<LPT>(open ? -(a.top_k < lanes ? hi : lo) : -INFINITY);
       lo = fmaxf(lo, top - 64.f);
-      const float range = fmaxf(top - lo, 1e-30f);
-      const float by = (float)((1 << kBits) - 64) / range;
+      const float by = (kPlaces - 64.f) * rcp(fmaxf(top - lo, 1e-30f));
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
-        const uint32_t f = (uint32_t)fminf(fmaxf(fmaf(k[i] - lo, by, 16.f), 1.f), (float)((1 << kBits) - 1));
-        key[i] = f << (32 - kBits) | (kSlots - 1 - (seat.lane * NPL + i));
+        const uint32_t f = (uint32_t)fminf(fmaxf(fmaf(s[i] - lo, by, 16.f), 1.f), kPlaces);
+        key[i] = f << kShift | (kSlots - 1 - (seat.lane * NPL + i));
       }
       // Rounding to places keeps the order of exact keys, or makes them equal; for the others
       // their error counts, and the roundings of the difference, below 4 places.
-      if (keyed) {
-        const float error = 1.25e-6f * s_max + 2.5e-7f * fmaxf(fabsf(top), fabsf(lo));
-        slack = 4 + (uint32_t)fminf(error * by, 4e9f);
-      }
+      if (keyed) slack = 4 + (uint32_t)fminf((s_error + 1.3e-7f * fmaxf(fabsf(top), fabsf(lo))) * by, 4e9f);
     }
 #pragma unroll
     for (int i = 0; i < NPL; ++i)
       if (!open || i >= (int)seat.n) key[i] = 0;
 
-    uint32_t won = 0;  // of rank `lane`
+    uint32_t won = 0;  // of rank `lane`; and of the first one not chosen
     if (NPL <= 8) {
       sort_down<NPL>(key);
     } else {
@@ -429,14 +584,8 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
         key[0] = hi;
       }
     }
-    uint32_t last = ~0u;
-    for (uint32_t r = 0; r < a.top_k + (exact ? 0 : 1); ++r) {
-      const uint32_t best = lanes_max_u32<LPT>(key[0]);
-      if (!exact) {
-        const uint32_t f = best >> (32 - kBits);
-        if (best != 0 && (last - f <= slack || (r < a.top_k && f < 8))) doubt = true;
-        last = f;
-      }
+    for (uint32_t r = 0; r <= a.top_k; ++r) {
+      const uint32_t best = lanes_top<LPT>(key[0]);
       if (seat.lane == r) won = best;
       if (key[0] == best) {
         if (NPL <= 8) {
@@ -454,44 +603,46 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
         }
       }
     }
-    const bool redo = __any_sync(~0u, doubt && live);
-    if (redo) select_exact<NPL, LPT>(a, x, bias, seat, keyed, worth, chosen);
+    if (!exact) {
+      const uint32_t f = won >> kShift, next = __shfl_down_sync(~0u, f, 1);
+      if (seat.lane < a.top_k && (f < 8 || (next != 0 && f - next <= slack))) doubt = true;
+    }
+    uint32_t slot = kSlots - 1 - (won & ((1u << (exact ? 16 : kShift)) - 1));
+    // (the whole warp takes part; a token that is not in doubt gets the same again)
+    if (__any_sync(~0u, (doubt || odd) && live && !later)) {
+      const bool close = resolve<T, NPL, LPT, GROUPED>(a, row, live, seat, keyed, &slot);
+      later = (__ballot_sync(~0u, later || odd || close) >> seat.base & kLanes<LPT>) != 0;
+    }
+    if (later && live && seat.lane == 0) which[atomicAdd(&left, 1u)] = (uint16_t)(step * kTokens + sub);
 
     // weights from the chosen logits, a lane each
-    float sum = 0.f;
-    for (uint32_t r = seat.lane; r < a.top_k; r += LPT) {
-      const uint32_t slot = redo ? chosen[r] : kSlots - 1 - (won & ((1u << (exact ? 16 : 32 - kBits)) - 1));
+    float sc = 0.f;
+    if (seat.lane < a.top_k && live && !later) {
       const uint32_t e = expert_of<NPL>(a, slot);
-      const float v = live ? to_f(row[e]) : 0.f;
-      float sc;
-      if (a.sigmoid) sc = 1.f / (1.f + expf(-v));
-      else sc = total == 0.f ? 0.f : expf(v - m) / total;
-      sum += sc;
-      if (live) {
-        if (!a.renorm) a.weights[t * a.ws + r * a.wk] = sc * a.scale;
-        if (a.wide) static_cast<int64_t*>(a.experts)[t * a.es + r * a.ek] = e;
-        else static_cast<int32_t*>(a.experts)[t * a.es + r * a.ek] = (int32_t)e;
-      }
-      won = __float_as_uint(sc);  // the only one of a lane where it is needed below
+      const float v = to_f(row[e]);
+      if (a.sigmoid) sc = rcp(1.f + expf(-v));
+      else sc = m == -INFINITY ? 0.f : expf(v - m) * rcp(total);
+      if (a.wide) static_cast<int64_t*>(a.experts)[t * a.es + seat.lane * a.ek] = e;
+      else static_cast<int32_t*>(a.experts)[t * a.es + seat.lane * a.ek] = (int32_t)e;
     }
+    float times = a.scale;
     if (a.renorm) {
-      sum = lanes_sum<LPT>(sum);
-      const float by = sum == 0.f ? 0.f : a.scale / sum;
-      for (uint32_t r = seat.lane; r < a.top_k; r += LPT) {
-        float sc = __uint_as_float(won);
-        if (a.top_k > LPT) {  // several ranks a lane: again
-          const float v = live ? to_f(row[expert_of<NPL>(a, chosen[r])]) : 0.f;
-          sc = a.sigmoid ? 1.f / (1.f + expf(-v)) : total == 0.f ? 0.f : expf(v - m) / total;
-        }
-        if (live) a.weights[t * a.ws + r * a.wk] = sc * by;
-      }
+      const float sum = lanes_sum<LPT>(sc);
+      times = sum == 0.f ? 0.f : a.scale / sum;
     }
-    __syncwarp();
+    if (seat.lane < a.top_k && live && !later) a.weights[t * a.ws + seat.lane * a.wk] = sc * times;
+  }
+
+  __syncthreads();
+  Key64* key = reinterpret_cast<Key64*>(smem) + (threadIdx.x / 32) * (a.n + a.groups);
+  for (uint32_t i = threadIdx.x / 32; i < left && threadIdx.x / 32 < a.exact_warps; i += a.exact_warps) {
+    const uint32_t step = which[i] / kTokens, token = which[i] - step * kTokens;
+    route_exact<T>(a, keyed, ((int64_t)step * gridDim.x + blockIdx.x) * kTokens + token, key, key + a.n);
   }
 }
 
 struct Chosen {
-  float score;
+  float value;
   uint32_t expert;
 };
 
@@ -499,65 +650,100 @@ struct Chosen {
 //   renormalised, S the sum of the chosen:  ds_j = scale (g_j - sum_i g_i s_i / S) / S,  else scale g_j
 //   sigmoid:  dx_j = ds_j s_j (1 - s_j)
 //   softmax:  dx_e = s_e (ds_e - sum_i ds_i s_i)        (ds = 0 where not chosen)
+// Of a renormalised softmax the last sum is 0 and s / S is the softmax of the
+// chosen logits alone; so only a plain softmax needs the whole row.
 template <typename T, int NPL, int LPT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, NPL <= 8 ? 4 : 1)
 gpuos_route_grad_kernel(const __grid_constant__ RouteArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   constexpr uint32_t kTokens = kThreads / LPT;
+  constexpr int NR = LPT == 32 ? kMaxTop / 32 : 1;
   const uint32_t sub = threadIdx.x / LPT, lane = threadIdx.x % LPT;
   float* dense = reinterpret_cast<float*>(smem) + sub * (LPT * NPL);
   Chosen* chosen = reinterpret_cast<Chosen*>(reinterpret_cast<float*>(smem) + kThreads * NPL) + sub * a.top_k;
-  const uint32_t at = lane * NPL;
+  const uint32_t at = lane * NPL, n = at < a.n ? min((uint32_t)NPL, a.n - at) : 0u;
+  const bool whole = !a.sigmoid && !a.renorm;
   for (int64_t t0 = (int64_t)blockIdx.x * kTokens; t0 < a.tokens; t0 += (int64_t)gridDim.x * kTokens) {
     const int64_t t = t0 + sub;
     const bool live = t < a.tokens;
     const T* row = static_cast<const T*>(a.x) + (live ? t * a.xs : 0);
-    float x[NPL], s[NPL];
-    load_logits<T, NPL>(row, at, at < a.n ? min((uint32_t)NPL, a.n - at) : 0u, a.vec, live, x);
-    float m = 0.f, total = 1.f;
-    score<float, NPL, LPT>(x, at < a.n ? min((uint32_t)NPL, a.n - at) : 0u, a.sigmoid, s, &m, &total);
-    // the chosen ones' scores and gradients, a lane each
-    float sum = 0.f, dot = 0.f;
-    for (uint32_t r = lane; r < a.top_k; r += LPT) {
-      int64_t e = -1;
-      if (live)
-        e = a.wide ? static_cast<const int64_t*>(a.experts)[t * a.es + r * a.ek]
-                   : (int64_t)static_cast<const int32_t*>(a.experts)[t * a.es + r * a.ek];
-      const bool in = e >= 0 && e < a.n;
-      const float g = in ? a.gw[t * a.gs + r * a.gk] : 0.f;
-      float sc = 0.f;
-      if (in) {
-        const float v = to_f(row[e]);
-        sc = a.sigmoid ? 1.f / (1.f + expf(-v)) : total == 0.f ? 0.f : expf(v - m) / total;
+    // the chosen ones, a lane each
+    float g[NR], v[NR];
+    uint32_t e[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      const uint32_t r = lane + i * LPT;
+      g[i] = 0.f;
+      v[i] = -INFINITY;
+      e[i] = ~0u;
+      if (r >= a.top_k || !live) continue;
+      const int64_t w = a.wide ? static_cast<const int64_t*>(a.experts)[t * a.es + r * a.ek]
+                               : (int64_t)static_cast<const int32_t*>(a.experts)[t * a.es + r * a.ek];
+      if (w < 0 || w >= a.n) continue;
+      e[i] = (uint32_t)w;
+      g[i] = a.gw[t * a.gs + r * a.gk];
+      v[i] = to_f(row[w]);
+    }
+    float p[NPL], m = -INFINITY, by = 1.f;
+    if (whole) {
+      load_logits<T, NPL>(row, at, n, a.vec, live, p);
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) m = fmaxf(m, p[i]);
+      m = lanes_top<LPT>(m);
+      const float shift = m == -INFINITY ? 0.f : m;
+      float total = 0.f;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) {
+        p[i] = ex2((p[i] - shift) * kLog2e);
+        total += p[i];
       }
-      sum += sc;
-      dot += g * sc;
-      chosen[r] = Chosen{g, in ? (uint32_t)e : ~0u};
+      total = lanes_sum<LPT>(total);
+      by = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) p[i] *= by;
+    } else if (!a.sigmoid) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i) m = fmaxf(m, v[i]);
+      m = lanes_top<LPT>(m);
+    }
+    float sc[NR], sum = 0.f, dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      if (a.sigmoid) sc[i] = e[i] == ~0u ? 0.f : 1.f / (1.f + expf(-v[i]));
+      else sc[i] = m == -INFINITY || e[i] == ~0u ? 0.f : expf(v[i] - m) * by;
+      sum += sc[i];
+      dot += g[i] * sc[i];
     }
     sum = lanes_sum<LPT>(sum);
     dot = lanes_sum<LPT>(dot);
-    float mul = a.scale, sub_ = 0.f, all;
-    if (a.renorm) {
-      mul = sum == 0.f ? 0.f : a.scale / sum;
-      sub_ = sum == 0.f ? 0.f : dot / sum;
-      all = 0.f;  // sum of ds_i s_i = scale (dot - dot) / S
-    } else {
-      all = a.scale * dot;
+    const float mul = !a.renorm ? a.scale : sum == 0.f ? 0.f : a.scale / sum;
+    const float less = !a.renorm || sum == 0.f ? 0.f : dot / sum;
+    const float all = a.scale * dot;  // of a plain softmax: the sum of ds_i s_i
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      const uint32_t r = lane + i * LPT;
+      float d = mul * (g[i] - less);
+      if (a.sigmoid) {
+        const float x = expf(-fabsf(v[i])), q = 1.f / (1.f + x);
+        d *= x * q * q;  // s (1 - s)
+      } else if (a.renorm) {
+        d *= sc[i];
+      }
+      if (r < a.top_k) chosen[r] = Chosen{d, e[i]};
     }
-    __syncwarp();
 #pragma unroll
     for (int i = 0; i < NPL; ++i) dense[at + i] = 0.f;
+    __syncwarp();
     // in order of rank, so that an expert named twice adds up the same way each time
     for (uint32_t r = 0; r < a.top_k; ++r) {
       const Chosen c = chosen[r];
-      if (c.expert / NPL == lane) dense[c.expert] += mul * (c.score - sub_);
+      if (c.expert / NPL == lane) dense[c.expert] += c.value;
     }
     float d[NPL];
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
-      const float ds = dense[at + i];
-      d[i] = a.sigmoid ? ds * s[i] * (1.f - s[i]) : s[i] * (ds - all);
-      if (s[i] == 0.f) d[i] = 0.f;
+      d[i] = dense[at + i];
+      if (whole) d[i] = p[i] == 0.f ? 0.f : p[i] * (d[i] - all);
     }
     if (live) {
       T* o = static_cast<T*>(a.gx) + t * a.os;
@@ -568,12 +754,12 @@ gpuos_route_grad_kernel(const __grid_constant__ RouteArgs a) {
           Pack<T, W> q;
 #pragma unroll
           for (int i = 0; i < W; ++i) q.v[i] = from_f<T>(d[k + i]);
-          if (at + k < a.n) store_pack<T, W>(o + at + k, q);
+          if (k < (int)n) store_pack<T, W>(o + at + k, q);
         }
       } else {
 #pragma unroll
         for (int i = 0; i < NPL; ++i)
-          if (at + i < a.n) o[at + i] = from_f<T>(d[i]);
+          if (i < (int)n) o[at + i] = from_f<T>(d[i]);
       }
     }
     __syncwarp();
@@ -584,7 +770,10 @@ template <typename T, int NPL, int LPT>
 void launch(RouteArgs a, bool grad, cudaStream_t s) {
   constexpr uint32_t kTokens = kThreads / LPT;
   const uint64_t ctas = ((uint64_t)a.tokens + kTokens - 1) / kTokens;
-  const unsigned grid = (unsigned)std::min<uint64_t>(ctas, (uint64_t)sm_count() * 8);
+  const uint64_t most = kCtaTokens / kTokens;  // steps of a CTA
+  const uint64_t wanted = std::max<uint64_t>(std::min<uint64_t>(ctas, (uint64_t)sm_count() * 8), (ctas + most - 1) / most);
+  need(wanted < 0x7fffffffull, "too many tokens");
+  const unsigned grid = (unsigned)wanted;
   a.seat_groups = a.groups;
   a.seat_per_group = a.per_group;
   if (a.groups * ((a.per_group + NPL - 1) / NPL) > LPT) {
@@ -599,8 +788,12 @@ void launch(RouteArgs a, bool grad, cudaStream_t s) {
                                    cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory");
     gpuos_route_grad_kernel<T, NPL, LPT><<<grid, kThreads, smem, s>>>(a);
   } else {
-    const size_t smem = kTokens * ((a.groups > 1 ? a.groups : 0) * sizeof(double) + a.top_k * sizeof(uint16_t));
-    gpuos_route_kernel<T, NPL, LPT><<<grid, kThreads, smem, s>>>(a);
+    // 16 KB of keys: 8 warps of 256 experts, fewer of more
+    const size_t keys = (a.n + a.groups) * sizeof(Key64);
+    a.exact_warps = (uint32_t)std::max<size_t>(1, std::min<size_t>(kThreads / 32, 18 * 1024 / keys));
+    const size_t smem = a.exact_warps * keys;
+    if (a.groups > 1) gpuos_route_kernel<T, NPL, LPT, true><<<grid, kThreads, smem, s>>>(a);
+    else gpuos_route_kernel<T, NPL, LPT, false><<<grid, kThreads, smem, s>>>(a);
   }
   cuda_ok(cudaGetLastError(), "launch");
 }
@@ -610,7 +803,8 @@ uint32_t lanes_for(const RouteArgs& a, uint32_t npl) { return a.groups * ((a.per
 
 template <typename T>
 void by_size(const RouteArgs& a, bool grad, cudaStream_t s) {
-  const uint32_t lanes = lanes_for(a, 8);
+  // a lane for each rank and the first one not chosen
+  const uint32_t lanes = std::max(lanes_for(a, 8), std::min<uint32_t>(a.top_k + 1, 32));
   if (lanes <= 4) launch<T, 8, 4>(a, grad, s);
   else if (lanes <= 8) launch<T, 8, 8>(a, grad, s);
   else if (lanes <= 16) launch<T, 8, 16>(a, grad, s);
