@@ -127,7 +127,7 @@ def build_ext(force=False, verbose=False) -> Path:
           "-DTORCH_EXTENSION_NAME=gpuos_ext", *inc, CSRC / "ext.cpp", CSRC / "rowops_ext.cpp",
           "-o", EXT,
           f"-L{HERE}", "-lgpuos_b200", f"-L{tlib}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
-          "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}"], verbose)
+          "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}"], verbose)
     return EXT
 
 

@@ -444,14 +444,14 @@ template <typename T, int F>
 void launch_write(const CacheArgs& a, bool vec, int n, cudaStream_t s) {
   const uint32_t per_cta = kThreads >> a.token_log;
   const dim3 grid((a.tokens + per_cta - 1) / per_cta, n);
-  if (vec) gpuos_cache_write_kernel<T, F, true><<<grid, kThreads, 0, s>>>(a);
-  else gpuos_cache_write_kernel<T, F, false><<<grid, kThreads, 0, s>>>(a);
+  if (vec) run(gpuos_cache_write_kernel<T, F, true>, grid, kThreads, 0, s, a);
+  else run(gpuos_cache_write_kernel<T, F, false>, grid, kThreads, 0, s, a);
 }
 
 template <typename T, int F>
 void launch_read(const CacheArgs& a, bool vec, dim3 grid, cudaStream_t s) {
-  if (vec) gpuos_cache_read_kernel<T, F, true><<<grid, kThreads, 0, s>>>(a);
-  else gpuos_cache_read_kernel<T, F, false><<<grid, kThreads, 0, s>>>(a);
+  if (vec) run(gpuos_cache_read_kernel<T, F, true>, grid, kThreads, 0, s, a);
+  else run(gpuos_cache_read_kernel<T, F, false>, grid, kThreads, 0, s, a);
 }
 
 template <typename L>
@@ -501,7 +501,6 @@ void cache_write(int32_t n, const gpuos_tensor* x, const gpuos_tensor* slots, co
   by_type(x[0].dtype, codes[0].dtype, [&](auto type, auto f) {
     launch_write<decltype(type), decltype(f)::value>(a, vec, n, stream);
   });
-  cuda_ok(cudaGetLastError(), "launch");
 }
 
 void cache_read(int32_t n, const gpuos_tensor* slots, const gpuos_tensor* codes, const gpuos_tensor* scales,
@@ -530,7 +529,6 @@ void cache_read(int32_t n, const gpuos_tensor* slots, const gpuos_tensor* codes,
   by_type(out[0].dtype, codes[0].dtype, [&](auto type, auto f) {
     launch_read<decltype(type), decltype(f)::value>(a, vec, grid, stream);
   });
-  cuda_ok(cudaGetLastError(), "launch");
 }
 
 }  // namespace

@@ -729,9 +729,8 @@ void backward(LogArgs a, cudaStream_t s) {
   need(a.rows * parts < 0x7fffffffll, "too many logits");
   a.parts = (uint32_t)parts;
   const unsigned grid = (unsigned)(a.rows * parts);
-  if (a.vec) gpuos_logprobs_grad_kernel<T, true><<<grid, kGradThreads, 0, s>>>(a);
-  else gpuos_logprobs_grad_kernel<T, false><<<grid, kGradThreads, 0, s>>>(a);
-  cuda_ok(cudaGetLastError(), "launch");
+  if (a.vec) run(gpuos_logprobs_grad_kernel<T, true>, grid, kGradThreads, 0, s, a);
+  else run(gpuos_logprobs_grad_kernel<T, false>, grid, kGradThreads, 0, s, a);
 }
 
 void logprobs_grad(const gpuos_tensor* x, const gpuos_tensor* targets, const gpuos_tensor* stats, const gpuos_tensor* entropy,

@@ -186,7 +186,7 @@ gpuos_rotary_kernel(const __grid_constant__ RotArgs a) {
 template <typename T>
 void launch(const RotArgs& a, int v, int vl, bool inter, dim3 grid, cudaStream_t s) {
   constexpr int W = 16 / sizeof(T);
-#define GPUOS_ROT(V, VL, I) gpuos_rotary_kernel<T, V, VL, I><<<grid, kThreads, 0, s>>>(a)
+#define GPUOS_ROT(V, VL, I) run(gpuos_rotary_kernel<T, V, VL, I>, grid, kThreads, 0, s, a)
   if (inter) {
     if (v == W) GPUOS_ROT(W, W, true);
     else if (v == W / 2 && vl == W / 2) GPUOS_ROT(W / 2, W / 2, true);
@@ -304,7 +304,6 @@ void rotary(int32_t n, const gpuos_tensor* x, const gpuos_tensor* out, const gpu
   if (x[0].dtype == GPUOS_F32) launch<float>(a, v, vl, inter, grid, stream);
   else if (x[0].dtype == GPUOS_F16) launch<__half>(a, v, vl, inter, grid, stream);
   else launch<__nv_bfloat16>(a, v, vl, inter, grid, stream);
-  cuda_ok(cudaGetLastError(), "launch");
 }
 
 }  // namespace

@@ -786,16 +786,15 @@ void launch(RouteArgs a, bool grad, cudaStream_t s) {
     if (smem > 48 * 1024)
       cuda_ok(cudaFuncSetAttribute(gpuos_route_grad_kernel<T, NPL, LPT>,
                                    cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory");
-    gpuos_route_grad_kernel<T, NPL, LPT><<<grid, kThreads, smem, s>>>(a);
+    run(gpuos_route_grad_kernel<T, NPL, LPT>, grid, kThreads, smem, s, a);
   } else {
     // 16 KB of keys: 8 warps of 256 experts, fewer of more
     const size_t keys = (a.n + a.groups) * sizeof(Key64);
     a.exact_warps = (uint32_t)std::max<size_t>(1, std::min<size_t>(kThreads / 32, 18 * 1024 / keys));
     const size_t smem = a.exact_warps * keys;
-    if (a.groups > 1) gpuos_route_kernel<T, NPL, LPT, true><<<grid, kThreads, smem, s>>>(a);
-    else gpuos_route_kernel<T, NPL, LPT, false><<<grid, kThreads, smem, s>>>(a);
+    if (a.groups > 1) run(gpuos_route_kernel<T, NPL, LPT, true>, grid, kThreads, smem, s, a);
+    else run(gpuos_route_kernel<T, NPL, LPT, false>, grid, kThreads, smem, s, a);
   }
-  cuda_ok(cudaGetLastError(), "launch");
 }
 
 // Lanes a token needs with NPL experts a lane, none of two groups.

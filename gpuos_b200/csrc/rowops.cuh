@@ -5,11 +5,20 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "rowops.h"
 
 namespace gpuos {
 namespace rowops {
+
+// One launch of a kernel that takes one parameter block.
+template <typename A>
+inline void run(void (*kernel)(A), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream,
+                const std::remove_const_t<A>& args) {
+  void* p[1] = {const_cast<std::remove_const_t<A>*>(&args)};
+  cuda_ok(cudaLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3(threads), p, smem, stream), "launch");
+}
 
 // n / d for n < 2^31 by one multiplication: with s = ceil(log2 d) and
 // m = ceil(2^(32+s-1) / d) the error of n * m / 2^(32+s-1) stays below 1 / d.

@@ -30,7 +30,9 @@ inline void need(bool ok, const char* msg) {
 }
 
 inline void cuda_ok(cudaError_t e, const char* what) {
-  if (e != cudaSuccess) throw Fail{GPUOS_ECUDA, std::string(what) + ": " + cudaGetErrorString(e)};
+  if (e == cudaSuccess) return;
+  cudaGetLastError();  // reported here, not by a later check
+  throw Fail{GPUOS_ECUDA, std::string(what) + ": " + cudaGetErrorString(e)};
 }
 
 // Runs an entry point's body; nothing is thrown past the C boundary.

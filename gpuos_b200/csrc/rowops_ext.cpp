@@ -4,14 +4,18 @@
 // callers use; it adds gradients and the order after a scheduler's requests.
 #include <Python.h>
 
-#include <ATen/ops/empty.h>
+#include <ATen/EmptyTensor.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <optional>
 #include <string>
+#include <vector>
 
 #include "../../include/gpuos_b200.h"
 
@@ -80,7 +84,49 @@ struct Place {
   }
   gpuos_tensor in(PyObject* o, const char* name) const { return in(tensor(o, name), name); }
   at::Tensor make(at::IntArrayRef sizes, at::ScalarType type) const {
-    return at::empty(sizes, at::TensorOptions().dtype(type).device(device));
+    return at::detail::empty_cuda(sizes, type, device, std::nullopt);
+  }
+};
+
+// A call's outputs, contiguous.  Small ones share one allocation, each at a
+// multiple of 256 bytes of it: an allocation costs the host about as much as all checks.
+struct Outputs {
+  static constexpr int kMost = 5;
+  static constexpr int64_t kSmall = 1 << 18;
+  at::Tensor t[kMost];
+  std::vector<int64_t> sizes[kMost];
+  at::ScalarType type[kMost];
+  int n = 0;
+  int add(std::vector<int64_t> size, at::ScalarType dt) {
+    sizes[n] = std::move(size);
+    type[n] = dt;
+    return n++;
+  }
+  void allocate(const Place& at) {
+    int64_t at_byte[kMost], total = 0;
+    bool small = n > 1;
+    for (int i = 0; i < n; ++i) {
+      int64_t bytes = (int64_t)c10::elementSize(type[i]);
+      for (const int64_t d : sizes[i]) {
+        if (d < 0 || d > kSmall) small = false;
+        bytes *= small ? d : 0;
+      }
+      at_byte[i] = total;
+      total += (bytes + 255) / 256 * 256;
+      if (total > kSmall) small = false;
+    }
+    if (!small) {
+      for (int i = 0; i < n; ++i) t[i] = at.make(sizes[i], type[i]);
+      return;
+    }
+    const at::Tensor whole = at.make({total}, at::kByte);
+    for (int i = 0; i < n; ++i) {
+      t[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()),
+                                                      c10::DispatchKeySet(c10::DispatchKey::CUDA),
+                                                      c10::scalarTypeToTypeMeta(type[i]));
+      t[i].unsafeGetTensorImpl()->set_sizes_contiguous(sizes[i]);
+      t[i].unsafeGetTensorImpl()->set_storage_offset(at_byte[i] / (int64_t)c10::elementSize(type[i]));
+    }
   }
 };
 
@@ -120,11 +166,36 @@ bool truth(PyObject* o) {
   return v != 0;
 }
 
-// One or two tensors: a tuple.
-Py_ssize_t pair(PyObject* o, const char* name) {
-  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) < 1 || PyTuple_GET_SIZE(o) > 2)
-    throw Raise{PyExc_TypeError, std::string(name) + " must be a tuple of one or two tensors"};
-  return PyTuple_GET_SIZE(o);
+// One tensor, or a tuple of one or two.
+struct Pair {
+  PyObject* o[2] = {nullptr, nullptr};
+  int n = 1;
+  bool tuple = false;
+  Pair(PyObject* arg, const char* name) {
+    if (!PyTuple_Check(arg)) {
+      o[0] = arg;
+      return;
+    }
+    tuple = true;
+    n = (int)PyTuple_GET_SIZE(arg);
+    if (n < 1 || n > 2)
+      throw Raise{PyExc_TypeError, std::string(name) + " must be a tensor, or a tuple of one or two tensors"};
+    for (int i = 0; i < n; ++i) o[i] = PyTuple_GET_ITEM(arg, i);
+  }
+};
+
+PyObject* wrap(const at::Tensor& t) {
+  PyObject* o = THPVariable_Wrap(t);
+  if (!o) throw PyFailed{};
+  return o;
+}
+
+// Whether autograd has to see the call (gpuos_b200.rowops then records it).
+bool recorded(const at::Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+
+PyObject* not_here() {
+  Py_INCREF(Py_NotImplemented);
+  return Py_NotImplemented;
 }
 
 void same_count(Py_ssize_t a, Py_ssize_t b, const char* what) {
@@ -166,81 +237,102 @@ PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 PyObject* rotary(PyObject* const* a, Py_ssize_t n) {
-  arity(n, 7, "(xs, outs, positions, inv_freq, scale, interleaved, inverse)");
-  const Py_ssize_t m = pair(a[0], "xs");
-  const Place at(tensor(PyTuple_GET_ITEM(a[0], 0), "x"));
+  arity(n, 7, "(x, out, positions, inv_freq, scale, interleaved, inverse)");
+  const Pair xs(a[0], "x");
+  const at::Tensor* xt[2];
+  for (int i = 0; i < xs.n; ++i) {
+    xt[i] = &tensor(xs.o[i], "x");
+    if (recorded(*xt[i])) return not_here();
+  }
+  const Place at(*xt[0]);
   gpuos_tensor x[2], o[2];
   at::Tensor out[2];
-  if (a[1] != Py_None) same_count(pair(a[1], "out"), m, "out must have a tensor for each x");
-  for (Py_ssize_t i = 0; i < m; ++i) {
-    const at::Tensor& t = tensor(PyTuple_GET_ITEM(a[0], i), "x");
-    x[i] = at.in(t, "x");
-    if (a[1] != Py_None) {
-      out[i] = tensor(PyTuple_GET_ITEM(a[1], i), "out");
-    } else {
-      out[i] = at::empty_like(t);
-      // an expanded or padded x keeps no layout in which the last dim is contiguous for sure
-      if (t.dim() && out[i].stride(-1) != 1) out[i] = at.make(t.sizes(), t.scalar_type());
+  if (a[1] != Py_None) {
+    const Pair given(a[1], "out");
+    same_count(given.n, xs.n, "out must have a tensor for each x");
+    for (int i = 0; i < xs.n; ++i) out[i] = tensor(given.o[i], "out");
+  } else {
+    Outputs outs;
+    for (int i = 0; i < xs.n; ++i)
+      if (xt[i]->is_contiguous()) outs.add(xt[i]->sizes().vec(), xt[i]->scalar_type());
+    outs.allocate(at);
+    for (int i = 0, k = 0; i < xs.n; ++i) {
+      if (xt[i]->is_contiguous()) {
+        out[i] = outs.t[k++];
+      } else {
+        // the layout of x, where its last dim is contiguous in it
+        out[i] = at::empty_like(*xt[i]);
+        if (xt[i]->dim() && out[i].stride(-1) != 1) out[i] = at.make(xt[i]->sizes(), xt[i]->scalar_type());
+      }
     }
+  }
+  for (int i = 0; i < xs.n; ++i) {
+    x[i] = at.in(*xt[i], "x");
     o[i] = at.in(out[i], "out");
   }
   const gpuos_tensor p = at.in(a[2], "positions"), f = at.in(a[3], "inv_freq");
   const double scale = real(a[4]);
   const int32_t flags = (truth(a[5]) ? GPUOS_ROTARY_INTERLEAVED : 0) | (truth(a[6]) ? GPUOS_ROTARY_INVERSE : 0);
-  done(gpuos_rotary((int32_t)m, x, o, &p, &f, (float)scale, flags, at.stream()));
-  return tuple_of(out, m);
+  done(gpuos_rotary(xs.n, x, o, &p, &f, (float)scale, flags, at.stream()));
+  return xs.tuple ? tuple_of(out, xs.n) : wrap(out[0]);
 }
 
 PyObject* cache_write(PyObject* const* a, Py_ssize_t n) {
-  arity(n, 4, "(xs, slots, codes, scales)");
-  const Py_ssize_t m = pair(a[0], "x");
-  same_count(pair(a[2], "codes"), m, "codes must have a tensor for each x");
-  same_count(pair(a[3], "scales"), m, "scales must have a tensor for each x");
-  const Place at(tensor(PyTuple_GET_ITEM(a[0], 0), "x"));
+  arity(n, 4, "(x, slots, codes, scales)");
+  const Pair xs(a[0], "x"), cs(a[2], "codes"), ss(a[3], "scales");
+  same_count(cs.n, xs.n, "codes must have a tensor for each x");
+  same_count(ss.n, xs.n, "scales must have a tensor for each x");
+  const Place at(tensor(xs.o[0], "x"));
   gpuos_tensor x[2], c[2], s[2];
-  for (Py_ssize_t i = 0; i < m; ++i) {
-    x[i] = at.in(PyTuple_GET_ITEM(a[0], i), "x");
-    c[i] = at.in(PyTuple_GET_ITEM(a[2], i), "codes");
-    s[i] = at.in(PyTuple_GET_ITEM(a[3], i), "scales");
+  for (int i = 0; i < xs.n; ++i) {
+    x[i] = at.in(xs.o[i], "x");
+    c[i] = at.in(cs.o[i], "codes");
+    s[i] = at.in(ss.o[i], "scales");
   }
   const gpuos_tensor slots = at.in(a[1], "slots");
-  done(gpuos_cache_write((int32_t)m, x, &slots, c, s, at.stream()));
+  done(gpuos_cache_write(xs.n, x, &slots, c, s, at.stream()));
   Py_RETURN_NONE;
 }
 
 PyObject* cache_read(PyObject* const* a, Py_ssize_t n) {
-  arity(n, 5, "(slots, codes, scales, outs, like)");
-  const Py_ssize_t m = pair(a[1], "codes");
-  same_count(pair(a[2], "scales"), m, "scales must have a tensor for each cache");
+  arity(n, 5, "(slots, codes, scales, out, dtype)");
+  const Pair cs(a[1], "codes"), ss(a[2], "scales");
+  same_count(ss.n, cs.n, "scales must have a tensor for each cache");
   const at::Tensor& slots_t = tensor(a[0], "slots");
   const Place at(slots_t);
   gpuos_tensor c[2], s[2], o[2];
   at::Tensor out[2];
-  if (a[3] != Py_None) same_count(pair(a[3], "out"), m, "out must have a tensor for each cache");
-  for (Py_ssize_t i = 0; i < m; ++i) {
-    const at::Tensor& codes = tensor(PyTuple_GET_ITEM(a[1], i), "codes");
-    c[i] = at.in(codes, "codes");
-    s[i] = at.in(PyTuple_GET_ITEM(a[2], i), "scales");
-    if (a[3] != Py_None) {
-      out[i] = tensor(PyTuple_GET_ITEM(a[3], i), "out");
-    } else {
-      if (codes.dim() != 4 || slots_t.dim() != 1)
-        throw Raise{PyExc_ValueError, "codes must be (page, row, head, code) and slots have one dim"};
-      const int32_t code = small(a[4], "dtype");
-      const at::ScalarType type = code == GPUOS_F32 ? at::kFloat : code == GPUOS_F16 ? at::kHalf : at::kBFloat16;
-      const int64_t head = codes.size(3) * (codes.scalar_type() == at::kByte ? 2 : 1);
-      out[i] = at.make({slots_t.size(0), codes.size(2), head}, type);
-    }
-    o[i] = at.in(out[i], "out");
+  Outputs outs;
+  if (a[3] != Py_None) {
+    const Pair given(a[3], "out");
+    same_count(given.n, cs.n, "out must have a tensor for each cache");
+    for (int i = 0; i < cs.n; ++i) out[i] = tensor(given.o[i], "out");
   }
+  const int32_t code = small(a[4], "dtype");
+  const at::ScalarType type = code == GPUOS_F32 ? at::kFloat : code == GPUOS_F16 ? at::kHalf : at::kBFloat16;
+  for (int i = 0; i < cs.n; ++i) {
+    const at::Tensor& codes = tensor(cs.o[i], "codes");
+    c[i] = at.in(codes, "codes");
+    s[i] = at.in(ss.o[i], "scales");
+    if (a[3] != Py_None) continue;
+    if (codes.dim() != 4 || slots_t.dim() != 1)
+      throw Raise{PyExc_ValueError, "codes must be (page, row, head, code) and slots have one dim"};
+    outs.add({slots_t.size(0), codes.size(2), codes.size(3) * (codes.scalar_type() == at::kByte ? 2 : 1)}, type);
+  }
+  if (a[3] == Py_None) {
+    outs.allocate(at);
+    for (int i = 0; i < cs.n; ++i) out[i] = outs.t[i];
+  }
+  for (int i = 0; i < cs.n; ++i) o[i] = at.in(out[i], "out");
   const gpuos_tensor slots = at.in(slots_t, "slots");
-  done(gpuos_cache_read((int32_t)m, &slots, c, s, o, at.stream()));
-  return tuple_of(out, m);
+  done(gpuos_cache_read(cs.n, &slots, c, s, o, at.stream()));
+  return cs.tuple ? tuple_of(out, cs.n) : wrap(out[0]);
 }
 
 PyObject* route(PyObject* const* a, Py_ssize_t n) {
   arity(n, 9, "(logits, bias, top_k, score, groups, top_groups, group_score, renormalize, scale)");
   const at::Tensor& x = tensor(a[0], "logits");
+  if (recorded(x)) return not_here();
   const Place at(x);
   const gpuos_tensor d = at.in(x, "logits");
   if (x.dim() != 2) throw Raise{PyExc_ValueError, "logits must have 2 dims, not " + std::to_string(x.dim())};
@@ -248,11 +340,14 @@ PyObject* route(PyObject* const* a, Py_ssize_t n) {
   if (a[1] != Py_None) bias = at.in(a[1], "bias");
   const int32_t k = small(a[2], "top_k");
   if (k < 1 || k > 64) throw Raise{PyExc_ValueError, "top_k must be in [1, 64]"};
-  at::Tensor out[2] = {at.make({x.size(0), k}, at::kFloat), at.make({x.size(0), k}, at::kLong)};
-  const gpuos_tensor w = at.in(out[0], "weights"), e = at.in(out[1], "experts");
+  Outputs out;
+  out.add({x.size(0), k}, at::kFloat);
+  out.add({x.size(0), k}, at::kLong);
+  out.allocate(at);
+  const gpuos_tensor w = at.in(out.t[0], "weights"), e = at.in(out.t[1], "experts");
   done(gpuos_route(&d, a[1] != Py_None ? &bias : nullptr, &w, &e, small(a[3], "score"), small(a[4], "groups"),
                    small(a[5], "top_groups"), small(a[6], "group_score"), truth(a[7]), (float)real(a[8]), at.stream()));
-  return tuple_of(out, 2);
+  return tuple_of(out.t, 2);
 }
 
 PyObject* route_grad(PyObject* const* a, Py_ssize_t n) {
@@ -263,12 +358,13 @@ PyObject* route_grad(PyObject* const* a, Py_ssize_t n) {
   const at::Tensor out = at.make(x.sizes(), x.scalar_type());
   const gpuos_tensor o = at.in(out, "grad_logits");
   done(gpuos_route_grad(&d, &e, &g, &o, small(a[3], "score"), truth(a[4]), (float)real(a[5]), at.stream()));
-  return THPVariable_Wrap(out);
+  return wrap(out);
 }
 
 PyObject* logprobs(PyObject* const* a, Py_ssize_t n) {
   arity(n, 6, "(logits, targets, top, entropy, temperature, stats)");
   const at::Tensor& x = tensor(a[0], "logits");
+  if (recorded(x)) return not_here();
   const Place at(x);
   const gpuos_tensor d = at.in(x, "logits"), y = at.in(a[1], "targets");
   if (x.dim() != 2) throw Raise{PyExc_ValueError, "logits must have 2 dims, not " + std::to_string(x.dim())};
@@ -276,17 +372,22 @@ PyObject* logprobs(PyObject* const* a, Py_ssize_t n) {
   if (k < 0 || k > 64) throw Raise{PyExc_ValueError, "top must be in [0, 64]"};
   const bool entropy = truth(a[3]), stats = truth(a[5]);
   const int64_t rows = x.size(0);
-  at::Tensor out[5];  // logprob, entropy, top_logprobs, top_tokens, stats
-  out[0] = at.make({rows}, at::kFloat);
-  if (entropy) out[1] = at.make({rows}, at::kFloat);
+  Outputs outs;
+  int which[5] = {outs.add({rows}, at::kFloat), -1, -1, -1, -1};
+  if (entropy) which[1] = outs.add({rows}, at::kFloat);
   if (k) {
-    out[2] = at.make({rows, k}, at::kFloat);
-    out[3] = at.make({rows, k}, at::kLong);
+    which[2] = outs.add({rows, k}, at::kFloat);
+    which[3] = outs.add({rows, k}, at::kLong);
   }
-  if (stats) out[4] = at.make({rows, 2}, at::kFloat);
+  if (stats) which[4] = outs.add({rows, 2}, at::kFloat);
+  outs.allocate(at);
+  at::Tensor out[5];  // logprob, entropy, top_logprobs, top_tokens, stats
   gpuos_tensor o[5];
   for (int i = 0; i < 5; ++i)
-    if (out[i].defined()) o[i] = at.in(out[i], "out");
+    if (which[i] >= 0) {
+      out[i] = outs.t[which[i]];
+      o[i] = at.in(out[i], "out");
+    }
   done(gpuos_logprobs(&d, &y, &o[0], entropy ? &o[1] : nullptr, k ? &o[2] : nullptr, k ? &o[3] : nullptr,
                       stats ? &o[4] : nullptr, (float)real(a[4]), at.stream()));
   return tuple_of(out, 5);
@@ -305,7 +406,7 @@ PyObject* logprobs_grad(PyObject* const* a, Py_ssize_t n) {
   const gpuos_tensor o = at.in(out, "out");
   done(gpuos_logprobs_grad(&d, &y, &st, a[3] != Py_None ? &opt[0] : nullptr, a[4] != Py_None ? &opt[1] : nullptr,
                            a[5] != Py_None ? &opt[2] : nullptr, &o, (float)real(a[6]), at.stream()));
-  return THPVariable_Wrap(out);
+  return wrap(out);
 }
 
 }  // namespace
@@ -314,9 +415,9 @@ PyObject* logprobs_grad(PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef* gpuos_rowops_methods() {
   static PyMethodDef methods[] = {
-      {"rotary", GPUOS_FAST(rotary), "rotary(xs, outs, positions, inv_freq, scale, interleaved, inverse): see rowops.rotary"},
-      {"cache_write", GPUOS_FAST(cache_write), "cache_write(xs, slots, codes, scales): see rowops.cache_write"},
-      {"cache_read", GPUOS_FAST(cache_read), "cache_read(slots, codes, scales, outs, dtype): see rowops.cache_read"},
+      {"rotary", GPUOS_FAST(rotary), "rotary(x, out, positions, inv_freq, scale, interleaved, inverse): see rowops.rotary"},
+      {"cache_write", GPUOS_FAST(cache_write), "cache_write(x, slots, codes, scales): see rowops.cache_write"},
+      {"cache_read", GPUOS_FAST(cache_read), "cache_read(slots, codes, scales, out, dtype): see rowops.cache_read"},
       {"route", GPUOS_FAST(route),
        "route(logits, bias, top_k, score, groups, top_groups, group_score, renormalize, scale): see rowops.route"},
       {"route_grad", GPUOS_FAST(route_grad),

@@ -27,7 +27,7 @@ from . import load as _load
 from . import scheduler as _scheduler
 
 _ext = _load()
-_entered = _scheduler._entered
+_entered = _scheduler.entered  # empty outside scheduler contexts
 
 _SCORE = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORE = {"max": 0, "top2": 1}
@@ -42,8 +42,9 @@ def _tuple(x) -> tuple:
 
 
 def _order(reads, writes=()):
-    if getattr(_entered, "modes", None):
-        _scheduler.order_after_pending([t for t in reads if t is not None], writes)
+    """Flush what a scheduler context of this thread has pending on a call's tensors."""
+    _scheduler.order_after_pending([t for t in reads if isinstance(t, torch.Tensor)],
+                                   [t for t in writes if isinstance(t, torch.Tensor)])
 
 
 def _choice(table, value, name):
@@ -103,22 +104,20 @@ def rotary(x: Tensors, positions: torch.Tensor, inv_freq: torch.Tensor, *, scale
     ``position * inv_freq`` (in 64 bits) and multiplied by `scale`, in pairs (i, i + half),
     or (2i, 2i + 1) if `interleaved`; the others are copied.  `inverse` rotates back
     (the transposed map, also the gradient).  `out` may be `x`.  Returns tensors as `x` is given."""
-    xs = _tuple(x)
-    outs = None if out is None else _tuple(out)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in xs):
-        if outs is not None:
+    if _entered:
+        _order((*_tuple(x), positions, inv_freq), () if out is None else _tuple(out))
+    got = _ext.rotary(x, out, positions, inv_freq, scale, interleaved, inverse)
+    if got is NotImplemented:  # autograd has to record it
+        if out is not None:
             raise ValueError("out cannot be given where a gradient is needed")
-        got = _Rotary.apply(positions, inv_freq, scale, interleaved, inverse, *xs)
-    else:
-        _order((*xs, positions, inv_freq), outs or ())
-        got = _ext.rotary(xs, outs, positions, inv_freq, scale, interleaved, inverse)
-    return got[0] if isinstance(x, torch.Tensor) else got
+        got = _Rotary.apply(positions, inv_freq, scale, interleaved, inverse, *_tuple(x))
+        return got[0] if isinstance(x, torch.Tensor) else got
+    return got
 
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, positions, inv_freq, scale, interleaved, inverse, *xs):
-        _order((*xs, positions, inv_freq))
         ctx.save_for_backward(positions, inv_freq)
         ctx.how = dict(scale=scale, interleaved=interleaved, inverse=not inverse)
         ctx.set_materialize_grads(False)
@@ -159,22 +158,21 @@ def cache_write(x: Tensors, slots: torch.Tensor, codes: Tensors, scales: Tensors
     through its pages.  A slot outside the cache (-1: padding) writes nothing; the
     slots inside it must differ.  `codes` and `scales` as from ``cache_alloc``, one of each
     for each of `x`; any strides but the last (a page may hold its heads before its rows)."""
-    xs, cs, ss = _tuple(x), _tuple(codes), _tuple(scales)
-    _order((*xs, slots), (*cs, *ss))
-    _ext.cache_write(xs, slots, cs, ss)
+    if _entered:
+        _order((*_tuple(x), slots), (*_tuple(codes), *_tuple(scales)))
+    _ext.cache_write(x, slots, codes, scales)
 
 
 def cache_read(slots: torch.Tensor, codes: Tensors, scales: Tensors, *, dtype: torch.dtype = torch.bfloat16,
                out: Optional[Tensors] = None) -> Tensors:
     """The rows of a cache at `slots` (token, head, element) in `dtype`, or written
     to `out`; zeros for a slot outside the cache.  Returns tensors as `codes` is given."""
-    cs, ss = _tuple(codes), _tuple(scales)
-    outs = None if out is None else _tuple(out)
-    _order((slots, *cs, *ss), outs or ())
-    if dtype not in _ROW_DTYPE:
+    if _entered:
+        _order((slots, *_tuple(codes), *_tuple(scales)), () if out is None else _tuple(out))
+    code = _ROW_DTYPE.get(dtype)
+    if code is None:
         raise TypeError("dtype must be float32, float16 or bfloat16")
-    got = _ext.cache_read(slots, cs, ss, outs, _ROW_DTYPE[dtype])
-    return got[0] if isinstance(codes, torch.Tensor) else got
+    return _ext.cache_read(slots, codes, scales, out, code)
 
 
 # ---- routing -----------------------------------------------------------------------
@@ -188,25 +186,26 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Opt
     worth its largest key, or with ``group_score="top2"`` the sum of its two
     largest.  Weights are the scores, divided by their sum if `renormalize`, times `scale`.
     The choice is that of exact arithmetic."""
-    how = (_choice(_SCORE, score, "score"), groups, top_groups, _choice(_GROUP_SCORE, group_score, "group_score"),
-           renormalize, scale)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _Route.apply(logits, bias, top_k, how)
-    _order((logits, bias))
-    return _ext.route(logits, bias, top_k, *how)
+    if _entered:
+        _order((logits, bias))
+    kind, rule = _choice(_SCORE, score, "score"), _choice(_GROUP_SCORE, group_score, "group_score")
+    got = _ext.route(logits, bias, top_k, kind, groups, top_groups, rule, renormalize, scale)
+    if got is NotImplemented:  # autograd has to record it
+        return _Route.apply(logits, bias, top_k, (kind, groups, top_groups, rule, renormalize, scale))
+    return got
 
 
 def route_grad(logits: torch.Tensor, experts: torch.Tensor, grad_weights: torch.Tensor, *, score: str = "softmax",
                renormalize: bool = False, scale: float = 1.0) -> torch.Tensor:
     """The gradient of the logits from that of ``route``'s weights (float32)."""
-    _order((logits, experts, grad_weights))
+    if _entered:
+        _order((logits, experts, grad_weights))
     return _ext.route_grad(logits, experts, grad_weights, _choice(_SCORE, score, "score"), renormalize, scale)
 
 
 class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, bias, top_k, how):
-        _order((logits, bias))
         weights, experts = _ext.route(logits, bias, top_k, *how)
         ctx.save_for_backward(logits, experts)
         ctx.how = (how[0], how[4], how[5])
@@ -217,7 +216,8 @@ class _Route(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_weights, _):
         logits, experts = ctx.saved_tensors
-        _order((logits, experts, grad_weights))
+        if _entered:
+            _order((logits, experts, grad_weights))
         return _ext.route_grad(logits, experts, grad_weights, *ctx.how), None, None, None
 
 
@@ -238,10 +238,12 @@ def logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0, entro
     most 64; of equal logits the lowest index first), with `stats` what
     ``logprobs_grad`` needs.  A negative target is padding (0).  Gradients flow to
     the logits from ``logprob`` and ``entropy``."""
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return LogProbs(*_LogProbs.apply(logits, targets, top, entropy, temperature))
-    _order((logits, targets))
-    return LogProbs(*_ext.logprobs(logits, targets, top, entropy, temperature, stats))
+    if _entered:
+        _order((logits, targets))
+    got = _ext.logprobs(logits, targets, top, entropy, temperature, stats)
+    if got is NotImplemented:  # autograd has to record it
+        got = _LogProbs.apply(logits, targets, top, entropy, temperature)
+    return LogProbs._make(got)
 
 
 def logprobs_grad(logits: torch.Tensor, targets: torch.Tensor, result: LogProbs,
@@ -252,14 +254,14 @@ def logprobs_grad(logits: torch.Tensor, targets: torch.Tensor, result: LogProbs,
     arguments.  `out` may be `logits`."""
     if result.stats is None:
         raise ValueError("result has no stats: call logprobs(..., stats=True)")
-    _order((logits, targets, result.stats, result.entropy, grad_logprob, grad_entropy), () if out is None else (out,))
+    if _entered:
+        _order((logits, targets, result.stats, result.entropy, grad_logprob, grad_entropy), (out,))
     return _ext.logprobs_grad(logits, targets, result.stats, result.entropy, grad_logprob, grad_entropy, temperature, out)
 
 
 class _LogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top, entropy, temperature):
-        _order((logits, targets))
         got = _ext.logprobs(logits, targets, top, entropy, temperature, True)
         ctx.save_for_backward(logits, targets, got[1], got[4])
         ctx.temperature = temperature
@@ -273,6 +275,7 @@ class _LogProbs(torch.autograd.Function):
         if grad_logprob is None and grad_entropy is None:
             return (None,) * 5
         logits, targets, entropy, stats = ctx.saved_tensors
-        _order((logits, targets, stats, entropy, grad_logprob, grad_entropy))
+        if _entered:
+            _order((logits, targets, stats, entropy, grad_logprob, grad_entropy))
         return (_ext.logprobs_grad(logits, targets, stats, entropy, grad_logprob, grad_entropy, ctx.temperature,
                                    None),) + (None,) * 4

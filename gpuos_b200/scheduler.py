@@ -467,7 +467,7 @@ class _GPUOSSchedulerMode(torch.utils._python_dispatch.TorchDispatchMode):
         return None
 
 
-_entered = threading.local()  # .modes: the modes of the scheduler contexts this thread is in
+entered: List[Tuple[int, "_GPUOSSchedulerMode"]] = []  # (thread, mode) of each context entered
 
 
 def order_after_pending(reads, writes) -> None:
@@ -475,10 +475,11 @@ def order_after_pending(reads, writes) -> None:
     dispatcher: inside a scheduler context of this thread, flush the pending
     requests that write what is in `reads`, or touch what is in `writes`, as an op that
     runs in torch does."""
-    for mode in getattr(_entered, "modes", ()):
-        if mode.pending and (any(_overlaps(_extent(t), mode._w) for t in reads) or
-                             any(_overlaps(_extent(t), tab) for t in writes
-                                 for tab in (mode._w, mode._r))):
+    me = threading.get_ident()
+    for thread, mode in entered:
+        if thread == me and mode.pending and (
+                any(_overlaps(_extent(t), mode._w) for t in reads) or
+                any(_overlaps(_extent(t), tab) for t in writes for tab in (mode._w, mode._r))):
             mode.sync()
 
 
@@ -503,7 +504,7 @@ class GPUOSScheduler:
                                          pending=self._pending, jit=not _jit_disabled(),
                                          fuse=_fuse_enabled())
         self._mode.__enter__()
-        _entered.modes = getattr(_entered, "modes", ()) + (self._mode,)
+        entered.append((threading.get_ident(), self._mode))
         return self
 
     def flush(self, sync: bool = False):
@@ -518,8 +519,7 @@ class GPUOSScheduler:
     def __exit__(self, exc_type, exc, tb):
         try:
             if self._mode is not None:
-                _entered.modes = tuple(m for m in getattr(_entered, "modes", ())
-                                       if m is not self._mode)
+                entered[:] = [e for e in entered if e[1] is not self._mode]
                 self._mode.close()
                 self._mode.submit_nodes()
                 self._mode.__exit__(exc_type, exc, tb)
