@@ -36,9 +36,11 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kMaxTop = 64;
-constexpr int kRowThreads = 256;  // of a CTA; short rows take 128
+constexpr int kRowThreads = 256;  // of a row; short rows take a warp each, 8 to a CTA
 constexpr int kList = 128;    // candidates a warp holds
-constexpr int kSeeds = 64;    // maxima that give the first bound
+constexpr int kWarpPacks = 128;  // 16-byte packs of a row that one warp takes,
+constexpr int kWarpPacksMany = 3200, kWarpRows = 8;  // and where there are many rows for each SM
+constexpr int kFewTop = 32;   // alternatives up to which 64 maxima give a close bound
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kLowest = -3.402823466e38f;  // the lowest finite number: where a maximum starts
 
@@ -158,7 +160,7 @@ __device__ __forceinline__ void add_two(Sums& r, float2 x, float k2) {
 }
 
 constexpr uint32_t kMarks = 16;    // maxima a thread leaves on its way along a row
-constexpr uint32_t kReach = 512;   // of them that may reach the bound, and
+constexpr uint32_t kReach = 4;     // of them a thread, on average, may reach the bound, and
 constexpr uint32_t kFew = 4;       // packs a thread then reads again, before the lists are used
 
 // Kept small: what the CTAs of an SM do not take of its memory holds their loads
@@ -168,11 +170,12 @@ struct TopShared {
   static constexpr uint32_t kWarps = THREADS / 32;
   static constexpr uint32_t kPool = std::max<uint32_t>(kMarks * THREADS * sizeof(T) / 8, kWarps * (kList + kMaxTop));
   static constexpr uint32_t kAll = std::min<uint32_t>(kPool, 1024);
+  static constexpr uint32_t kReached = kReach * THREADS;
   unsigned long long bound;          // no candidate below it is needed
   uint32_t count;                    // of the candidates
   uint32_t reached;                  // of `reach`
-  float seeds[kSeeds];
-  uint32_t reach[kReach];            // (mark, thread) whose maximum reaches the bound
+  alignas(16) float seeds[THREADS];
+  uint32_t reach[kReached];           // (mark, thread) whose maximum reaches the bound
   unsigned long long last[kMaxTop];  // the top_k, sorted
   // one after the other: the marks; the candidates; where those are too many, each
   // warp's list, and behind them the lists joined
@@ -182,6 +185,21 @@ struct TopShared {
   __device__ unsigned long long* list(uint32_t warp) { return pool + warp * kList; }
   __device__ unsigned long long* joined() { return pool + kWarps * kList; }
 };
+
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// The threads of a row: a CTA, or a warp of one.
+template <int THREADS>
+__device__ __forceinline__ void row_sync() {
+  if constexpr (THREADS == 32) __syncwarp();
+  else __syncthreads();
+}
+
+template <int THREADS> constexpr int kRowsOfCta = THREADS == 32 ? 8 : 1;
 
 template <int THREADS> struct RowShared;
 template <int THREADS> constexpr size_t kTopAt = (sizeof(RowShared<THREADS>) + 15) / 16 * 16;
@@ -263,32 +281,88 @@ __device__ __forceinline__ uint32_t candidates(const Pack<T, N>& x, uint32_t at,
 // below k go to out, sorted.
 template <int THREADS>
 __device__ __forceinline__ void rank_into(const unsigned long long* keys, uint32_t n, uint32_t k, unsigned long long* out) {
+  const uint32_t tid = threadIdx.x % THREADS;
   for (uint32_t i0 = 0; i0 < n; i0 += THREADS / 8) {
-    const uint32_t i = i0 + threadIdx.x / 8;
+    const uint32_t i = i0 + tid / 8;
     const unsigned long long mine = i < n ? keys[i] : 0;
     uint32_t rank = 0;
-    for (uint32_t j = threadIdx.x & 7; j < n; j += 8) rank += keys[j] > mine;
+#pragma unroll 4
+    for (uint32_t j = tid & 7; j < n; j += 8) rank += keys[j] > mine;
 #pragma unroll
     for (int d = 1; d < 8; d <<= 1) rank += __shfl_xor_sync(~0u, rank, d);
-    if ((threadIdx.x & 7) == 0 && i < n && rank < k) out[rank] = mine;
+    if ((tid & 7) == 0 && i < n && rank < k) out[rank] = mine;
   }
+}
+
+// The bound: a value that k of the row's elements reach, from the threads' maxima.
+// For few alternatives the k-th largest of 64 maxima over neighbouring threads is close;
+// for more each thread's counts
+// (64 alternatives of 8 x 32000: 23 us, 48 us from 64 maxima, whose last one is far too low;
+// 20: 12.2 us, 8.6 us from 64).
+template <typename T, int THREADS>
+__device__ __forceinline__ void find_bound(TopShared<T, THREADS>& top, float m, uint32_t k) {
+  const int tid = threadIdx.x % THREADS;
+  uint32_t rank = 0;
+  float me = m;
+  bool mine = true;
+  if constexpr (THREADS == 32) {
+    // a round for each alternative: the largest of those left
+    for (uint32_t i = 0; i < k; ++i) {
+      me = warp_max(m);
+      if (tid == __ffs(__ballot_sync(~0u, m == me)) - 1) m = -INFINITY;
+    }
+    mine = tid == 0;
+    rank = k - 1;
+  } else if (k <= kFewTop) {
+    constexpr int S = 64, L = THREADS / S;
+#pragma unroll
+    for (int d = 1; d < L; d <<= 1) me = fmaxf(me, __shfl_xor_sync(~0u, me, d));
+    if (tid % L == 0) top.seeds[tid / L] = me;
+    __syncthreads();
+#pragma unroll
+    for (int j = tid % L; j < S; j += L) {
+      const float o = top.seeds[j];
+      rank += o > me || (o == me && j < tid / L);
+    }
+#pragma unroll
+    for (int d = 1; d < L; d <<= 1) rank += __shfl_xor_sync(~0u, rank, d);
+    mine = tid % L == 0;
+  } else {
+    top.seeds[tid] = me;
+    __syncthreads();
+#pragma unroll 4
+    for (int j = 0; j < THREADS; j += 4) {
+      const float4 o = *reinterpret_cast<const float4*>(top.seeds + j);
+      rank += (o.x > me || (o.x == me && j < tid)) + (o.y > me || (o.y == me && j + 1 < tid)) +
+              (o.z > me || (o.z == me && j + 2 < tid)) + (o.w > me || (o.w == me && j + 3 < tid));
+    }
+  }
+  // A maximum that is still where it started was reached by nothing: no bound.
+  // Otherwise every element of this value and above counts, whatever its index.
+  if (mine && rank == k - 1 && me > kLowest) top.bound = key_of(me, 0) & ~0xffffffffull;
+  row_sync<THREADS>();
 }
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
+template <typename T, int THREADS, bool TOP>
+constexpr size_t kSharedOfRow = (kTopAt<THREADS> + (TOP ? sizeof(TopShared<T, THREADS>) : 0) + 15) / 16 * 16;
+
 template <typename T, int THREADS, bool ENT, bool TOP>
-__global__ void __launch_bounds__(THREADS, THREADS == kRowThreads ? 6 : 1)
+__global__ void __launch_bounds__(THREADS * kRowsOfCta<THREADS>, THREADS == 32 ? 5 : 6)
 gpuos_logprobs_kernel(const __grid_constant__ LogArgs a) {
   constexpr int W = 16 / sizeof(T);
   constexpr int U = 4;  // packs a thread has in flight
   extern __shared__ __align__(16) uint8_t smem[];
-  RowShared<THREADS>& sh = *reinterpret_cast<RowShared<THREADS>*>(smem);
-  TopShared<T, THREADS>& top = *reinterpret_cast<TopShared<T, THREADS>*>(smem + kTopAt<THREADS>);
+  const uint32_t tid = threadIdx.x % THREADS, lane = tid & 31, warp = tid / 32;
+  uint8_t* mem = smem + threadIdx.x / THREADS * kSharedOfRow<T, THREADS, TOP>;
+  RowShared<THREADS>& sh = *reinterpret_cast<RowShared<THREADS>*>(mem);
+  TopShared<T, THREADS>& top = *reinterpret_cast<TopShared<T, THREADS>*>(mem + kTopAt<THREADS>);
   cg::cluster_group cluster = cg::this_cluster();
-  const uint32_t parts = cluster.num_blocks(), part = cluster.block_rank();
-  const int64_t row = blockIdx.x / parts;
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  const uint32_t parts = THREADS == 32 ? 1 : cluster.num_blocks(), part = THREADS == 32 ? 0 : cluster.block_rank();
+  const int64_t row = (int64_t)(blockIdx.x / parts) * kRowsOfCta<THREADS> + threadIdx.x / THREADS;
+  if (THREADS == 32 && row >= a.rows) return;
   const T* x = static_cast<const T*>(a.x) + row * a.xs;
 
   // the row is a head up to the first 16-byte boundary, whole packs, and a tail
@@ -300,20 +374,23 @@ gpuos_logprobs_kernel(const __grid_constant__ LogArgs a) {
   const uint32_t tail = head + packs * W;
   const T* body = x + head;
 
-  // read ahead: the row's last step needs it
+  // read ahead: the row's end needs it
   int64_t target = -1;
   float target_x = 0.f;
-  if (part == 0 && threadIdx.x == 0) {
+  if (part == 0 && tid == 0) {
     target = load_index(a.targets, a.target_wide, row * a.ts);
     if (target >= 0 && target < a.cols) target_x = to_f(x[target]);
   }
   if (parts > 1) cluster_arrive();
 
   Sums r;
-  if (TOP && threadIdx.x == 0) {
-    top.bound = 0;
-    top.count = 0;
-    top.reached = 0;
+  if (TOP) {
+    if (tid == 0) {
+      top.bound = 0;
+      top.count = 0;
+      top.reached = 0;
+    }
+    for (uint32_t i = tid; i < a.top_k; i += THREADS) top.last[i] = 0;
   }
 
   // the loose elements, at most 2 (W - 1), go to the last part's first warp
@@ -325,8 +402,26 @@ gpuos_logprobs_kernel(const __grid_constant__ LogArgs a) {
     if (has_loose) {
       loose_at = lane < head ? lane : tail + (lane - head);
       loose.v[0] = x[loose_at];
+      raise<ENT>(r, to_f(loose.v[0]), a.k2);
+      add_two<ENT>(r, make_float2(to_f(loose.v[0]), -INFINITY), a.k2);
     }
   }
+
+  // the candidates of a pack at index `at`, of `bound` and above
+  auto push = [&](const auto& q, uint32_t at, unsigned long long bound) {
+    constexpr int N = sizeof(q.v) / sizeof(T);
+    uint32_t open = candidates<T, N>(q, at, bound);
+    while (open) {
+      const int e = __ffs(open) - 1;
+      open &= open - 1;
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (e == i) v = to_f(q.v[i]);
+      const uint32_t n = atomicAdd(&top.count, 1u);
+      if (n < top.kAll) top.pool[n] = key_of(v, at + e);
+    }
+  };
 
   const uint32_t steps = (p1 - p0 + THREADS * U - 1) / (THREADS * U);
   const uint32_t stretch = (steps + kMarks - 1) / kMarks;  // steps a mark covers
@@ -335,7 +430,7 @@ gpuos_logprobs_kernel(const __grid_constant__ LogArgs a) {
   for (uint32_t base = p0; base < p1; base += THREADS * U) {
     // a step: U packs a thread, all of them or (the last step) those below p1
     Pack<T, W> q[U];
-    const uint32_t mine = base + threadIdx.x;
+    const uint32_t mine = base + tid;
     const bool whole = base + THREADS * U <= p1;
     if (whole) {
 #pragma unroll
@@ -356,11 +451,22 @@ gpuos_logprobs_kernel(const __grid_constant__ LogArgs a) {
     for (int u = 1; u < U; ++u) cm = fmaxf(cm, max_of(q[u]));
     raise<ENT>(r, cm, a.k2);
     if (TOP) {
-      marked = fmaxf(marked, cm);
-      if (--left == 0 || base + THREADS * U >= p1) {
-        top.marks()[mark++ * THREADS + threadIdx.x] = from_f<T>(marked);
-        marked = -INFINITY;
-        left = stretch;
+      if (THREADS == 32 && steps == 1) {
+        // the whole row is in registers: its candidates are taken from there
+        find_bound<T, THREADS>(top, r.m, a.top_k);
+        const unsigned long long bound = top.bound;
+        if (!(cm < value_of(bound)))
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (mine + u * THREADS < p1) push(q[u], head + (mine + u * THREADS) * W, bound);
+        if (has_loose) push(loose, loose_at, bound);
+      } else {
+        marked = fmaxf(marked, cm);
+        if (--left == 0 || base + THREADS * U >= p1) {
+          top.marks()[mark++ * THREADS + tid] = from_f<T>(marked);
+          marked = -INFINITY;
+          left = stretch;
+        }
       }
     }
     // a last step's missing packs are -inf: terms of 0
@@ -369,95 +475,56 @@ gpuos_logprobs_kernel(const __grid_constant__ LogArgs a) {
 #pragma unroll
       for (int i = 0; i < W; i += 2) add_two<ENT>(r, make_float2(to_f(q[u].v[i]), to_f(q[u].v[i + 1])), a.k2);
   }
-  if (has_loose) {
-    const float v = to_f(loose.v[0]);
-    raise<ENT>(r, v, a.k2);
-    add_two<ENT>(r, make_float2(v, -INFINITY), a.k2);
-  }
 
   // join: lanes, warps, then the cluster's CTAs, always in the same order
   const Running t = join_lanes<32, ENT>(Running{r.m, r.s.x + r.s.y, r.w.x + r.w.y}, a.k2);
-  if (lane == 0) {
+  if (THREADS > 32 && lane == 0) {
     sh.m[warp] = t.m;
     sh.s[warp] = t.s;
     sh.w[warp] = t.w;
   }
-  constexpr int L = THREADS / kSeeds;  // lanes to a seed
-  if (TOP) {
-    float m = r.m;
-#pragma unroll
-    for (int d = 1; d < L; d <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
-    if (threadIdx.x % L == 0) top.seeds[threadIdx.x / L] = m;
-  }
-  __syncthreads();
-  if (TOP) {
-    const int seed = threadIdx.x / L;
-    const float me = top.seeds[seed];
-    uint32_t rank = 0;
-#pragma unroll
-    for (int j = threadIdx.x % L; j < kSeeds; j += L) {
-      const float o = top.seeds[j];
-      rank += o > me || (o == me && j < seed);
-    }
-#pragma unroll
-    for (int d = 1; d < L; d <<= 1) rank += __shfl_xor_sync(~0u, rank, d);
-    // A maximum that is still where it started was reached by nothing: no bound.
-    // Otherwise every element of this value and above counts, whatever its index.
-    if (threadIdx.x % L == 0 && rank == a.top_k - 1 && me > kLowest) top.bound = key_of(me, 0) & ~0xffffffffull;
-    for (uint32_t i = threadIdx.x; i < a.top_k; i += THREADS) top.last[i] = 0;
-    __syncthreads();
+  bool few = true;
+  if (TOP && !(THREADS == 32 && steps == 1)) {
+    find_bound<T, THREADS>(top, r.m, a.top_k);
     const unsigned long long bound = top.bound;
     if (r.m >= value_of(bound))
       for (uint32_t i = 0; i < mark; ++i)
-        if (to_f(top.marks()[i * THREADS + threadIdx.x]) >= value_of(bound)) {
+        if (to_f(top.marks()[i * THREADS + tid]) >= value_of(bound)) {
           const uint32_t n = atomicAdd(&top.reached, 1u);
-          if (n < kReach) top.reach[n] = i << 16 | threadIdx.x;
+          if (n < top.kReached) top.reach[n] = i << 16 | tid;
         }
-    __syncthreads();
+    row_sync<THREADS>();
     // the packs under those marks, a lane each
     const uint32_t each = stretch * U;
-    const bool few = top.reached <= kReach && (uint64_t)top.reached * each <= kFew * THREADS;
+    few = top.reached <= top.kReached && (uint64_t)top.reached * each <= kFew * THREADS;
     if (few) {
       const uint32_t items = top.reached * each;
       Pack<T, W> q[kFew];
       uint32_t at[kFew];
 #pragma unroll
       for (int u = 0; u < kFew; ++u) {
-        const uint32_t it = u * THREADS + threadIdx.x;
+        const uint32_t it = u * THREADS + tid;
         at[u] = p1;
         if (it < items) {
           const uint32_t i = it / each, to = top.reach[i];
           at[u] = p0 + ((to >> 16) * each + (it - i * each)) * THREADS + (to & 0xffff);
         }
-        if (at[u] < p1) q[u] = load_pack<T, W>(body + (uint64_t)at[u] * W);
+        if (at[u] < p1) q[u] = load_pack<T, W, false>(body + (uint64_t)at[u] * W);
       }
 #pragma unroll
-      for (int u = 0; u < kFew; ++u) {
-        if (at[u] >= p1) continue;
-        uint32_t open = candidates<T, W>(q[u], head + at[u] * W, bound);
-        while (open) {
-          const int e = __ffs(open) - 1;
-          open &= open - 1;
-          float v = 0.f;
-#pragma unroll
-          for (int i = 0; i < W; ++i)
-            if (e == i) v = to_f(q[u].v[i]);
-          const uint32_t n = atomicAdd(&top.count, 1u);
-          if (n < top.kAll) top.pool[n] = key_of(v, head + at[u] * W + e);
-        }
-      }
-      if (has_loose && candidates<T, 1>(loose, loose_at, bound)) {
-        const uint32_t n = atomicAdd(&top.count, 1u);
-        if (n < top.kAll) top.pool[n] = key_of(to_f(loose.v[0]), loose_at);
-      }
+      for (int u = 0; u < kFew; ++u)
+        if (at[u] < p1) push(q[u], head + at[u] * W, bound);
+      if (has_loose) push(loose, loose_at, bound);
     }
-    __syncthreads();
+  }
+  row_sync<THREADS>();
+  if (TOP) {
     if (!few || top.count > top.kAll) {
       // many equal or masked logits: the row again, through lists that are cut
-      __syncthreads();
-      if (threadIdx.x == 0) top.count = 0;
+      row_sync<THREADS>();
+      if (tid == 0) top.count = 0;
       uint32_t count = 0;  // of this warp's list
-      for (uint32_t p = p0 + threadIdx.x; __any_sync(~0u, p < p1); p += THREADS) {
+      for (uint32_t p = p0 + tid; __any_sync(~0u, p < p1); p += THREADS) {
         Pack<T, W> q;
         uint32_t open = 0;
         if (p < p1) {
@@ -470,13 +537,13 @@ gpuos_logprobs_kernel(const __grid_constant__ LogArgs a) {
         offer<T, 1>(loose, has_loose ? candidates<T, 1>(loose, loose_at, *(volatile unsigned long long*)&top.bound) : 0u,
                     loose_at, a.top_k, top.list(warp), count, &top.bound);
       if (count > a.top_k) count = cut(top.list(warp), count, a.top_k, &top.bound);
-      __syncthreads();
+      row_sync<THREADS>();
       const unsigned long long b = *(volatile unsigned long long*)&top.bound;
       for (uint32_t i = lane; i < count; i += 32) {
         const unsigned long long key = top.list(warp)[i];
         if (key >= b) top.joined()[atomicAdd(&top.count, 1u)] = key;
       }
-      __syncthreads();
+      row_sync<THREADS>();
       rank_into<THREADS>(top.joined(), top.count, a.top_k, top.last);
     } else {
       rank_into<THREADS>(top.pool, top.count, a.top_k, top.last);
@@ -491,10 +558,10 @@ gpuos_logprobs_kernel(const __grid_constant__ LogArgs a) {
     to = cluster.map_shared_rank(to, 0);
     if (TOP) {
       unsigned long long* best = cluster.map_shared_rank(top.best, 0) + part * a.top_k;
-      for (uint32_t i = threadIdx.x; i < a.top_k; i += THREADS) best[i] = top.last[i];
+      for (uint32_t i = tid; i < a.top_k; i += THREADS) best[i] = top.last[i];
     }
   }
-  if (warp == THREADS / 32 - 1) {
+  if (THREADS > 32 && warp == THREADS / 32 - 1) {
     Running c;
     if (lane < THREADS / 32) c = Running{sh.m[lane], sh.s[lane], sh.w[lane]};
     c = join_lanes<THREADS / 32, ENT>(c, a.k2);
@@ -504,14 +571,29 @@ gpuos_logprobs_kernel(const __grid_constant__ LogArgs a) {
     cluster_arrive();
     if (part != 0) return;
     cluster_wait();
-    if (TOP) rank_into<THREADS>(top.best, parts * a.top_k, a.top_k, top.last);
+    if (TOP) {
+      // each part has `share` keys no smaller than the smallest of the parts' share-th ones, so
+      // all together top_k or more: smaller ones drop out before the rest are ranked
+      const uint32_t share = (a.top_k + parts - 1) / parts;
+      unsigned long long least = ~0ull;
+      for (uint32_t i = 0; i < parts; ++i) least = min(least, top.best[i * a.top_k + share - 1]);
+      if (tid == 0) top.count = 0;
+      __syncthreads();
+      for (uint32_t i = tid; i < parts * a.top_k; i += THREADS)
+        if (top.best[i] >= least && top.best[i] != 0) top.pool[atomicAdd(&top.count, 1u)] = top.best[i];
+      __syncthreads();
+      rank_into<THREADS>(top.pool, top.count, a.top_k, top.last);
+    }
   }
-  __syncthreads();
+  row_sync<THREADS>();
   if (warp != 0) return;
-  Running c;
-  if (lane < parts) c = sh.part[lane];
-  c = join_lanes<8, ENT>(c, a.k2);
-  c = Running{__shfl_sync(~0u, c.m, 0), __shfl_sync(~0u, c.s, 0), __shfl_sync(~0u, c.w, 0)};
+  Running c = THREADS == 32 ? t : sh.part[0];
+  if (parts > 1) {
+    c = Running{};
+    if (lane < parts) c = sh.part[lane];
+    c = join_lanes<8, ENT>(c, a.k2);
+    c = Running{__shfl_sync(~0u, c.m, 0), __shfl_sync(~0u, c.s, 0), __shfl_sync(~0u, c.w, 0)};
+  }
   const float ln_s = logf(c.s);
   const bool none = c.s == 0.f;  // every logit is -inf
   if (lane == 0) {
@@ -537,37 +619,19 @@ gpuos_logprobs_kernel(const __grid_constant__ LogArgs a) {
   }
 }
 
-constexpr int kGradThreads = 256;
+constexpr int kGradThreads = 128;
 constexpr int kGradPacks = 4;
 
 // One CTA a stretch of a row: the row's constants are folded into
 // dx = e (A + B y) with y = (x - m) log2(e) / t, e = 2^y.
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool ENT>
 __global__ void __launch_bounds__(kGradThreads)
 gpuos_logprobs_grad_kernel(const __grid_constant__ LogArgs a) {
   constexpr int W = VEC ? 16 / sizeof(T) : 1;
-  // from the last row on: forward read it last, so that it may still be in L2
-  const uint32_t from_end = blockIdx.x / a.parts, part = blockIdx.x - from_end * a.parts;
-  const int64_t row = a.rows - 1 - from_end;
+  const int64_t row = blockIdx.x / a.parts;
+  const uint32_t part = blockIdx.x - (uint32_t)row * a.parts;
   const T* x = static_cast<const T*>(a.x) + row * a.xs;
   T* o = static_cast<T*>(a.gx) + row * a.gs;
-  const int64_t y = load_index(a.targets, a.target_wide, row * a.ts);
-  const float m = a.stats[row * a.ss], s = a.stats[row * a.ss + a.sk];
-  float g = a.gl && y >= 0 ? a.gl[row * a.gls] : 0.f;
-  if (a.gl && y >= a.cols) g = NAN;
-  const float h = a.ge ? a.ge[row * a.ges] : 0.f;
-  const float H = a.ge ? a.entropy[row * a.es] : 0.f;
-  const bool none = s == 0.f;
-  const float c0 = none ? 0.f : -a.inv_t / s;
-  const float A = none ? 0.f : c0 * (g + h * (H - logf(s))), B = c0 * h * (kLn2);
-  const float hit = none ? 0.f : g * a.inv_t;
-
-  auto value = [&](float v, int64_t at) {
-    const float y2 = fmaxf((v - m) * a.k2, -1e4f);
-    float d = v == v ? ex2(y2) * fmaf(B, y2, A) : NAN;
-    if (at == y) d += hit;
-    return d;
-  };
   const uint32_t cols = (uint32_t)a.cols;
   uint32_t head = 0;
   if (VEC) {
@@ -576,36 +640,77 @@ gpuos_logprobs_grad_kernel(const __grid_constant__ LogArgs a) {
   }
   const uint32_t packs = (cols - head) / W, tail = head + packs * W;
   const uint32_t base = part * (kGradThreads * kGradPacks) + threadIdx.x;
-  if (VEC && part == 0) {
-    for (uint32_t i = threadIdx.x; i < head; i += kGradThreads) o[i] = from_f<T>(value(to_f(x[i]), i));
-    for (uint32_t i = tail + threadIdx.x; i < cols; i += kGradThreads) o[i] = from_f<T>(value(to_f(x[i]), i));
-  }
   Pack<T, W> q[kGradPacks];
 #pragma unroll
   for (int u = 0; u < kGradPacks; ++u) {
     const uint32_t p = base + u * kGradThreads;
     if (p < packs) q[u] = load_pack<T, W>(x + head + (uint64_t)p * W);
   }
+
+  const int64_t y = load_index(a.targets, a.target_wide, row * a.ts);
+  const float m = a.stats[row * a.ss], s = a.stats[row * a.ss + a.sk];
+  float g = a.gl && y >= 0 ? a.gl[row * a.gls] : 0.f;
+  if (a.gl && y >= a.cols) g = NAN;
+  const float h = ENT ? a.ge[row * a.ges] : 0.f, H = ENT ? a.entropy[row * a.es] : 0.f;
+  const bool none = s == 0.f;
+  const float c0 = none ? 0.f : -a.inv_t / s;
+  const float A = none ? 0.f : ENT ? c0 * (g + h * (H - logf(s))) : c0 * g, B = c0 * h * kLn2;
+  const float hit = none ? 0.f : g * a.inv_t;
+  const uint32_t at_y = y >= 0 && y < a.cols ? (uint32_t)y : ~0u;
+
+  auto two = [&](float2 v) {
+    const float2 z = mul2(add2(v, both(-m)), both(a.k2));
+    const float2 e = make_float2(ex2(z.x), ex2(z.y));
+    if (!ENT) return mul2(e, both(A));
+    // a masked element's z is -inf: e is 0, and its factor must stay finite
+    return mul2(e, fma2(make_float2(fmaxf(z.x, -1e4f), fmaxf(z.y, -1e4f)), both(B), both(A)));
+  };
+  auto one = [&](uint32_t i) {
+    const float d = two(make_float2(to_f(x[i]), 0.f)).x + (i == at_y ? hit : 0.f);
+    o[i] = from_f<T>(d);
+  };
+  if (VEC && part == 0) {
+    if (threadIdx.x < head) one(threadIdx.x);
+    if (threadIdx.x < cols - tail) one(tail + threadIdx.x);
+  }
 #pragma unroll
   for (int u = 0; u < kGradPacks; ++u) {
     const uint32_t p = base + u * kGradThreads;
     if (p >= packs) break;
-    const int64_t at = head + (int64_t)p * W;
+    const uint32_t at = head + p * W;
+    float d[W];
+    if constexpr (W == 1) {
+      d[0] = two(make_float2(to_f(q[u].v[0]), 0.f)).x;
+    } else {
 #pragma unroll
-    for (int i = 0; i < W; ++i) q[u].v[i] = from_f<T>(value(to_f(q[u].v[i]), at + i));
-    store_pack<T, W>(o + at, q[u]);
+      for (int i = 0; i < W; i += 2) {
+        const float2 r = two(make_float2(to_f(q[u].v[i]), to_f(q[u].v[i + 1])));
+        d[i] = r.x;
+        d[i + 1] = r.y;
+      }
+    }
+    if (at_y - at < (uint32_t)W) {
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        if (at + i == at_y) d[i] += hit;
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) q[u].v[i] = from_f<T>(d[i]);
+    if constexpr (VEC) __stcs(reinterpret_cast<uint4*>(o + at), *reinterpret_cast<const uint4*>(&q[u]));
+    else o[at] = q[u].v[0];
   }
 }
 
 template <typename T, int THREADS, bool ENT, bool TOP>
 void launch(const LogArgs& a, uint32_t parts, cudaStream_t s) {
-  const size_t smem = kTopAt<THREADS> + (TOP ? sizeof(TopShared<T, THREADS>) + (parts > 1 ? parts * a.top_k * 8 : 0) : 0);
+  constexpr int kRows = kRowsOfCta<THREADS>;
+  const size_t smem = kRows * kSharedOfRow<T, THREADS, TOP> + (TOP && parts > 1 ? parts * a.top_k * 8 : 0);
   auto kernel = gpuos_logprobs_kernel<T, THREADS, ENT, TOP>;
   if (smem > 48 * 1024)
     cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory");
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(a.rows * parts));
-  cfg.blockDim = dim3(THREADS);
+  cfg.gridDim = dim3((unsigned)((a.rows + kRows - 1) / kRows * parts));
+  cfg.blockDim = dim3(THREADS * kRows);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
@@ -613,7 +718,7 @@ void launch(const LogArgs& a, uint32_t parts, cudaStream_t s) {
   at[0].val.clusterDim.x = parts;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = parts > 1 ? 1 : 0;
   cuda_ok(cudaLaunchKernelEx(&cfg, kernel, a), "launch");
 }
 
@@ -628,11 +733,17 @@ void by_outputs(const LogArgs& a, uint32_t parts, cudaStream_t s) {
 template <typename T>
 void forward(const LogArgs& a, cudaStream_t s) {
   constexpr int64_t kStep = kRowThreads * 16 / sizeof(T);  // elements a CTA reads at once
+  const int64_t sms = sm_count();
+  // A warp a row, where that is one step, or where there are rows enough for every warp of the
+  // GPU.  32 maxima bound 32 alternatives; those under marks are few enough for a warp up to 16.
+  const int64_t packs = a.cols * (int64_t)sizeof(T) / 16;
+  if ((packs <= kWarpPacks && a.top_k <= 32) ||
+      (packs <= kWarpPacksMany && a.rows >= kWarpRows * sms && a.top_k <= 16))
+    return by_outputs<T, 32>(a, 1, s);
   uint32_t parts = 1;
-  while (parts < 8 && a.rows * parts < 2 * sm_count() && a.cols >= kStep * parts * 2) parts *= 2;
-  // a row of one pack for each of 128 threads leaves most of a larger CTA idle
-  if (parts == 1 && a.cols <= kStep / 2) by_outputs<T, 128>(a, parts, s);
-  else by_outputs<T, kRowThreads>(a, parts, s);
+  // (8 x 32000 with 20 alternatives: 8.4 us over 4 CTAs a row, 9.3 over 8, 8.8 over 2)
+  while (parts < 8 && a.rows * parts < 2 * sms && a.cols >= kStep * parts * 4) parts *= 2;
+  by_outputs<T, kRowThreads>(a, parts, s);
 }
 
 LogArgs prepare(const gpuos_tensor* x, const gpuos_tensor* targets, float temperature) {
@@ -729,8 +840,10 @@ void backward(LogArgs a, cudaStream_t s) {
   need(a.rows * parts < 0x7fffffffll, "too many logits");
   a.parts = (uint32_t)parts;
   const unsigned grid = (unsigned)(a.rows * parts);
-  if (a.vec) run(gpuos_logprobs_grad_kernel<T, true>, grid, kGradThreads, 0, s, a);
-  else run(gpuos_logprobs_grad_kernel<T, false>, grid, kGradThreads, 0, s, a);
+  if (a.vec && a.ge) run(gpuos_logprobs_grad_kernel<T, true, true>, grid, kGradThreads, 0, s, a);
+  else if (a.vec) run(gpuos_logprobs_grad_kernel<T, true, false>, grid, kGradThreads, 0, s, a);
+  else if (a.ge) run(gpuos_logprobs_grad_kernel<T, false, true>, grid, kGradThreads, 0, s, a);
+  else run(gpuos_logprobs_grad_kernel<T, false, false>, grid, kGradThreads, 0, s, a);
 }
 
 void logprobs_grad(const gpuos_tensor* x, const gpuos_tensor* targets, const gpuos_tensor* stats, const gpuos_tensor* entropy,
