@@ -7,16 +7,17 @@
 //   top_k largest keys of the open groups; of equal ones the lowest index
 //   w    = s of the chosen (/ their sum) * scale
 //
-// The chosen experts are those of exact arithmetic, at the price of a fast
-// selection: every key becomes one unsigned integer, the key's place in the
-// row's range above the expert's slot, so that a maximum over lanes gives key and
-// expert at once and of equal keys the lowest index.  16-bit logits without a
-// bias fit whole; other keys are computed in 32 bits, with a known error bound, and rounded
-// to 22 to 24 bits of the range that the largest ones span.  Where two keys whose
-// order matters come out closer than the error, about one token in two thousand of random
-// logits, its lanes do it again in 64 bits.  What that does not settle (keys
-// within 2^-38, NaN, more ranks than lanes, groups that fit no seats) is left for the
-// CTA's second part, a warp to a token.
+// The chosen experts are those of 64-bit arithmetic, by a selection in 32-bit integers, so that a
+// maximum over lanes is one or a few instructions.  16-bit logits without a bias fit whole above the
+// expert's slot; 32-bit logits become their place among 2^24 (2^22) of the range that the row's
+// largest ones span.  Scores are computed in 64 bits (the exponential as a series,
+// to 2^-32: the half-rate pipe has room beside the integers) and become places among 2^29
+// of the range that scores and bias can take; groups add places.
+// Where places whose order matters are equal, or for scores next to each other, the
+// token's lanes do it again with 64-bit keys.  (Scores in 32 bits put one token in two
+// thousand in doubt, and those set the time: 16384 tokens over 256 experts took 25.7 us with groups,
+// 17.3 without.)  What that does not settle (keys within 2^-38, NaN, more
+// ranks than lanes, groups that fit no seats) is left for the CTA's second part, a warp to a token.
 //
 // A token belongs to LPT lanes of a warp, each holding NPL neighbouring experts
 // of one group in registers: up to 256 experts take 8 a lane and as many lanes as
@@ -293,6 +294,40 @@ __device__ __forceinline__ double inverse(double d) {
   return r * fma(-d, r, 2.0);
 }
 
+// Conversions by the bits, for finite values within 2^-126..2^127 and 0 (which becomes 2^-127): a
+// conversion instruction between 32 and 64 bits takes eight times an integer one's time.
+__device__ __forceinline__ double widen(float x) {
+  const int b = __float_as_int(x);
+  return __hiloint2double(((b >> 3) & 0x8fffffff) + 0x38000000, b << 29);
+}
+__device__ __forceinline__ float narrow(double x) {  // x > 0; cut, not rounded
+  return __uint_as_float(__funnelshift_l(__double2loint(x), __double2hiint(x) - 0x38000000, 3));
+}
+
+// e^a for |a| at most 60 to 2^-32: the exponential series of what is left of a without multiples
+// of ln 2, to r^8 (the rest is below 0.35^9 / 9!).
+__device__ __forceinline__ double exp_series(double a) {
+  const double whole = 6755399441055744.0;  // 3 * 2^51: a sum's low word is its integer
+  const double t = fma(a, 1.44269504088896340736, whole);
+  const double r = fma(t - whole, -0.69314718055994530942, a);
+  double p = 1.0 / 40320.0;
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
+}
+
+// 1 / d for d of 1 to 2^100, by one Newton step from 20 bits: to 2^-39.
+__device__ __forceinline__ double inverse_of_sum(double d) {
+  const double r = widen(rcp(narrow(d)));
+  return r * fma(-d, r, 2.0);
+}
+
 // One token's selection in 64 bits by its own lanes: lane r gets the slot of rank r.
 // Returns whether two keys whose order matters are still too close.
 template <typename T, int NPL, int LPT, bool GROUPED>
@@ -417,7 +452,7 @@ __device__ __forceinline__ void sort_down(uint32_t (&k)[N]) {
           }
 }
 
-template <typename T, int NPL, int LPT, bool GROUPED>
+template <typename T, int NPL, int LPT, bool GROUPED, bool SIGMOID>
 __global__ void __launch_bounds__(kThreads, NPL <= 8 ? 4 : 1)
 gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
@@ -426,6 +461,9 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
   constexpr int kShift = kSlots <= 256 ? 8 : 10;  // bits of a slot, below the key's
   constexpr float kPlaces = (float)((1u << (32 - kShift)) - 1);
   constexpr bool kHalf = sizeof(T) == 2;
+  constexpr int kLow = NPL <= 8 ? 3 : NPL <= 16 ? 4 : 5;  // bits of a place in the lane, below a score's place
+  constexpr float kScorePlaces = (float)(1u << (32 - kLow)) - 64.f;
+  __shared__ double shift[kSlots];       // the place of a slot's bias; lane l's i-th at [i][l]
   __shared__ uint32_t left;              // tokens in doubt,
   __shared__ uint16_t which[kCtaTokens];  // and which of this CTA's
   const uint32_t sub = threadIdx.x / LPT;
@@ -440,9 +478,10 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
   seat.at = seat.group * a.seat_per_group + in_group;
   seat.n = seat.group < a.seat_groups && in_group < a.seat_per_group
                ? min((uint32_t)NPL, a.seat_per_group - in_group) : 0;
-  float bias[NPL];
-  bool keyed = a.bias != nullptr;
+  bool keyed = a.bias != nullptr, lost = false;
+  double times = kScorePlaces;  // places of a score of 1
   if (keyed) {
+    float bias[NPL], hi = -INFINITY, lo = INFINITY;
     // a bias that is the same for all does not change the order
     const float b0 = __ldg(a.bias);
     bool same = b0 - b0 == 0.f;
@@ -450,8 +489,20 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
     for (int i = 0; i < NPL; ++i) {
       bias[i] = i < (int)seat.n ? __ldg(a.bias + (seat.at + i) * a.bs) : b0;
       same = same && bias[i] == b0;
+      hi = fmaxf(hi, bias[i]);
+      lo = fminf(lo, bias[i]);
+      lost = lost || bias[i] - bias[i] != 0.f;  // infinities and NaN have no places
     }
     keyed = !__syncthreads_and(same);
+    lost = __syncthreads_or(lost);
+    hi = lanes_top<LPT>(hi);
+    lo = -lanes_top<LPT>(-lo);
+    times = (double)kScorePlaces / (1.0 + (double)hi - (double)lo);
+    if (sub == 0) {
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) shift[i * LPT + seat.lane] = ((double)bias[i] - (double)lo) * times;
+    }
+    __syncthreads();
   }
   const bool scored = keyed || (GROUPED && a.top2);
 
@@ -467,107 +518,118 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
     float check = x[0];
 #pragma unroll
     for (int i = 1; i < NPL; ++i) check += x[i];
-    const bool odd = check != check;
-    bool later = a.top_k >= LPT || (GROUPED && a.groups != a.seat_groups), doubt = false;
+    bool later = a.top_k >= LPT || (GROUPED && a.groups != a.seat_groups) || lost, doubt = false;
 
-    // scores, as far as the order or the weights need all of them
-    float s[NPL], m = 0.f, total = 1.f;
-    if (!a.sigmoid) {
+    float m = 0.f, total = 1.f;  // of a softmax
+    if (!SIGMOID) {
       m = x[0];
 #pragma unroll
       for (int i = 1; i < NPL; ++i) m = fmaxf(m, x[i]);
       m = lanes_top<LPT>(m);
-      // a row of -inf: every difference is -inf, not NaN
-      const float shift = m == -INFINITY ? 0.f : m;
+    }
+    // a row of -inf: every difference is -inf, not NaN
+    const float top_x = m == -INFINITY ? 0.f : m;
+    const bool odd = check != check || m == INFINITY;
+    uint32_t key[NPL];
+    if (scored) {
+      double e[NPL], by = 1.0;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) {
+        // beyond 60 a score is 0 or 1 as far as its place goes
+        const float v = SIGMOID ? fminf(fmaxf(-x[i], -60.f), 60.f) : x[i] - top_x;
+        e[i] = exp_series(SIGMOID ? widen(v) : v < -60.f ? -60.0 : (double)x[i] - (double)top_x);
+      }
+      if (!SIGMOID) {
+        double sum = 0;
+#pragma unroll
+        for (int i = 0; i < NPL; ++i)
+          if (x[i] != -INFINITY) sum += e[i];
+        sum = lanes_sum<LPT>(sum);
+        total = (float)sum;
+        by = sum == 0.0 ? 0.0 : inverse_of_sum(sum);
+      }
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) {
+        const double sc = SIGMOID ? inverse_of_sum(1.0 + e[i]) : e[i] * by;
+        // an integer in the low word: below 2^52 a double's last bit is one place
+        const double place = fma(sc, times, keyed ? shift[i * LPT + seat.lane] : 0.0) + (4503599627370496.0 + 16.0);
+        key[i] = (uint32_t)__double2loint(place);
+      }
+    } else if (!SIGMOID) {
       total = 0.f;
 #pragma unroll
-      for (int i = 0; i < NPL; ++i) {
-        s[i] = ex2((x[i] - shift) * kLog2e);
-        total += s[i];
-      }
+      for (int i = 0; i < NPL; ++i) total += ex2((x[i] - top_x) * kLog2e);
       total = lanes_sum<LPT>(total);
-      if (scored) {
-        const float by = total == 0.f ? 0.f : rcp(total);
-#pragma unroll
-        for (int i = 0; i < NPL; ++i) s[i] *= by;
-      }
-    } else if (scored) {
-#pragma unroll
-      for (int i = 0; i < NPL; ++i) s[i] = rcp(1.f + ex2(x[i] * -kLog2e));
     }
-    // A sigmoid is off by at most 2e-7: (1 - s) s times the exponential's 2^-22 and 2^-24 |x| log2 e,
-    // the sum's and the reciprocal's roundings.  A softmax by 6.2e-7 of the row's largest:
-    // the exponential's error, at most 1.1 * 2^-24 of it from its argument, the sum's, the products'.
-    // Two keys by twice that, and by 2^-24 of themselves each.
-    const float s_error = a.sigmoid ? 4.2e-7f : 1.25e-6f * rcp(total);
     bool open = seat.n > 0;
     if (GROUPED && a.groups == a.seat_groups) {
-      float v1 = -INFINITY, v2 = -INFINITY;
+      // the group's two largest, of places or (without scores) of logits in their order
+      uint32_t v1 = 0, v2 = 0;
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
-        float v = keyed ? s[i] + bias[i] : a.top2 ? s[i] : x[i];
-        if (i >= (int)seat.n) v = -INFINITY;
-        v2 = fmaxf(v2, fminf(v1, v));
-        v1 = fmaxf(v1, v);
+        uint32_t v = key[i];
+        if (!scored) {
+          const uint32_t b = __float_as_uint(x[i] + 0.f);
+          v = (b >> 31) ? ~b : b | 0x80000000u;
+        }
+        if (i >= (int)seat.n) v = 0;
+        v2 = max(v2, min(v1, v));
+        v1 = max(v1, v);
       }
-      float w1 = v1, w2 = v2;
+      uint32_t w1 = v1, w2 = v2;
       for (uint32_t i = 1; i < a.lanes.d; ++i) {
         uint32_t from = seat.lane + i;
         if (from >= seat.first_lane + a.lanes.d) from -= a.lanes.d;
-        const float o1 = __shfl_sync(~0u, v1, seat.base + from), o2 = __shfl_sync(~0u, v2, seat.base + from);
-        w2 = fmaxf(fminf(w1, o1), fmaxf(w2, o2));
-        w1 = fmaxf(w1, o1);
+        const uint32_t o1 = __shfl_sync(~0u, v1, seat.base + from), o2 = __shfl_sync(~0u, v2, seat.base + from);
+        w2 = max(min(w1, o1), max(w2, o2));
+        w1 = max(w1, o1);
       }
-      const bool two = a.top2 && a.per_group > 1;
-      const float w = two ? w1 + w2 : w1;
-      // Without scores the largest logits are exact.  With them, how many other groups are
-      // clearly better, and how many may be: their order is within the error.
-      const float error = scored ? (two ? 2.f : 1.f) * s_error + 5e-7f * fabsf(w) : 0.f;
-      uint32_t better = 0, before = 0, worse = 0;
+      const uint32_t w = a.top2 && a.per_group > 1 ? w1 + w2 : w1;
+      uint32_t before = 0;  // groups that are better, or as good and before it
+#pragma unroll 4
       for (uint32_t h = 0; h < a.groups; ++h) {
-        const float o = __shfl_sync(~0u, w, seat.base + h * a.lanes.d);
+        const uint32_t o = __shfl_sync(~0u, w, seat.base + h * a.lanes.d);
         before += o > w || (o == w && h < seat.group);
-        better += o - w > error;
-        worse += w - o > error;
       }
       open = open && before < a.top_groups;
-      // it matters where it could open this group or close it
-      if (seat.n && error > 0.f && (better < a.top_groups) != (worse >= a.groups - a.top_groups)) doubt = true;
+      if (scored) {
+        // A place is off by 0.8 at most: its rounding, and the series' 2.8e-10 of a score (twice of a
+        // softmax) times 2^29; two sums of two places are in doubt within 4.
+        const uint32_t in = ~lanes_top<LPT>(open ? ~w : 0u), out = lanes_top<LPT>(seat.n && !open ? w : 0u);
+        if (in <= out + 4) doubt = true;
+      }
     }
 
-    uint32_t key[NPL];
     const bool exact = kHalf && !keyed;
-    uint32_t slack = 0;  // keys this close are in doubt
-    if (exact) {
+    if (keyed) {
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) key[i] = key[i] << kLow | (NPL - 1 - i);
+    } else if (exact) {
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
         const uint32_t b = half_bits<T>(x[i]);
         key[i] = (((b & 0x8000u) ? ~b & 0xffffu : b | 0x8000u) << 16) | (kSlots - 1 - (seat.lane * NPL + i));
       }
     } else {
-      // the range from the largest key down to one that top_k + 1 others reach
+      // the range from the largest logit down to one that top_k + 1 others reach
       float hi = -INFINITY, lo = INFINITY;
 #pragma unroll
-      for (int i = 0; i < NPL; ++i) {
-        s[i] = keyed ? s[i] + bias[i] : x[i];
+      for (int i = 0; i < NPL; ++i)
         if (i < (int)seat.n) {
-          hi = fmaxf(hi, s[i]);
-          lo = fminf(lo, s[i]);
+          hi = fmaxf(hi, x[i]);
+          lo = fminf(lo, x[i]);
         }
-      }
       const uint32_t lanes = __popc(__ballot_sync(~0u, open) >> seat.base & kLanes<LPT>);
       const float top = lanes_top<LPT>(open ? hi : -INFINITY);
       lo = -lanes_top<LPT>(open ? -(a.top_k < lanes ? hi : lo) : -INFINITY);
       lo = fmaxf(lo, top - 64.f);
       const float by = (kPlaces - 64.f) * rcp(fmaxf(top - lo, 1e-30f));
+      // rounding to places keeps the order, or makes logits equal
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
-        const uint32_t f = (uint32_t)fminf(fmaxf(fmaf(s[i] - lo, by, 16.f), 1.f), kPlaces);
+        const uint32_t f = (uint32_t)fminf(fmaxf(fmaf(x[i] - lo, by, 16.f), 1.f), kPlaces);
         key[i] = f << kShift | (kSlots - 1 - (seat.lane * NPL + i));
       }
-      // Rounding to places keeps the order of exact keys, or makes them equal; for the others
-      // their error counts, and the roundings of the difference, below 4 places.
-      if (keyed) slack = 4 + (uint32_t)fminf((s_error + 1.3e-7f * fmaxf(fabsf(top), fabsf(lo))) * by, 4e9f);
     }
 #pragma unroll
     for (int i = 0; i < NPL; ++i)
@@ -584,10 +646,16 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
         key[0] = hi;
       }
     }
+    uint32_t from = 0;  // the lane it is from
     for (uint32_t r = 0; r <= a.top_k; ++r) {
       const uint32_t best = lanes_top<LPT>(key[0]);
-      if (seat.lane == r) won = best;
-      if (key[0] == best) {
+      // (scores' places of several lanes may be equal: the lowest lane's counts)
+      const uint32_t owner = __ffs(__ballot_sync(~0u, key[0] == best) >> seat.base) - 1;
+      if (seat.lane == r) {
+        won = best;
+        from = owner;
+      }
+      if (seat.lane == owner) {
         if (NPL <= 8) {
 #pragma unroll
           for (int i = 0; i + 1 < NPL; ++i) key[i] = key[i + 1];
@@ -604,10 +672,12 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
       }
     }
     if (!exact) {
-      const uint32_t f = won >> kShift, next = __shfl_down_sync(~0u, f, 1);
-      if (seat.lane < a.top_k && (f < 8 || (next != 0 && f - next <= slack))) doubt = true;
+      const int down = keyed ? kLow : kShift;
+      const uint32_t f = won >> down, next = __shfl_down_sync(~0u, f, 1);
+      if (seat.lane < a.top_k && (f < 8 || (next != 0 && f - next <= (keyed ? 2u : 0u)))) doubt = true;
     }
-    uint32_t slot = kSlots - 1 - (won & ((1u << (exact ? 16 : kShift)) - 1));
+    uint32_t slot = keyed ? from * NPL + (NPL - 1 - (won & ((1u << kLow) - 1)))
+                          : kSlots - 1 - (won & ((1u << (exact ? 16 : kShift)) - 1));
     // (the whole warp takes part; a token that is not in doubt gets the same again)
     if (__any_sync(~0u, (doubt || odd) && live && !later)) {
       const bool close = resolve<T, NPL, LPT, GROUPED>(a, row, live, seat, keyed, &slot);
@@ -620,17 +690,17 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
     if (seat.lane < a.top_k && live && !later) {
       const uint32_t e = expert_of<NPL>(a, slot);
       const float v = to_f(row[e]);
-      if (a.sigmoid) sc = rcp(1.f + expf(-v));
+      if (SIGMOID) sc = rcp(1.f + expf(-v));
       else sc = m == -INFINITY ? 0.f : expf(v - m) * rcp(total);
       if (a.wide) static_cast<int64_t*>(a.experts)[t * a.es + seat.lane * a.ek] = e;
       else static_cast<int32_t*>(a.experts)[t * a.es + seat.lane * a.ek] = (int32_t)e;
     }
-    float times = a.scale;
+    float norm = a.scale;
     if (a.renorm) {
       const float sum = lanes_sum<LPT>(sc);
-      times = sum == 0.f ? 0.f : a.scale / sum;
+      norm = sum == 0.f ? 0.f : a.scale / sum;
     }
-    if (seat.lane < a.top_k && live && !later) a.weights[t * a.ws + seat.lane * a.wk] = sc * times;
+    if (seat.lane < a.top_k && live && !later) a.weights[t * a.ws + seat.lane * a.wk] = sc * norm;
   }
 
   __syncthreads();
@@ -792,8 +862,10 @@ void launch(RouteArgs a, bool grad, cudaStream_t s) {
     const size_t keys = (a.n + a.groups) * sizeof(Key64);
     a.exact_warps = (uint32_t)std::max<size_t>(1, std::min<size_t>(kThreads / 32, 18 * 1024 / keys));
     const size_t smem = a.exact_warps * keys;
-    if (a.groups > 1) run(gpuos_route_kernel<T, NPL, LPT, true>, grid, kThreads, smem, s, a);
-    else run(gpuos_route_kernel<T, NPL, LPT, false>, grid, kThreads, smem, s, a);
+    if (a.groups > 1 && a.sigmoid) run(gpuos_route_kernel<T, NPL, LPT, true, true>, grid, kThreads, smem, s, a);
+    else if (a.groups > 1) run(gpuos_route_kernel<T, NPL, LPT, true, false>, grid, kThreads, smem, s, a);
+    else if (a.sigmoid) run(gpuos_route_kernel<T, NPL, LPT, false, true>, grid, kThreads, smem, s, a);
+    else run(gpuos_route_kernel<T, NPL, LPT, false, false>, grid, kThreads, smem, s, a);
   }
 }
 
