@@ -6,8 +6,7 @@ Each call runs one kernel at once on torch's current stream of its tensors'
 device; it allocates its outputs (where `out` gives none) and nothing else, so it
 may be captured into a CUDA graph.  As with an op of torch's own, requests
 submitted to an executor are seen once they are flushed; inside a
-``scheduler_context`` of the calling thread, pending requests on the call's
-tensors are flushed first.  Tensors are CUDA tensors of one device.  A call that
+``scheduler_context``, pending requests on the call's tensors are flushed first.  Tensors are CUDA tensors of one device.  A call that
 breaks a rule raises ``ValueError`` (``TypeError`` for a dtype, ``RuntimeError``
 for a device) and launches nothing.
 
@@ -42,7 +41,7 @@ def _tuple(x) -> tuple:
 
 
 def _order(reads, writes=()):
-    """Flush what a scheduler context of this thread has pending on a call's tensors."""
+    """Flush what a scheduler context has pending on a call's tensors."""
     _scheduler.order_after_pending([t for t in reads if isinstance(t, torch.Tensor)],
                                    [t for t in writes if isinstance(t, torch.Tensor)])
 
@@ -185,7 +184,7 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Opt
     first.  With `groups`, only experts of the best `top_groups` groups are chosen from; a group is
     worth its largest key, or with ``group_score="top2"`` the sum of its two
     largest.  Weights are the scores, divided by their sum if `renormalize`, times `scale`.
-    The choice is that of exact arithmetic."""
+    The choice is that of keys in 64 bits."""
     if _entered:
         _order((logits, bias))
     kind, rule = _choice(_SCORE, score, "score"), _choice(_GROUP_SCORE, group_score, "group_score")

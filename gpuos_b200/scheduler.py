@@ -467,19 +467,19 @@ class _GPUOSSchedulerMode(torch.utils._python_dispatch.TorchDispatchMode):
         return None
 
 
-entered: List[Tuple[int, "_GPUOSSchedulerMode"]] = []  # (thread, mode) of each context entered
+entered: List[_GPUOSSchedulerMode] = []  # the modes of the contexts entered
 
 
 def order_after_pending(reads, writes) -> None:
     """For code that launches on tensors without going through torch's
-    dispatcher: inside a scheduler context of this thread, flush the pending
-    requests that write what is in `reads`, or touch what is in `writes`, as an op that
-    runs in torch does."""
-    me = threading.get_ident()
-    for thread, mode in entered:
-        if thread == me and mode.pending and (
-                any(_overlaps(_extent(t), mode._w) for t in reads) or
-                any(_overlaps(_extent(t), tab) for t in writes for tab in (mode._w, mode._r))):
+    dispatcher: inside a scheduler context, flush the pending requests that
+    write what is in `reads`, or touch what is in `writes`, as an op that runs in torch
+    does.  Every context counts, not this thread's alone: a backward pass
+    runs, and schedules, on a thread of autograd's."""
+    for mode in tuple(entered):
+        if mode.pending and (any(_overlaps(_extent(t), mode._w) for t in reads) or
+                             any(_overlaps(_extent(t), tab) for t in writes
+                                 for tab in (mode._w, mode._r))):
             mode.sync()
 
 
@@ -504,7 +504,7 @@ class GPUOSScheduler:
                                          pending=self._pending, jit=not _jit_disabled(),
                                          fuse=_fuse_enabled())
         self._mode.__enter__()
-        entered.append((threading.get_ident(), self._mode))
+        entered.append(self._mode)
         return self
 
     def flush(self, sync: bool = False):
@@ -519,7 +519,7 @@ class GPUOSScheduler:
     def __exit__(self, exc_type, exc, tb):
         try:
             if self._mode is not None:
-                entered[:] = [e for e in entered if e[1] is not self._mode]
+                entered[:] = [m for m in entered if m is not self._mode]
                 self._mode.close()
                 self._mode.submit_nodes()
                 self._mode.__exit__(exc_type, exc, tb)

@@ -394,7 +394,7 @@ int32_t gpuos_cache_read(int32_t n, const gpuos_tensor* slots, const gpuos_tenso
  * `top_groups` stay open.  experts (i32 or i64, (token, top_k), top_k at most 64)
  * gets the largest keys of the open groups in falling order, weights (f32) their
  * scores without bias, divided by their sum with `renormalize`, times `scale`.
- * The choice is that of exact arithmetic; of equal keys, and of equal groups, the
+ * The choice is that of keys in 64 bits; of equal keys, and of equal groups, the
  * lowest index comes first.  A NaN logit counts as -inf in the choice; a row of
  * -inf has scores 0 (softmax), and where the chosen scores sum to 0 the
  * renormalised weights are 0. */

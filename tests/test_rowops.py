@@ -1183,3 +1183,156 @@ def test_errors_leave_the_device_usable():
         R.rotary(torch.zeros(4, 1, 8, device=DEV), torch.arange(4), torch.ones(4, device=DEV))
     w, e = R.route(x, 2)
     assert torch.equal(e.cpu(), torch.tensor([[0, 1]]).expand(4, 2))
+
+
+@gpu
+def test_backward_inside_a_scheduler_context(monkeypatch):
+    """A backward pass schedules its small ops from a thread of autograd's; the
+    row operators' gradients read what those have pending."""
+    monkeypatch.setenv("GPUOS_MODE", "stream")
+    monkeypatch.setenv("GPUOS_SCHEDULER_DISABLE_JIT", "0")
+    g = gen(22)
+    x, gw, lg = randn(g, 6, 16).to(DEV), randn(g, 6, 3).to(DEV), randn(g, 6).to(DEV)
+    q, pos, f = randn(g, 6, 2, 32).to(DEV), torch.arange(6, device=DEV), R.rotary_frequencies(32, device=DEV)
+    y = torch.arange(6, device=DEV)
+
+    def grads():
+        a, b, c = (t.clone().requires_grad_() for t in (x, x, q))
+        w, _ = R.route(a * 1.5, 3)
+        r = R.logprobs(b * 2.0, y, entropy=True)
+        z = R.rotary(c * 0.5, pos, f)
+        # the products' backward makes gradients that the operators' backward reads
+        return torch.autograd.grad([w * gw, r.logprob * lg, r.entropy * lg, z * z], [a, b, c],
+                                   [torch.ones_like(gw), lg, lg, torch.ones_like(z)])
+
+    want = grads()
+    with S.scheduler_context(auto_flush_ms=None):
+        got = grads()
+    torch.cuda.synchronize()
+    for u, v in zip(got, want):
+        assert torch.equal(u, v)
+
+
+# ---------------------------------------------------------------------------
+# Sizes that choose other kernels
+# ---------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("cols", [300, 1000, 4999, 13001])
+@pytest.mark.parametrize("top", [0, 5, 16, 17, 33, 64])
+def test_logprobs_many_rows(dtype, cols, top):
+    """Rows enough for a warp each, with rows that make many candidates among
+    them, and alternatives on both sides of every limit."""
+    g = torch.Generator(device=DEV).manual_seed(cols + top)
+    x = (torch.randn(1301, cols, generator=g, device=DEV) * 3).to(dtype)
+    low = torch.finfo(dtype).min
+    x[3] = 1.5
+    x[10] = -math.inf
+    x[17, 2:] = -math.inf
+    x[24] = low
+    x[31] = torch.linspace(-4, 4, cols, device=DEV).to(dtype)
+    x[38] = torch.linspace(4, -4, cols, device=DEV).to(dtype)
+    x[45, ::3] = -math.inf
+    x[1300, : cols - 1] = low
+    y = torch.randint(0, cols, (1301,), generator=g, device=DEV)
+    y[1] = -1
+    r = R.logprobs(x, y, top=min(top, cols), entropy=True)
+    rows = torch.cat((torch.arange(60), torch.arange(1200, 1301)))
+    keep = R.LogProbs(*(None if t is None else t[rows.to(DEV)] for t in r))
+    check_logprobs(keep, x.cpu()[rows], y.cpu()[rows], min(top, cols), 1.0, True)
+    if top:  # every row's tokens
+        assert torch.equal(r.top_tokens, x.float().sort(dim=-1, descending=True, stable=True)[1][:, :min(top, cols)])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("cols,rows", [(50000, 3), (140001, 40), (262144, 1)])
+@pytest.mark.parametrize("top", [1, 20, 40, 64])
+def test_logprobs_long_rows_of_candidates(dtype, cols, rows, top):
+    """Rows split over CTAs, and rows whose ties overflow the candidates."""
+    g = torch.Generator(device=DEV).manual_seed(cols)
+    x = (torch.randn(rows, cols, generator=g, device=DEV) * 3).to(dtype)
+    x[rows - 1, cols // 3:] = 9.0                       # most are equal, and the largest
+    x[0, : cols - 7] = -math.inf                        # seven left
+    y = torch.zeros(rows, dtype=torch.int64, device=DEV)
+    r = R.logprobs(x, y, top=top, entropy=True)
+    assert torch.equal(r.top_tokens, x.float().sort(dim=-1, descending=True, stable=True)[1][:, :top])
+    check_logprobs(r, x.cpu(), y.cpu(), top, 1.0, True)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups,top_groups,top_k", [(256, 8, 4, 8), (64, 1, 1, 6), (128, 4, 2, 31), (384, 6, 3, 8)])
+def test_route_many_tokens_with_ties(dtype, score, experts, groups, top_groups, top_k):
+    """Tokens enough for every CTA to take several, logits and biases of few
+    distinct values, so that keys tie or nearly tie in every row."""
+    g = torch.Generator(device=DEV).manual_seed(experts)
+    x = (torch.randn(20011, experts, generator=g, device=DEV) * 4).round().div(4).to(dtype)
+    x[::2] += torch.randn(10006, experts, generator=g, device=DEV).mul(1e-3).to(dtype)
+    bias = torch.randn(experts, generator=g, device=DEV).mul(8).round().div(64)
+    for b, rule in ((None, "max"), (bias, "max"), (bias, "top2"), (None, "top2")):
+        how = dict(score=score, groups=groups, top_groups=top_groups, group_score=rule, renormalize=True)
+        w, e = R.route(x, top_k, bias=b, **how)
+        torch.set_default_device(DEV)
+        try:
+            ww, we = route_oracle(x, top_k, bias=b, **how)
+        finally:
+            torch.set_default_device("cpu")
+        # The oracle's 64-bit keys carry 2^-50 of error: rows whose order two such keys leave open say nothing
+        s = (x.double().softmax(-1) if score == "softmax" else torch.sigmoid(x.double()))
+        k = x.double() if b is None else s + b.double()
+        diff = (e != we).any(-1)
+        near = torch.zeros_like(diff)
+        if bool(diff.any()):
+            a, c = k[diff].gather(-1, e[diff]), k[diff].gather(-1, we[diff])
+            near[diff] = ((a - c).abs() <= 2.0 ** -50).all(-1)
+            if groups > 1:
+                # Nor do groups: with biases that are multiples of 1/64, (s1 + b1) + (s2 + b2) and
+                # (s1 + b2) + (s2 + b1) are equal, but three additions of values below 4 leave up to
+                # 3 * 2^-52 between their 64-bit sums (the rows that differed had 2^-52 or 2^-53 there).
+                by = (s if b is None and rule == "top2" else k)[diff].unflatten(-1, (groups, -1))
+                by = by.amax(-1) if rule == "max" else by.sort(-1, descending=True)[0][..., :2].sum(-1)
+                by = by.sort(-1, descending=True)[0]
+                near[diff] |= by[:, top_groups - 1] - by[:, top_groups] <= 2.0 ** -50
+        assert not bool((diff & ~near).any())
+        assert bool(((w.double() - ww).abs() <= ROUTE_REL * ww.abs() + 1e-37)[~diff].all())
+
+
+@gpu
+def test_more_pairs_than_threads_and_no_heads():
+    g = gen(30)
+    x = randn(g, 3, 2, 4200).to(DEV)
+    pos, f = torch.tensor([0, 7, 900], device=DEV), R.rotary_frequencies(4096, device=DEV)
+    for inter in (False, True):
+        check_rotary(R.rotary(x, pos, f, interleaved=inter), x, pos, f, interleaved=inter)
+    assert R.rotary(x[:, :0], pos, f).shape == (3, 0, 4200)
+    c, s = R.cache_alloc(2, 4, 0, 16, device=DEV)
+    R.cache_write(x[:, :0, :16], pos, c, s)
+    assert R.cache_read(pos, c, s).shape == (3, 0, 16)
+
+
+@gpu
+def test_first_calls_inside_a_capture():
+    """A process whose first call of each operator is captured."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from gpuos_b200 import rowops as R
+x = torch.randn(9, 64, device="cuda"); y = torch.arange(9, device="cuda"); q = torch.randn(9, 2, 32, device="cuda")
+f = R.rotary_frequencies(32, device="cuda"); c, s = R.cache_alloc(2, 8, 2, 32)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    a = R.rotary(q, y, f); R.cache_write(a, y, c, s); b = R.cache_read(y, c, s, dtype=torch.float32)
+    w, e = R.route(x, 4); r = R.logprobs(x, y, top=3, entropy=True, stats=True)
+    d = R.logprobs_grad(x, y, r, r.logprob, r.entropy); h = R.route_grad(x, e, w)
+g.replay(); torch.cuda.synchronize()
+assert torch.equal(a, R.rotary(q, y, f)) and torch.equal(e, R.route(x, 4)[1])
+assert torch.equal(r.logprob, R.logprobs(x, y).logprob) and float((a - b).abs().max()) < 0.05
+print("captured")
+"""
+    from pathlib import Path
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240,
+                         cwd=Path(__file__).resolve().parents[1])
+    assert "captured" in out.stdout, out.stderr[-2000:]
