@@ -40,6 +40,8 @@ constexpr int kRowThreads = 256;  // of a row; short rows take a warp each, 8 to
 constexpr int kList = 128;    // candidates a warp holds
 constexpr int kWarpPacks = 128;  // 16-byte packs of a row that one warp takes,
 constexpr int kWarpPacksMany = 3200, kWarpRows = 8;  // and where there are many rows for each SM
+constexpr int kLongPacks = 14000;  // of a row whose threads have eight packs in flight
+
 constexpr int kFewTop = 32;   // alternatives up to which 64 maxima give a close bound
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kLowest = -3.402823466e38f;  // the lowest finite number: where a maximum starts
@@ -174,7 +176,7 @@ struct TopShared {
   unsigned long long bound;          // no candidate below it is needed
   uint32_t count;                    // of the candidates
   uint32_t reached;                  // of `reach`
-  alignas(16) float seeds[THREADS];
+  alignas(16) float seeds[THREADS < 256 ? THREADS : 256];
   uint32_t reach[kReached];           // (mark, thread) whose maximum reaches the bound
   unsigned long long last[kMaxTop];  // the top_k, sorted
   // one after the other: the marks; the candidates; where those are too many, each
@@ -295,10 +297,9 @@ __device__ __forceinline__ void rank_into(const unsigned long long* keys, uint32
 }
 
 // The bound: a value that k of the row's elements reach, from the threads' maxima.
-// For few alternatives the k-th largest of 64 maxima over neighbouring threads is close;
-// for more each thread's counts
-// (64 alternatives of 8 x 32000: 23 us, 48 us from 64 maxima, whose last one is far too low;
-// 20: 12.2 us, 8.6 us from 64).
+// For few alternatives the k-th largest of 64 maxima over neighbouring threads is close,
+// for more it takes 256
+// (64 alternatives of 8 x 32000: 12 us, 48 from 64 maxima, whose last one is far too low).
 template <typename T, int THREADS>
 __device__ __forceinline__ void find_bound(TopShared<T, THREADS>& top, float m, uint32_t k) {
   const int tid = threadIdx.x % THREADS;
@@ -313,29 +314,26 @@ __device__ __forceinline__ void find_bound(TopShared<T, THREADS>& top, float m, 
     }
     mine = tid == 0;
     rank = k - 1;
-  } else if (k <= kFewTop) {
-    constexpr int S = 64, L = THREADS / S;
-#pragma unroll
-    for (int d = 1; d < L; d <<= 1) me = fmaxf(me, __shfl_xor_sync(~0u, me, d));
-    if (tid % L == 0) top.seeds[tid / L] = me;
-    __syncthreads();
-#pragma unroll
-    for (int j = tid % L; j < S; j += L) {
-      const float o = top.seeds[j];
-      rank += o > me || (o == me && j < tid / L);
-    }
-#pragma unroll
-    for (int d = 1; d < L; d <<= 1) rank += __shfl_xor_sync(~0u, rank, d);
-    mine = tid % L == 0;
   } else {
-    top.seeds[tid] = me;
-    __syncthreads();
+    auto among = [&](auto seeds) {
+      constexpr int S = decltype(seeds)::value, L = THREADS / S;  // L lanes to a seed
+#pragma unroll
+      for (int d = 1; d < L; d <<= 1) me = fmaxf(me, __shfl_xor_sync(~0u, me, d));
+      if (tid % L == 0) top.seeds[tid / L] = me;
+      __syncthreads();
 #pragma unroll 4
-    for (int j = 0; j < THREADS; j += 4) {
-      const float4 o = *reinterpret_cast<const float4*>(top.seeds + j);
-      rank += (o.x > me || (o.x == me && j < tid)) + (o.y > me || (o.y == me && j + 1 < tid)) +
-              (o.z > me || (o.z == me && j + 2 < tid)) + (o.w > me || (o.w == me && j + 3 < tid));
-    }
+      for (int j = tid % L * 4; j < S; j += L * 4) {
+        const float4 o = *reinterpret_cast<const float4*>(top.seeds + j);
+        const int at = tid / L;
+        rank += (o.x > me || (o.x == me && j < at)) + (o.y > me || (o.y == me && j + 1 < at)) +
+                (o.z > me || (o.z == me && j + 2 < at)) + (o.w > me || (o.w == me && j + 3 < at));
+      }
+#pragma unroll
+      for (int d = 1; d < L; d <<= 1) rank += __shfl_xor_sync(~0u, rank, d);
+      mine = tid % L == 0;
+    };
+    if (k <= kFewTop) among(std::integral_constant<int, 64>());
+    else among(std::integral_constant<int, 256>());
   }
   // A maximum that is still where it started was reached by nothing: no bound.
   // Otherwise every element of this value and above counts, whatever its index.
@@ -349,11 +347,11 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 template <typename T, int THREADS, bool TOP>
 constexpr size_t kSharedOfRow = (kTopAt<THREADS> + (TOP ? sizeof(TopShared<T, THREADS>) : 0) + 15) / 16 * 16;
 
-template <typename T, int THREADS, bool ENT, bool TOP>
-__global__ void __launch_bounds__(THREADS * kRowsOfCta<THREADS>, THREADS == 32 ? 5 : 6)
+// U packs a thread in flight: four, with more CTAs of an SM, or eight, with fewer.
+template <typename T, int THREADS, int U, bool ENT, bool TOP>
+__global__ void __launch_bounds__(THREADS * kRowsOfCta<THREADS>, THREADS == 32 ? 5 : U == 4 ? 6 : 4)
 gpuos_logprobs_kernel(const __grid_constant__ LogArgs a) {
   constexpr int W = 16 / sizeof(T);
-  constexpr int U = 4;  // packs a thread has in flight
   extern __shared__ __align__(16) uint8_t smem[];
   const uint32_t tid = threadIdx.x % THREADS, lane = tid & 31, warp = tid / 32;
   uint8_t* mem = smem + threadIdx.x / THREADS * kSharedOfRow<T, THREADS, TOP>;
@@ -701,11 +699,11 @@ gpuos_logprobs_grad_kernel(const __grid_constant__ LogArgs a) {
   }
 }
 
-template <typename T, int THREADS, bool ENT, bool TOP>
+template <typename T, int THREADS, int U, bool ENT, bool TOP>
 void launch(const LogArgs& a, uint32_t parts, cudaStream_t s) {
   constexpr int kRows = kRowsOfCta<THREADS>;
   const size_t smem = kRows * kSharedOfRow<T, THREADS, TOP> + (TOP && parts > 1 ? parts * a.top_k * 8 : 0);
-  auto kernel = gpuos_logprobs_kernel<T, THREADS, ENT, TOP>;
+  auto kernel = gpuos_logprobs_kernel<T, THREADS, U, ENT, TOP>;
   if (smem > 48 * 1024)
     cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory");
   cudaLaunchConfig_t cfg{};
@@ -722,12 +720,12 @@ void launch(const LogArgs& a, uint32_t parts, cudaStream_t s) {
   cuda_ok(cudaLaunchKernelEx(&cfg, kernel, a), "launch");
 }
 
-template <typename T, int THREADS>
+template <typename T, int THREADS, int U>
 void by_outputs(const LogArgs& a, uint32_t parts, cudaStream_t s) {
-  if (a.entropy && a.top_k) launch<T, THREADS, true, true>(a, parts, s);
-  else if (a.entropy) launch<T, THREADS, true, false>(a, parts, s);
-  else if (a.top_k) launch<T, THREADS, false, true>(a, parts, s);
-  else launch<T, THREADS, false, false>(a, parts, s);
+  if (a.entropy && a.top_k) launch<T, THREADS, U, true, true>(a, parts, s);
+  else if (a.entropy) launch<T, THREADS, U, true, false>(a, parts, s);
+  else if (a.top_k) launch<T, THREADS, U, false, true>(a, parts, s);
+  else launch<T, THREADS, U, false, false>(a, parts, s);
 }
 
 template <typename T>
@@ -739,11 +737,14 @@ void forward(const LogArgs& a, cudaStream_t s) {
   const int64_t packs = a.cols * (int64_t)sizeof(T) / 16;
   if ((packs <= kWarpPacks && a.top_k <= 32) ||
       (packs <= kWarpPacksMany && a.rows >= kWarpRows * sms && a.top_k <= 16))
-    return by_outputs<T, 32>(a, 1, s);
+    return by_outputs<T, 32, 4>(a, 1, s);
   uint32_t parts = 1;
   // (8 x 32000 with 20 alternatives: 8.4 us over 4 CTAs a row, 9.3 over 8, 8.8 over 2)
   while (parts < 8 && a.rows * parts < 2 * sms && a.cols >= kStep * parts * 4) parts *= 2;
-  by_outputs<T, kRowThreads>(a, parts, s);
+  // Long whole rows: fewer CTAs with more in flight each keep the memory busy while the last rows
+  // run (1000 x 128000 bf16: 45 us, 53 with four packs in flight; 3000 x 50257: 69 and 61).
+  if (parts == 1 && packs >= kLongPacks) by_outputs<T, kRowThreads, 8>(a, parts, s);
+  else by_outputs<T, kRowThreads, 4>(a, parts, s);
 }
 
 LogArgs prepare(const gpuos_tensor* x, const gpuos_tensor* targets, float temperature) {

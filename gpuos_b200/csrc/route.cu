@@ -840,8 +840,13 @@ template <typename T, int NPL, int LPT>
 void launch(RouteArgs a, bool grad, cudaStream_t s) {
   constexpr uint32_t kTokens = kThreads / LPT;
   const uint64_t ctas = ((uint64_t)a.tokens + kTokens - 1) / kTokens;
-  const uint64_t most = kCtaTokens / kTokens;  // steps of a CTA
-  const uint64_t wanted = std::max<uint64_t>(std::min<uint64_t>(ctas, (uint64_t)sm_count() * 8), (ctas + most - 1) / most);
+  // weights: CTAs that stay, as each first looks at the bias, but take at most kCtaTokens;
+  // their gradient has nothing to set up
+  uint64_t wanted = ctas;
+  if (!grad) {
+    const uint64_t most = kCtaTokens / kTokens;
+    wanted = std::max<uint64_t>(std::min<uint64_t>(ctas, (uint64_t)sm_count() * 8), (ctas + most - 1) / most);
+  }
   need(wanted < 0x7fffffffull, "too many tokens");
   const unsigned grid = (unsigned)wanted;
   a.seat_groups = a.groups;
