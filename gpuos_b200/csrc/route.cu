@@ -786,18 +786,18 @@ gpuos_route_grad_kernel(const __grid_constant__ RouteArgs a) {
     }
     sum = lanes_sum<LPT>(sum);
     dot = lanes_sum<LPT>(dot);
-    const float mul = !a.renorm ? a.scale : sum == 0.f ? 0.f : a.scale / sum;
     const float less = !a.renorm || sum == 0.f ? 0.f : dot / sum;
     const float all = a.scale * dot;  // of a plain softmax: the sum of ds_i s_i
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       const uint32_t r = lane + i * LPT;
-      float d = mul * (g[i] - less);
+      float d = a.scale * (g[i] - less);
+      // (a score over the sum first: the sum's own inverse leaves the range where scores are near 2^-127)
+      if (a.renorm) d *= sum == 0.f ? 0.f : sc[i] / sum;
+      else if (a.sigmoid) d *= sc[i];
       if (a.sigmoid) {
         const float x = expf(-fabsf(v[i])), q = 1.f / (1.f + x);
-        d *= x * q * q;  // s (1 - s)
-      } else if (a.renorm) {
-        d *= sc[i];
+        d *= v[i] > 0.f ? x * q : q;  // 1 - s
       }
       if (r < a.top_k) chosen[r] = Chosen{d, e[i]};
     }
@@ -857,10 +857,8 @@ void launch(RouteArgs a, bool grad, cudaStream_t s) {
   }
   a.lanes = FastDiv((a.seat_per_group + NPL - 1) / NPL);
   if (grad) {
+    // (36 KB at most)
     const size_t smem = kThreads * NPL * sizeof(float) + kTokens * a.top_k * sizeof(Chosen);
-    if (smem > 48 * 1024)
-      cuda_ok(cudaFuncSetAttribute(gpuos_route_grad_kernel<T, NPL, LPT>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory");
     run(gpuos_route_grad_kernel<T, NPL, LPT>, grid, kThreads, smem, s, a);
   } else {
     // 16 KB of keys: 8 warps of 256 experts, fewer of more

@@ -1336,3 +1336,18 @@ print("captured")
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240,
                          cwd=Path(__file__).resolve().parents[1])
     assert "captured" in out.stdout, out.stderr[-2000:]
+
+
+@gpu
+@pytest.mark.parametrize("by", [-80.0, -88.5])
+def test_route_gradient_of_scores_near_the_smallest(by):
+    """Renormalised sigmoid scores whose sum has no 32-bit inverse still have shares."""
+    x = torch.tensor([[0.0, -0.125, -0.0625, 0.0]]) + by
+    e, g = torch.tensor([[0, 1]]), torch.tensor([[1.0, -0.5]])
+    got = R.route_grad(x.to(DEV), e.to(DEV), g.to(DEV), score="sigmoid", renormalize=True, scale=2.5)
+    want, _ = route_grad_oracle(x, e, g, "sigmoid", True, 2.5)
+    # Near 2^-128 the spacing of 2^-149 makes a rounding up to 2^-22 of a score.  A share takes three
+    # (its score, the sum, the quotient), the mean of g five more; exp adds 2^-22 each: below 16 of
+    # 2^-22, of terms up to 2.5 * 1.5.
+    assert bool(((got.cpu().double() - want).abs() <= 16 * 2.0 ** -22 * 2.5 * 1.5).all()), got
+    assert bool((got[0, 2:] == 0).all())
