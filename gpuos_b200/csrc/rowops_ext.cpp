@@ -193,6 +193,18 @@ PyObject* wrap(const at::Tensor& t) {
 // Whether autograd has to see the call (gpuos_b200.rowops then records it).
 bool recorded(const at::Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
 
+// A tensor of the caller's was written: autograd then refuses a backward pass that saved it.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// A tensor to be written, which autograd must not be following.
+const at::Tensor& given_out(PyObject* o) {
+  const at::Tensor& t = tensor(o, "out");
+  if (recorded(t)) throw Raise{PyExc_ValueError, "out cannot be a tensor that requires a gradient"};
+  return t;
+}
+
 PyObject* not_here() {
   Py_INCREF(Py_NotImplemented);
   return Py_NotImplemented;
@@ -240,6 +252,8 @@ PyObject* rotary(PyObject* const* a, Py_ssize_t n) {
   arity(n, 7, "(x, out, positions, inv_freq, scale, interleaved, inverse)");
   const Pair xs(a[0], "x");
   const at::Tensor* xt[2];
+  if (recorded(tensor(a[3], "inv_freq")))
+    throw Raise{PyExc_ValueError, "inv_freq takes no gradient: detach it"};
   for (int i = 0; i < xs.n; ++i) {
     xt[i] = &tensor(xs.o[i], "x");
     if (recorded(*xt[i])) return not_here();
@@ -250,7 +264,7 @@ PyObject* rotary(PyObject* const* a, Py_ssize_t n) {
   if (a[1] != Py_None) {
     const Pair given(a[1], "out");
     same_count(given.n, xs.n, "out must have a tensor for each x");
-    for (int i = 0; i < xs.n; ++i) out[i] = tensor(given.o[i], "out");
+    for (int i = 0; i < xs.n; ++i) out[i] = given_out(given.o[i]);
   } else {
     Outputs outs;
     for (int i = 0; i < xs.n; ++i)
@@ -274,6 +288,8 @@ PyObject* rotary(PyObject* const* a, Py_ssize_t n) {
   const double scale = real(a[4]);
   const int32_t flags = (truth(a[5]) ? GPUOS_ROTARY_INTERLEAVED : 0) | (truth(a[6]) ? GPUOS_ROTARY_INVERSE : 0);
   done(gpuos_rotary(xs.n, x, o, &p, &f, (float)scale, flags, at.stream()));
+  if (a[1] != Py_None)
+    for (int i = 0; i < xs.n; ++i) written(out[i]);
   return xs.tuple ? tuple_of(out, xs.n) : wrap(out[0]);
 }
 
@@ -291,6 +307,10 @@ PyObject* cache_write(PyObject* const* a, Py_ssize_t n) {
   }
   const gpuos_tensor slots = at.in(a[1], "slots");
   done(gpuos_cache_write(xs.n, x, &slots, c, s, at.stream()));
+  for (int i = 0; i < xs.n; ++i) {
+    written(tensor(cs.o[i], "codes"));
+    written(tensor(ss.o[i], "scales"));
+  }
   Py_RETURN_NONE;
 }
 
@@ -306,7 +326,7 @@ PyObject* cache_read(PyObject* const* a, Py_ssize_t n) {
   if (a[3] != Py_None) {
     const Pair given(a[3], "out");
     same_count(given.n, cs.n, "out must have a tensor for each cache");
-    for (int i = 0; i < cs.n; ++i) out[i] = tensor(given.o[i], "out");
+    for (int i = 0; i < cs.n; ++i) out[i] = given_out(given.o[i]);
   }
   const int32_t code = small(a[4], "dtype");
   const at::ScalarType type = code == GPUOS_F32 ? at::kFloat : code == GPUOS_F16 ? at::kHalf : at::kBFloat16;
@@ -326,6 +346,8 @@ PyObject* cache_read(PyObject* const* a, Py_ssize_t n) {
   for (int i = 0; i < cs.n; ++i) o[i] = at.in(out[i], "out");
   const gpuos_tensor slots = at.in(slots_t, "slots");
   done(gpuos_cache_read(cs.n, &slots, c, s, o, at.stream()));
+  if (a[3] != Py_None)
+    for (int i = 0; i < cs.n; ++i) written(out[i]);
   return cs.tuple ? tuple_of(out, cs.n) : wrap(out[0]);
 }
 
@@ -406,6 +428,7 @@ PyObject* logprobs_grad(PyObject* const* a, Py_ssize_t n) {
   const gpuos_tensor o = at.in(out, "out");
   done(gpuos_logprobs_grad(&d, &y, &st, a[3] != Py_None ? &opt[0] : nullptr, a[4] != Py_None ? &opt[1] : nullptr,
                            a[5] != Py_None ? &opt[2] : nullptr, &o, (float)real(a[6]), at.stream()));
+  if (a[7] != Py_None) written(out);
   return wrap(out);
 }
 

@@ -6,13 +6,15 @@ Each call runs one kernel at once on torch's current stream of its tensors'
 device; it allocates its outputs (where `out` gives none) and nothing else, so it
 may be captured into a CUDA graph.  As with an op of torch's own, requests
 submitted to an executor are seen once they are flushed; inside a
-``scheduler_context``, pending requests on the call's tensors are flushed first.  Tensors are CUDA tensors of one device.  A call that
-breaks a rule raises ``ValueError`` (``TypeError`` for a dtype, ``RuntimeError``
-for a device) and launches nothing.
+``scheduler_context``, pending requests on the call's tensors are flushed first.
+Tensors are CUDA tensors of one device.  A call that breaks a rule raises ``ValueError`` (``TypeError`` for a dtype,
+``RuntimeError`` for a device) and launches nothing.
 
 ``rotary``, ``route`` and ``logprobs`` take part in autograd; their gradients
 are also there as calls of their own (``rotary(..., inverse=True)``,
 ``route_grad``, ``logprobs_grad``), for steps that are captured or keep no graph.
+A given `out` and a written cache count as changed in place: a backward pass that saved
+one of them raises, as after an in-place op of torch's.
 include/gpuos_b200.h states each operator's formula and its edge cases.
 """
 from __future__ import annotations

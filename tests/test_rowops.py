@@ -1351,3 +1351,51 @@ def test_route_gradient_of_scores_near_the_smallest(by):
     # 2^-22, of terms up to 2.5 * 1.5.
     assert bool(((got.cpu().double() - want).abs() <= 16 * 2.0 ** -22 * 2.5 * 1.5).all()), got
     assert bool((got[0, 2:] == 0).all())
+
+
+@gpu
+def test_written_tensors_count_as_changed_in_place():
+    """A backward pass that saved a tensor which an operator wrote over raises; what autograd
+    follows is not written to behind its back."""
+    g = gen(31)
+    pos, f = torch.arange(4, device=DEV), R.rotary_frequencies(16, device=DEV)
+    rows = randn(g, 4, 2, 16).to(DEV)
+
+    def saved(shape):
+        w = torch.ones(shape, device=DEV, requires_grad=True)
+        t = torch.ones(shape, device=DEV)
+        return t, (w * t).sum()
+
+    q, loss = saved((4, 2, 16))
+    R.rotary(q, pos, f, out=q)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    c, s = R.cache_alloc(1, 8, 2, 16, device=DEV)
+    out, loss = saved((4, 2, 16))
+    before = c._version, s._version
+    R.cache_write(rows, pos, c, s)
+    assert c._version > before[0] and s._version > before[1]
+    R.cache_read(pos, c, s, out=out, dtype=F32)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    x, loss = saved((4, 16))
+    r = R.logprobs(x, pos, stats=True)
+    R.logprobs_grad(x, pos, r, torch.ones(4, device=DEV), out=x)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    # calls with new outputs leave their inputs as they are
+    before = rows._version
+    R.rotary(rows, pos, f)
+    assert rows._version == before
+    followed = torch.zeros(4, 2, 16, device=DEV, requires_grad=True)
+    with pytest.raises(ValueError, match="requires a gradient"):
+        R.rotary(rows, pos, f, out=followed)
+    with pytest.raises(ValueError, match="requires a gradient"):
+        R.cache_read(pos, c, s, out=followed, dtype=F32)
+    with pytest.raises(ValueError, match="inv_freq takes no gradient"):
+        R.rotary(rows, pos, f.clone().requires_grad_())
+    assert not bool(followed.any())
+    with torch.inference_mode():
+        z = torch.zeros(4, 2, 16, device=DEV)
+        assert torch.equal(R.rotary(rows, pos, f, out=z), R.rotary(rows, pos, f))
+    assert torch.equal(R.rotary(rows, pos, f, out=z), R.rotary(rows, pos, f))
