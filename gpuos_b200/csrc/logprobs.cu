@@ -14,7 +14,7 @@
 // weighted sum in 32 bits, rescaled when a step of U 16-byte packs raises the
 // maximum; they are joined at the row's end.  The alternatives cost nothing
 // while the row streams but a maximum that each thread leaves behind now and
-// then.  At the row's end the k-th largest of 64 maxima over threads is a bound
+// then.  At the row's end the k-th largest of the threads' maxima is a bound
 // that k elements reach, and only packs under a maximum that reaches it are read
 // again (a few KB).  Rows of many equal or masked logits make more candidates than that:
 // they are read again whole, through lists of a warp each, cut back when full
@@ -25,6 +25,8 @@
 // At 16 bits an SM's share of the memory rate is about 12 elements a cycle,
 // its exponentials 16, its instructions 128 lanes: the loop is kept to about 5
 // instructions an element (maxima of two elements at once, packed 32-bit sums and products).
+// 2048 x 128257 bf16 take 85 us (6.2 TB/s), with 5 alternatives 96; 1500 x 50257 fp32 with entropy
+// 49 (6.1 TB/s); their gradient, which reads and writes, 89 (6.7 TB/s).
 #include <cooperative_groups.h>
 
 #include "rowops.cuh"
@@ -38,11 +40,14 @@ namespace cg = cooperative_groups;
 constexpr int kMaxTop = 64;
 constexpr int kRowThreads = 256;  // of a row; short rows take a warp each, 8 to a CTA
 constexpr int kList = 128;    // candidates a warp holds
-constexpr int kWarpPacks = 128;  // 16-byte packs of a row that one warp takes,
-constexpr int kWarpPacksMany = 3200, kWarpRows = 8;  // and where there are many rows for each SM
+constexpr int kWarpPacks = 128;  // 16-byte packs of a row that a warp has in flight at once
+constexpr int kWarpTop = 24;     // alternatives of a row that a warp takes, at most
+constexpr int kWarpReads = 16000;  // packs times alternatives of such a row
 constexpr int kLongPacks = 14000;  // of a row whose threads have eight packs in flight
 
+constexpr int kSeeds = 64;
 constexpr int kFewTop = 32;   // alternatives up to which 64 maxima give a close bound
+constexpr int kFewRounds = 8;  // and up to which a warp takes a round for each (8192 x 300 with 5: 14.1 us, by bits 14.7)
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kLowest = -3.402823466e38f;  // the lowest finite number: where a maximum starts
 
@@ -163,7 +168,7 @@ __device__ __forceinline__ void add_two(Sums& r, float2 x, float k2) {
 
 constexpr uint32_t kMarks = 16;    // maxima a thread leaves on its way along a row
 constexpr uint32_t kReach = 4;     // of them a thread, on average, may reach the bound, and
-constexpr uint32_t kFew = 4;       // packs a thread then reads again, before the lists are used
+constexpr uint32_t kFew = 4;       // packs a thread then reads again at once
 
 // Kept small: what the CTAs of an SM do not take of its memory holds their loads
 // in flight (at 45 KB a CTA the loop ran a third slower than at 15).
@@ -176,7 +181,7 @@ struct TopShared {
   unsigned long long bound;          // no candidate below it is needed
   uint32_t count;                    // of the candidates
   uint32_t reached;                  // of `reach`
-  alignas(16) float seeds[THREADS < 256 ? THREADS : 256];
+  alignas(16) float seeds[kSeeds];
   uint32_t reach[kReached];           // (mark, thread) whose maximum reaches the bound
   unsigned long long last[kMaxTop];  // the top_k, sorted
   // one after the other: the marks; the candidates; where those are too many, each
@@ -279,65 +284,72 @@ __device__ __forceinline__ uint32_t candidates(const Pack<T, N>& x, uint32_t at,
   return open;
 }
 
-// Ranks n unique keys by counting the larger ones, 8 lanes to a key; those
-// below k go to out, sorted.
+// Ranks n unique keys by counting the larger ones; those below k go to out, sorted.
+// In a CTA 8 lanes count for a key; a warp's lanes take a key each and read all keys together.
 template <int THREADS>
 __device__ __forceinline__ void rank_into(const unsigned long long* keys, uint32_t n, uint32_t k, unsigned long long* out) {
+  constexpr uint32_t L = THREADS == 32 ? 1 : 8;  // lanes to a key
   const uint32_t tid = threadIdx.x % THREADS;
-  for (uint32_t i0 = 0; i0 < n; i0 += THREADS / 8) {
-    const uint32_t i = i0 + tid / 8;
+  for (uint32_t i0 = 0; i0 < n; i0 += THREADS / L) {
+    const uint32_t i = i0 + tid / L;
     const unsigned long long mine = i < n ? keys[i] : 0;
     uint32_t rank = 0;
 #pragma unroll 4
-    for (uint32_t j = tid & 7; j < n; j += 8) rank += keys[j] > mine;
+    for (uint32_t j = tid % L; j < n; j += L) rank += keys[j] > mine;
 #pragma unroll
-    for (int d = 1; d < 8; d <<= 1) rank += __shfl_xor_sync(~0u, rank, d);
-    if ((tid & 7) == 0 && i < n && rank < k) out[rank] = mine;
+    for (uint32_t d = 1; d < L; d <<= 1) rank += __shfl_xor_sync(~0u, rank, d);
+    if (tid % L == 0 && i < n && rank < k) out[rank] = mine;
   }
 }
 
-// The bound: a value that k of the row's elements reach, from the threads' maxima.
-// For few alternatives the k-th largest of 64 maxima over neighbouring threads is close,
-// for more it takes 256
-// (64 alternatives of 8 x 32000: 12 us, 48 from 64 maxima, whose last one is far too low).
+template <int THREADS>
+__device__ __forceinline__ uint32_t row_count(bool p) {
+  if constexpr (THREADS == 32) return __popc(__ballot_sync(~0u, p));
+  else return __syncthreads_count(p);
+}
+
+// The bound: a value that k of the row's elements reach, from the threads' maxima.  A maximum
+// that is still where it started was reached by nothing and does not count: with fewer than k
+// others there is no bound.  (8 x 32000 with 20 alternatives: 7.7 us by 64 maxima, 8.2 by bits; with 64,
+// too many for 64 maxima, 10.5 by bits.)
 template <typename T, int THREADS>
-__device__ __forceinline__ void find_bound(TopShared<T, THREADS>& top, float m, uint32_t k) {
+__device__ __forceinline__ void find_bound(TopShared<T, THREADS>& top, float m, uint32_t k, uint32_t packs) {
   const int tid = threadIdx.x % THREADS;
-  uint32_t rank = 0;
-  float me = m;
-  bool mine = true;
-  if constexpr (THREADS == 32) {
+  if (THREADS == 32 && k <= kFewRounds) {
     // a round for each alternative: the largest of those left
+    float me = m;
     for (uint32_t i = 0; i < k; ++i) {
       me = warp_max(m);
       if (tid == __ffs(__ballot_sync(~0u, m == me)) - 1) m = -INFINITY;
     }
-    mine = tid == 0;
-    rank = k - 1;
+    if (tid == 0 && me > kLowest) top.bound = key_of(me, 0) & ~0xffffffffull;
+  } else if (THREADS > 32 && k <= kFewTop && packs >= THREADS) {
+    // the k-th largest of 64 maxima over neighbouring threads, 4 lanes to each
+    constexpr int S = kSeeds, L = THREADS > S ? THREADS / S : 1;
+    const int at = tid / L;
+    uint32_t rank = 0;
+#pragma unroll
+    for (int d = 1; d < L; d <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+    if (tid % L == 0) top.seeds[at] = m;
+    row_sync<THREADS>();
+#pragma unroll
+    for (int j = tid % L * 4; j < S; j += L * 4) {
+      const float4 o = *reinterpret_cast<const float4*>(top.seeds + j);
+      rank += (o.x > m || (o.x == m && j < at)) + (o.y > m || (o.y == m && j + 1 < at)) +
+              (o.z > m || (o.z == m && j + 2 < at)) + (o.w > m || (o.w == m && j + 3 < at));
+    }
+#pragma unroll
+    for (int d = 1; d < L; d <<= 1) rank += __shfl_xor_sync(~0u, rank, d);
+    if (tid % L == 0 && rank == k - 1 && m > kLowest) top.bound = key_of(m, 0) & ~0xffffffffull;
   } else {
-    auto among = [&](auto seeds) {
-      constexpr int S = decltype(seeds)::value, L = THREADS / S;  // L lanes to a seed
-#pragma unroll
-      for (int d = 1; d < L; d <<= 1) me = fmaxf(me, __shfl_xor_sync(~0u, me, d));
-      if (tid % L == 0) top.seeds[tid / L] = me;
-      __syncthreads();
-#pragma unroll 4
-      for (int j = tid % L * 4; j < S; j += L * 4) {
-        const float4 o = *reinterpret_cast<const float4*>(top.seeds + j);
-        const int at = tid / L;
-        rank += (o.x > me || (o.x == me && j < at)) + (o.y > me || (o.y == me && j + 1 < at)) +
-                (o.z > me || (o.z == me && j + 2 < at)) + (o.w > me || (o.w == me && j + 3 < at));
-      }
-#pragma unroll
-      for (int d = 1; d < L; d <<= 1) rank += __shfl_xor_sync(~0u, rank, d);
-      mine = tid % L == 0;
-    };
-    if (k <= kFewTop) among(std::integral_constant<int, 64>());
-    else among(std::integral_constant<int, 256>());
+    // the largest leading bits that k of all the maxima reach (of 32 bits the value to 2^-11)
+    constexpr int kBits = std::is_same_v<T, __nv_bfloat16> ? 16 : 20;
+    const uint32_t mine = m > kLowest ? (uint32_t)(key_of(m, 0) >> 32) : 0;
+    uint32_t t = 0;
+    for (int b = 31; b >= 32 - kBits; --b)
+      if (row_count<THREADS>(mine >= (t | 1u << b)) >= k) t |= 1u << b;
+    if (tid == 0) top.bound = (unsigned long long)t << 32;
   }
-  // A maximum that is still where it started was reached by nothing: no bound.
-  // Otherwise every element of this value and above counts, whatever its index.
-  if (mine && rank == k - 1 && me > kLowest) top.bound = key_of(me, 0) & ~0xffffffffull;
   row_sync<THREADS>();
 }
 
@@ -451,7 +463,7 @@ gpuos_logprobs_kernel(const __grid_constant__ LogArgs a) {
     if (TOP) {
       if (THREADS == 32 && steps == 1) {
         // the whole row is in registers: its candidates are taken from there
-        find_bound<T, THREADS>(top, r.m, a.top_k);
+        find_bound<T, THREADS>(top, r.m, a.top_k, p1 - p0);
         const unsigned long long bound = top.bound;
         if (!(cm < value_of(bound)))
 #pragma unroll
@@ -483,7 +495,7 @@ gpuos_logprobs_kernel(const __grid_constant__ LogArgs a) {
   }
   bool few = true;
   if (TOP && !(THREADS == 32 && steps == 1)) {
-    find_bound<T, THREADS>(top, r.m, a.top_k);
+    find_bound<T, THREADS>(top, r.m, a.top_k, p1 - p0);
     const unsigned long long bound = top.bound;
     if (r.m >= value_of(bound))
       for (uint32_t i = 0; i < mark; ++i)
@@ -494,24 +506,27 @@ gpuos_logprobs_kernel(const __grid_constant__ LogArgs a) {
     row_sync<THREADS>();
     // the packs under those marks, a lane each
     const uint32_t each = stretch * U;
-    few = top.reached <= top.kReached && (uint64_t)top.reached * each <= kFew * THREADS;
+    few = top.reached <= top.kReached &&
+          (uint64_t)top.reached * each <= max(kFew * THREADS, (p1 - p0) / 4);
     if (few) {
       const uint32_t items = top.reached * each;
-      Pack<T, W> q[kFew];
-      uint32_t at[kFew];
+      for (uint32_t i0 = 0; i0 < items; i0 += kFew * THREADS) {
+        Pack<T, W> q[kFew];
+        uint32_t at[kFew];
 #pragma unroll
-      for (int u = 0; u < kFew; ++u) {
-        const uint32_t it = u * THREADS + tid;
-        at[u] = p1;
-        if (it < items) {
-          const uint32_t i = it / each, to = top.reach[i];
-          at[u] = p0 + ((to >> 16) * each + (it - i * each)) * THREADS + (to & 0xffff);
+        for (int u = 0; u < kFew; ++u) {
+          const uint32_t it = i0 + u * THREADS + tid;
+          at[u] = p1;
+          if (it < items) {
+            const uint32_t i = it / each, to = top.reach[i];
+            at[u] = p0 + ((to >> 16) * each + (it - i * each)) * THREADS + (to & 0xffff);
+          }
+          if (at[u] < p1) q[u] = load_pack<T, W, false>(body + (uint64_t)at[u] * W);
         }
-        if (at[u] < p1) q[u] = load_pack<T, W, false>(body + (uint64_t)at[u] * W);
-      }
 #pragma unroll
-      for (int u = 0; u < kFew; ++u)
-        if (at[u] < p1) push(q[u], head + at[u] * W, bound);
+        for (int u = 0; u < kFew; ++u)
+          if (at[u] < p1) push(q[u], head + at[u] * W, bound);
+      }
       if (has_loose) push(loose, loose_at, bound);
     }
   }
@@ -703,9 +718,7 @@ template <typename T, int THREADS, int U, bool ENT, bool TOP>
 void launch(const LogArgs& a, uint32_t parts, cudaStream_t s) {
   constexpr int kRows = kRowsOfCta<THREADS>;
   const size_t smem = kRows * kSharedOfRow<T, THREADS, TOP> + (TOP && parts > 1 ? parts * a.top_k * 8 : 0);
-  auto kernel = gpuos_logprobs_kernel<T, THREADS, U, ENT, TOP>;
-  if (smem > 48 * 1024)
-    cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory");
+  auto kernel = gpuos_logprobs_kernel<T, THREADS, U, ENT, TOP>;  // (up to 30 KB of shared memory)
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((a.rows + kRows - 1) / kRows * parts));
   cfg.blockDim = dim3(THREADS * kRows);
@@ -732,11 +745,14 @@ template <typename T>
 void forward(const LogArgs& a, cudaStream_t s) {
   constexpr int64_t kStep = kRowThreads * 16 / sizeof(T);  // elements a CTA reads at once
   const int64_t sms = sm_count();
-  // A warp a row, where that is one step, or where there are rows enough for every warp of the
-  // GPU.  32 maxima bound 32 alternatives; those under marks are few enough for a warp up to 16.
-  const int64_t packs = a.cols * (int64_t)sizeof(T) / 16;
-  if ((packs <= kWarpPacks && a.top_k <= 32) ||
-      (packs <= kWarpPacksMany && a.rows >= kWarpRows * sms && a.top_k <= 16))
+  // A warp a row: short rows with few alternatives (8 x 250 with 8: 5.5 us, a CTA a row 7.0), or rows
+  // enough for the warps of every SM, the more the longer they are (1183 x 24000 with 5 alternatives:
+  // 33 us, CTAs 24; 4096 x 24000: 57 and 64; 4096 x 1000: 10 and 42).  Its 32 maxima give a loose
+  // bound, so that what it reads again grows with the alternatives and the row (4096 x 8000 with 16: 34
+  // us, CTAs 46, with 24: 58 and 48; x 24000 with 16: 76 and 67).
+  const int64_t packs = a.cols * (int64_t)sizeof(T) / 16, k = a.top_k;
+  if ((packs <= kWarpPacks && k <= kFewRounds) ||
+      (a.rows >= sms * (2 + packs / 160) && k <= kWarpTop && packs * std::max<int64_t>(k, 5) <= kWarpReads))
     return by_outputs<T, 32, 4>(a, 1, s);
   uint32_t parts = 1;
   // (8 x 32000 with 20 alternatives: 8.4 us over 4 CTAs a row, 9.3 over 8, 8.8 over 2)

@@ -212,6 +212,7 @@ void rotary(int32_t n, const gpuos_tensor* x, const gpuos_tensor* out, const gpu
   need(inv_freq->dtype == GPUOS_F64 || inv_freq->dtype == GPUOS_F32, "inv_freq must be float64 or float32");
   need(is_index(positions->dtype), "positions must be int32 or int64");
   const int64_t half = inv_freq->sizes[0];
+  need(half <= kTablePairs, "inv_freq has more than 2048 pairs");
   const int nd = x[0].ndim;
   need(nd == 3 || nd == 4, "x must have 3 dims (token, head, element) or 4 (batch, token, head, element)");
   check_tensor(positions, nd - 2, "positions");
@@ -234,7 +235,6 @@ void rotary(int32_t n, const gpuos_tensor* x, const gpuos_tensor* out, const gpu
            "the last dim of x and out must be contiguous");
     check_output(out[i], "out");
   }
-  need(half <= kTablePairs, "inv_freq has more than 2048 pairs");
   for (int i = 0; i < n; ++i) {
     need(same_view(x[i], out[i]) || !overlap(x[i], out[i]), "out must be x or not overlap it");
     need(!overlap(out[i], *positions) && !overlap(out[i], *inv_freq), "out overlaps an input");

@@ -1,5 +1,5 @@
 // Device helpers of the row operators: vector loads and stores of 32- and
-// 16-bit elements, division by a launch constant, warp reductions.
+// 16-bit elements, division by a launch constant, packed 32-bit arithmetic.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

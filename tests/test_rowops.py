@@ -1399,3 +1399,31 @@ def test_written_tensors_count_as_changed_in_place():
         z = torch.zeros(4, 2, 16, device=DEV)
         assert torch.equal(R.rotary(rows, pos, f, out=z), R.rotary(rows, pos, f))
     assert torch.equal(R.rotary(rows, pos, f, out=z), R.rotary(rows, pos, f))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,cols,top", [(3011, 24001, 5), (3011, 11999, 5), (1403, 7999, 16), (1301, 1990, 24), (1301, 1990, 25), (9, 901, 24)])
+def test_logprobs_rows_of_a_warp_and_just_past_them(dtype, rows, cols, top):
+    """Long rows by a warp each: several packs under a mark, more marks than are read at once, ties that overflow."""
+    g = torch.Generator(device=DEV).manual_seed(cols + top)
+    x = (torch.randn(rows, cols, generator=g, device=DEV) * 2).to(dtype)
+    x[0] = 0.5
+    x[1] = -math.inf
+    x[2, 1:] = -math.inf
+    x[3] = torch.linspace(-8, 8, cols, device=DEV).to(dtype)          # the largest all in the last mark
+    x[4] = x[3].flip(0)
+    x[5, cols // 2:] = 20.0
+    x[6] = 0
+    x[6, ::max(cols // 40, 1)] = 1.0                                  # forty of them, over all marks
+    x[7, 7::97] = math.nan
+    x[8, :] = torch.finfo(dtype).min
+    y = torch.randint(0, cols, (rows,), generator=g, device=DEV)
+    r = R.logprobs(x, y, top=top, entropy=True)
+    order = torch.where(x != x, torch.tensor(-math.inf, device=DEV), x.float()).sort(dim=-1, descending=True, stable=True)[1]
+    assert torch.equal(r.top_tokens, order[:, :top])
+    assert bool(r.logprob[7].isnan())
+    some = [i for i in range(min(rows, 40)) if i != 7] + list(range(rows - 3, rows))
+    some = torch.tensor([i for i in some if i != 7])
+    keep = R.LogProbs(*(None if t is None else t[some.to(DEV)] for t in r))
+    check_logprobs(keep, x.cpu()[some], y.cpu()[some], top, 1.0, True)
