@@ -2,7 +2,9 @@
 
 `gpuos_b200.gpuos_ext` is a drop-in for the reference's `gpuos_ext` module
 (init / submit_* / flush / register_* / shutdown); `gpuos_b200.scheduler`
-mirrors the reference's TorchDispatch scheduler.  The compute path is the
+mirrors the reference's TorchDispatch scheduler; `gpuos_b200.rowops` holds the
+row operators of a language model's step (rotary positions, a quantised cache,
+routing to experts, log probabilities).  The compute path is the
 CUDA code in `libgpuos_b200.so`; there is no CPU fallback: if the native
 library is missing, `load()` (and `from gpuos_b200 import gpuos_ext`) fails.
 """

@@ -5,8 +5,8 @@
 
 Outputs (next to this file, git-ignored, shipped with the tree):
     libgpuos_b200.so   the executor (CUDA kernels + C++ runtime + C ABI, with
-                       the multi-process IPC server and client),
-                       cudart linked statically
+                       the multi-process IPC server and client) and the row
+                       operators, cudart linked statically
     gpuos_ext*.so      the Python module with the reference's API
 
 No GPU is needed to build: nvcc cross-compiles for sm_100a.

@@ -17,6 +17,8 @@
 // above that are instructions, so each token's row of the cache is found once by the lanes that
 // share the token, which then walk over its heads; a write holds a group in the
 // registers of neighbouring lanes and joins its maximum by shuffles.
+// 16000 tokens x 2 x 8 heads x 128 bf16 as e4m3: written in 20.4 us, read in 18.3 (99.5 MB each: 4.9 and
+// 5.4 TB/s); 100003 tokens of 4 bits in groups of 32 to fp16: read in 96.8 us (5.6 TB/s).
 #include <cuda_fp8.h>
 
 #include "rowops.cuh"
@@ -279,6 +281,8 @@ gpuos_cache_write_kernel(const __grid_constant__ CacheArgs a) {
   }
 }
 
+// Eight heads' codes in flight a thread (four where the results are 32 bits wide: 64 registers, four
+// CTAs of an SM), since a code's load waits for the token's slot first.
 template <typename T, int F, bool VEC>
 __global__ void __launch_bounds__(kThreads, 4)
 gpuos_cache_read_kernel(const __grid_constant__ CacheArgs a) {

@@ -199,7 +199,9 @@ inline int sm_count() {
 // How tokens of `heads` rows of `units` groups are spread over CTAs: a thread
 // belongs to one token and one group and walks over about 8 heads in steps of
 // groups * split; with few tokens the heads are spread over more threads, then
-// over more CTAs, so that their loads start at once on many SMs.
+// over more CTAs, so that their loads start at once on many SMs.  (Rotary positions of 8 tokens x 40 heads:
+// 2.4 us, 16.4 with one thread for all heads; of 9001 tokens 35 and 49; a cache's read of 64 tokens 1.8
+// and 2.5.)
 struct Spread {
   uint32_t lanes;   // threads side by side over a head's groups
   uint32_t groups;  // heads a CTA takes at once

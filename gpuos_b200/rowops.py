@@ -7,8 +7,9 @@ device; it allocates its outputs (where `out` gives none) and nothing else, so i
 may be captured into a CUDA graph.  As with an op of torch's own, requests
 submitted to an executor are seen once they are flushed; inside a
 ``scheduler_context``, pending requests on the call's tensors are flushed first.
-Tensors are CUDA tensors of one device.  A call that breaks a rule raises ``ValueError`` (``TypeError`` for a dtype,
-``RuntimeError`` for a device) and launches nothing.
+Tensors are CUDA tensors of one device.  A call that breaks a rule raises
+``ValueError`` (``TypeError`` for a dtype, ``RuntimeError`` for a device) and
+launches nothing.
 
 ``rotary``, ``route`` and ``logprobs`` take part in autograd; their gradients
 are also there as calls of their own (``rotary(..., inverse=True)``,

@@ -376,7 +376,9 @@ int32_t gpuos_rotary(int32_t n, const gpuos_tensor* x, const gpuos_tensor* out,
  * 32 bits with each step rounded: scale = a * (1/Q), code = x * ((1/a) * Q)
  * rounded to the format, nearest even; Q = 127, 448, 7.  Where a < 2^-100
  * scale and codes are 0.  An infinity takes the largest code and does not count
- * for a, nor does NaN, which takes code 0 (E4M3: NaN). */
+ * for a, nor does NaN, which takes code 0 (E4M3: NaN).  Limits of a call: fewer
+ * than 2^31 units of 8 elements (or groups), cache rows below 2^31, and strides
+ * below 2^32 elements; a larger call is refused. */
 int32_t gpuos_cache_write(int32_t n, const gpuos_tensor* x, const gpuos_tensor* slots,
                           const gpuos_tensor* codes, const gpuos_tensor* scales, void* stream);
 
@@ -396,8 +398,8 @@ int32_t gpuos_cache_read(int32_t n, const gpuos_tensor* slots, const gpuos_tenso
  * scores without bias, divided by their sum with `renormalize`, times `scale`.
  * The choice is that of keys in 64 bits; of equal keys, and of equal groups, the
  * lowest index comes first.  A NaN logit counts as -inf in the choice; a row of
- * -inf has scores 0 (softmax), and where the chosen scores sum to 0 the
- * renormalised weights are 0. */
+ * -inf has scores 0 (softmax); a sigmoid below 2^-126 counts as 0; where the
+ * chosen scores sum to 0 the renormalised weights are 0. */
 #define GPUOS_SCORE_SOFTMAX 0
 #define GPUOS_SCORE_SIGMOID 1
 #define GPUOS_GROUP_MAX 0
