@@ -48,6 +48,7 @@ struct RotArgs {
   FastDiv per_token;    // threads of a token: lanes * head groups
   uint32_t head_step;   // head groups of all CTAs that share a token
   uint32_t tile;        // tokens a CTA takes
+  uint32_t two;         // 1: two heads in flight (interleaved, nothing copied)
   float scale;
   int pos_wide, freq_wide;
 };
@@ -83,6 +84,13 @@ __device__ __forceinline__ uint32_t table_at(uint32_t token, uint32_t pair, uint
   if constexpr (P == 1) return token * half + pair;
   const uint32_t j = pair / P, i = pair % P;
   return token * half + (i / 2) * (half / P) * 2 + j * 2 + (i & 1);
+}
+
+template <typename T>
+__device__ __forceinline__ void turn(T& first, T& second, float2 cd) {
+  const float v = to_f(first), w = to_f(second);
+  first = from_f<T>(v * cd.x - w * cd.y);
+  second = from_f<T>(w * cd.x + v * cd.y);
 }
 
 template <typename T, int V, int VL, bool INTER>
@@ -123,6 +131,7 @@ gpuos_rotary_kernel(const __grid_constant__ RotArgs a) {
     const T* x = from(h) + j * V;
     fetch<T, V, VL>(x, p);
     if (!INTER) fetch<T, V, VL>(x + half, q);
+    else if (a.two && h + a.head_step < heads) fetch<T, V, VL>(from(h + a.head_step) + j * V, q);
     if (j < a.t[h >= a.t[0].heads].copies) fetch<T, V, VL>(x + 2 * half, r);
   };
   if (live && j0 < a.units && h0 < heads) load(h0, j0);
@@ -154,20 +163,21 @@ gpuos_rotary_kernel(const __grid_constant__ RotArgs a) {
         cd[2 * k + 1] = make_float2(w.z, w.w);
       }
     }
-    for (uint32_t h = h0; h < heads; h += a.head_step) {
+    for (uint32_t h = h0; h < heads; h += INTER ? a.head_step << a.two : a.head_step) {
       if (j != j0 || h != h0) load(h, j);
       T* o = to(h) + j * V;
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        T& first = p.v[INTER ? 2 * i : i];
-        T& second = INTER ? p.v[2 * i + 1] : q.v[i];
-        const float v = to_f(first), w = to_f(second);
-        first = from_f<T>(v * cd[i].x - w * cd[i].y);
-        second = from_f<T>(w * cd[i].x + v * cd[i].y);
-      }
+      for (int i = 0; i < P; ++i) turn(p.v[INTER ? 2 * i : i], INTER ? p.v[2 * i + 1] : q.v[i], cd[i]);
       put<T, V, VL>(o, p);
       if (!INTER) put<T, V, VL>(o + half, q);
       if (j < a.t[h >= a.t[0].heads].copies) put<T, V, VL>(o + 2 * half, r);
+      if constexpr (INTER) {
+        if (a.two && h + a.head_step < heads) {
+#pragma unroll
+          for (int i = 0; i < P; ++i) turn(q.v[2 * i], q.v[2 * i + 1], cd[i]);
+          put<T, V, VL>(to(h + a.head_step) + j * V, q);
+        }
+      }
     }
   }
   // where more is copied than rotated
@@ -301,6 +311,9 @@ void rotary(int32_t n, const gpuos_tensor* x, const gpuos_tensor* out, const gpu
   a.per_token = FastDiv(sp.lanes * sp.groups);
   a.head_step = sp.groups * sp.split;
   a.tile = sp.tile;
+  // An interleaved group is one load a head, half of what a split one keeps in flight: two heads at once
+  // (15715 x 18 x 80 fp32: 37.0 us, 45.5 with one; 9001 x 40 x 128 bf16: 39.8 and 47.5).
+  a.two = inter && copies == 0;
   const dim3 grid(sp.tiles, sp.split);
   if (x[0].dtype == GPUOS_F32) launch<float>(a, v, vl, inter, grid, stream);
   else if (x[0].dtype == GPUOS_F16) launch<__half>(a, v, vl, inter, grid, stream);

@@ -1427,3 +1427,23 @@ def test_logprobs_rows_of_a_warp_and_just_past_them(dtype, rows, cols, top):
     some = torch.tensor([i for i in some if i != 7])
     keep = R.LogProbs(*(None if t is None else t[some.to(DEV)] for t in r))
     check_logprobs(keep, x.cpu()[some], y.cpu()[some], top, 1.0, True)
+
+
+@gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rot,dq,dk", [(32, 128, 32), (16, 128, 64), (96, 192, 104), (8, 264, 8), (64, 64, 64), (2, 50, 6)])
+def test_rotary_shares_of_a_head(dtype, interleaved, rot, dq, dk):
+    """More copied than rotated elements, heads of two sizes, one tensor in place beside one that is not, odd numbers of heads."""
+    g = gen(rot + dq)
+    f = R.rotary_frequencies(rot).to(DEV)
+    how = dict(interleaved=interleaved, scale=1.25)
+    for tokens, hq, hk in ((1, 7, 1), (37, 9, 3), (700, 5, 2)):
+        q, k = randn(g, tokens, hq, dq, dtype=dtype).to(DEV), randn(g, tokens, hk, dk, dtype=dtype).to(DEV)
+        pos = torch.randint(0, 5000, (tokens,), generator=g).to(DEV)
+        room = torch.full((tokens, hq + 1, dq), 7.0, dtype=dtype, device=DEV)
+        was = k.clone()
+        a, b = R.rotary((q, k), pos, f, out=(room[:, :hq], k), **how)
+        check_rotary(a, q, pos, f, **how)
+        check_rotary(b, was, pos, f, **how)
+        assert b.data_ptr() == k.data_ptr() and bool((room[:, hq] == 7).all())
