@@ -242,7 +242,7 @@ __device__ __forceinline__ void route_exact(const RouteArgs& a, bool keyed, int6
       }
   };
   again();
-  float sum = 0.f;
+  float low = -INFINITY, high = -INFINITY;  // the logits of ranks lane and lane + 32
 #pragma unroll 1
   for (uint32_t r = 0; r < a.top_k; ++r) {
     const Key64 best = lanes_top<32>(mine);
@@ -251,20 +251,25 @@ __device__ __forceinline__ void route_exact(const RouteArgs& a, bool keyed, int6
       key[e] = 0;
       again();
     }
-    const float s = (float)score(to_f(row[e]));
-    sum += s;
+    if (lane == r % 32) (r < 32 ? low : high) = to_f(row[e]);
     if (lane == 0) {
-      a.weights[t * a.ws + r * a.wk] = a.renorm ? s : s * a.scale;
       if (a.wide) static_cast<int64_t*>(a.experts)[t * a.es + r * a.ek] = e;
       else static_cast<int32_t*>(a.experts)[t * a.es + r * a.ek] = (int32_t)e;
     }
   }
-  if (a.renorm) {
-    const float by = sum == 0.f ? 0.f : a.scale / sum;
-    if (lane == 0)
-#pragma unroll 1
-      for (uint32_t r = 0; r < a.top_k; ++r) a.weights[t * a.ws + r * a.wk] *= by;
-  }
+  const float top = lanes_top<32>(fmaxf(low, high));
+  auto weight = [&](float v) {
+    if (!a.renorm || a.sigmoid || total != total) return (float)score(v);
+    return top == -INFINITY ? 0.f : expf(v - top);  // (as in the lanes' part)
+  };
+  low = lane < a.top_k ? weight(low) : 0.f;
+  high = lane + 32 < a.top_k ? weight(high) : 0.f;
+  const float sum = a.renorm ? lanes_sum<32>(low + high) : 1.f;
+  auto put = [&](uint32_t r, float s) {
+    if (r < a.top_k) a.weights[t * a.ws + r * a.wk] = sum == 0.f ? 0.f : s / sum * a.scale;
+  };
+  put(lane, low);
+  put(lane + 32, high);
   __syncwarp();
 }
 
@@ -686,21 +691,30 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
     if (later && live && seat.lane == 0) which[atomicAdd(&left, 1u)] = (uint16_t)(step * kTokens + sub);
 
     // weights from the chosen logits, a lane each
-    float sc = 0.f;
-    if (seat.lane < a.top_k && live && !later) {
+    const bool mine = seat.lane < a.top_k && live && !later;
+    float v = -INFINITY, sc = 0.f;
+    if (mine) {
       const uint32_t e = expert_of<NPL>(a, slot);
-      const float v = to_f(row[e]);
-      if (SIGMOID) sc = rcp(1.f + expf(-v));
-      else sc = m == -INFINITY ? 0.f : expf(v - m) * rcp(total);
+      v = to_f(row[e]);
       if (a.wide) static_cast<int64_t*>(a.experts)[t * a.es + seat.lane * a.ek] = e;
       else static_cast<int32_t*>(a.experts)[t * a.es + seat.lane * a.ek] = (int32_t)e;
     }
-    float norm = a.scale;
-    if (a.renorm) {
-      const float sum = lanes_sum<LPT>(sc);
-      norm = sum == 0.f ? 0.f : a.scale / sum;
+    if (SIGMOID) {
+      if (mine) sc = rcp(1.f + expf(-v));
+    } else if (a.renorm) {
+      // The chosen may lie far below the row's largest logit, where scores leave 32 bits: their shares
+      // are the softmax of the chosen alone.  (Ordered by logits, the chosen have the largest.)
+      const float top = scored ? lanes_top<LPT>(v) : m;
+      if (mine && top != -INFINITY) sc = expf(v - top);
+    } else if (mine && m != -INFINITY) {
+      sc = expf(v - m) * rcp(total);
     }
-    if (seat.lane < a.top_k && live && !later) a.weights[t * a.ws + seat.lane * a.wk] = sc * norm;
+    if (a.renorm) {
+      // a score over the sum first: the sum's own inverse times the scale may leave 32 bits
+      const float sum = lanes_sum<LPT>(sc);
+      sc = sum == 0.f ? 0.f : sc / sum;
+    }
+    if (mine) a.weights[t * a.ws + seat.lane * a.wk] = sc * a.scale;
   }
 
   __syncthreads();

@@ -1,0 +1,63 @@
+"""The row operators where 32-bit scores leave their range, where keys tie, where
+autograd looks at a call in other ways than by a gradient, and where several threads meet.
+
+Tolerances count roundings as in test_rowops.py, whose oracles these tests use.
+"""
+import itertools
+import math
+
+import pytest
+import torch
+
+from gpuos_b200 import rowops as R
+from test_rowops import BF, DEV, F32, FP, ROUTE_REL, TYPES, gen, gpu, randn, route_oracle
+
+
+# ---------------------------------------------------------------------------
+# Routing
+# ---------------------------------------------------------------------------
+def check_weights(got, want, rel=ROUTE_REL):
+    got = got.cpu().double()
+    assert bool(torch.isfinite(got).all()), got
+    assert bool(((got - want).abs() <= rel * want.abs()).all()), (got, want)
+
+
+@gpu
+@pytest.mark.parametrize("scale", [1.0, 10.0, 1e30])
+def test_renormalised_sigmoids_near_the_smallest_normal_number(scale):
+    """scale / sum would leave 32 bits; the shares are ordinary numbers."""
+    x = torch.tensor([[-86.5, -89.0, -95.0, -96.0], [-85.0, -85.5, -86.0, -100.0], [-86.25, -86.25, -87.0, -100.0]])
+    for top_k in (1, 2):
+        w, e = R.route(x.to(DEV), top_k, score="sigmoid", renormalize=True, scale=scale)
+        ww, we = route_oracle(x, top_k, score="sigmoid", renormalize=True, scale=scale)
+        assert torch.equal(e.cpu(), we)
+        keep = [1, 2] if top_k == 2 else [0, 1, 2]
+        check_weights(w[keep], ww[keep])
+    # more ranks than a warp has lanes: the other selection
+    x = -85.0 - torch.arange(40.0)[None] / 32
+    w, e = R.route(x.to(DEV), 36, score="sigmoid", renormalize=True, scale=scale)
+    ww, we = route_oracle(x, 36, score="sigmoid", renormalize=True, scale=scale)
+    assert torch.equal(e.cpu(), we)
+    check_weights(w, ww)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("below", [10.0, 80.0, 88.0, 96.0, 104.0, 200.0])
+@pytest.mark.parametrize("experts,top_k,groups", [(3, 2, 1), (32, 4, 4), (256, 8, 8), (64, 36, 1), (48, 33, 2)])
+def test_renormalised_softmax_of_experts_far_below_the_largest(dtype, below, experts, top_k, groups):
+    """The bias picks experts whose scores leave 32 bits: their shares are those of their logits alone."""
+    g = gen(experts + int(below))
+    x = torch.zeros(5, experts)
+    x[:, 1:] = -below - torch.rand(5, experts - 1, generator=g) * 4
+    x = x.to(dtype)
+    bias = 4.0 - torch.arange(experts).float() / 64  # falling by more than any picked score
+    bias[0] = -4.0
+    for rule in ("max", "top2"):
+        how = dict(groups=groups, top_groups=max(1, groups // 2), group_score=rule, renormalize=True, scale=2.5)
+        if top_k > experts // groups * how["top_groups"]:
+            how["top_groups"] = groups
+        w, e = R.route(x.to(DEV), top_k, bias=bias.to(DEV), **how)
+        ww, we = route_oracle(x, top_k, bias=bias, **how)
+        assert torch.equal(e.cpu(), we) and not bool((we == 0).any())
+        check_weights(w, ww)
