@@ -155,6 +155,16 @@ __device__ __forceinline__ float rcp(float x) {
 }
 constexpr float kLog2e = 1.44269504088896341f;
 
+// The sigmoid of a chosen logit over e^top.  Shares of a sum take the smaller of 0 and the largest chosen
+// logit as top, so that sigmoids too small for 32 bits keep their ratios; a sigmoid by itself takes 0.
+// e^-v leaves 64 bits at the limit: the sigmoid is 0 from there on.
+__device__ __forceinline__ float sigmoid_over(float v, float top) {
+  const float a = expf(-fabsf(v)), q = rcp(1.f + a);
+  if (v <= -709.78271484375f) return 0.f;
+  if (v > 0.f) return q;
+  return (top == 0.f ? a : expf(v - top)) * q;
+}
+
 // Where a lane's experts are.
 struct Seat {
   uint32_t lane, base;  // in the token; of the token in the warp
@@ -259,8 +269,10 @@ __device__ __forceinline__ void route_exact(const RouteArgs& a, bool keyed, int6
   }
   const float top = lanes_top<32>(fmaxf(low, high));
   auto weight = [&](float v) {
-    if (!a.renorm || a.sigmoid || total != total) return (float)score(v);
-    return top == -INFINITY ? 0.f : expf(v - top);  // (as in the lanes' part)
+    // (as in the lanes' part)
+    if (a.sigmoid) return sigmoid_over(v, a.renorm ? fminf(top, 0.f) : 0.f);
+    if (!a.renorm || total != total) return (float)score(v);
+    return top == -INFINITY ? 0.f : expf(v - top);
   };
   low = lane < a.top_k ? weight(low) : 0.f;
   high = lane + 32 < a.top_k ? weight(high) : 0.f;
@@ -700,7 +712,7 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
       else static_cast<int32_t*>(a.experts)[t * a.es + seat.lane * a.ek] = (int32_t)e;
     }
     if (SIGMOID) {
-      if (mine) sc = rcp(1.f + expf(-v));
+      sc = sigmoid_over(v, a.renorm ? fminf(lanes_top<LPT>(v), 0.f) : 0.f);  // (0 of v = -inf)
     } else if (a.renorm) {
       // The chosen may lie far below the row's largest logit, where scores leave 32 bits: their shares
       // are the softmax of the chosen alone.  (Ordered by logits, the chosen have the largest.)
@@ -785,15 +797,16 @@ gpuos_route_grad_kernel(const __grid_constant__ RouteArgs a) {
       by = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
       for (int i = 0; i < NPL; ++i) p[i] *= by;
-    } else if (!a.sigmoid) {
+    } else {
 #pragma unroll
       for (int i = 0; i < NR; ++i) m = fmaxf(m, v[i]);
       m = lanes_top<LPT>(m);
+      if (a.sigmoid) m = a.renorm ? fminf(m, 0.f) : 0.f;
     }
     float sc[NR], sum = 0.f, dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
-      if (a.sigmoid) sc[i] = e[i] == ~0u ? 0.f : 1.f / (1.f + expf(-v[i]));
+      if (a.sigmoid) sc[i] = sigmoid_over(v[i], m);
       else sc[i] = m == -INFINITY || e[i] == ~0u ? 0.f : expf(v[i] - m) * by;
       sum += sc[i];
       dot += g[i] * sc[i];
@@ -806,7 +819,7 @@ gpuos_route_grad_kernel(const __grid_constant__ RouteArgs a) {
     for (int i = 0; i < NR; ++i) {
       const uint32_t r = lane + i * LPT;
       float d = a.scale * (g[i] - less);
-      // (a score over the sum first: the sum's own inverse leaves the range where scores are near 2^-127)
+      // (a score over the sum first, as in the forward: the sum's own inverse may leave 32 bits)
       if (a.renorm) d *= sum == 0.f ? 0.f : sc[i] / sum;
       else if (a.sigmoid) d *= sc[i];
       if (a.sigmoid) {

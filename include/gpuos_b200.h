@@ -398,8 +398,9 @@ int32_t gpuos_cache_read(int32_t n, const gpuos_tensor* slots, const gpuos_tenso
  * scores without bias, divided by their sum with `renormalize`, times `scale`.
  * The choice is that of keys in 64 bits; of equal keys, and of equal groups, the
  * lowest index comes first.  A NaN logit counts as -inf in the choice; a row of
- * -inf has scores 0 (softmax); a sigmoid below 2^-126 counts as 0; where the
- * chosen scores sum to 0 the renormalised weights are 0. */
+ * -inf has scores 0 (softmax); a sigmoid is 0 where e^-x leaves 64 bits (x below
+ * -709.78).  Renormalised weights are the shares of the chosen scores however
+ * small those are, and 0 where all of them are 0. */
 #define GPUOS_SCORE_SOFTMAX 0
 #define GPUOS_SCORE_SIGMOID 1
 #define GPUOS_GROUP_MAX 0

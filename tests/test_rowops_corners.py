@@ -61,3 +61,51 @@ def test_renormalised_softmax_of_experts_far_below_the_largest(dtype, below, exp
         ww, we = route_oracle(x, top_k, bias=bias, **how)
         assert torch.equal(e.cpu(), we) and not bool((we == 0).any())
         check_weights(w, ww)
+
+
+# Below 2^-126 a 32-bit score and its product with the scale are rounded to multiples of 2^-149: expf's
+# 2 ulp, and half a step of each of two products.
+SMALLEST = 3 * 2.0 ** -149
+
+
+def sigmoid_weights_and_gradient(x, e, g, renormalize, scale):
+    """In 64 bits from the logits: shares by e^(x - the largest), and their gradient on the chosen."""
+    v = x.double().gather(-1, e)
+    zero = v < -709.7827128933840
+    top = v.amax(-1, keepdim=True).clamp(max=0) if renormalize else torch.zeros(len(x), 1).double()
+    t = torch.where(v > 0, 1 / (1 + (-v).exp()), (v - top).exp() / (1 + v.exp()))
+    t = torch.where(zero, torch.zeros(()).double(), t)
+    d, size = g.double() * scale, g.double().abs() * scale
+    if renormalize:
+        total = t.sum(-1, keepdim=True)
+        t = torch.where(total == 0, torch.zeros(()).double(), t / total)
+        d, size = d - (d * t).sum(-1, keepdim=True), size + (size * t).sum(-1, keepdim=True)
+    slope = t / (1 + v.exp())
+    zeros = torch.zeros_like(x).double()
+    return t * scale, zeros.scatter(-1, e, d * slope), zeros.scatter(-1, e, size * slope)
+
+
+@gpu
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("by", [0.0, -60.0, -87.0, -87.5, -90.0, -100.0, -104.5, -300.0, -705.0, -712.0])
+@pytest.mark.parametrize("experts,top_k", [(4, 2), (64, 8), (48, 40)])
+def test_small_sigmoids_have_one_rule(renormalize, by, experts, top_k):
+    """Weights by the lanes, by a warp (40 ranks) and their gradient keep scores that 32 bits flush."""
+    g = gen(experts - int(by))
+    x = torch.rand(6, experts, generator=g) * 4 + by
+    x[1] = by                              # equal ones
+    x[2, 1:] = -math.inf                   # one left
+    x[3] = -math.inf
+    gw = randn(g, 6, top_k)
+    for scale in (1.5, 4096.0):
+        how = dict(score="sigmoid", renormalize=renormalize, scale=scale)
+        w, e = R.route(x.to(DEV), top_k, **how)
+        assert torch.equal(e.cpu(), x.double().sort(dim=-1, descending=True, stable=True)[1][:, :top_k])
+        ww, dd, size = sigmoid_weights_and_gradient(x, e.cpu(), gw, renormalize, scale)
+        tiny = 0.0 if renormalize else SMALLEST * scale
+        assert bool(((w.cpu().double() - ww).abs() <= ROUTE_REL * ww + tiny).all()), (w, ww)
+        dx = R.route_grad(x.to(DEV), e, gw.to(DEV), **how).cpu().double()
+        # a share of 2^-126 and less of the sum is rounded to multiples of 2^-149 too
+        tiny = 4 * SMALLEST * scale * (1 + gw.abs().amax().double())
+        assert bool(((dx - dd).abs() <= 2 * ROUTE_REL * size + tiny).all()), (dx - dd).abs().max()
+        assert bool((dx[3] == 0).all())
