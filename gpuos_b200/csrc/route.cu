@@ -285,7 +285,7 @@ __device__ __forceinline__ void route_exact(const RouteArgs& a, bool keyed, int6
   __syncwarp();
 }
 
-// 2^y to 2^-41, |y| at most 1000: the exponential series of the fraction, to t^10 (the rest is
+// 2^y to 2^-41; beyond 1000 either way that of the limit: the exponential series of the fraction, to t^10 (the rest is
 // below 0.35^11 / 11!).
 __device__ __forceinline__ double exp2_series(double y) {
   y = fmin(fmax(y, -1000.0), 1000.0);
@@ -346,7 +346,7 @@ __device__ __forceinline__ double inverse_of_sum(double d) {
 }
 
 // One token's selection in 64 bits by its own lanes: lane r gets the slot of rank r.
-// Returns whether two keys whose order matters are still too close.
+// Returns whether two keys whose order matters are still too close, or a score is too small for the series.
 template <typename T, int NPL, int LPT, bool GROUPED>
 __device__ __forceinline__ bool resolve(const RouteArgs& a, const T* row, bool live, const Seat& seat, bool keyed,
                                         uint32_t* slot) {
@@ -354,12 +354,25 @@ __device__ __forceinline__ bool resolve(const RouteArgs& a, const T* row, bool l
   float x[NPL];
   load_logits<T, NPL>(row, seat.at, seat.n, a.vec, live, x);
   double v[NPL];
+  bool close = false, open = seat.n > 0;
+  // e^d for d at most 0.  Between kLeast and `gone`, from where on the score is 0 in 64 bits (masked
+  // logits, most of all), the series' limit would make different scores equal.
+  constexpr double kLeast = -690.0;
+  auto power = [&](double d, double gone) {
+    close = close || (d < kLeast && d > gone);
+    return d <= gone ? 0.0 : exp2_series(d * kLog2eD);
+  };
   if (!keyed && !(GROUPED && a.top2)) {
 #pragma unroll
     for (int i = 0; i < NPL; ++i) v[i] = (double)x[i];
   } else if (a.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) v[i] = inverse(1.0 + exp2_series((double)x[i] * -kLog2eD));
+    for (int i = 0; i < NPL; ++i) {
+      // e^x / (1 + e^x) of a negative logit, whose e^-x would have no inverse from 2^126 on
+      const double e = x[i] < 0.f ? power((double)x[i], -710.0) : exp2_series((double)x[i] * -kLog2eD);
+      const double r = inverse(1.0 + e);
+      v[i] = x[i] < 0.f ? e * r : r;
+    }
   } else {
     float m = x[0];
 #pragma unroll
@@ -368,7 +381,7 @@ __device__ __forceinline__ bool resolve(const RouteArgs& a, const T* row, bool l
     double total = 0;
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
-      v[i] = x[i] == -INFINITY ? 0.0 : exp2_series(((double)x[i] - (double)m) * kLog2eD);
+      v[i] = x[i] == -INFINITY ? 0.0 : power((double)x[i] - (double)m, -746.0);
       total += v[i];
     }
     total = lanes_sum<LPT>(total);
@@ -381,7 +394,6 @@ __device__ __forceinline__ bool resolve(const RouteArgs& a, const T* row, bool l
     for (int i = 0; i < NPL; ++i)
       if (i < (int)seat.n) v[i] += (double)__ldg(a.bias + (seat.at + i) * a.bs);
   }
-  bool close = false, open = seat.n > 0;
   if (GROUPED) {
     double l1 = -INFINITY, l2 = -INFINITY;
 #pragma unroll
@@ -407,7 +419,7 @@ __device__ __forceinline__ bool resolve(const RouteArgs& a, const T* row, bool l
       before += o > w || (o == w && h < seat.group);
       near += o != w && fabs(o - w) < kClose;
     }
-    close = seat.n && near != 0;
+    close = close || (seat.n && near != 0);
     open = open && before < a.top_groups;
     if (!keyed && a.top2) {
 #pragma unroll

@@ -109,3 +109,54 @@ def test_small_sigmoids_have_one_rule(renormalize, by, experts, top_k):
         tiny = 4 * SMALLEST * scale * (1 + gw.abs().amax().double())
         assert bool(((dx - dd).abs() <= 2 * ROUTE_REL * size + tiny).all()), (dx - dd).abs().max()
         assert bool((dx[3] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, FP, BF])
+@pytest.mark.parametrize("experts,top_k", [(4, 2), (32, 8), (200, 8), (64, 34)])
+def test_bias_of_experts_whose_scores_leave_the_series(dtype, experts, top_k):
+    """Softmax scores hundreds below the largest logit differ in 64 bits until e^-745, in every path."""
+    if experts == 4 and dtype == F32:
+        x, bias = torch.tensor([[0.0, -700.0, -695.0, -800.0]]), torch.tensor([0.5, 0.0, 0.0, 0.0])
+        w, e = R.route(x.to(DEV), 2, bias=bias.to(DEV))
+        assert e.cpu().tolist() == [[0, 2]]
+    g = gen(experts)
+    # (steps that scores near 2^-1074, multiples of it, still tell apart)
+    step = 4.0 if dtype == BF else 0.5
+    x = -680.0 - torch.randint(0, int(60 / step) + 1, (40, experts), generator=g) * step
+    x[20:] -= 80 * (torch.rand(20, experts, generator=g) < 0.3)  # and some of them 0
+    x[:, 0] = 0.0
+    x[5:10, 1:] += 500.0
+    x[10, 3:] = -math.inf
+    x[11, 3:] = torch.finfo(dtype).min
+    x = x.to(dtype)
+    bias = torch.zeros(experts)
+    bias[0] = 0.5
+    for renormalize in (False, True):
+        w, e = R.route(x.to(DEV), top_k, bias=bias.to(DEV), renormalize=renormalize)
+        ww, we = route_oracle(x, top_k, bias=bias, renormalize=renormalize)
+        assert torch.equal(e.cpu(), we)
+        assert bool(((w.cpu().double() - ww).abs() <= ROUTE_REL * ww + 1e-37).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, FP, BF])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups,top_groups,top_k", [(32, 4, 2, 4), (256, 8, 4, 8), (64, 8, 3, 10), (1024, 64, 5, 8),
+                                                             (128, 2, 1, 40)])
+def test_groups_of_scores_near_nothing(dtype, score, experts, groups, top_groups, top_k):
+    """The sum of a group's two largest scores, where those are far below 32 bits' smallest."""
+    g = gen(experts + groups)
+    for low, high in ((-120, -86), (-708, -640), (-760, -690)):
+        step = 4.0 if dtype == BF else 0.5
+        x = low + torch.randint(0, int((high - low) / step), (24, experts), generator=g) * step
+        x[3] = low                                     # all equal: the first groups
+        x[4, : experts // 2] = -math.inf
+        if score == "softmax":
+            x[::2, 5] = 0.0
+        x = x.to(dtype)
+        how = dict(score=score, groups=groups, top_groups=top_groups, group_score="top2")
+        for bias in (None, torch.arange(experts).remainder(3) * 0.0):
+            w, e = R.route(x.to(DEV), top_k, bias=None if bias is None else bias.to(DEV), **how)
+            ww, we = route_oracle(x, top_k, **how)
+            assert torch.equal(e.cpu(), we)
