@@ -1,7 +1,7 @@
 // gpuos_route / gpuos_route_grad: routing of tokens to experts.
 //
 //   s    = softmax(x) or sigmoid(x)          over a token's E logits
-//   key  = s + bias                          (without a bias: x, which orders as s does)
+//   key  = s + bias                          (without one, or with one number for all: x, which orders as s does)
 //   groups of E / groups neighbours: a group is worth its largest key, or the sum of its two
 //   largest; the best `top_groups` stay open
 //   top_k largest keys of the open groups; of equal ones the lowest index
@@ -511,7 +511,8 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
   double times = kScorePlaces;  // places of a score of 1
   if (keyed) {
     float bias[NPL], hi = -INFINITY, lo = INFINITY;
-    // a bias that is the same for all does not change the order
+    // A bias that is the same for all (zeros, before balancing starts) counts as none: the order is the
+    // logits', as without it.
     const float b0 = __ldg(a.bias);
     bool same = b0 - b0 == 0.f;
 #pragma unroll

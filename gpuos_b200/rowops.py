@@ -183,8 +183,8 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Opt
           scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
     """(weights float32, experts int64), both (token, top_k), of logits (token,
     expert): the `top_k` experts with the largest score (+ `bias`, float32 [expert], for balance:
-    it chooses and does not weigh), in falling order, of equal ones the lowest index
-    first.  With `groups`, only experts of the best `top_groups` groups are chosen from; a group is
+    it chooses and does not weigh; one number for all is no bias), in falling order, of equal
+    ones the lowest index first.  With `groups`, only experts of the best `top_groups` groups are chosen from; a group is
     worth its largest key, or with ``group_score="top2"`` the sum of its two
     largest.  Weights are the scores, divided by their sum if `renormalize`, times `scale`.
     The choice is that of keys in 64 bits."""

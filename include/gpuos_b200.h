@@ -390,8 +390,9 @@ int32_t gpuos_cache_read(int32_t n, const gpuos_tensor* slots, const gpuos_tenso
 
 /* Route tokens to experts.  logits: f32, f16 or bf16 (token, expert), last
  * stride 1, at most 1024 experts.  Scores s are the softmax or the sigmoid of a
- * row, keys are s + bias (bias: f32 [expert] or NULL; without one experts are
- * ordered by their logits).  The experts form `groups` (at most 64) groups of neighbours;
+ * row, keys are s + bias (bias: f32 [expert] or NULL; without one, and with one
+ * that is the same finite number for all, experts are ordered by their logits,
+ * which also tells scores apart that are equal in 64 bits).  The experts form `groups` (at most 64) groups of neighbours;
  * a group is worth its largest key or the sum of its two largest, and the best
  * `top_groups` stay open.  experts (i32 or i64, (token, top_k), top_k at most 64)
  * gets the largest keys of the open groups in falling order, weights (f32) their

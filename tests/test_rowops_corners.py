@@ -160,3 +160,19 @@ def test_groups_of_scores_near_nothing(dtype, score, experts, groups, top_groups
             w, e = R.route(x.to(DEV), top_k, bias=None if bias is None else bias.to(DEV), **how)
             ww, we = route_oracle(x, top_k, **how)
             assert torch.equal(e.cpu(), we)
+
+
+@gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("top_k,groups", [(2, 1), (2, 2), (40, 1)])
+def test_one_bias_for_all_is_no_bias(score, top_k, groups):
+    """Scores that 64 bits cannot tell apart (1 - e^-40, or a small one beside 0.5) are ordered by their logits."""
+    x = torch.full((3, 48), -50.0)
+    x[0, :4] = torch.tensor([40.0, 41.0, 42.0, 41.0])
+    x[1, 20:24] = torch.tensor([-49.0, -48.0, -47.0, 90.0])
+    how = dict(score=score, groups=groups)
+    w, e = R.route(x.to(DEV), top_k, **how)
+    assert torch.equal(e.cpu(), route_oracle(x, top_k, score="softmax", groups=groups)[1])
+    for b in (0.0, 0.5, -3.0):
+        wb, eb = R.route(x.to(DEV), top_k, bias=torch.full((48,), b, device=DEV), **how)
+        assert torch.equal(e, eb) and torch.equal(w, wb)
