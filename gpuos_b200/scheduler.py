@@ -56,6 +56,7 @@ import threading
 from typing import Any, Dict, List, Optional, Set, Tuple
 
 import torch
+from torch.utils._python_dispatch import _get_current_dispatch_mode_stack
 
 from . import load as _load
 
@@ -474,12 +475,13 @@ def order_after_pending(reads, writes) -> None:
     """For code that launches on tensors without going through torch's
     dispatcher: inside a scheduler context, flush the pending requests that
     write what is in `reads`, or touch what is in `writes`, as an op that runs in torch
-    does.  Every context counts, not this thread's alone: a backward pass
-    runs, and schedules, on a thread of autograd's."""
-    for mode in tuple(entered):
-        if mode.pending and (any(_overlaps(_extent(t), mode._w) for t in reads) or
-                             any(_overlaps(_extent(t), tab) for t in writes
-                                 for tab in (mode._w, mode._r))):
+    does: of the contexts that this thread's ops go through.  A backward pass
+    takes its caller's contexts to a thread of autograd's, while the caller waits;
+    any other thread's tables may be changing."""
+    for mode in _get_current_dispatch_mode_stack():
+        if (isinstance(mode, _GPUOSSchedulerMode) and mode.pending and
+                (any(_overlaps(_extent(t), mode._w) for t in reads) or
+                 any(_overlaps(_extent(t), tab) for t in writes for tab in (mode._w, mode._r)))):
             mode.sync()
 
 

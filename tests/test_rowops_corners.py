@@ -5,11 +5,13 @@ Tolerances count roundings as in test_rowops.py, whose oracles these tests use.
 """
 import itertools
 import math
+import threading
 
 import pytest
 import torch
 
 from gpuos_b200 import rowops as R
+from gpuos_b200 import scheduler as S
 from test_rowops import BF, DEV, F32, FP, ROUTE_REL, TYPES, gen, gpu, randn, route_oracle
 
 
@@ -176,3 +178,53 @@ def test_one_bias_for_all_is_no_bias(score, top_k, groups):
     for b in (0.0, 0.5, -3.0):
         wb, eb = R.route(x.to(DEV), top_k, bias=torch.full((48,), b, device=DEV), **how)
         assert torch.equal(e, eb) and torch.equal(w, wb)
+
+
+# ---------------------------------------------------------------------------
+# Around the calls
+# ---------------------------------------------------------------------------
+class Recorder:
+    """In place of the extension: what a mode submits and flushes, and on which thread."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        return lambda *a, **k: self.calls.append((name, threading.get_ident()))
+
+
+def test_only_the_threads_own_contexts_are_flushed():
+    """Another thread's tables may be changing, and the addresses in them may be of tensors long gone."""
+    def mode():
+        return S._GPUOSSchedulerMode(Recorder(), size_threshold=1 << 16, auto_flush_ms=None, pending=set(), jit=True, fuse=True)
+
+    shared = torch.zeros(8)
+    mine, theirs = mode(), mode()
+    entered, done = threading.Event(), threading.Event()
+
+    def other():
+        with theirs:
+            S.entered.append(theirs)
+            theirs._done(shared)
+            entered.set()
+            done.wait(30)
+            S.entered.remove(theirs)
+
+    t = threading.Thread(target=other)
+    t.start()
+    try:
+        assert entered.wait(30)
+        S.order_after_pending([shared], [shared])
+        assert theirs.ext.calls == [] and theirs.pending
+        with mine:
+            S.entered.append(mine)
+            mine._done(shared[2:4])
+            S.order_after_pending([shared[4:]], [])
+            assert mine.ext.calls == []            # reads nothing that is pending
+            S.order_after_pending([shared], [])
+            S.entered.remove(mine)
+        assert mine.ext.calls == [("flush", threading.get_ident())] and not mine.pending
+        assert theirs.ext.calls == [] and theirs.pending
+    finally:
+        done.set()
+        t.join(30)
