@@ -7,7 +7,7 @@
 #include <ATen/EmptyTensor.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty_like.h>
-#include <c10/core/GradMode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -190,8 +190,12 @@ PyObject* wrap(const at::Tensor& t) {
   return o;
 }
 
-// Whether autograd has to see the call (gpuos_b200.rowops then records it).
-bool recorded(const at::Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+// Whether torch has to see the call (gpuos_b200.rowops then makes it an autograd function's): for
+// a gradient, or for a tangent of forward mode.
+bool recorded(const at::Tensor& t) {
+  const c10::AutogradState& state = c10::AutogradState::get_tls_state();
+  return (state.get_grad_mode() && t.requires_grad()) || (state.get_fw_grad_mode() && t._fw_grad(0).defined());
+}
 
 // A tensor of the caller's was written: autograd then refuses a backward pass that saved it.
 void written(const at::Tensor& t) {

@@ -14,6 +14,7 @@ launches nothing.
 ``rotary``, ``route`` and ``logprobs`` take part in autograd; their gradients
 are also there as calls of their own (``rotary(..., inverse=True)``,
 ``route_grad``, ``logprobs_grad``), for steps that are captured or keep no graph.
+In forward mode ``rotary`` carries tangents; ``route`` and ``logprobs`` raise.
 A given `out` and a written cache count as changed in place: a backward pass that saved
 one of them raises, as after an in-place op of torch's.
 include/gpuos_b200.h states each operator's formula and its edge cases.
@@ -121,19 +122,35 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, positions, inv_freq, scale, interleaved, inverse, *xs):
         ctx.save_for_backward(positions, inv_freq)
-        ctx.how = dict(scale=scale, interleaved=interleaved, inverse=not inverse)
+        ctx.save_for_forward(positions, inv_freq)
+        ctx.how = dict(scale=scale, interleaved=interleaved)
+        ctx.inverse = inverse
+        ctx.like = [(x.shape, x.dtype, x.device) for x in xs]
         ctx.set_materialize_grads(False)
         return _ext.rotary(xs, None, positions, inv_freq, scale, interleaved, inverse)
 
     @staticmethod
-    def backward(ctx, *grads):
+    def _turn(ctx, vectors, inverse):
+        """The map, or its transpose, of those vectors that there are."""
         positions, inv_freq = ctx.saved_tensors
-        need = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[5 + i]]
-        got = [None] * len(grads)
+        need = [i for i, v in enumerate(vectors) if v is not None]
+        got = [None] * len(vectors)
         if need:
-            for i, g in zip(need, rotary(tuple(_row(grads[i]) for i in need), positions, inv_freq, **ctx.how)):
-                got[i] = g
-        return (None,) * 5 + tuple(got)
+            turned = rotary(tuple(_row(vectors[i]) for i in need), positions, inv_freq, inverse=inverse, **ctx.how)
+            for i, v in zip(need, turned):
+                got[i] = v
+        return tuple(got)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        grads = [g if need else None for g, need in zip(grads, ctx.needs_input_grad[5:])]
+        return (None,) * 5 + _Rotary._turn(ctx, grads, not ctx.inverse)
+
+    @staticmethod
+    def jvp(ctx, *tangents):  # linear: the map itself
+        got = _Rotary._turn(ctx, tangents[5:], ctx.inverse)
+        return tuple(torch.zeros(size, dtype=dtype, device=device) if t is None else t
+                     for t, (size, dtype, device) in zip(got, ctx.like))
 
 
 # ---- quantised cache -------------------------------------------------------------

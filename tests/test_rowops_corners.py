@@ -9,6 +9,7 @@ import threading
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from gpuos_b200 import rowops as R
 from gpuos_b200 import scheduler as S
@@ -228,3 +229,40 @@ def test_only_the_threads_own_contexts_are_flushed():
     finally:
         done.set()
         t.join(30)
+
+
+@gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_forward_mode(interleaved):
+    """Rotary's tangent is the operator of the tangent; the others have none and say so."""
+    g = gen(40)
+    q, k, tq = randn(g, 5, 3, 32).to(DEV), randn(g, 5, 1, 32).to(DEV), randn(g, 5, 3, 32).to(DEV)
+    pos, f = torch.arange(5, device=DEV) * 100, R.rotary_frequencies(16, device=DEV)
+    how = dict(interleaved=interleaved, scale=1.5)
+    want = R.rotary(tq, pos, f, **how)
+    for inverse in (False, True):
+        with fwd.dual_level():
+            a, b = R.rotary((fwd.make_dual(q, tq), k), pos, f, inverse=inverse, **how)
+            assert torch.equal(fwd.unpack_dual(a).tangent, R.rotary(tq, pos, f, inverse=inverse, **how))
+            assert fwd.unpack_dual(b).tangent is None or not bool(fwd.unpack_dual(b).tangent.any())
+            assert torch.equal(fwd.unpack_dual(a).primal, R.rotary(q, pos, f, inverse=inverse, **how))
+    with torch.no_grad(), fwd.dual_level():  # which leaves forward mode on
+        a = R.rotary(fwd.make_dual(q, tq), pos, f, **how)
+        assert torch.equal(fwd.unpack_dual(a).tangent, want)
+        wide = fwd.make_dual(q, tq.transpose(0, 2).contiguous().transpose(0, 2))  # elements of a tangent's row apart
+        assert torch.equal(fwd.unpack_dual(R.rotary(wide, pos, f, **how)).tangent, want)
+        with pytest.raises(ValueError, match="out cannot"):
+            R.rotary(fwd.make_dual(q, tq), pos, f, out=torch.empty_like(q))
+        with pytest.raises(ValueError, match="inv_freq takes no gradient"):
+            R.rotary(q, pos, fwd.make_dual(f, torch.ones_like(f)))
+        x = fwd.make_dual(q[:, 0], tq[:, 0])
+        with pytest.raises(NotImplementedError):
+            R.route(x, 2)
+        with pytest.raises(NotImplementedError):
+            R.logprobs(x, pos // 100, entropy=True)
+    # a gradient through the tangent
+    t = tq.clone().requires_grad_()
+    with fwd.dual_level():
+        a = fwd.unpack_dual(R.rotary(fwd.make_dual(q, t), pos, f, **how)).tangent
+        (dt,) = torch.autograd.grad(a, t, tq)
+    assert torch.equal(dt, R.rotary(tq, pos, f, inverse=True, **how))
