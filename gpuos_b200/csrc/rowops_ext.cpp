@@ -7,6 +7,7 @@
 #include <ATen/EmptyTensor.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty_like.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -197,6 +198,19 @@ bool recorded(const at::Tensor& t) {
   return (state.get_grad_mode() && t.requires_grad()) || (state.get_fw_grad_mode() && t._fw_grad(0).defined());
 }
 
+// A call whose result torch.jit.trace would take for a constant: to be made an autograd function's, which
+// is an operation of the trace, or refused.  Inside such a function forward mode is off; in
+// inference mode it is off everywhere, so that nothing tells the two apart.
+bool tracing() { return at::tracer::impl::is_dispatch_enabled(); }
+void not_traced() {
+  if (tracing()) throw Raise{PyExc_RuntimeError, "torch.jit.trace cannot record this call"};
+}
+bool traced() {
+  if (!tracing()) return false;
+  if (c10::AutogradState::get_tls_state().get_inference_mode()) not_traced();
+  return c10::AutogradState::get_tls_state().get_fw_grad_mode();
+}
+
 // A tensor of the caller's was written: autograd then refuses a backward pass that saved it.
 void written(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -260,7 +274,7 @@ PyObject* rotary(PyObject* const* a, Py_ssize_t n) {
     throw Raise{PyExc_ValueError, "inv_freq takes no gradient: detach it"};
   for (int i = 0; i < xs.n; ++i) {
     xt[i] = &tensor(xs.o[i], "x");
-    if (recorded(*xt[i])) return not_here();
+    if (recorded(*xt[i]) || traced()) return not_here();
   }
   const Place at(*xt[0]);
   gpuos_tensor x[2], o[2];
@@ -299,6 +313,7 @@ PyObject* rotary(PyObject* const* a, Py_ssize_t n) {
 
 PyObject* cache_write(PyObject* const* a, Py_ssize_t n) {
   arity(n, 4, "(x, slots, codes, scales)");
+  not_traced();
   const Pair xs(a[0], "x"), cs(a[2], "codes"), ss(a[3], "scales");
   same_count(cs.n, xs.n, "codes must have a tensor for each x");
   same_count(ss.n, xs.n, "scales must have a tensor for each x");
@@ -320,6 +335,7 @@ PyObject* cache_write(PyObject* const* a, Py_ssize_t n) {
 
 PyObject* cache_read(PyObject* const* a, Py_ssize_t n) {
   arity(n, 5, "(slots, codes, scales, out, dtype)");
+  not_traced();
   const Pair cs(a[1], "codes"), ss(a[2], "scales");
   same_count(ss.n, cs.n, "scales must have a tensor for each cache");
   const at::Tensor& slots_t = tensor(a[0], "slots");
@@ -358,7 +374,7 @@ PyObject* cache_read(PyObject* const* a, Py_ssize_t n) {
 PyObject* route(PyObject* const* a, Py_ssize_t n) {
   arity(n, 9, "(logits, bias, top_k, score, groups, top_groups, group_score, renormalize, scale)");
   const at::Tensor& x = tensor(a[0], "logits");
-  if (recorded(x)) return not_here();
+  if (recorded(x) || traced()) return not_here();
   const Place at(x);
   const gpuos_tensor d = at.in(x, "logits");
   if (x.dim() != 2) throw Raise{PyExc_ValueError, "logits must have 2 dims, not " + std::to_string(x.dim())};
@@ -378,6 +394,7 @@ PyObject* route(PyObject* const* a, Py_ssize_t n) {
 
 PyObject* route_grad(PyObject* const* a, Py_ssize_t n) {
   arity(n, 6, "(logits, experts, grad_weights, score, renormalize, scale)");
+  not_traced();
   const at::Tensor& x = tensor(a[0], "logits");
   const Place at(x);
   const gpuos_tensor d = at.in(x, "logits"), e = at.in(a[1], "experts"), g = at.in(a[2], "grad_weights");
@@ -390,7 +407,7 @@ PyObject* route_grad(PyObject* const* a, Py_ssize_t n) {
 PyObject* logprobs(PyObject* const* a, Py_ssize_t n) {
   arity(n, 6, "(logits, targets, top, entropy, temperature, stats)");
   const at::Tensor& x = tensor(a[0], "logits");
-  if (recorded(x)) return not_here();
+  if (recorded(x) || traced()) return not_here();
   const Place at(x);
   const gpuos_tensor d = at.in(x, "logits"), y = at.in(a[1], "targets");
   if (x.dim() != 2) throw Raise{PyExc_ValueError, "logits must have 2 dims, not " + std::to_string(x.dim())};
@@ -421,6 +438,7 @@ PyObject* logprobs(PyObject* const* a, Py_ssize_t n) {
 
 PyObject* logprobs_grad(PyObject* const* a, Py_ssize_t n) {
   arity(n, 8, "(logits, targets, stats, entropy, grad_logprob, grad_entropy, temperature, out)");
+  not_traced();
   const at::Tensor& x = tensor(a[0], "logits");
   const Place at(x);
   const gpuos_tensor d = at.in(x, "logits"), y = at.in(a[1], "targets"), st = at.in(a[2], "stats");

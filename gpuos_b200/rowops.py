@@ -112,7 +112,7 @@ def rotary(x: Tensors, positions: torch.Tensor, inv_freq: torch.Tensor, *, scale
     got = _ext.rotary(x, out, positions, inv_freq, scale, interleaved, inverse)
     if got is NotImplemented:  # autograd has to record it
         if out is not None:
-            raise ValueError("out cannot be given where a gradient is needed")
+            raise ValueError("out cannot be given where a gradient is needed, nor in a trace")
         got = _Rotary.apply(positions, inv_freq, scale, interleaved, inverse, *_tuple(x))
         return got[0] if isinstance(x, torch.Tensor) else got
     return got

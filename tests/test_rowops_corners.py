@@ -266,3 +266,37 @@ def test_forward_mode(interleaved):
         a = fwd.unpack_dual(R.rotary(fwd.make_dual(q, t), pos, f, **how)).tangent
         (dt,) = torch.autograd.grad(a, t, tq)
     assert torch.equal(dt, R.rotary(tq, pos, f, inverse=True, **how))
+
+
+@gpu
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("how", [torch.enable_grad, torch.no_grad])
+def test_a_trace_keeps_the_calls(how):
+    g = gen(41)
+    x, other = randn(g, 5, 32).to(DEV), randn(g, 5, 32).to(DEV)
+    pos, f = torch.arange(5, device=DEV), R.rotary_frequencies(16, device=DEV)
+
+    def step(x):
+        y = R.rotary(x[:, None], pos, f)[:, 0]
+        w, e = R.route(y, 4)
+        return y, w, e, R.logprobs(y, pos, top=2).top_logprobs
+
+    with how():
+        traced = torch.jit.trace(step, x, check_trace=False)
+        for got, want in zip(traced(other), step(other)):
+            assert torch.equal(got, want)
+        c, s = R.cache_alloc(1, 8, 1, 32, device=DEV)
+        with pytest.raises(RuntimeError, match="cannot record"):
+            torch.jit.trace(lambda x: R.cache_read(pos, c, s), x)
+        with pytest.raises(RuntimeError, match="cannot record"):
+            torch.jit.trace(lambda x: R.cache_write(x[:, None], pos, c, s), x)
+        r = R.logprobs(x, pos, stats=True)
+        with pytest.raises(RuntimeError, match="cannot record"):
+            torch.jit.trace(lambda x: R.logprobs_grad(x, pos, r, r.logprob), x)
+        w, e = R.route(x, 2)
+        with pytest.raises(RuntimeError, match="cannot record"):
+            torch.jit.trace(lambda x: R.route_grad(x, e, w), x)
+    with torch.inference_mode():
+        for call in (lambda x: R.rotary(x[:, None], pos, f), lambda x: R.route(x, 2), lambda x: R.logprobs(x, pos).logprob):
+            with pytest.raises(RuntimeError, match="cannot record"):
+                torch.jit.trace(call, x)
