@@ -217,9 +217,9 @@ void written(const at::Tensor& t) {
 }
 
 // A tensor to be written, which autograd must not be following.
-const at::Tensor& given_out(PyObject* o) {
-  const at::Tensor& t = tensor(o, "out");
-  if (recorded(t)) throw Raise{PyExc_ValueError, "out cannot be a tensor that requires a gradient"};
+const at::Tensor& given_out(PyObject* o, const char* name = "out") {
+  const at::Tensor& t = tensor(o, name);
+  if (recorded(t)) throw Raise{PyExc_ValueError, std::string(name) + " cannot be a tensor that requires a gradient"};
   return t;
 }
 
@@ -321,8 +321,8 @@ PyObject* cache_write(PyObject* const* a, Py_ssize_t n) {
   gpuos_tensor x[2], c[2], s[2];
   for (int i = 0; i < xs.n; ++i) {
     x[i] = at.in(xs.o[i], "x");
-    c[i] = at.in(cs.o[i], "codes");
-    s[i] = at.in(ss.o[i], "scales");
+    c[i] = at.in(given_out(cs.o[i], "codes"), "codes");
+    s[i] = at.in(given_out(ss.o[i], "scales"), "scales");
   }
   const gpuos_tensor slots = at.in(a[1], "slots");
   done(gpuos_cache_write(xs.n, x, &slots, c, s, at.stream()));
@@ -446,7 +446,7 @@ PyObject* logprobs_grad(PyObject* const* a, Py_ssize_t n) {
   const char* names[3] = {"entropy", "grad_logprob", "grad_entropy"};
   for (int i = 0; i < 3; ++i)
     if (a[3 + i] != Py_None) opt[i] = at.in(a[3 + i], names[i]);
-  const at::Tensor out = a[7] != Py_None ? tensor(a[7], "out") : at.make(x.sizes(), x.scalar_type());
+  const at::Tensor out = a[7] != Py_None ? given_out(a[7]) : at.make(x.sizes(), x.scalar_type());
   const gpuos_tensor o = at.in(out, "out");
   done(gpuos_logprobs_grad(&d, &y, &st, a[3] != Py_None ? &opt[0] : nullptr, a[4] != Py_None ? &opt[1] : nullptr,
                            a[5] != Py_None ? &opt[2] : nullptr, &o, (float)real(a[6]), at.stream()));

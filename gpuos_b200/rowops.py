@@ -176,7 +176,8 @@ def cache_write(x: Tensors, slots: torch.Tensor, codes: Tensors, scales: Tensors
     values), (token, head, element); token t goes to row ``slots[t]`` of the cache, counted
     through its pages.  A slot outside the cache (-1: padding) writes nothing; the
     slots inside it must differ.  `codes` and `scales` as from ``cache_alloc``, one of each
-    for each of `x`; any strides but the last (a page may hold its heads before its rows)."""
+    for each of `x`; any strides but the last (a page may hold its heads before its rows).
+    `x` counts as detached: no gradient goes through a cache."""
     if _entered:
         _order((*_tuple(x), slots), (*_tuple(codes), *_tuple(scales)))
     _ext.cache_write(x, slots, codes, scales)
@@ -270,7 +271,7 @@ def logprobs_grad(logits: torch.Tensor, targets: torch.Tensor, result: LogProbs,
                   temperature: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The gradient of the logits from those of ``logprobs``'s logprob and entropy
     (float32 [row]); `result` is what ``logprobs(..., stats=True)`` gave for the same
-    arguments.  `out` may be `logits`."""
+    arguments.  `out` may be `logits`, if autograd does not follow those (detach them)."""
     if result.stats is None:
         raise ValueError("result has no stats: call logprobs(..., stats=True)")
     if _entered:

@@ -300,3 +300,29 @@ def test_a_trace_keeps_the_calls(how):
         for call in (lambda x: R.rotary(x[:, None], pos, f), lambda x: R.route(x, 2), lambda x: R.logprobs(x, pos).logprob):
             with pytest.raises(RuntimeError, match="cannot record"):
                 torch.jit.trace(call, x)
+
+
+@gpu
+def test_outputs_that_autograd_follows_are_refused():
+    g = gen(42)
+    x, y = randn(g, 4, 16).to(DEV), torch.arange(4, device=DEV)
+    r = R.logprobs(x, y, stats=True)
+    gl = torch.ones(4, device=DEV)
+    want = R.logprobs_grad(x, y, r, gl)
+    for followed in (x.clone().requires_grad_(), x.clone().requires_grad_() * 1):
+        before = followed.detach().clone()
+        with pytest.raises(ValueError, match="out cannot be a tensor that requires a gradient"):
+            R.logprobs_grad(followed, y, r, gl, out=followed)
+        with pytest.raises(ValueError, match="out cannot be a tensor that requires a gradient"):
+            R.logprobs_grad(x, y, r, gl, out=followed)
+        assert torch.equal(followed, before)
+        assert torch.equal(R.logprobs_grad(followed, y, r, gl), want)   # read, not written
+        with torch.no_grad():
+            assert R.logprobs_grad(followed, y, r, gl, out=followed) is followed
+        assert torch.equal(followed, want)
+    c, s = R.cache_alloc(1, 8, 1, 16, device=DEV)
+    rows = x[:, None].clone().requires_grad_()
+    with pytest.raises(ValueError, match="scales cannot be a tensor that requires a gradient"):
+        R.cache_write(rows, y, c, s.clone().requires_grad_())
+    R.cache_write(rows, y, c, s)                                     # rows count as detached
+    assert not s.requires_grad and bool(s.flatten()[:4].all())
