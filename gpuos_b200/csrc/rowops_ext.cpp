@@ -4,19 +4,17 @@
 // callers use; it adds gradients and the order after a scheduler's requests.
 #include <Python.h>
 
-#include <ATen/EmptyTensor.h>
-#include <ATen/cuda/EmptyTensor.h>
+#include <ATen/core/Tensor.h>
 #include <ATen/ops/empty_like.h>
 #include <ATen/TracerMode.h>
 #include <c10/core/AutogradState.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
-#include <optional>
 #include <string>
-#include <vector>
 
 #include "../../include/gpuos_b200.h"
 
@@ -84,50 +82,19 @@ struct Place {
     return describe(t, name);
   }
   gpuos_tensor in(PyObject* o, const char* name) const { return in(tensor(o, name), name); }
+  // A new contiguous tensor with a storage of its own, as torch.empty's: without the latter's
+  // choices, which cost a call of several outputs about as much as all checks.
   at::Tensor make(at::IntArrayRef sizes, at::ScalarType type) const {
-    return at::detail::empty_cuda(sizes, type, device, std::nullopt);
-  }
-};
-
-// A call's outputs, contiguous.  Small ones share one allocation, each at a
-// multiple of 256 bytes of it: an allocation costs the host about as much as all checks.
-struct Outputs {
-  static constexpr int kMost = 5;
-  static constexpr int64_t kSmall = 1 << 18;
-  at::Tensor t[kMost];
-  std::vector<int64_t> sizes[kMost];
-  at::ScalarType type[kMost];
-  int n = 0;
-  int add(std::vector<int64_t> size, at::ScalarType dt) {
-    sizes[n] = std::move(size);
-    type[n] = dt;
-    return n++;
-  }
-  void allocate(const Place& at) {
-    int64_t at_byte[kMost], total = 0;
-    bool small = n > 1;
-    for (int i = 0; i < n; ++i) {
-      int64_t bytes = (int64_t)c10::elementSize(type[i]);
-      for (const int64_t d : sizes[i]) {
-        if (d < 0 || d > kSmall) small = false;
-        bytes *= small ? d : 0;
-      }
-      at_byte[i] = total;
-      total += (bytes + 255) / 256 * 256;
-      if (total > kSmall) small = false;
-    }
-    if (!small) {
-      for (int i = 0; i < n; ++i) t[i] = at.make(sizes[i], type[i]);
-      return;
-    }
-    const at::Tensor whole = at.make({total}, at::kByte);
-    for (int i = 0; i < n; ++i) {
-      t[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()),
-                                                      c10::DispatchKeySet(c10::DispatchKey::CUDA),
-                                                      c10::scalarTypeToTypeMeta(type[i]));
-      t[i].unsafeGetTensorImpl()->set_sizes_contiguous(sizes[i]);
-      t[i].unsafeGetTensorImpl()->set_storage_offset(at_byte[i] / (int64_t)c10::elementSize(type[i]));
-    }
+    int64_t bytes = (int64_t)c10::elementSize(type);
+    for (const int64_t d : sizes)
+      if (d < 0 || __builtin_mul_overflow(bytes, d, &bytes)) throw Raise{PyExc_ValueError, "an output is too large"};
+    c10::Allocator* const from = c10::cuda::CUDACachingAllocator::get();
+    const at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(
+        c10::make_intrusive<c10::StorageImpl>(c10::StorageImpl::use_byte_size_t(), (size_t)bytes,
+                                              from->allocate((size_t)bytes), from, /*resizable=*/true),
+        c10::DispatchKeySet(c10::DispatchKey::CUDA), c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    return t;
   }
 };
 
@@ -284,18 +251,11 @@ PyObject* rotary(PyObject* const* a, Py_ssize_t n) {
     same_count(given.n, xs.n, "out must have a tensor for each x");
     for (int i = 0; i < xs.n; ++i) out[i] = given_out(given.o[i]);
   } else {
-    Outputs outs;
-    for (int i = 0; i < xs.n; ++i)
-      if (xt[i]->is_contiguous()) outs.add(xt[i]->sizes().vec(), xt[i]->scalar_type());
-    outs.allocate(at);
-    for (int i = 0, k = 0; i < xs.n; ++i) {
-      if (xt[i]->is_contiguous()) {
-        out[i] = outs.t[k++];
-      } else {
-        // the layout of x, where its last dim is contiguous in it
-        out[i] = at::empty_like(*xt[i]);
-        if (xt[i]->dim() && out[i].stride(-1) != 1) out[i] = at.make(xt[i]->sizes(), xt[i]->scalar_type());
-      }
+    for (int i = 0; i < xs.n; ++i) {
+      // the layout of x, where its last dim is contiguous in it
+      const bool plain = xt[i]->is_contiguous();
+      if (!plain) out[i] = at::empty_like(*xt[i]);
+      if (plain || (xt[i]->dim() && out[i].stride(-1) != 1)) out[i] = at.make(xt[i]->sizes(), xt[i]->scalar_type());
     }
   }
   for (int i = 0; i < xs.n; ++i) {
@@ -342,7 +302,6 @@ PyObject* cache_read(PyObject* const* a, Py_ssize_t n) {
   const Place at(slots_t);
   gpuos_tensor c[2], s[2], o[2];
   at::Tensor out[2];
-  Outputs outs;
   if (a[3] != Py_None) {
     const Pair given(a[3], "out");
     same_count(given.n, cs.n, "out must have a tensor for each cache");
@@ -357,11 +316,7 @@ PyObject* cache_read(PyObject* const* a, Py_ssize_t n) {
     if (a[3] != Py_None) continue;
     if (codes.dim() != 4 || slots_t.dim() != 1)
       throw Raise{PyExc_ValueError, "codes must be (page, row, head, code) and slots have one dim"};
-    outs.add({slots_t.size(0), codes.size(2), codes.size(3) * (codes.scalar_type() == at::kByte ? 2 : 1)}, type);
-  }
-  if (a[3] == Py_None) {
-    outs.allocate(at);
-    for (int i = 0; i < cs.n; ++i) out[i] = outs.t[i];
+    out[i] = at.make({slots_t.size(0), codes.size(2), codes.size(3) * (codes.scalar_type() == at::kByte ? 2 : 1)}, type);
   }
   for (int i = 0; i < cs.n; ++i) o[i] = at.in(out[i], "out");
   const gpuos_tensor slots = at.in(slots_t, "slots");
@@ -382,14 +337,11 @@ PyObject* route(PyObject* const* a, Py_ssize_t n) {
   if (a[1] != Py_None) bias = at.in(a[1], "bias");
   const int32_t k = small(a[2], "top_k");
   if (k < 1 || k > 64) throw Raise{PyExc_ValueError, "top_k must be in [1, 64]"};
-  Outputs out;
-  out.add({x.size(0), k}, at::kFloat);
-  out.add({x.size(0), k}, at::kLong);
-  out.allocate(at);
-  const gpuos_tensor w = at.in(out.t[0], "weights"), e = at.in(out.t[1], "experts");
+  const at::Tensor out[2] = {at.make({x.size(0), k}, at::kFloat), at.make({x.size(0), k}, at::kLong)};
+  const gpuos_tensor w = at.in(out[0], "weights"), e = at.in(out[1], "experts");
   done(gpuos_route(&d, a[1] != Py_None ? &bias : nullptr, &w, &e, small(a[3], "score"), small(a[4], "groups"),
                    small(a[5], "top_groups"), small(a[6], "group_score"), truth(a[7]), (float)real(a[8]), at.stream()));
-  return tuple_of(out.t, 2);
+  return tuple_of(out, 2);
 }
 
 PyObject* route_grad(PyObject* const* a, Py_ssize_t n) {
@@ -415,22 +367,17 @@ PyObject* logprobs(PyObject* const* a, Py_ssize_t n) {
   if (k < 0 || k > 64) throw Raise{PyExc_ValueError, "top must be in [0, 64]"};
   const bool entropy = truth(a[3]), stats = truth(a[5]);
   const int64_t rows = x.size(0);
-  Outputs outs;
-  int which[5] = {outs.add({rows}, at::kFloat), -1, -1, -1, -1};
-  if (entropy) which[1] = outs.add({rows}, at::kFloat);
-  if (k) {
-    which[2] = outs.add({rows, k}, at::kFloat);
-    which[3] = outs.add({rows, k}, at::kLong);
-  }
-  if (stats) which[4] = outs.add({rows, 2}, at::kFloat);
-  outs.allocate(at);
   at::Tensor out[5];  // logprob, entropy, top_logprobs, top_tokens, stats
+  out[0] = at.make({rows}, at::kFloat);
+  if (entropy) out[1] = at.make({rows}, at::kFloat);
+  if (k) {
+    out[2] = at.make({rows, k}, at::kFloat);
+    out[3] = at.make({rows, k}, at::kLong);
+  }
+  if (stats) out[4] = at.make({rows, 2}, at::kFloat);
   gpuos_tensor o[5];
   for (int i = 0; i < 5; ++i)
-    if (which[i] >= 0) {
-      out[i] = outs.t[which[i]];
-      o[i] = at.in(out[i], "out");
-    }
+    if (out[i].defined()) o[i] = at.in(out[i], "out");
   done(gpuos_logprobs(&d, &y, &o[0], entropy ? &o[1] : nullptr, k ? &o[2] : nullptr, k ? &o[3] : nullptr,
                       stats ? &o[4] : nullptr, (float)real(a[4]), at.stream()));
   return tuple_of(out, 5);

@@ -326,3 +326,29 @@ def test_outputs_that_autograd_follows_are_refused():
         R.cache_write(rows, y, c, s.clone().requires_grad_())
     R.cache_write(rows, y, c, s)                                     # rows count as detached
     assert not s.requires_grad and bool(s.flatten()[:4].all())
+
+
+@gpu
+def test_results_of_a_call_have_storages_of_their_own():
+    """One may be resized, saved or kept without the others."""
+    g = gen(43)
+    x, y = randn(g, 6, 32).to(DEV), torch.arange(6, device=DEV)
+    q = randn(g, 6, 2, 32).to(DEV)
+    f = R.rotary_frequencies(32, device=DEV)
+    c, s = R.cache_alloc(1, 8, 2, 32, device=DEV)
+    calls = [lambda: R.route(x, 4), lambda: R.rotary((q, q), y, f), lambda: R.cache_read(y, (c, c), (s, s)),
+             lambda: R.logprobs(x, y, top=3, entropy=True, stats=True)]
+    for call in calls:
+        got = list(call())
+        kept = [t.clone() for t in got]
+        assert len({t.untyped_storage().data_ptr() for t in got}) == len(got)
+        for t in got:
+            assert t.storage_offset() == 0 and t.untyped_storage().nbytes() == t.numel() * t.element_size()
+        got[0].resize_(4096).fill_(7)
+        assert all(torch.equal(a, b) for a, b in zip(got[1:], kept[1:]))
+    # as other tensors' memory: kept for another stream that uses it, and none for no rows
+    w, e = R.route(x, 4)
+    w.record_stream(torch.cuda.Stream())
+    assert R.route(x[:0], 4)[0].shape == (0, 4)
+    with torch.inference_mode():
+        assert R.route(x, 4)[0].is_inference()
