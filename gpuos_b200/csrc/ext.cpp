@@ -492,11 +492,23 @@ PyObject* py_flush(PyObject*, PyObject* args, PyObject* kw) {
     if (!current_stream(d, &s)) return nullptr;
     int32_t rc;
     uint64_t ticket = 0;
+    // A request that another thread submits while this one waits may be behind the ticket: its
+    // tensors stay for the next flush.  One that this flush still takes is kept longer than needed.
+    std::vector<PyObject*> refs;
+    refs.swap(g_pending_refs[d]);
     Py_BEGIN_ALLOW_THREADS rc = gpuos_flush(ex, sync, s, &ticket);
-    Py_END_ALLOW_THREADS if (rc != GPUOS_OK) return raise_status(rc);
-    if (!g_pending_refs[d].empty()) {
-      g_inflight_refs[d].push_back(Keep{ticket, std::move(g_pending_refs[d])});
-      g_pending_refs[d].clear();
+    Py_END_ALLOW_THREADS
+    if (rc != GPUOS_OK) {
+      auto& p = g_pending_refs[d];
+      p.insert(p.begin(), refs.begin(), refs.end());
+      return raise_status(rc);
+    }
+    if (!refs.empty()) {
+      // (a flush of another thread may have come first with a later ticket)
+      auto& q = g_inflight_refs[d];
+      auto at = q.end();
+      while (at != q.begin() && std::prev(at)->ticket > ticket) --at;
+      q.insert(at, Keep{ticket, std::move(refs)});
     }
     release_done(d, false);
   }

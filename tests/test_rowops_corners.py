@@ -6,11 +6,14 @@ Tolerances count roundings as in test_rowops.py, whose oracles these tests use.
 import itertools
 import math
 import threading
+import time
+import weakref
 
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
+from gpuos_b200 import load
 from gpuos_b200 import rowops as R
 from gpuos_b200 import scheduler as S
 from test_rowops import BF, DEV, F32, FP, ROUTE_REL, TYPES, gen, gpu, randn, route_oracle
@@ -352,3 +355,33 @@ def test_results_of_a_call_have_storages_of_their_own():
     assert R.route(x[:0], 4)[0].shape == (0, 4)
     with torch.inference_mode():
         assert R.route(x, 4)[0].is_inference()
+
+
+@gpu
+def test_tensors_of_a_request_submitted_during_a_flush_stay():
+    """A flush waits outside the interpreter's lock; a request that another thread submits meanwhile
+    is not among those it waits for, nor are its tensors."""
+    ext = load()
+    ext.init(mode="stream")
+    try:
+        x = torch.arange(64.0, device=DEV)
+        first, out = torch.empty_like(x), x * 0 + 5.0    # (which loads the kernels that the wait must not meet)
+        torch.cuda.synchronize()
+        ext.submit_add(x, x, first)
+        torch.cuda._sleep(1 << 30)                      # half a second, for which the flush waits
+        waiting = threading.Thread(target=lambda: ext.flush(sync=True))
+        waiting.start()
+        time.sleep(0.1)
+        assert waiting.is_alive()
+        y = x * 0 + 5.0
+        ext.submit_add(x, y, out)
+        alive = weakref.ref(y)
+        del y
+        assert waiting.is_alive()
+        waiting.join(60)
+        assert alive() is not None
+        ext.flush(sync=True)
+        ext.flush(sync=True)                             # what the one before left is released here at the latest
+        assert alive() is None and torch.equal(out, x + 5)
+    finally:
+        ext.shutdown()
