@@ -758,7 +758,9 @@ void forward(const LogArgs& a, cudaStream_t s) {
   // (8 x 32000 with 20 alternatives: 8.4 us over 4 CTAs a row, 9.3 over 8, 8.8 over 2)
   while (parts < 8 && a.rows * parts < 2 * sms && a.cols >= kStep * parts * 4) parts *= 2;
   // Long whole rows: fewer CTAs with more in flight each keep the memory busy while the last rows
-  // run (1000 x 128000 bf16: 45 us, 53 with four packs in flight; 3000 x 50257: 69 and 61).
+  // run (1000 x 128000 bf16: 46.5 us, 53.6 with four packs in flight).  Many shorter rows of 16 bits lose
+  // by it: 1000 and 3000 of them take 0.94 and 1.06 of the time at 13000 packs, 0.90 and 1.01
+  // at 14000, 0.87 and 1.01 at 16000 (6282: 1.02 and 1.12; of 32 bits 0.91 and 1.00 at 13000, 0.87 and 0.98 above).
   if (parts == 1 && packs >= kLongPacks) by_outputs<T, kRowThreads, 8>(a, parts, s);
   else by_outputs<T, kRowThreads, 4>(a, parts, s);
 }

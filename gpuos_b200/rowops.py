@@ -105,7 +105,7 @@ def rotary(x: Tensors, positions: torch.Tensor, inv_freq: torch.Tensor, *, scale
     strides but the last, which is 1.  `positions` (int32 or int64) has the token
     dims.  The first ``2 * len(inv_freq)`` elements of each head are rotated by
     ``position * inv_freq`` (in 64 bits) and multiplied by `scale`, in pairs (i, i + half),
-    or (2i, 2i + 1) if `interleaved`; the others are copied.  `inverse` rotates back
+    or (2i, 2i + 1) if `interleaved` (of an even head size); the others are copied.  `inverse` rotates back
     (the transposed map, also the gradient).  `out` may be `x`.  Returns tensors as `x` is given."""
     if _entered:
         _order((*_tuple(x), positions, inv_freq), () if out is None else _tuple(out))

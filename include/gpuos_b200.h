@@ -356,7 +356,7 @@ int32_t gpuos_reduce_rows_noalloc(int32_t variant, const void* x, int32_t x_dtyp
  * a = position * inv_freq[i] (in 64 bits), pair (x1, x2) of the head's first
  * 2 * pairs elements becomes scale * (x1 cos a - x2 sin a, x2 cos a + x1 sin a);
  * the other elements are copied unscaled.  Pair i is elements (i, i + pairs), or
- * (2i, 2i + 1) with GPUOS_ROTARY_INTERLEAVED.  GPUOS_ROTARY_INVERSE takes -a:
+ * (2i, 2i + 1) with GPUOS_ROTARY_INTERLEAVED (heads are then of even size).  GPUOS_ROTARY_INVERSE takes -a:
  * the transposed map, which is also the gradient.  out[i] may be x[i]. */
 #define GPUOS_ROTARY_INTERLEAVED 1
 #define GPUOS_ROTARY_INVERSE 2
