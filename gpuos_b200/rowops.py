@@ -25,6 +25,7 @@ import math
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
+import torch.autograd.forward_ad as _fwd
 
 from . import load as _load
 from . import scheduler as _scheduler
@@ -62,6 +63,10 @@ def _row(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     if g is None or g.dim() == 0 or g.stride(-1) == 1 or g.size(-1) == 1:
         return g
     return g.contiguous()
+
+
+def _followed(t: torch.Tensor) -> bool:
+    return (t.requires_grad and torch.is_grad_enabled()) or _fwd.unpack_dual(t).tangent is not None
 
 
 # ---- rotary positions ----------------------------------------------------------
@@ -113,7 +118,10 @@ def rotary(x: Tensors, positions: torch.Tensor, inv_freq: torch.Tensor, *, scale
     if got is NotImplemented:  # autograd has to record it
         if out is not None:
             raise ValueError("out cannot be given where a gradient is needed, nor in a trace")
-        got = _Rotary.apply(positions, inv_freq, scale, interleaved, inverse, *_tuple(x))
+        xs = _tuple(x)
+        got = _Rotary.apply(positions, inv_freq, scale, interleaved, inverse, *xs)
+        # (of a pair, one whose input needs none follows no gradient)
+        got = tuple(y if _followed(t) else y.detach() for t, y in zip(xs, got))
         return got[0] if isinstance(x, torch.Tensor) else got
     return got
 

@@ -385,3 +385,19 @@ def test_tensors_of_a_request_submitted_during_a_flush_stay():
         assert alive() is None and torch.equal(out, x + 5)
     finally:
         ext.shutdown()
+
+
+@gpu
+def test_of_a_pair_only_what_needs_a_gradient_is_followed():
+    g = gen(44)
+    q, k = randn(g, 5, 3, 32).to(DEV), randn(g, 5, 1, 32).to(DEV)
+    pos, f = torch.arange(5, device=DEV), R.rotary_frequencies(32, device=DEV)
+    for needs in ((True, False), (False, True), (True, True)):
+        a, b = q.clone().requires_grad_(needs[0]), k.clone().requires_grad_(needs[1])
+        y, z = R.rotary((a, b), pos, f)
+        assert (y.requires_grad, z.requires_grad) == needs
+        assert torch.equal(y, R.rotary(q, pos, f)) and torch.equal(z, R.rotary(k, pos, f))
+        grads = torch.autograd.grad([t for t in (y, z) if t.requires_grad], [t for t in (a, b) if t.requires_grad],
+                                    [w for t, w in ((y, q), (z, k)) if t.requires_grad])
+        for got, w in zip(grads, [w for n, w in zip(needs, (q, k)) if n]):
+            assert torch.equal(got, R.rotary(w, pos, f, inverse=True))
