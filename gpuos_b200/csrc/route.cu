@@ -155,14 +155,16 @@ __device__ __forceinline__ float rcp(float x) {
 }
 constexpr float kLog2e = 1.44269504088896341f;
 
-// The sigmoid of a chosen logit over e^top.  Shares of a sum take the smaller of 0 and the largest chosen
-// logit as top, so that sigmoids too small for 32 bits keep their ratios; a sigmoid by itself takes 0.
-// e^-v leaves 64 bits at the limit: the sigmoid is 0 from there on.
-__device__ __forceinline__ float sigmoid_over(float v, float top) {
+__device__ __forceinline__ float sigmoid(float v) {
   const float a = expf(-fabsf(v)), q = rcp(1.f + a);
+  return v > 0.f ? q : a * q;
+}
+// The sigmoid of a chosen logit over e^top, top the smaller of 0 and the largest chosen logit: of a
+// sum of those, sigmoids too small for 32 bits keep their shares.  e^-v leaves 64 bits at the limit: the
+// sigmoid is 0 from there on.
+__device__ __forceinline__ float sigmoid_over(float v, float top) {
   if (v <= -709.78271484375f) return 0.f;
-  if (v > 0.f) return q;
-  return (top == 0.f ? a : expf(v - top)) * q;
+  return v > 0.f ? sigmoid(v) : expf(v - top) * rcp(1.f + expf(v));
 }
 
 // Where a lane's experts are.
@@ -270,7 +272,7 @@ __device__ __forceinline__ void route_exact(const RouteArgs& a, bool keyed, int6
   const float top = lanes_top<32>(fmaxf(low, high));
   auto weight = [&](float v) {
     // (as in the lanes' part)
-    if (a.sigmoid) return sigmoid_over(v, a.renorm ? fminf(top, 0.f) : 0.f);
+    if (a.sigmoid) return a.renorm ? sigmoid_over(v, fminf(top, 0.f)) : sigmoid(v);
     if (!a.renorm || total != total) return (float)score(v);
     return top == -INFINITY ? 0.f : expf(v - top);
   };
@@ -725,7 +727,7 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
       else static_cast<int32_t*>(a.experts)[t * a.es + seat.lane * a.ek] = (int32_t)e;
     }
     if (SIGMOID) {
-      sc = sigmoid_over(v, a.renorm ? fminf(lanes_top<LPT>(v), 0.f) : 0.f);  // (0 of v = -inf)
+      sc = sigmoid(v);  // (0 of v = -inf)
     } else if (a.renorm) {
       // The chosen may lie far below the row's largest logit, where scores leave 32 bits: their shares
       // are the softmax of the chosen alone.  (Ordered by logits, the chosen have the largest.)
@@ -735,9 +737,15 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
       sc = expf(v - m) * rcp(total);
     }
     if (a.renorm) {
-      // a score over the sum first: the sum's own inverse times the scale may leave 32 bits
-      const float sum = lanes_sum<LPT>(sc);
-      sc = sum == 0.f ? 0.f : sc / sum;
+      float sum = lanes_sum<LPT>(sc);
+      if (SIGMOID && __any_sync(~0u, live && sum < 0.25f)) {
+        // none of the chosen is above -1: their sigmoids over the largest (for a token of larger ones the same again)
+        sc = sigmoid_over(v, fminf(lanes_top<LPT>(v), 0.f));
+        sum = lanes_sum<LPT>(sc);
+      }
+      // the share first: the scale over the sum may leave 32 bits.  The sum is 0 or at least a half
+      // (that of the largest chosen), so it has an inverse.
+      sc = sum == 0.f ? 0.f : sc * __frcp_rn(sum);
     }
     if (mine) a.weights[t * a.ws + seat.lane * a.wk] = sc * a.scale;
   }
@@ -814,26 +822,26 @@ gpuos_route_grad_kernel(const __grid_constant__ RouteArgs a) {
 #pragma unroll
       for (int i = 0; i < NR; ++i) m = fmaxf(m, v[i]);
       m = lanes_top<LPT>(m);
-      if (a.sigmoid) m = a.renorm ? fminf(m, 0.f) : 0.f;
+      if (a.sigmoid) m = fminf(m, 0.f);
     }
     float sc[NR], sum = 0.f, dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
-      if (a.sigmoid) sc[i] = sigmoid_over(v[i], m);
+      if (a.sigmoid) sc[i] = a.renorm ? sigmoid_over(v[i], m) : sigmoid(v[i]);
       else sc[i] = m == -INFINITY || e[i] == ~0u ? 0.f : expf(v[i] - m) * by;
       sum += sc[i];
       dot += g[i] * sc[i];
     }
     sum = lanes_sum<LPT>(sum);
     dot = lanes_sum<LPT>(dot);
-    const float less = !a.renorm || sum == 0.f ? 0.f : dot / sum;
+    // (as in the forward: the sum is 0 or at least a half)
+    const float over = !a.renorm || sum == 0.f ? 0.f : __frcp_rn(sum), less = dot * over;
     const float all = a.scale * dot;  // of a plain softmax: the sum of ds_i s_i
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       const uint32_t r = lane + i * LPT;
       float d = a.scale * (g[i] - less);
-      // (a score over the sum first, as in the forward: the sum's own inverse may leave 32 bits)
-      if (a.renorm) d *= sum == 0.f ? 0.f : sc[i] / sum;
+      if (a.renorm) d *= sc[i] * over;
       else if (a.sigmoid) d *= sc[i];
       if (a.sigmoid) {
         const float x = expf(-fabsf(v[i])), q = 1.f / (1.f + x);
