@@ -401,7 +401,8 @@ int32_t gpuos_cache_read(int32_t n, const gpuos_tensor* slots, const gpuos_tenso
  * lowest index comes first.  A NaN logit counts as -inf in the choice; a row of
  * -inf has scores 0 (softmax); a sigmoid is 0 where e^-x leaves 64 bits (x below
  * -709.78).  Renormalised weights are the shares of the chosen scores however
- * small those are, and 0 where all of them are 0. */
+ * small those are (of a softmax: the softmax of the chosen logits alone), and 0
+ * where all the chosen are masked by -inf or have a sigmoid of 0. */
 #define GPUOS_SCORE_SOFTMAX 0
 #define GPUOS_SCORE_SIGMOID 1
 #define GPUOS_GROUP_MAX 0

@@ -401,3 +401,22 @@ def test_of_a_pair_only_what_needs_a_gradient_is_followed():
                                     [w for t, w in ((y, q), (z, k)) if t.requires_grad])
         for got, w in zip(grads, [w for n, w in zip(needs, (q, k)) if n]):
             assert torch.equal(got, R.rotary(w, pos, f, inverse=True))
+
+
+@gpu
+@pytest.mark.parametrize("top_k", [2, 33])
+def test_renormalised_softmax_of_masked_experts(top_k):
+    """A bias that closes all experts but masked ones: by -inf nothing is left of those, by a finite
+    number they share alike, in the weights as in their gradient."""
+    x = torch.zeros(2, 48)
+    x[0, 8:], x[1, 8:] = -math.inf, -65504.0
+    bias = torch.zeros(48)
+    bias[:8] = -2.0
+    gw = randn(gen(45), 2, top_k)
+    w, e = R.route(x.to(DEV), top_k, bias=bias.to(DEV), renormalize=True)
+    assert bool((e >= 8).all())
+    want = torch.stack((torch.zeros(top_k), torch.full((top_k,), 1 / top_k))).double()
+    assert bool(((w.cpu().double() - want).abs() <= ROUTE_REL * want).all())
+    dx = R.route_grad(x.to(DEV), e, gw.to(DEV), renormalize=True).cpu().double()
+    d = torch.zeros(2, 48).double().scatter(-1, e.cpu(), want * (gw.double() - (gw.double() * want).sum(-1, keepdim=True)))
+    assert bool(((dx - d).abs() <= 2 * ROUTE_REL * (gw.abs().amax().double() + 1)).all()) and not bool(dx[0].any())
