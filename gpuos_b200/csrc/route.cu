@@ -744,8 +744,8 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
         sc = sigmoid_over(v, fminf(lanes_top<LPT>(v), 0.f));
         sum = lanes_sum<LPT>(sc);
       }
-      // the share first: the scale over the sum may leave 32 bits.  The sum is 0 or at least a half
-      // (that of the largest chosen), so it has an inverse.
+      // the share first: the scale over the sum may leave 32 bits.  The sum is 0 or at least a quarter,
+      // so it has an inverse.
       sc = sum == 0.f ? 0.f : sc * __frcp_rn(sum);
     }
     if (mine) a.weights[t * a.ws + seat.lane * a.wk] = sc * a.scale;
