@@ -740,8 +740,9 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
     if (a.renorm) {
       float sum = lanes_sum<LPT>(sc);
       if (SIGMOID && __any_sync(~0u, live && sum < 0.25f)) {
-        // none of the chosen is above -1: their sigmoids over the largest (for a token of larger ones the same again)
-        sc = sigmoid_over(v, fminf(lanes_top<LPT>(v), 0.f));
+        // none of the chosen is above -1: their sigmoids over the largest (other tokens of the warp keep theirs)
+        const float over = sigmoid_over(v, fminf(lanes_top<LPT>(v), 0.f));
+        if (sum < 0.25f) sc = over;
         sum = lanes_sum<LPT>(sc);
       }
       // the share first: the scale over the sum may leave 32 bits.  The sum is 0 or at least a quarter,

@@ -420,3 +420,15 @@ def test_renormalised_softmax_of_masked_experts(top_k):
     dx = R.route_grad(x.to(DEV), e, gw.to(DEV), renormalize=True).cpu().double()
     d = torch.zeros(2, 48).double().scatter(-1, e.cpu(), want * (gw.double() - (gw.double() * want).sum(-1, keepdim=True)))
     assert bool(((dx - d).abs() <= 2 * ROUTE_REL * (gw.abs().amax().double() + 1)).all()) and not bool(dx[0].any())
+
+
+@gpu
+@pytest.mark.parametrize("experts", [8, 24, 64, 200])
+def test_small_sigmoids_leave_the_other_tokens_of_a_warp_as_they_are(experts):
+    x = -0.3 - torch.rand(64, experts, generator=gen(46))
+    w, e = R.route(x.to(DEV), 3, score="sigmoid", renormalize=True)
+    x[1::2] -= 95.0
+    x[6] = -math.inf
+    w2, e2 = R.route(x.to(DEV), 3, score="sigmoid", renormalize=True)
+    keep = [i for i in range(0, 64, 2) if i != 6]
+    assert torch.equal(w[keep], w2[keep]) and torch.equal(e[keep], e2[keep])
