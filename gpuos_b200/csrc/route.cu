@@ -711,10 +711,15 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
     }
     uint32_t slot = keyed ? from * NPL + (NPL - 1 - (won & ((1u << kLow) - 1)))
                           : kSlots - 1 - (won & ((1u << (exact ? 16 : kShift)) - 1));
-    // (the whole warp takes part; a token that is not in doubt gets the same again)
+    // (the whole warp takes part; a token that is not in doubt keeps what it has, whatever is beside it)
     if (__any_sync(~0u, (doubt || odd) && live && !later)) {
-      const bool close = resolve<T, NPL, LPT, GROUPED>(a, row, live, seat, keyed, &slot);
-      later = (__ballot_sync(~0u, later || odd || close) >> seat.base & kLanes<LPT>) != 0;
+      uint32_t again = slot;
+      const bool close = resolve<T, NPL, LPT, GROUPED>(a, row, live, seat, keyed, &again);
+      const uint32_t asked = __ballot_sync(~0u, doubt || odd), open_still = __ballot_sync(~0u, odd || close);
+      if ((asked >> seat.base & kLanes<LPT>) != 0) {
+        slot = again;
+        later = later || (open_still >> seat.base & kLanes<LPT>) != 0;
+      }
     }
     if (later && live && seat.lane == 0) which[atomicAdd(&left, 1u)] = (uint16_t)(step * kTokens + sub);
 

@@ -432,3 +432,22 @@ def test_small_sigmoids_leave_the_other_tokens_of_a_warp_as_they_are(experts):
     w2, e2 = R.route(x.to(DEV), 3, score="sigmoid", renormalize=True)
     keep = [i for i in range(0, 64, 2) if i != 6]
     assert torch.equal(w[keep], w2[keep]) and torch.equal(e[keep], e2[keep])
+
+
+@gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts", [8, 24, 64])
+def test_doubt_about_one_token_leaves_the_others_of_a_warp_as_they_are(score, experts):
+    """Ties in every other row send them to later passes; the rows between have a score that those passes
+    would not settle, but which decides nothing there."""
+    g = gen(47)
+    x, tied = randn(g, 256, experts), torch.zeros(256, experts)
+    x[:, 5] = -700.0
+    bias = torch.rand(experts, generator=g)
+    bias[2] = bias[3] = 3.0                # the tie of a row of equal logits
+    bias[5] = -3.0
+    tied[::2] = x[::2]
+    w, e = R.route(x.to(DEV), 3, score=score, bias=bias.to(DEV))
+    w2, e2 = R.route(tied.to(DEV), 3, score=score, bias=bias.to(DEV))
+    assert torch.equal(e2.cpu(), route_oracle(tied, 3, score=score, bias=bias)[1])
+    assert torch.equal(w[::2], w2[::2]) and torch.equal(e[::2], e2[::2])
