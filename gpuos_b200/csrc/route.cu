@@ -733,7 +733,13 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
       else static_cast<int32_t*>(a.experts)[t * a.es + seat.lane * a.ek] = (int32_t)e;
     }
     if (SIGMOID) {
-      sc = sigmoid(v);  // (0 of v = -inf)
+      sc = mine ? rcp(1.f + expf(-v)) : 0.f;
+      // below -60, on the way out of 32 bits, by e^v, and shares over the largest chosen
+      const uint32_t low = __ballot_sync(~0u, mine && v < -60.f);
+      if (low != 0) {
+        const float over = sigmoid_over(v, a.renorm ? fminf(lanes_top<LPT>(v), 0.f) : 0.f);
+        if ((low >> seat.base & kLanes<LPT>) != 0) sc = over;  // (other tokens of the warp keep theirs)
+      }
     } else if (a.renorm) {
       // The chosen may lie far below the row's largest logit, where scores leave 32 bits: their shares
       // are the softmax of the chosen alone.  (Ordered by logits, the chosen have the largest.)
@@ -743,15 +749,9 @@ gpuos_route_kernel(const __grid_constant__ RouteArgs a) {
       sc = expf(v - m) * rcp(total);
     }
     if (a.renorm) {
-      float sum = lanes_sum<LPT>(sc);
-      if (SIGMOID && __any_sync(~0u, live && sum < 0.25f)) {
-        // none of the chosen is above -1: their sigmoids over the largest (other tokens of the warp keep theirs)
-        const float over = sigmoid_over(v, fminf(lanes_top<LPT>(v), 0.f));
-        if (sum < 0.25f) sc = over;
-        sum = lanes_sum<LPT>(sc);
-      }
-      // the share first: the scale over the sum may leave 32 bits.  The sum is 0 or at least a quarter,
-      // so it has an inverse.
+      // the share first: the scale over the sum may leave 32 bits.  The sum is 0 or at least e^-60, so
+      // it has an inverse.
+      const float sum = lanes_sum<LPT>(sc);
       sc = sum == 0.f ? 0.f : sc * __frcp_rn(sum);
     }
     if (mine) a.weights[t * a.ws + seat.lane * a.wk] = sc * a.scale;
