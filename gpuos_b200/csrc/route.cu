@@ -23,9 +23,9 @@
 // needed, so that one warp serves up to 8 tokens of few experts.  A lane sorts its
 // keys once; a round of the selection is then a maximum over the lanes' first ones.
 // Few experts make the kernel a matter of instructions, not of bytes: 16384
-// tokens of 256 fp32 logits in 8 groups are 18 MB, 2.8 us, and 1236 instructions of a warp each, 23.6 us
-// at three quarters of the issue slots; 32749 of 128 bf16 without groups take 14.6 us, the gradient 10.0.
-// Tokens that all go to the second part cost several times that: 8192 x 64 with 40 ranks 58 us.
+// tokens of 256 fp32 logits in 8 groups are 18 MB, 2.8 us, and 1236 instructions of a warp each, 23.8 us
+// at three quarters of the issue slots; 32749 of 128 bf16 without groups take 14.7 us, the gradient 10.0.
+// Tokens that all go to the second part cost several times that: 8192 x 64 with 40 ranks 59 us.
 #include "rowops.cuh"
 
 namespace gpuos {
