@@ -17,6 +17,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -32,8 +33,8 @@ EXT = HERE / ("gpuos_ext" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 DEV_HEADERS = [CSRC / "gpuos_abi.h", CSRC / "ops.cuh", CSRC / "executor.cuh", CSRC / "batch.cuh",
                CSRC / "lean.cuh"]
-# one object each: gpuos_rotary, gpuos_cache_*, gpuos_route*, gpuos_logprobs*
-ROWOPS = ["rotary", "cache", "route", "logprobs"]
+# gpuos_rotary, gpuos_cache_*, gpuos_attend, gpuos_route*, gpuos_order / dispatch / combine*, gpuos_logprobs*, gpuos_verify
+ROWOPS = ["rotary", "cache", "attend", "attend_int8", "attend_e4m3", "route", "experts", "logprobs", "verify"]
 HOST_HEADERS = [CSRC / "gpuos_abi.h", CSRC / "runtime.h", CSRC / "jit.h", ROOT / "include" / "gpuos_b200.h"]
 
 
@@ -56,59 +57,54 @@ def _run(cmd, verbose):
 
 def build_lib(force=False, verbose=False) -> Path:
     BUILD.mkdir(exist_ok=True)
-    kobj = BUILD / "kernels.o"
-    robj = BUILD / "runtime.o"
-    if force or _stale(kobj, [CSRC / "kernels.cu", *DEV_HEADERS]):
-        _run([NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
-              "-c", CSRC / "kernels.cu", "-o", kobj], verbose)
-    nobj = BUILD / "noalloc.o"
-    if force or _stale(nobj, [CSRC / "noalloc.cu", ROOT / "include" / "gpuos_b200.h", *DEV_HEADERS]):
-        _run([NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
-              "-c", CSRC / "noalloc.cu", "-o", nobj], verbose)
-    # the row operators
-    robj2 = BUILD / "rowops.o"
-    if force or _stale(robj2, [CSRC / "rowops.cpp"]):
-        _run(["g++", "-std=c++17", "-O2", "-fPIC", "-Wall", f"-I{CUDA_HOME / 'include'}",
-              "-c", CSRC / "rowops.cpp", "-o", robj2], verbose)
-    rowobjs = [robj2]
+    abi = ROOT / "include" / "gpuos_b200.h"
+    nvcc = [NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
+    gxx = ["g++", "-std=c++17", "-O2", "-fPIC", "-Wall", "-Wno-unused-parameter", f"-I{CUDA_HOME / 'include'}"]
+    # (object, its command up to -o, what it depends on)
+    steps = [(BUILD / "kernels.o", [*nvcc, "-c", CSRC / "kernels.cu"], [CSRC / "kernels.cu", *DEV_HEADERS]),
+             (BUILD / "noalloc.o", [*nvcc, "-c", CSRC / "noalloc.cu"], [CSRC / "noalloc.cu", abi, *DEV_HEADERS]),
+             (BUILD / "rowops.o", [*gxx, "-c", CSRC / "rowops.cpp"], [CSRC / "rowops.cpp"]),
+             (BUILD / "jit.o", [*gxx, "-c", CSRC / "jit.cpp"], [CSRC / "jit.cpp", CSRC / "jit.h", *HOST_HEADERS]),
+             (BUILD / "runtime.o", [*gxx, "-c", CSRC / "runtime.cpp"], [CSRC / "runtime.cpp", *HOST_HEADERS]),
+             (BUILD / "ipc.o", [*gxx, "-c", CSRC / "ipc.cpp"], [CSRC / "ipc.cpp", *HOST_HEADERS])]
     for name in ROWOPS:
-        obj = BUILD / f"{name}.o"
-        rowobjs.append(obj)
-        if force or _stale(obj, [CSRC / f"{name}.cu", CSRC / "rowops.cuh", CSRC / "rowops.h",
-                                 ROOT / "include" / "gpuos_b200.h"]):
-            _run([NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
-                  "-c", CSRC / f"{name}.cu", "-o", obj], verbose)
-    # the relocatable batch kernel for custom expressions, embedded as bytes
+        src = CSRC / f"{name}.cu"
+        deps = [src, CSRC / "rowops.cuh", CSRC / "rowops.h", abi]
+        if name.startswith("attend"):
+            deps += [CSRC / "attend.h", CSRC / "attend.cuh"]
+        steps.append((BUILD / f"{name}.o", [*nvcc, "-c", src], deps))
     jcubin = BUILD / "jit_kernel.cubin"
     jblob = BUILD / "jit_blob.cpp"
     jbobj = BUILD / "jit_blob.o"
-    jobj = BUILD / "jit.o"
-    if force or _stale(jcubin, [CSRC / "jit_kernel.cu", *DEV_HEADERS]):
-        _run([NVCC, *ARCH, "-O3", "-std=c++17", "-rdc=true", "-cubin",
-              CSRC / "jit_kernel.cu", "-o", jcubin], verbose)
-    if force or _stale(jbobj, [jcubin]):
-        data = jcubin.read_bytes()
-        lines = ["// generated by _build.py from jit_kernel.cu: the relocatable batch kernel",
-                 'extern "C" const unsigned long long gpuos_jit_cubin_size = %d;' % len(data),
-                 'extern "C" alignas(64) const unsigned char gpuos_jit_cubin[] = {']
-        for k in range(0, len(data), 24):
-            lines.append(",".join(str(b) for b in data[k:k + 24]) + ",")
-        lines.append("};")
-        jblob.write_text("\n".join(lines) + "\n")
-        _run(["g++", "-O0", "-fPIC", "-c", jblob, "-o", jbobj], verbose)
-    if force or _stale(jobj, [CSRC / "jit.cpp", CSRC / "jit.h", *HOST_HEADERS]):
-        _run(["g++", "-std=c++17", "-O2", "-fPIC", "-Wall", "-Wno-unused-parameter",
-              f"-I{CUDA_HOME / 'include'}", "-c", CSRC / "jit.cpp", "-o", jobj], verbose)
-    if force or _stale(robj, [CSRC / "runtime.cpp", *HOST_HEADERS]):
-        _run(["g++", "-std=c++17", "-O2", "-fPIC", "-Wall", "-Wno-unused-parameter",
-              f"-I{CUDA_HOME / 'include'}", "-c", CSRC / "runtime.cpp", "-o", robj], verbose)
-    iobj = BUILD / "ipc.o"
-    if force or _stale(iobj, [CSRC / "ipc.cpp", *HOST_HEADERS]):
-        _run(["g++", "-std=c++17", "-O2", "-fPIC", "-Wall", "-Wno-unused-parameter",
-              f"-I{CUDA_HOME / 'include'}", "-c", CSRC / "ipc.cpp", "-o", iobj], verbose)
-    if force or _stale(LIB, [kobj, robj, nobj, jobj, jbobj, iobj, *rowobjs]):
-        _run([NVCC, *ARCH, "-shared", "-cudart", "static", "-o", LIB, kobj, robj, nobj, jobj, jbobj,
-              iobj, *rowobjs, "-Xlinker", "--no-undefined", "-lpthread", "-ldl", "-lrt"], verbose)
+
+    def embed():
+        # the relocatable batch kernel for custom expressions, embedded as bytes
+        if force or _stale(jcubin, [CSRC / "jit_kernel.cu", *DEV_HEADERS]):
+            _run([NVCC, *ARCH, "-O3", "-std=c++17", "-rdc=true", "-cubin",
+                  CSRC / "jit_kernel.cu", "-o", jcubin], verbose)
+        if force or _stale(jbobj, [jcubin]):
+            data = jcubin.read_bytes()
+            lines = ["// generated by _build.py from jit_kernel.cu: the relocatable batch kernel",
+                     'extern "C" const unsigned long long gpuos_jit_cubin_size = %d;' % len(data),
+                     'extern "C" alignas(64) const unsigned char gpuos_jit_cubin[] = {']
+            for k in range(0, len(data), 24):
+                lines.append(",".join(str(b) for b in data[k:k + 24]) + ",")
+            lines.append("};")
+            jblob.write_text("\n".join(lines) + "\n")
+            _run(["g++", "-O0", "-fPIC", "-c", jblob, "-o", jbobj], verbose)
+
+    def compile_one(step):
+        out, cmd, deps = step
+        if force or _stale(out, deps):
+            _run([*cmd, "-o", out], verbose)
+
+    with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+        for f in [pool.submit(embed), *(pool.submit(compile_one, s) for s in steps)]:
+            f.result()
+    objs = [out for out, _, _ in steps] + [jbobj]
+    if force or _stale(LIB, objs):
+        _run([NVCC, *ARCH, "-shared", "-cudart", "static", "-o", LIB, *objs,
+              "-Xlinker", "--no-undefined", "-lpthread", "-ldl", "-lrt"], verbose)
     return LIB
 
 

@@ -1,0 +1,722 @@
+// gpuos_attend for few rows: query rows over a paged cache of 8-bit codes.
+// With s_j = scale * q . (K_j kappa_j), K and V codes, kappa and nu their scales,
+//
+//   m = max s_j     l = sum e^(s_j - m)     out = sum e^(s_j - m) nu_j V_j / l
+//
+// over the positions j that a query sees.  Each code is read once for all query heads
+// of its key head and, of drafted tokens, for all queries: a block of 8, 16 or 32
+// rows.  At so few rows memory is the bound, and an SM's share of it is 24 codes a
+// cycle, so what a code costs in instructions counts:
+//   - codes are whole numbers, or e4m3 numbers, that 16-bit floats hold exactly: a
+//     code becomes one in about 1.3 instructions, unscaled.  kappa_j multiplies the
+//     finished product; nu_j goes into the 16-bit weight e^(s_j - m) nu_j;
+//   - the codes are the matrix product's first operand (16 positions, or 16 elements of
+//     the head, a step) and the 8 rows its second one, so that no row of it is idle;
+//   - a row's maximum is raised only when a score passes it by 2^4;
+//   - q is held as 16-bit floats times a power of two a row, nu_j relative to a
+//     power of two that follows the largest seen: 16-bit floats then lose nothing of a 16-bit q,
+//     and half a step, 2^-11, of a weight down to 2^-22 of the largest: an eighth of what a bf16 result is
+//     rounded by.  32-bit queries take q and weights in two parts (2^-22), 16-bit floats of 11 bits the weights.
+// A warp takes 32 positions at a time through a ring of its own (no barrier in the
+// loop).  Items (sequence, key head, block of rows) are laid end to end and the CTAs
+// take equal shares of all units; what is split is joined by a second launch in a fixed order.
+#pragma once
+#include "attend.h"
+
+namespace gpuos {
+namespace rowops {
+namespace attend {
+namespace {
+
+constexpr uint32_t kTile = 32;
+constexpr float kSmallestUnit = 0x1p-100f;
+
+// How a kernel lays out its shared memory.
+template <int DT, int NT, bool GEN>
+struct Layout {
+  static constexpr uint32_t rows = 8 * NT;
+  static constexpr uint32_t stages = GEN ? 2 : 3;
+  static constexpr uint32_t scales = GEN ? DT / 32 : 1;                 // of a row, room for
+  static constexpr uint32_t codes = kTile * DT;                         // bytes, of K or V
+  static constexpr uint32_t stage = 2 * codes + 2 * kTile * scales * 4 + 16;
+  static constexpr uint32_t ring = stages * stage > rows * DT * 4 ? stages * stage : rows * DT * 4;  // of a warp
+  static constexpr uint32_t q_row = DT * 2 + 64;                        // bytes: 4 of 8 16-byte banks further each row
+  static constexpr uint32_t q = rows * q_row * (GEN ? 2 : 1);
+  static constexpr uint32_t total = kWarps * ring + q;
+};
+
+// Where the 16 bytes x of a row of codes lie: rows of 8 (K) and every second row (V) are read
+// together without two of them in a bank.
+template <int DT>
+__device__ __forceinline__ uint32_t place(uint32_t row, uint32_t x) {
+  if constexpr (DT == 64) {
+    const uint32_t line = row >> 1;
+    return line * 128 + ((((row & 1) * 4 + x) ^ ((line & 3) << 1)) << 4);
+  } else {
+    return row * DT + ((x ^ ((((row >> 1) & 3) << 1) ^ ((row & 1) << 2))) << 4);
+  }
+}
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool has) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(has ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void* from, bool has) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(has ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float2 unpack(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
+
+// Of an item, laid out in units: blocks of a head, heads of a sequence.
+struct Item {
+  uint32_t seq, head;
+  int64_t block;
+  int64_t units, from;  // all of it, and where the search's unit lies
+};
+
+template <uint32_t RB>
+__device__ __forceinline__ int64_t blocks(const Args& a, const Sequence& s) {
+  const int64_t rows = s.n * a.each;
+  return a.few && rows > a.few ? 0 : (rows + RB - 1) / RB;
+}
+template <uint32_t RB>
+__device__ __forceinline__ Range block_range(const Args& a, const Sequence& s, int64_t b) {
+  const int64_t last = min((b + 1) * RB, s.n * a.each) - 1;
+  return seen(a, s, a.each_div.div((uint32_t)(b * RB)), a.each_div.div((uint32_t)last));
+}
+__device__ __forceinline__ int64_t units_of(const Range& r) { return max((r.hi - r.lo + kUnit - 1) / kUnit, (int64_t)1); }
+
+// Units of a head of a sequence.
+template <uint32_t RB>
+__device__ __forceinline__ int64_t head_units(const Args& a, const Sequence& s) {
+  const int64_t n = blocks<RB>(a, s);
+  int64_t u = 0;
+  for (int64_t b = 0; b < n; ++b) u += units_of(block_range<RB>(a, s, b));
+  return u;
+}
+
+// The item that unit `u` of sequence s lies in.
+template <uint32_t RB>
+__device__ __forceinline__ Item find(const Args& a, uint32_t seq, const Sequence& s, int64_t u) {
+  Item it;
+  it.seq = seq;
+  const int64_t per_head = head_units<RB>(a, s);
+  it.head = (uint32_t)(u / per_head);
+  u -= it.head * per_head;
+  for (it.block = 0;; ++it.block) {
+    it.units = units_of(block_range<RB>(a, s, it.block));
+    if (u < it.units) break;
+    u -= it.units;
+  }
+  it.from = u;
+  return it;
+}
+
+template <int F, int DT, int NT, bool GEN>
+__global__ void __launch_bounds__(kThreads, DT == 256 ? 1 : 2)
+gpuos_attend_kernel(const __grid_constant__ Args a) {
+  using L = Layout<DT, NT, GEN>;
+  constexpr uint32_t RB = L::rows, kStages = L::stages;
+  constexpr uint32_t MT = DT / 16;             // steps over the head's elements
+  constexpr uint32_t HB = DT / 32;             // blocks of 32 elements
+  // Weights are at most 2^14: 2^kSlack from scores that pass the row's maximum, 2^kSlackV from scales that pass
+  // their unit, and the rest as a factor, so that small weights stay among the normal 16-bit numbers.
+  constexpr int kSlack = GEN ? 0 : 4, kSlackV = GEN ? 0 : 2, kUp = 14 - kSlack - kSlackV;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int64_t thread_units[kThreads + 1];
+  __shared__ uint32_t edge_seq[2];
+  __shared__ int64_t edge_unit[2], edge_at[2];
+  __shared__ float row_scale[RB];              // of a row's q, times scale * log2(e)
+  __shared__ int64_t row_lo[RB], row_hi[RB];   // positions a row sees
+  __shared__ float part_m[kWarps][RB], part_l[kWarps][RB], part_e[kWarps];
+
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  uint8_t* const ring = smem + warp * L::ring;
+  uint8_t* const sq = smem + kWarps * L::ring;
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+
+  // tokens of no sequence get zeros
+  if (a.offsets) {
+    const int64_t end = min(max(load_index(a.offsets, a.offset_wide, (int64_t)a.sequences * a.os), (int64_t)0), (int64_t)a.tokens);
+    const int64_t before = min(max(load_index(a.offsets, a.offset_wide, 0), (int64_t)0), end);
+    const uint32_t heads = a.k_heads * a.each;
+    for (int64_t i = blockIdx.x * kWarps + warp; i < (before + a.tokens - end) * heads; i += (int64_t)a.grid * kWarps) {
+      int64_t t = i / heads;
+      const int64_t h = i - t * heads;
+      if (t >= before) t += end - before;
+      for (uint32_t e = lane; e < a.head; e += 32) store_real(a.out, a.type, t * a.ot + h * a.oh + e, 0.f);
+      if (a.lse && lane == 0) a.lse[t * a.lt + h * a.lh] = -INFINITY;
+    }
+  }
+
+  // ---- this CTA's share: where unit blockIdx.x * per begins, and the next CTA's
+  const uint32_t per_thread = (a.sequences + kThreads - 1) / kThreads;
+  const uint32_t s0 = min(tid * per_thread, a.sequences), s1 = min(s0 + per_thread, a.sequences);
+  {
+    int64_t u = 0;
+    for (uint32_t s = s0; s < s1; ++s) u += a.k_heads * head_units<RB>(a, sequence(a, s));
+    int64_t sum = u;
+    for (uint32_t d = 1; d < 32; d <<= 1) {
+      const int64_t o = __shfl_up_sync(~0u, sum, d);
+      if (lane >= d) sum += o;
+    }
+    thread_units[tid + 1] = sum;  // within the warp
+    __syncthreads();
+    int64_t ahead = 0;
+    for (uint32_t w = 0; w < warp; ++w) ahead += thread_units[(w + 1) * 32];
+    __syncthreads();
+    thread_units[tid + 1] = sum + ahead;
+    if (tid == 0) thread_units[0] = 0;
+    if (tid < 2) {
+      edge_seq[tid] = a.sequences;
+      edge_unit[tid] = 0;
+    }
+    __syncthreads();
+  }
+  const int64_t all = thread_units[kThreads];
+  const int64_t per = max((all + a.grid - 1) / a.grid, (int64_t)kLeast);
+  if (blockIdx.x * per >= all) {
+    if (tid == 0 && a.split) a.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
+  }
+  for (int i = 0; i < 2; ++i) {
+    int64_t u = (blockIdx.x + i) * per;
+    if (u >= all) {
+      if (tid == 0) edge_at[i] = all;
+    } else if (thread_units[tid] <= u && u < thread_units[tid + 1]) {
+      int64_t at = thread_units[tid];
+      for (uint32_t s = s0; s < s1; ++s) {
+        const Sequence q = sequence(a, s);
+        const int64_t n = a.k_heads * head_units<RB>(a, q);
+        if (u < at + n) {
+          const Item it = find<RB>(a, s, q, u - at);
+          if (it.from && it.units <= kWhole) u += it.units - it.from;  // short items stay whole
+          edge_seq[i] = s;
+          edge_unit[i] = u - at;  // (may be n: the next sequence's first)
+          edge_at[i] = u;
+          break;
+        }
+        at += n;
+      }
+    }
+  }
+  __syncthreads();
+  int64_t todo = edge_at[1] - edge_at[0];
+  uint32_t seq = edge_seq[0];
+  int64_t unit = edge_unit[0];
+  int4 goes_on = make_int4(0, 0, 0, 0);
+
+  while (todo > 0) {
+    // ---- the item, and how much of it is this CTA's
+    Sequence s = sequence(a, seq);
+    int64_t n = blocks<RB>(a, s) ? a.k_heads * head_units<RB>(a, s) : 0;
+    if (unit >= n) {
+      unit -= n;
+      ++seq;
+      continue;
+    }
+    const Item it = find<RB>(a, seq, s, unit);
+    const int64_t take = min(it.units - it.from, todo);
+    const Range range = block_range<RB>(a, s, it.block);
+    const int64_t begin = range.lo + it.from * kUnit + warp * kTile;
+    const uint32_t row0 = (uint32_t)(it.block * RB), row_count = (uint32_t)min((int64_t)RB, s.n * a.each - row0);
+    // positions that every row sees
+    const int64_t all_hi = last_seen(a, s, a.each_div.div(row0)) + 1;
+    const int64_t all_lo = first_seen(a, last_seen(a, s, a.each_div.div(row0 + row_count - 1)));
+
+    // ---- loads: 32 positions of this warp into a stage
+    const int64_t table = it.seq * a.ps;
+    auto page_at = [&](int64_t j) -> int64_t {  // of position j; -1 where there is none
+      if (j >= range.hi) return -1;
+      const int64_t p = load_index(a.pages, a.page_wide, table + a.page.div((uint32_t)j) * a.pp);
+      return p >= 0 && p < a.pool ? p : -1;
+    };
+    int64_t next_page = page_at(begin + lane);
+    auto issue = [&](int64_t i) {  // unit i of the share
+      if (i < take) {
+        const uint32_t to = ring_at + (uint32_t)(i % kStages) * L::stage;
+        const int64_t j = begin + i * kUnit + lane;
+        const int64_t page = next_page;
+        if (i + 1 < take) next_page = page_at(j + kUnit);
+        const uint32_t row = (uint32_t)j - a.page.div((uint32_t)j) * a.page.d;
+        const bool has = page >= 0;
+        const int64_t k_at = has ? page * a.k.cp + row * a.k.cr + it.head * a.k.ch : 0;
+        const int64_t v_at = has ? page * a.v.cp + row * a.v.cr + it.head * a.v.ch : 0;
+        constexpr uint32_t X = DT / 16;
+        if (a.vec == 16) {
+#pragma unroll
+          for (uint32_t r0 = 0; r0 < X; ++r0) {
+            const uint32_t r = r0 * (32 / X) + lane / X, x = lane % X;
+            const int64_t ko = __shfl_sync(~0u, k_at, r), vo = __shfl_sync(~0u, v_at, r);
+            const bool in = __shfl_sync(~0u, has, r) && x * 16 < a.head;
+            const uint32_t at = place<DT>(r, x);
+            copy16(to + at, a.k.codes + ko + (in ? x * 16 : 0), in);
+            copy16(to + L::codes + at, a.v.codes + vo + (in ? x * 16 : 0), in);
+          }
+        } else {
+          uint8_t* const stage = ring + (i % kStages) * L::stage;
+          for (uint32_t r = 0; r < kTile; ++r) {
+            const int64_t ko = __shfl_sync(~0u, k_at, r), vo = __shfl_sync(~0u, v_at, r);
+            const bool in = __shfl_sync(~0u, has, r);
+            for (uint32_t e = lane * 4; e < DT; e += 128) {
+              const uint32_t at = place<DT>(r, e >> 4) + (e & 15);
+              if (a.vec == 4) {
+                copy4(to + at, a.k.codes + ko + (in && e < a.head ? e : 0), in && e < a.head);
+                copy4(to + L::codes + at, a.v.codes + vo + (in && e < a.head ? e : 0), in && e < a.head);
+              } else {
+#pragma unroll
+                for (uint32_t b = 0; b < 4; ++b) {
+                  stage[at + b] = in && e < a.head ? a.k.codes[ko + e + b] : 0;
+                  stage[L::codes + at + b] = in && e < a.head ? a.v.codes[vo + e + b] : 0;
+                }
+              }
+            }
+          }
+        }
+        const uint32_t sc = to + 2 * L::codes;
+        const int64_t ks = has ? page * a.k.sp + row * a.k.sr + it.head * a.k.sh : 0;
+        const int64_t vs = has ? page * a.v.sp + row * a.v.sr + it.head * a.v.sh : 0;
+        for (uint32_t gr = 0; gr < (GEN ? a.groups : 1); ++gr) {
+          copy4(sc + (gr * kTile + lane) * 4, a.k.scales + ks + gr * a.k.sg, has);
+          copy4(sc + ((L::scales + gr) * kTile + lane) * 4, a.v.scales + vs + gr * a.v.sg, has);
+        }
+        const uint32_t valid = __ballot_sync(~0u, has);
+        if (lane == 0) *reinterpret_cast<uint32_t*>(ring + (i % kStages) * L::stage + 2 * L::codes + 2 * kTile * L::scales * 4) = valid;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (uint32_t i = 0; i + 1 < kStages; ++i) issue(i);
+
+    // ---- the block's rows of q: a warp takes a row
+    for (uint32_t r = warp; r < RB; r += kWarps) {
+      constexpr uint32_t E = DT / 32;
+      float v[E];
+      float most = 0.f;
+      int64_t base = 0;
+      uint32_t query = 0;
+      if (r < row_count) {
+        query = a.each_div.div(row0 + r);
+        base = (s.first + query) * a.qt + (int64_t)(it.head * a.each + row0 + r - query * a.each) * a.qh;
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < E; ++i) {
+        const uint32_t e = i * 32 + lane;
+        v[i] = r < row_count && e < a.head ? load_real(a.q, a.type, base + e) : 0.f;
+        most = fmaxf(most, fabsf(v[i]));
+      }
+      most = warp_max(most);
+      // times a power of two that puts the largest into [2^14, 2^15): 16-bit floats reach 2^-29 of it
+      int shift = 14 - (int)((__float_as_uint(most) >> 23) - 127);
+      if (!(most > 0.f)) shift = 0;
+      const float up = __uint_as_float((uint32_t)(min(max(shift, -126), 126) + 127) << 23);  // (in two steps for the smallest)
+      const float more = __uint_as_float((uint32_t)(shift - min(max(shift, -126), 126) + 127) << 23);
+#pragma unroll
+      for (uint32_t i = 0; i < E; ++i) {
+        const uint32_t e = i * 32 + lane;
+        const float y = v[i] * up * more;
+        const __half hi = __float2half_rn(y);
+        *reinterpret_cast<__half*>(sq + r * L::q_row + e * 2) = hi;
+        if (GEN) *reinterpret_cast<__half*>(sq + (RB + r) * L::q_row + e * 2) = __float2half_rn(a.split_q ? y - __half2float(hi) : 0.f);
+      }
+      if (lane == 0) {
+        row_scale[r] = a.scale2 / up / more;
+        const int64_t last = last_seen(a, s, query);
+        row_lo[r] = r < row_count ? first_seen(a, last) : 1;
+        row_hi[r] = r < row_count ? last + 1 : 0;
+      }
+    }
+    __syncthreads();
+    float scale[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      scale[t][0] = row_scale[8 * t + 2 * c];
+      scale[t][1] = row_scale[8 * t + 2 * c + 1];
+    }
+    uint4 qf[NT == 1 && !GEN ? HB : 1];
+    if constexpr (NT == 1 && !GEN) {
+#pragma unroll
+      for (uint32_t b = 0; b < HB; ++b) qf[b] = *reinterpret_cast<const uint4*>(sq + g * L::q_row + b * 64 + c * 16);
+    }
+
+    float o[MT][NT][4];
+#pragma unroll
+    for (uint32_t i = 0; i < MT; ++i)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[i][t][k] = 0.f;
+    float m[NT][2], l[NT][2], unit_v = 0.f;  // unit_v: the power of two that nu is relative to
+#pragma unroll
+    for (int t = 0; t < NT; ++t) m[t][0] = m[t][1] = -INFINITY, l[t][0] = l[t][1] = 0.f;
+
+    for (int64_t i = 0; i < take; ++i) {
+      __syncwarp();  // the stage that is filled next has been read by all
+      issue(i + kStages - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      __syncwarp();
+      const uint8_t* const stage = ring + (i % kStages) * L::stage;
+      const float* const kappa = reinterpret_cast<const float*>(stage + 2 * L::codes);
+      const float* const nu = kappa + L::scales * kTile;
+      const uint32_t valid = *reinterpret_cast<const uint32_t*>(nu + L::scales * kTile);
+
+      // scores of 32 positions (rows g and g + 8 of two products) x NT * 8 rows
+      float sc[2][NT][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) sc[h][t][k] = 0.f;
+      float acc[GEN ? 2 : 1][GEN ? NT : 1][4];
+      if constexpr (GEN) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[h][t][k] = 0.f;
+      }
+#pragma unroll
+      for (uint32_t b = 0; b < HB; ++b) {
+        uint4 qb[NT], ql[GEN ? NT : 1];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if constexpr (NT == 1 && !GEN) qb[t] = qf[b];
+          else qb[t] = *reinterpret_cast<const uint4*>(sq + (8 * t + g) * L::q_row + b * 64 + c * 16);
+          if constexpr (GEN) ql[t] = *reinterpret_cast<const uint4*>(sq + (RB + 8 * t + g) * L::q_row + b * 64 + c * 16);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint2 w0 = *reinterpret_cast<const uint2*>(stage + place<DT>(16 * h + g, 2 * b + (c >> 1)) + (c & 1) * 8);
+          const uint2 w1 = *reinterpret_cast<const uint2*>(stage + place<DT>(16 * h + g + 8, 2 * b + (c >> 1)) + (c & 1) * 8);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t x0 = raw<F>(k ? w0.y : w0.x), x1 = raw<F>(k ? w1.y : w1.x);
+            const uint32_t a0 = pair_low<F>(x0), a1 = pair_low<F>(x1), a2 = pair_high<F>(x0), a3 = pair_high<F>(x1);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              if constexpr (GEN) {
+                mma(acc[h][t], a0, a1, a2, a3, k ? qb[t].z : qb[t].x, k ? qb[t].w : qb[t].y);
+                if (a.split_q) mma(acc[h][t], a0, a1, a2, a3, k ? ql[t].z : ql[t].x, k ? ql[t].w : ql[t].y);
+              } else {
+                mma(sc[h][t], a0, a1, a2, a3, k ? qb[t].z : qb[t].x, k ? qb[t].w : qb[t].y);
+              }
+            }
+          }
+        }
+        if constexpr (GEN) {
+          if ((b + 1) * 32 % a.group == 0 || b + 1 == HB) {
+            const uint32_t gr = min(b * 32 / a.group, a.groups - 1);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float k0 = kappa[gr * kTile + 16 * h + g], k1 = kappa[gr * kTile + 16 * h + g + 8];
+#pragma unroll
+              for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  sc[h][t][k] = fmaf(acc[h][t][k], k < 2 ? k0 : k1, sc[h][t][k]);
+                  acc[h][t][k] = 0.f;
+                }
+            }
+          }
+        }
+      }
+      const int64_t j0 = begin + i * kUnit;
+      const bool plain = valid == ~0u && j0 >= all_lo && j0 + kTile <= all_hi;
+      bool higher = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float k0 = GEN ? 1.f : kappa[16 * h + g], k1 = GEN ? 1.f : kappa[16 * h + g + 8];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) sc[h][t][k] *= scale[t][k & 1] * (k < 2 ? k0 : k1);
+      }
+      if (!plain) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int64_t lo = row_lo[8 * t + 2 * c + k] - j0, hi = row_hi[8 * t + 2 * c + k] - j0;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+              const int at = g + 8 * p;
+              if (!(at >= lo && at < hi && (valid >> at & 1))) sc[p >> 1][t][(p & 1) * 2 + k] = -INFINITY;
+            }
+          }
+      }
+      float top[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          top[t][k] = fmaxf(fmaxf(sc[0][t][k], sc[0][t][k + 2]), fmaxf(sc[1][t][k], sc[1][t][k + 2]));
+          higher |= top[t][k] > m[t][k] + (float)kSlack;  // (from nothing: -inf)
+        }
+      if (__any_sync(~0u, higher)) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float x = fmaxf(top[t][k], m[t][k]);
+            for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
+            const float f = x == m[t][k] ? 1.f : ex2(m[t][k] - x);
+            l[t][k] *= f;
+            m[t][k] = x;
+#pragma unroll
+            for (uint32_t d = 0; d < MT; ++d) o[d][t][k] *= f, o[d][t][k + 2] *= f;
+          }
+      }
+      // the scales of V relative to a power of two, which is raised when they pass it by 2^kSlackV
+      float most = nu[lane];
+      if constexpr (GEN)
+        for (uint32_t gr = 1; gr < a.groups; ++gr) most = fmaxf(most, nu[gr * kTile + lane]);
+      most = warp_max(most);
+      if (most > (float)(1 << kSlackV) * unit_v) {
+        const float up = fmaxf(__uint_as_float(min((__float_as_uint(most) & 0x7f800000u) + 0x00800000u, 0x7e800000u)), kSmallestUnit);
+        const float f = unit_v / up;
+#pragma unroll
+        for (uint32_t d = 0; d < MT; ++d)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[d][t][k] *= f;
+        unit_v = up;
+      }
+      // 2^kUp / unit_v
+      const float per_v = unit_v > 0.f ? __uint_as_float(0x7f000000u + (kUp << 23) - __float_as_uint(unit_v)) : 0.f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float from = m[t][k] == -INFINITY ? 0.f : m[t][k];
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            float& x = sc[p >> 1][t][(p & 1) * 2 + k];
+            x = ex2(x - from);
+            l[t][k] += x;
+          }
+        }
+      uint32_t bf[2][NT][2], bl[GEN ? 2 : 1][GEN ? NT : 1][2];
+      auto weights = [&](uint32_t gr) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const float w = nu[gr * kTile + 16 * h + 8 * q + g] * per_v;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              // (a weight of 0 stays 0 whatever the scale is)
+              const float x0 = sc[h][t][2 * q], x1 = sc[h][t][2 * q + 1];
+              const float y0 = x0 == 0.f ? 0.f : x0 * w, y1 = x1 == 0.f ? 0.f : x1 * w;
+              const uint32_t hi = pack(y0, y1);
+              bf[h][t][q] = transposed(hi);
+              if constexpr (GEN) {
+                const float2 r = unpack(hi);
+                bl[h][t][q] = transposed(pack(y0 - r.x, y1 - r.y));
+              }
+            }
+          }
+      };
+      if constexpr (!GEN) weights(0);
+      const uint8_t* const vs = stage + L::codes;
+      if constexpr (!GEN) {
+        // a lane's elements: 16 neighbours (8 of heads of 64) of each 128, those of a step two of them
+        constexpr uint32_t HALVES = DT == 256 ? 2 : 1, W = DT == 64 ? 2 : 4;
+#pragma unroll
+        for (uint32_t half = 0; half < HALVES; ++half)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t w[4][W];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+              const uint32_t r = 16 * h + 2 * c + (p & 1) + (p >> 1) * 8;
+              if constexpr (DT == 64) {
+                const uint2 x = *reinterpret_cast<const uint2*>(vs + place<DT>(r, g >> 1) + (g & 1) * 8);
+                w[p][0] = raw<F>(x.x), w[p][1] = raw<F>(x.y);
+              } else {
+                const uint4 x = *reinterpret_cast<const uint4*>(vs + place<DT>(r, half * 8 + g));
+                w[p][0] = raw<F>(x.x), w[p][1] = raw<F>(x.y), w[p][2] = raw<F>(x.z), w[p][3] = raw<F>(x.w);
+              }
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < W; ++k)
+#pragma unroll
+              for (uint32_t e = 0; e < 2; ++e) {
+                const uint32_t x = __byte_perm(w[0][k], w[1][k], e ? 0x7362 : 0x5140);
+                const uint32_t y = __byte_perm(w[2][k], w[3][k], e ? 0x7362 : 0x5140);
+                const uint32_t a0 = pair_low<F>(x), a1 = pair_high<F>(x), a2 = pair_low<F>(y), a3 = pair_high<F>(y);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) mma(o[half * 8 + 2 * k + e][t], a0, a1, a2, a3, bf[h][t][0], bf[h][t][1]);
+              }
+          }
+      } else {
+        // four neighbours of each 32
+#pragma unroll
+        for (uint32_t b = 0; b < HB; ++b) {
+          if (b * 32 % a.group == 0) weights(min(b * 32 / a.group, a.groups - 1));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t w[4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+              const uint32_t r = 16 * h + 2 * c + (p & 1) + (p >> 1) * 8;
+              w[p] = raw<F>(*reinterpret_cast<const uint32_t*>(vs + place<DT>(r, 2 * b + (g >> 2)) + (g & 3) * 4));
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 2; ++e) {
+              const uint32_t x = __byte_perm(w[0], w[1], e ? 0x7362 : 0x5140);
+              const uint32_t y = __byte_perm(w[2], w[3], e ? 0x7362 : 0x5140);
+              const uint32_t a0 = pair_low<F>(x), a1 = pair_high<F>(x), a2 = pair_low<F>(y), a3 = pair_high<F>(y);
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                mma(o[2 * b + e][t], a0, a1, a2, a3, bf[h][t][0], bf[h][t][1]);
+                if (a.split_p) mma(o[2 * b + e][t], a0, a1, a2, a3, bl[h][t][0], bl[h][t][1]);
+              }
+            }
+          }
+        }
+      }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+
+    // ---- the warps' results joined
+    float* const part = reinterpret_cast<float*>(ring);  // (row, element) of this warp
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float x = l[t][k];
+        for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(~0u, x, d);
+        const uint32_t r = 8 * t + 2 * c + k;
+        if (g == 0) part_m[warp][r] = m[t][k], part_l[warp][r] = x;
+#pragma unroll
+        for (uint32_t d = 0; d < MT; ++d) {
+          const uint32_t e = GEN ? (d >> 1) * 32 + g * 4 + (d & 1) * 2
+                                 : DT == 64 ? g * 8 + d * 2 : (d >> 3) * 128 + g * 16 + (d & 7) * 2;
+          part[r * DT + e] = o[d][t][k];
+          part[r * DT + e + 1] = o[d][t][k + 2];
+        }
+      }
+    if (lane == 0) part_e[warp] = unit_v > 0.f ? unit_v * (1.f / (1 << kUp)) : 1.f;
+    __syncthreads();
+    const bool whole = it.from == 0 && take == it.units;
+    float* const slot = a.partial + ((size_t)blockIdx.x * 2 + (it.from == 0)) * RB * (a.head + 2);
+    for (uint32_t r = warp; r < row_count; r += kWarps) {
+      float top = part_m[0][r];
+#pragma unroll
+      for (uint32_t w = 1; w < kWarps; ++w) top = fmaxf(top, part_m[w][r]);
+      float f[kWarps], sum = 0.f;
+#pragma unroll
+      for (uint32_t w = 0; w < kWarps; ++w) {
+        f[w] = part_m[w][r] == -INFINITY ? 0.f : ex2(part_m[w][r] - top);
+        sum += f[w] * part_l[w][r];
+        f[w] *= part_e[w];
+      }
+      const uint32_t query = a.each_div.div(row0 + r), h = it.head * a.each + row0 + r - query * a.each;
+      const int64_t t = s.first + query;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      for (uint32_t e = lane; e < a.head; e += 32) {
+        float x = 0.f;
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; ++w)
+          if (f[w] != 0.f) x += f[w] * reinterpret_cast<const float*>(smem + w * L::ring)[r * DT + e];
+        if (whole) store_real(a.out, a.type, t * a.ot + h * a.oh + e, x * inv);
+        else slot[r * (a.head + 2) + e] = x;
+      }
+      if (lane == 0) {
+        if (!whole) {
+          slot[r * (a.head + 2) + a.head] = top;
+          slot[r * (a.head + 2) + a.head + 1] = sum;
+        } else if (a.lse) {
+          a.lse[t * a.lt + h * a.lh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718056f;
+        }
+      }
+    }
+    if (it.from == 0 && !whole) {
+      // the CTAs behind this one go on with it, a share each
+      const int64_t rest = it.units - take;
+      goes_on = make_int4((int)it.seq, (int)it.head, (int)it.block, (int)((rest + per - 1) / per));
+    }
+    __syncthreads();
+    todo -= take;
+    unit += take;
+  }
+  if (tid == 0 && a.split) a.split[blockIdx.x] = goes_on;
+}
+
+// Joins the parts of split items, in the order of the CTAs that made them.
+template <uint32_t RB>
+__global__ void __launch_bounds__(kThreads) gpuos_attend_join_kernel(const __grid_constant__ Args a) {
+  const int4 it = a.split[blockIdx.x];
+  if (it.w == 0) return;
+  const Sequence s = sequence(a, (uint32_t)it.x);
+  const uint32_t row0 = (uint32_t)it.z * RB;
+  const uint32_t rows = (uint32_t)min((int64_t)RB, s.n * a.each - row0);
+  const uint32_t stride = a.head + 2;
+  for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    auto part = [&](int i) { return a.partial + (((size_t)blockIdx.x + i) * 2 + (i == 0)) * RB * stride + r * stride; };
+    float top = -INFINITY;
+    for (int i = 0; i <= it.w; ++i) top = fmaxf(top, part(i)[a.head]);
+    const uint32_t query = a.each_div.div(row0 + r), h = it.y * a.each + row0 + r - query * a.each;
+    const int64_t t = s.first + query;
+    float sum = 0.f;
+    for (int i = 0; i <= it.w; ++i) {
+      const float m = part(i)[a.head];
+      if (m != -INFINITY) sum += ex2(m - top) * part(i)[a.head + 1];
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    for (uint32_t e = threadIdx.x; e < a.head; e += kThreads) {
+      float x = 0.f;
+      for (int i = 0; i <= it.w; ++i) {
+        const float m = part(i)[a.head];
+        if (m != -INFINITY) x += ex2(m - top) * part(i)[e];
+      }
+      store_real(a.out, a.type, t * a.ot + h * a.oh + e, x * inv);
+    }
+    if (a.lse && threadIdx.x == 0) a.lse[t * a.lt + h * a.lh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718056f;
+  }
+}
+
+template <int F, int DT, int NT, bool GEN>
+void start(const Args& a, cudaStream_t stream) {
+  using L = Layout<DT, NT, GEN>;
+  void (*const kernel)(const Args) = gpuos_attend_kernel<F, DT, NT, GEN>;
+  cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::total), "shared memory");
+  run(kernel, dim3(a.grid), kThreads, L::total, stream, a);
+  if (a.split) run(gpuos_attend_join_kernel<L::rows>, dim3(a.grid, 8), kThreads, 0, stream, a);
+}
+
+template <int F, int DT>
+void start(const Plan& p, const Args& a, cudaStream_t stream) {
+  if (p.general) start<F, DT, 2, true>(a, stream);
+  else if (p.tiles == 1) start<F, DT, 1, false>(a, stream);
+  else start<F, DT, DT == 256 ? 2 : 4, false>(a, stream);
+}
+
+}  // namespace
+
+template <int F>
+void launch(const Plan& p, const Args& a, cudaStream_t stream) {
+  if (p.padded == 64) start<F, 64>(p, a, stream);
+  else if (p.padded == 128) start<F, 128>(p, a, stream);
+  else start<F, 256>(p, a, stream);
+}
+
+}  // namespace attend
+}  // namespace rowops
+}  // namespace gpuos

@@ -1,0 +1,169 @@
+// What the attention's kernels share: the parameter block, and how the work of a
+// call is cut into units, items and the CTAs' shares of them.
+#pragma once
+#include "rowops.cuh"
+
+namespace gpuos {
+namespace rowops {
+namespace attend {
+
+constexpr uint32_t kUnit = 128;      // positions a CTA takes at once, 32 a warp
+constexpr uint32_t kWarps = 4, kThreads = 32 * kWarps;
+constexpr uint32_t kLeast = 4;       // units of a CTA, at least
+constexpr uint32_t kWhole = 8;       // units up to which an item is not split
+constexpr uint32_t kMaxHead = 256;
+
+// A slice of the cache.
+struct Held {
+  const uint8_t* codes;
+  const float* scales;
+  int64_t cp, cr, ch;      // strides of page, row, head (bytes)
+  int64_t sp, sr, sh, sg;  // of the scales (elements)
+};
+
+struct Args {
+  const void* q;
+  int64_t qt, qh;          // strides of token and head
+  void* out;
+  int64_t ot, oh;
+  float* lse;              // may be NULL
+  int64_t lt, lh;
+  Held k, v;
+  const void* pages;
+  int64_t ps, pp;
+  const void* lengths;
+  int64_t ls;
+  const void* offsets;     // may be NULL: one query a sequence
+  int64_t os;
+  float* partial;          // of split items: 2 slots a CTA, each rows x (head + 2)
+  int4* split;             // of each CTA: the item it begins and does not end, w: CTAs that go on with it; NULL: none can be
+  int64_t pool;            // pages of the cache
+  int64_t capacity;        // positions a row of the table has
+  uint32_t tokens, sequences;
+  uint32_t k_heads, each;  // query heads of a key head
+  uint32_t head, groups;   // elements; scales of a head
+  uint32_t group;          // elements of a scale
+  uint32_t grid;           // CTAs over which the work is spread
+  uint32_t few;            // 0, or: sequences of more rows than this are another kernel's
+  int64_t window;          // 0: none
+  float scale2;            // scale * log2(e)
+  FastDiv page, each_div;
+  int causal, type;        // type: of q and out
+  int page_wide, length_wide, offset_wide;
+  int vec;                 // bytes of codes loaded at once: 16, 4 or 1
+  int split_q, split_p;    // 16-bit parts of q and p: one, or two
+};
+
+// The queries of a sequence and what is cached of it.
+struct Sequence {
+  int64_t first;   // token
+  int64_t n;       // queries
+  int64_t length;
+};
+
+__device__ __forceinline__ Sequence sequence(const Args& a, uint32_t s) {
+  Sequence q;
+  if (a.offsets) {
+    const int64_t lo = load_index(a.offsets, a.offset_wide, s * a.os), hi = load_index(a.offsets, a.offset_wide, (s + 1) * a.os);
+    q.first = min(max(lo, (int64_t)0), (int64_t)a.tokens);
+    q.n = max(min(hi, (int64_t)a.tokens) - q.first, (int64_t)0);
+  } else {
+    q.first = s;
+    q.n = 1;
+  }
+  const int64_t len = load_index(a.lengths, a.length_wide, s * a.ls);
+  q.length = min(max(len, (int64_t)0), a.capacity);
+  return q;
+}
+
+// The positions that queries [qa, qb] of a sequence see between them.
+struct Range {
+  int64_t lo, hi;
+};
+
+__device__ __forceinline__ int64_t last_seen(const Args& a, const Sequence& s, int64_t query) {
+  return a.causal ? s.length - s.n + query : s.length - 1;
+}
+__device__ __forceinline__ int64_t first_seen(const Args& a, int64_t last) {
+  return a.window ? max(last - a.window + 1, (int64_t)0) : 0;
+}
+__device__ __forceinline__ Range seen(const Args& a, const Sequence& s, int64_t qa, int64_t qb) {
+  Range r;
+  r.hi = max(last_seen(a, s, qb) + 1, (int64_t)0);
+  r.lo = min(first_seen(a, last_seen(a, s, qa)), r.hi);
+  return r;
+}
+
+// ---- e4m3 and int8 codes as 16-bit numbers, exactly ---------------------------------
+enum Format { kInt8, kE4M3 };
+
+// The two codes in the low (high) half of x.  The NaN code of e4m3 counts as 0.
+template <int F>
+__device__ __forceinline__ uint32_t pair_low(uint32_t x) {
+  if constexpr (F == kInt8) {  // x holds code ^ 0x80; 0x6400 + u is 1024 + u
+    const uint32_t w = __byte_perm(x, 0x64646464u, 0x4140);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&w), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    uint32_t r;
+    asm("{ .reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, l; }" : "=r"(r) : "r"(x));
+    return r & __heq2_mask(*reinterpret_cast<const __half2*>(&r), *reinterpret_cast<const __half2*>(&r));
+  }
+}
+template <int F>
+__device__ __forceinline__ uint32_t pair_high(uint32_t x) {
+  if constexpr (F == kInt8) {
+    const uint32_t w = __byte_perm(x, 0x64646464u, 0x4342);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&w), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    uint32_t r;
+    asm("{ .reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, h; }" : "=r"(r) : "r"(x));
+    return r & __heq2_mask(*reinterpret_cast<const __half2*>(&r), *reinterpret_cast<const __half2*>(&r));
+  }
+}
+template <int F>
+__device__ __forceinline__ uint32_t raw(uint32_t codes) { return F == kInt8 ? codes ^ 0x80808080u : codes; }
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+__device__ __forceinline__ float load_real(const void* p, int type, int64_t i) {
+  if (type == GPUOS_F32) return __ldg(static_cast<const float*>(p) + i);
+  if (type == GPUOS_F16) return to_f(static_cast<const __half*>(p)[i]);
+  return to_f(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void store_real(void* p, int type, int64_t i, float v) {
+  if (type == GPUOS_F32) static_cast<float*>(p)[i] = v;
+  else if (type == GPUOS_F16) static_cast<__half*>(p)[i] = from_f<__half>(v);
+  else static_cast<__nv_bfloat16*>(p)[i] = from_f<__nv_bfloat16>(v);
+}
+
+// Launches of one format (attend_int8.cu, attend_e4m3.cu).  `rows`: of a block.
+struct Plan {
+  uint32_t tiles;   // of 8 rows
+  bool general;     // scales of a part of the head, or numbers in two parts
+  uint32_t padded;  // head, as the kernel holds it
+  uint32_t per_sm;  // CTAs
+};
+inline Plan plan(uint32_t head, uint32_t groups, bool split, int64_t rows) {
+  Plan p;
+  p.padded = head <= 64 ? 64 : head <= 128 ? 128 : 256;
+  p.general = groups > 1 || split;
+  p.tiles = p.general ? 2 : rows <= 8 ? 1 : p.padded == 256 ? 2 : 4;
+  p.per_sm = p.padded == 256 ? 1 : 2;
+  return p;
+}
+template <int F> void launch(const Plan& p, const Args& a, cudaStream_t stream);
+
+}  // namespace attend
+}  // namespace rowops
+}  // namespace gpuos

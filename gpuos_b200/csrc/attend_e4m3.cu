@@ -1,0 +1,4 @@
+// gpuos_attend's kernels for a cache of e4m3 codes.
+#include "attend.cuh"
+
+template void gpuos::rowops::attend::launch<gpuos::rowops::attend::kE4M3>(const Plan&, const Args&, cudaStream_t);

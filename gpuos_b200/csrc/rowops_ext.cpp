@@ -1,4 +1,5 @@
-// The row operators (gpuos_rotary, gpuos_cache_*, gpuos_route*, gpuos_logprobs*)
+// The row operators (gpuos_rotary, gpuos_cache_*, gpuos_attend, gpuos_route*, gpuos_order, gpuos_dispatch, gpuos_combine*,
+// gpuos_logprobs*, gpuos_verify)
 // in the Python module `gpuos_ext`: tensors in, new or given tensors out, on
 // torch's current stream of the tensors' device.  gpuos_b200/rowops.py is what
 // callers use; it adds gradients and the order after a scheduler's requests.
@@ -14,6 +15,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <cmath>
 #include <string>
 
 #include "../../include/gpuos_b200.h"
@@ -326,6 +329,47 @@ PyObject* cache_read(PyObject* const* a, Py_ssize_t n) {
   return cs.tuple ? tuple_of(out, cs.n) : wrap(out[0]);
 }
 
+PyObject* attend(PyObject* const* a, Py_ssize_t n) {
+  arity(n, 12, "(q, codes, scales, pages, lengths, offsets, longest, causal, window, scale, lse, out)");
+  not_traced();
+  const at::Tensor& x = tensor(a[0], "q");
+  if (recorded(x)) throw Raise{PyExc_ValueError, "q takes no gradient here: detach it"};
+  const Pair cs(a[1], "codes"), ss(a[2], "scales");
+  if (cs.n != 2 || ss.n != 2) throw Raise{PyExc_ValueError, "codes and scales must have a tensor each for keys and for values"};
+  const Place at(x);
+  const gpuos_tensor q = at.in(x, "q");
+  gpuos_tensor c[2], s[2], offsets;
+  for (int i = 0; i < 2; ++i) {
+    c[i] = at.in(cs.o[i], "codes");
+    s[i] = at.in(ss.o[i], "scales");
+  }
+  const gpuos_tensor pages = at.in(a[3], "pages"), lengths = at.in(a[4], "lengths");
+  const bool ragged = a[5] != Py_None;
+  if (ragged) offsets = at.in(a[5], "offsets");
+  if (x.dim() != 3) throw Raise{PyExc_ValueError, "q must have 3 dims, not " + std::to_string(x.dim())};
+  const int64_t longest = a[6] != Py_None ? (int64_t)integer(a[6]) : ragged ? std::max<int64_t>(x.size(0), 1) : 1;
+  const int64_t window = a[8] != Py_None ? (int64_t)integer(a[8]) : 0;
+  if (a[8] != Py_None && window < 1) throw Raise{PyExc_ValueError, "window must be at least 1"};
+  const double scale = a[9] != Py_None ? real(a[9]) : 1.0 / std::sqrt((double)std::max<int64_t>(x.size(2), 1));
+  const at::Tensor out = a[11] != Py_None ? given_out(a[11]) : at.make(x.sizes(), x.scalar_type());
+  const gpuos_tensor o = at.in(out, "out");
+  at::Tensor lse, work;
+  gpuos_tensor l;
+  if (truth(a[10])) {
+    lse = at.make({x.size(0), x.size(1)}, at::kFloat);
+    l = at.in(lse, "lse");
+  }
+  const int64_t bytes = gpuos_attend_workspace(&q, &c[0], &s[0], &pages, std::min(longest, std::max<int64_t>(x.size(0), 1)));
+  if (bytes) work = at.make({bytes}, at::kByte);
+  done(gpuos_attend(&q, c, s, &pages, &lengths, ragged ? &offsets : nullptr, &o, lse.defined() ? &l : nullptr,
+                    bytes ? const_cast<void*>(work.const_data_ptr()) : nullptr, bytes, longest, window, (float)scale,
+                    truth(a[7]) ? GPUOS_ATTEND_CAUSAL : 0, at.stream()));
+  if (a[11] != Py_None) written(out);
+  if (!lse.defined()) return wrap(out);
+  const at::Tensor both[2] = {out, lse};
+  return tuple_of(both, 2);
+}
+
 PyObject* route(PyObject* const* a, Py_ssize_t n) {
   arity(n, 9, "(logits, bias, top_k, score, groups, top_groups, group_score, renormalize, scale)");
   const at::Tensor& x = tensor(a[0], "logits");
@@ -401,6 +445,111 @@ PyObject* logprobs_grad(PyObject* const* a, Py_ssize_t n) {
   return wrap(out);
 }
 
+// The order of a token's choices: (places, sources, ...) as a tuple.
+struct Given {
+  const at::Tensor *places, *sources;
+  gpuos_tensor p, s;
+  Given(const Place& at, PyObject* o) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) throw Raise{PyExc_TypeError, "order must be what rowops.order returned"};
+    places = &tensor(PyTuple_GET_ITEM(o, 0), "places");
+    sources = &tensor(PyTuple_GET_ITEM(o, 1), "sources");
+    p = at.in(*places, "places");
+    s = at.in(*sources, "sources");
+    if (places->dim() != 2 || sources->dim() != 1)
+      throw Raise{PyExc_ValueError, "order: places must be (token, choice) and sources have one dim"};
+  }
+};
+
+void two_dims(const at::Tensor& t, const char* name) {
+  if (t.dim() != 2) throw Raise{PyExc_ValueError, std::string(name) + " must have 2 dims, not " + std::to_string(t.dim())};
+}
+
+PyObject* order(PyObject* const* a, Py_ssize_t n) {
+  arity(n, 3, "(experts, count, align)");
+  not_traced();
+  const at::Tensor& x = tensor(a[0], "experts");
+  const Place at(x);
+  const gpuos_tensor d = at.in(x, "experts");
+  two_dims(x, "experts");
+  const int32_t count = small(a[1], "count"), align = small(a[2], "align");
+  if (count < 1 || count > 1024) throw Raise{PyExc_ValueError, "count must be in [1, 1024]"};
+  const int64_t rows = gpuos_order_rows(x.numel(), count, align);
+  if (rows < 0) throw Raise{PyExc_ValueError, "align must be in [1, 65536]"};
+  const at::Tensor out[4] = {at.make(x.sizes(), at::kInt), at.make({rows}, at::kInt), at.make({count + 1}, at::kInt),
+                             at.make({count}, at::kInt)};
+  const gpuos_tensor o[4] = {at.in(out[0], "places"), at.in(out[1], "sources"), at.in(out[2], "offsets"), at.in(out[3], "counts")};
+  done(gpuos_order(&d, align, &o[0], &o[1], &o[2], &o[3], at.stream()));
+  return tuple_of(out, 4);
+}
+
+PyObject* dispatch(PyObject* const* a, Py_ssize_t n) {
+  arity(n, 2, "(x, order)");
+  const at::Tensor& x = tensor(a[0], "x");
+  if (recorded(x) || traced()) return not_here();
+  const Place at(x);
+  const Given by(at, a[1]);
+  const gpuos_tensor d = at.in(x, "x");
+  two_dims(x, "x");
+  const at::Tensor out = at.make({by.sources->size(0), x.size(1)}, x.scalar_type());
+  const gpuos_tensor o = at.in(out, "rows");
+  done(gpuos_dispatch(&d, &by.p, &by.s, &o, at.stream()));
+  return wrap(out);
+}
+
+PyObject* combine(PyObject* const* a, Py_ssize_t n) {
+  arity(n, 3, "(y, order, weights)");
+  const at::Tensor& y = tensor(a[0], "y");
+  if (recorded(y) || traced() || (a[2] != Py_None && recorded(tensor(a[2], "weights")))) return not_here();
+  const Place at(y);
+  const Given by(at, a[1]);
+  const gpuos_tensor d = at.in(y, "y");
+  two_dims(y, "y");
+  gpuos_tensor w;
+  if (a[2] != Py_None) w = at.in(a[2], "weights");
+  const at::Tensor out = at.make({by.places->size(0), y.size(1)}, y.scalar_type());
+  const gpuos_tensor o = at.in(out, "out");
+  done(gpuos_combine(&d, &by.p, &by.s, a[2] != Py_None ? &w : nullptr, &o, at.stream()));
+  return wrap(out);
+}
+
+PyObject* combine_grad(PyObject* const* a, Py_ssize_t n) {
+  arity(n, 6, "(grad, y, order, weights, want_y, want_weights)");
+  not_traced();
+  const at::Tensor& g = tensor(a[0], "grad");
+  const Place at(g);
+  const Given by(at, a[2]);
+  const gpuos_tensor d = at.in(g, "grad"), w = at.in(a[3], "weights");
+  two_dims(g, "grad");
+  const bool want[2] = {truth(a[4]), truth(a[5])};
+  gpuos_tensor y, o[2];
+  if (a[1] != Py_None) y = at.in(a[1], "y");
+  at::Tensor out[2];
+  if (want[0]) out[0] = at.make({by.sources->size(0), g.size(1)}, g.scalar_type());
+  if (want[1]) out[1] = at.make(by.places->sizes(), at::kFloat);
+  for (int i = 0; i < 2; ++i)
+    if (want[i]) o[i] = at.in(out[i], i ? "grad_weights" : "grad_y");
+  done(gpuos_combine_grad(&d, a[1] != Py_None ? &y : nullptr, &by.p, &by.s, &w, want[0] ? &o[0] : nullptr,
+                          want[1] ? &o[1] : nullptr, at.stream()));
+  return tuple_of(out, 2);
+}
+
+PyObject* verify(PyObject* const* a, Py_ssize_t n) {
+  arity(n, 5, "(logits, drafts, uniforms, probs, temperature)");
+  not_traced();
+  const at::Tensor& x = tensor(a[0], "logits");
+  const Place at(x);
+  const gpuos_tensor d = at.in(x, "logits"), y = at.in(a[1], "drafts");
+  if (x.dim() != 3) throw Raise{PyExc_ValueError, "logits must have 3 dims, not " + std::to_string(x.dim())};
+  gpuos_tensor u, q;
+  if (a[2] != Py_None) u = at.in(a[2], "uniforms");
+  if (a[3] != Py_None) q = at.in(a[3], "probs");
+  const at::Tensor out[2] = {at.make({x.size(0), x.size(1)}, at::kLong), at.make({x.size(0)}, at::kLong)};
+  const gpuos_tensor o[2] = {at.in(out[0], "tokens"), at.in(out[1], "accepted")};
+  done(gpuos_verify(&d, &y, a[2] != Py_None ? &u : nullptr, a[3] != Py_None ? &q : nullptr, &o[0], &o[1], real(a[4]),
+                    at.stream()));
+  return tuple_of(out, 2);
+}
+
 }  // namespace
 
 #define GPUOS_FAST(f) (PyCFunction)(void (*)(void))guarded<f>, METH_FASTCALL
@@ -410,6 +559,8 @@ PyMethodDef* gpuos_rowops_methods() {
       {"rotary", GPUOS_FAST(rotary), "rotary(x, out, positions, inv_freq, scale, interleaved, inverse): see rowops.rotary"},
       {"cache_write", GPUOS_FAST(cache_write), "cache_write(x, slots, codes, scales): see rowops.cache_write"},
       {"cache_read", GPUOS_FAST(cache_read), "cache_read(slots, codes, scales, out, dtype): see rowops.cache_read"},
+      {"attend", GPUOS_FAST(attend),
+       "attend(q, codes, scales, pages, lengths, offsets, longest, causal, window, scale, lse, out): see rowops.attend"},
       {"route", GPUOS_FAST(route),
        "route(logits, bias, top_k, score, groups, top_groups, group_score, renormalize, scale): see rowops.route"},
       {"route_grad", GPUOS_FAST(route_grad),
@@ -418,6 +569,12 @@ PyMethodDef* gpuos_rowops_methods() {
       {"logprobs_grad", GPUOS_FAST(logprobs_grad),
        "logprobs_grad(logits, targets, stats, entropy, grad_logprob, grad_entropy, temperature, out): see "
        "rowops.logprobs_grad"},
+      {"order", GPUOS_FAST(order), "order(experts, count, align): see rowops.order"},
+      {"dispatch", GPUOS_FAST(dispatch), "dispatch(x, order): see rowops.dispatch"},
+      {"combine", GPUOS_FAST(combine), "combine(y, order, weights): see rowops.combine"},
+      {"combine_grad", GPUOS_FAST(combine_grad),
+       "combine_grad(grad, y, order, weights, want_y, want_weights): see rowops.combine_grad"},
+      {"verify", GPUOS_FAST(verify), "verify(logits, drafts, uniforms, probs, temperature): see rowops.verify"},
       {nullptr, nullptr, 0, nullptr}};
   return methods;
 }

@@ -1,0 +1,501 @@
+// gpuos_verify: drafted tokens d_0 .. d_(n-1) of a sequence checked against the
+// target's n + 1 rows of logits x from given random numbers u_0 .. u_n, and the
+// next token drawn.  With temperature t, m_i = max x_i,
+//
+//   w_ij = e^((x_ij - m_i) / t)      S_i = sum_j w_ij      p_ij = w_ij / S_i
+//
+// draft i is accepted where u_i q_i(d_i) S_i < w_i(d_i) (q: the draft's
+// probabilities; 1 at d_i where none are given).  At the first that is not, a, the
+// next token is drawn from r_j = max(w_aj - q_aj S_a, 0), or from w_a where
+// that leaves nothing; where all are accepted, from r = w_n: the lowest j with
+//
+//   sum_(i <= j) r_i  >  u_n sum_i r_i
+//
+// which gives tokens as the target alone would.  t = 0 takes the likeliest token instead.
+// Counts and tokens are those of 64-bit arithmetic.  A cluster takes a sequence, so
+// that nothing but its tokens leaves it:
+//   1. every row is read once for m_i and S_i in 32 bits, whose error is below 2^-15;
+//   2. a draft for which that could matter has S_i summed again in 64 bits;
+//   3. the one row that is drawn from is read again (from L2) and summed in 64 bits:
+//      an SM's 64-bit rate is half its 32-bit rate, and it is one row of a sequence.
+#include <cooperative_groups.h>
+
+#include "rowops.cuh"
+
+namespace gpuos {
+namespace rowops {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr uint32_t kThreads = 512, kWarps = kThreads / 32;
+constexpr uint32_t kCluster = 8;
+constexpr uint32_t kMaxDrafts = 63;
+constexpr uint32_t kMaxTokens = 1u << 24;  // of a row
+constexpr int kPack = 8;                   // elements a lane takes at once
+constexpr int kFlight = 4;                 // packs a lane has in flight
+constexpr float kLowest = -3.402823466e38f;
+
+struct VerifyArgs {
+  const void* x;
+  int64_t xs, xr;       // strides of sequence and row
+  const void* drafts;
+  int64_t ds, di;
+  const float* u;
+  int64_t us, ui;
+  const void* q;        // may be NULL
+  int64_t qs, qr;
+  int64_t* tokens;      // (sequence, n + 1)
+  int64_t* accepted;
+  uint32_t n, cols;
+  double inv_t;
+  float k2;             // log2(e) / t
+  int draft_wide, greedy, q_type;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// A row as packs of 8 elements that start on 16 bytes (of 16-bit elements; 32 of 32-bit ones): the first and the last
+// may lie partly outside the row.
+template <typename T>
+struct Row {
+  const T* x;
+  uint32_t cols, shift;  // elements of the first pack that are before the row
+  __device__ Row(const T* p, uint32_t n)
+      : x(p), cols(n), shift((uint32_t)(reinterpret_cast<uintptr_t>(p) % (kPack * sizeof(T)) / sizeof(T))) {}
+  __device__ uint32_t packs() const { return (cols + shift + kPack - 1) / kPack; }
+  // the 8 elements from `first()` of pack p on; -inf outside the row
+  __device__ int64_t first(uint32_t p) const { return (int64_t)p * kPack - shift; }
+  __device__ void load(uint32_t p, float (&v)[kPack]) const {
+    const int64_t e = first(p);
+    if (e >= 0 && e + kPack <= cols) {
+      constexpr int W = 16 / sizeof(T);
+#pragma unroll
+      for (int k = 0; k < kPack; k += W) {
+        const Pack<T, W> q = load_pack<T, W, false>(x + e + k);
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[k + i] = to_f(q.v[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPack; ++i) v[i] = e + i >= 0 && e + i < cols ? to_f(x[e + i]) : -INFINITY;
+    }
+  }
+};
+
+__device__ __forceinline__ float prob(const void* q, int type, int64_t i) {
+  if (type == GPUOS_F32) return __ldg(static_cast<const float*>(q) + i);
+  if (type == GPUOS_F16) return to_f(static_cast<const __half*>(q)[i]);
+  return to_f(static_cast<const __nv_bfloat16*>(q)[i]);
+}
+
+// An integer that orders as (x, lowest index first) does.
+__device__ __forceinline__ unsigned long long key_of(float x, uint32_t index) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  const uint32_t k = (b >> 31) ? ~b : b | 0x80000000u;
+  return ((unsigned long long)k << 32) | (uint32_t)~index;
+}
+
+// A row's maximum, and its sum in units of e^(maximum / t); greedy: the key of the likeliest token, and NaN where there is no such.
+struct Stat {
+  float m, s;
+  unsigned long long key;
+};
+
+__device__ __forceinline__ void join(Stat& a, const Stat& b, float k2) {
+  const float m = fmaxf(a.m, b.m);
+  a.s = a.s * ex2(fmaxf((a.m - m) * k2, -1e4f)) + b.s * ex2(fmaxf((b.m - m) * k2, -1e4f));
+  a.m = m;
+  a.key = max(a.key, b.key);
+}
+
+__device__ __forceinline__ Stat join_warp(Stat v, float k2) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    const Stat o{__shfl_xor_sync(~0u, v.m, d), __shfl_xor_sync(~0u, v.s, d), __shfl_xor_sync(~0u, v.key, d)};
+    join(v, o, k2);
+  }
+  return v;
+}
+
+// Sums over a warp, the same in all lanes.
+__device__ __forceinline__ double sum_warp(double v) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+  return v;
+}
+
+struct Shared {
+  Stat part[kMaxDrafts + 1][kWarps];
+  Stat mine[kMaxDrafts + 1];   // of this CTA, read by the others
+  Stat all[kMaxDrafts + 1];
+  double warp[kWarps];
+  double sum[2];               // of this CTA, read by the others (two, taken in turn)
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+gpuos_verify_kernel(const __grid_constant__ VerifyArgs a) {
+  __shared__ Shared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const uint32_t rank = cluster.block_rank(), parts = cluster.num_blocks();
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t seq = blockIdx.x / parts;
+  const T* x0 = static_cast<const T*>(a.x) + seq * a.xs;
+  const uint32_t rows = a.n + 1;
+
+  // the packs of a row that this warp takes, neighbours
+  auto share = [&](const Row<T>& r, uint32_t& lo, uint32_t& hi) {
+    const uint32_t packs = r.packs(), each = (packs + parts * kWarps - 1) / (parts * kWarps);
+    lo = min((rank * kWarps + warp) * each, packs);
+    hi = min(lo + each, packs);
+  };
+
+  // 1. maxima and sums of all rows
+  for (uint32_t i = 0; i < rows; ++i) {
+    const Row<T> row(x0 + i * a.xr, a.cols);
+    uint32_t lo, hi;
+    share(row, lo, hi);
+    Stat st{a.greedy ? -INFINITY : kLowest, 0.f, 0};
+    bool odd = false;  // greedy: NaN or +inf seen
+    for (uint32_t p = lo + lane; p < hi; p += 32 * kFlight) {
+      float v[kFlight][kPack];
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f) {
+        if (p + 32 * f < hi) {
+          row.load(p + 32 * f, v[f]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < kPack; ++c) v[f][c] = -INFINITY;
+        }
+      }
+      float m = st.m;
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f)
+#pragma unroll
+        for (int c = 0; c < kPack; ++c) m = fmaxf(m, v[f][c]);
+      if (a.greedy) {
+#pragma unroll
+        for (int f = 0; f < kFlight; ++f)
+#pragma unroll
+          for (int c = 0; c < kPack; ++c) {
+            odd |= !(v[f][c] < INFINITY);
+            if (v[f][c] == m && m > st.m)
+              st.key = max(st.key, key_of(m, (uint32_t)(row.first(p + 32 * f) + c)));
+          }
+        if (m > st.m) st.m = m;
+        continue;
+      }
+      if (m > st.m) {
+        st.s *= ex2(fmaxf((st.m - m) * a.k2, -1e4f));
+        st.m = m;
+      }
+      float2 sum = {0.f, 0.f};
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f)
+#pragma unroll
+        for (int c = 0; c < kPack; c += 2) {
+          const float2 y = mul2(add2(make_float2(v[f][c], v[f][c + 1]), both(-m)), both(a.k2));
+          sum = add2(sum, make_float2(ex2(y.x), ex2(y.y)));
+        }
+      st.s += sum.x + sum.y;
+    }
+    if (a.greedy) st.s = odd ? NAN : 0.f;
+    st = join_warp(st, a.greedy ? 0.f : a.k2);
+    if (lane == 0) sh.part[i][warp] = st;
+  }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < rows; i += kThreads) {
+    Stat st = sh.part[i][0];
+    for (uint32_t w = 1; w < kWarps; ++w) join(st, sh.part[i][w], a.greedy ? 0.f : a.k2);
+    sh.mine[i] = st;
+  }
+  cluster.sync();
+  for (uint32_t i = threadIdx.x; i < rows; i += kThreads) {
+    Stat st = *cluster.map_shared_rank(&sh.mine[i], 0);
+    for (uint32_t c = 1; c < parts; ++c) join(st, *cluster.map_shared_rank(&sh.mine[i], c), a.greedy ? 0.f : a.k2);
+    sh.all[i] = st;
+  }
+  __syncthreads();
+
+  // From here on all threads of the cluster take the same way.
+  uint32_t turn = 0;
+  // the sum over the cluster of what the warps have, and what lies before this warp
+  auto sum_all = [&](double v, double& before) {
+    if (lane == 0) sh.warp[warp] = v;
+    __syncthreads();
+    double mine = 0.0, ahead = 0.0;
+    for (uint32_t w = 0; w < kWarps; ++w) {
+      if (w == warp) ahead = mine;
+      mine += sh.warp[w];
+    }
+    if (threadIdx.x == 0) sh.sum[turn & 1] = mine;
+    cluster.sync();
+    double total = 0.0;
+    before = 0.0;
+    for (uint32_t c = 0; c < parts; ++c) {
+      if (c == rank) before = total;
+      total += *cluster.map_shared_rank(&sh.sum[turn & 1], c);
+    }
+    // a warp's range ends exactly where the next one's begins
+    before += ahead;
+    ++turn;
+    __syncthreads();
+    return total;
+  };
+  auto weight = [&](float v, float m) { return exp(((double)v - m) * a.inv_t); };
+  auto whole_sum = [&](uint32_t i) {
+    const Row<T> row(x0 + i * a.xr, a.cols);
+    uint32_t lo, hi;
+    share(row, lo, hi);
+    const float m = sh.all[i].m;
+    double s = 0.0, unused;
+    for (uint32_t p = lo + lane; p < hi; p += 32) {
+      float v[kPack];
+      row.load(p, v);
+#pragma unroll
+      for (int c = 0; c < kPack; ++c) s += weight(v[c], m);
+    }
+    return sum_all(sum_warp(s), unused);
+  };
+  auto draft = [&](uint32_t i) { return load_index(a.drafts, a.draft_wide, seq * a.ds + i * a.di); };
+  auto valid = [&](uint32_t i) {
+    const Stat& st = sh.all[i];
+    return a.greedy ? st.s == 0.f && st.key != 0 : st.s > 0.f && st.s < INFINITY && st.m < INFINITY;
+  };
+
+  // 2. drafts from the first on, until one is refused or there is none
+  uint32_t at = 0;
+  bool refused = false;
+  for (; at < a.n; ++at) {
+    const int64_t d = draft(at);
+    if (d < 0 || d >= a.cols) break;  // the drafts end here
+    if (!valid(at)) {
+      refused = true;
+      break;
+    }
+    if (a.greedy) {
+      refused = d != (uint32_t)~(uint32_t)sh.all[at].key;
+    } else {
+      const double w = weight(to_f(x0[at * a.xr + d]), sh.all[at].m);
+      const double q = a.q ? (double)prob(a.q, a.q_type, seq * a.qs + at * a.qr + d) : 1.0;
+      const double uq = (double)__ldg(a.u + seq * a.us + at * a.ui) * q;
+      double bound = uq * sh.all[at].s;
+      // the sum's error: at most 16 + 128 additions in a thread, 29 joins of 6 roundings each (2^-24 is one), and of the
+      // exponents' arguments 1.8 roundings times the sum of w |log2 w| / S, at most log2 of the tokens: below 2^-15
+      if (fabs(bound - w) <= 0x1p-14 * w && w > 0.0) bound = uq * whole_sum(at);
+      refused = !(bound < w);
+    }
+    if (refused) break;
+  }
+
+  // 3. the next token
+  int64_t* out = a.tokens + seq * rows;
+  if (rank == 0) {
+    for (uint32_t i = threadIdx.x; i < rows; i += kThreads)
+      if (i != at || !valid(at) || a.greedy)
+        out[i] = i < at ? draft(i) : i == at && valid(at) ? (int64_t)(uint32_t)~(uint32_t)sh.all[at].key : -1;
+    if (threadIdx.x == 0) a.accepted[seq] = at;
+  }
+  if (a.greedy || !valid(at)) {
+    cluster.sync();  // no CTA leaves while another reads its `mine`
+    return;
+  }
+  const Row<T> row(x0 + at * a.xr, a.cols);
+  uint32_t lo, hi;
+  share(row, lo, hi);
+  const float m = sh.all[at].m;
+  const int64_t gone = refused && !a.q ? draft(at) : -1;   // the draft itself, where it had all
+  const double total_w = refused && a.q ? whole_sum(at) : 0.0;
+  bool less = refused;
+  auto weights = [&](uint32_t p, double (&r)[kPack]) {
+    float v[kPack];
+    row.load(p, v);
+    const int64_t e = row.first(p);
+#pragma unroll
+    for (int c = 0; c < kPack; ++c) {
+      r[c] = weight(v[c], m);
+      if (!less) continue;
+      if (!a.q) {
+        if (e + c == gone) r[c] = 0.0;
+      } else if (r[c] > 0.0) {
+        const double rest = r[c] - (double)prob(a.q, a.q_type, seq * a.qs + at * a.qr + e + c) * total_w;
+        r[c] = rest > 0.0 ? rest : 0.0;  // (a NaN leaves nothing)
+      }
+    }
+  };
+  double before, own, total;
+  for (;;) {
+    double s = 0.0;
+    for (uint32_t p = lo + lane; p < hi; p += 32) {
+      double r[kPack];
+      weights(p, r);
+#pragma unroll
+      for (int c = 0; c < kPack; ++c) s += r[c];
+    }
+    own = sum_warp(s);
+    total = sum_all(own, before);
+    if (total > 0.0 || !less) break;
+    less = false;
+  }
+  double u = (double)__ldg(a.u + seq * a.us + a.n * a.ui);
+  u = u > 0.0 ? u : 0.0;
+  double goal = u * total;
+  if (!(goal < total)) goal = __longlong_as_double(__double_as_longlong(total) - 1);
+  // the warp that the goal lies in: this one's end is the next one's beginning
+  __shared__ double starts[kWarps];
+  if (lane == 0) starts[warp] = before;
+  __syncthreads();
+  double end = total;
+  if (warp + 1 < kWarps) {
+    end = starts[warp + 1];
+  } else if (rank + 1 < parts) {
+    double sum = 0.0;
+    for (uint32_t c = 0; c <= rank; ++c) sum += *cluster.map_shared_rank(&sh.sum[(turn - 1) & 1], c);
+    end = sum;
+  }
+  if (before <= goal && goal < end) {
+    double run = before;
+    int64_t found = -1, last = -1;
+    for (uint32_t p0 = lo; p0 < hi && found < 0; p0 += 32) {
+      const uint32_t p = p0 + lane;
+      double r[kPack], s = 0.0;
+      const bool in = p < hi;
+      if (in) weights(p, r);
+#pragma unroll
+      for (int c = 0; c < kPack; ++c) {
+        if (!in) r[c] = 0.0;
+        s += r[c];
+      }
+      double sum = s;
+      for (uint32_t d = 1; d < 32; d <<= 1) {
+        const double o = __shfl_up_sync(~0u, sum, d);
+        if (lane >= d) sum += o;
+      }
+      // the first lane whose sum passes the goal; its elements one by one
+      const uint32_t past = __ballot_sync(~0u, run + sum > goal);
+      const uint32_t some = __ballot_sync(~0u, s > 0.0);
+      const uint32_t who = past ? __ffs(past) - 1 : 32 - __clz(some) - 1;
+      int64_t pick = -1, high = -1;
+      if (past || some) {
+        if (lane == who) {
+          double acc = run + (sum - s);
+          for (int c = 0; c < kPack; ++c) {
+            acc += r[c];
+            if (r[c] > 0.0) {
+              high = row.first(p) + c;
+              if (pick < 0 && acc > goal) pick = high;
+            }
+          }
+        }
+        high = __shfl_sync(~0u, high, who);
+        pick = __shfl_sync(~0u, pick, who);
+        if (high >= 0) last = high;
+        if (past) found = pick >= 0 ? pick : last;
+      }
+      run += __shfl_sync(~0u, sum, 31);
+    }
+    if (lane == 0) out[at] = found >= 0 ? found : last;
+  }
+  cluster.sync();  // no CTA leaves while another reads its sums
+}
+
+}  // namespace
+}  // namespace rowops
+}  // namespace gpuos
+
+using namespace gpuos::rowops;
+
+extern "C" int32_t gpuos_verify(const gpuos_tensor* logits, const gpuos_tensor* drafts, const gpuos_tensor* uniforms,
+                                const gpuos_tensor* probs, const gpuos_tensor* tokens, const gpuos_tensor* accepted,
+                                double temperature, void* stream) {
+  return entry("gpuos_verify", [&] {
+    check_tensor(logits, 3, "logits");
+    need(is_real(logits->dtype), "logits must be float32, float16 or bfloat16");
+    const int64_t b = logits->sizes[0], rows = logits->sizes[1], v = logits->sizes[2];
+    need(rows >= 1 && rows <= (int64_t)kMaxDrafts + 1, "logits must be (sequence, draft + 1, token) with at most 63 drafts");
+    need(v >= 1 && v < kMaxTokens, "logits must have between 1 and 2^24 - 1 tokens a row");
+    need(v == 1 || logits->strides[2] == 1, "logits: the last dim must be contiguous");
+    // (k2 stays a 32-bit number)
+    need(temperature == 0.0 || (temperature >= 1e-30 && temperature <= 1e30), "temperature must be 0, or in [1e-30, 1e30]");
+    check_tensor(drafts, 2, "drafts");
+    need(is_index(drafts->dtype), "drafts must be int32 or int64");
+    need(drafts->sizes[0] == b && drafts->sizes[1] == rows - 1, "drafts must be (sequence, draft), one less than logits has rows");
+    const bool greedy = temperature == 0.0;
+    if (!greedy) need(uniforms != nullptr, "uniforms are needed (but for temperature 0)");
+    if (uniforms) {
+      check_tensor(uniforms, 2, "uniforms");
+      need(uniforms->dtype == GPUOS_F32, "uniforms must be float32");
+      need(uniforms->sizes[0] == b && uniforms->sizes[1] == rows, "uniforms must be (sequence, draft + 1)");
+    }
+    if (probs) {
+      check_tensor(probs, 3, "probs");
+      need(is_real(probs->dtype), "probs must be float32, float16 or bfloat16");
+      need(probs->sizes[0] == b && probs->sizes[1] == rows - 1 && probs->sizes[2] == v, "probs must be (sequence, draft, token)");
+      need(v == 1 || probs->sizes[1] == 0 || probs->strides[2] == 1, "probs: the last dim must be contiguous");
+    }
+    check_tensor(tokens, 2, "tokens");
+    check_tensor(accepted, 1, "accepted");
+    need(tokens->dtype == GPUOS_I64 && accepted->dtype == GPUOS_I64, "tokens and accepted must be int64");
+    need(tokens->sizes[0] == b && tokens->sizes[1] == rows, "tokens must be (sequence, draft + 1)");
+    need(accepted->sizes[0] == b, "accepted must be [sequence]");
+    need((rows == 1 || tokens->strides[1] == 1) && (b <= 1 || tokens->strides[0] == rows), "tokens must be contiguous");
+    need(b <= 1 || accepted->strides[0] == 1, "accepted must be contiguous");
+    for (const gpuos_tensor* o : {tokens, accepted})
+      for (const gpuos_tensor* i : {logits, drafts, uniforms, probs})
+        if (i) no_overlap(*o, *i, "an output must not overlap an input");
+    no_overlap(*tokens, *accepted, "outputs overlap");
+    need(b < (1ll << 27), "too many sequences");
+    if (b == 0) return;
+    VerifyArgs a{};
+    a.x = logits->data;
+    a.xs = logits->strides[0];
+    a.xr = logits->strides[1];
+    a.drafts = drafts->data;
+    a.draft_wide = drafts->dtype == GPUOS_I64;
+    a.ds = drafts->strides[0];
+    a.di = drafts->strides[1];
+    if (!greedy) {
+      a.u = static_cast<const float*>(uniforms->data);
+      a.us = uniforms->strides[0];
+      a.ui = uniforms->strides[1];
+      a.inv_t = 1.0 / temperature;
+      a.k2 = (float)(1.44269504088896340736 / temperature);
+    }
+    if (probs && rows > 1 && !greedy) {
+      a.q = probs->data;
+      a.q_type = probs->dtype;
+      a.qs = probs->strides[0];
+      a.qr = probs->strides[1];
+    }
+    a.tokens = static_cast<int64_t*>(tokens->data);
+    a.accepted = static_cast<int64_t*>(accepted->data);
+    a.n = (uint32_t)rows - 1;
+    a.cols = (uint32_t)v;
+    a.greedy = greedy;
+    // CTAs of a sequence: each with a pack for every thread at least; of very many sequences fewer, but
+    // for rows so long that a thread's sums in 32 bits would lose their bound
+    uint32_t parts = 1;
+    while (parts < kCluster && (uint64_t)parts * kThreads * kPack < (uint64_t)v &&
+           ((uint64_t)b * parts < 8u * (uint32_t)sm_count() || v > (1 << 20)))
+      parts *= 2;
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3((uint32_t)b * parts);
+    c.blockDim = dim3(kThreads);
+    c.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {parts, 1, 1};
+    c.attrs = at;
+    c.numAttrs = 1;
+    const VerifyArgs args = a;
+    cuda_ok(logits->dtype == GPUOS_F32   ? cudaLaunchKernelEx(&c, gpuos_verify_kernel<float>, args)
+            : logits->dtype == GPUOS_F16 ? cudaLaunchKernelEx(&c, gpuos_verify_kernel<__half>, args)
+                                         : cudaLaunchKernelEx(&c, gpuos_verify_kernel<__nv_bfloat16>, args),
+            "launch");
+  });
+}

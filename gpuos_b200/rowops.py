@@ -203,6 +203,28 @@ def cache_read(slots: torch.Tensor, codes: Tensors, scales: Tensors, *, dtype: t
     return _ext.cache_read(slots, codes, scales, out, code)
 
 
+# ---- attention over the cache ----------------------------------------------------------
+def attend(q: torch.Tensor, codes: Tuple[torch.Tensor, torch.Tensor], scales: Tuple[torch.Tensor, torch.Tensor],
+           pages: torch.Tensor, lengths: torch.Tensor, *, offsets: Optional[torch.Tensor] = None,
+           longest: Optional[int] = None, causal: bool = True, window: Optional[int] = None,
+           scale: Optional[float] = None, lse: bool = False, out: Optional[torch.Tensor] = None) -> Tensors:
+    """Attention of queries (token, query head, element) over a cache of keys and values
+    (int8 or e4m3; `codes` and `scales` as from ``cache_alloc``, pairs).  ``pages`` (int32 or int64
+    (sequence, page)) says which pages of the cache hold a sequence's positions, `lengths` [sequence] how
+    many there are; a sequence's queries are the last of its positions: one each, or
+    with `offsets` [sequence + 1] tokens ``offsets[s]`` to ``offsets[s + 1]`` of `q`.  `causal`: a query sees
+    the positions up to its own, with `window` the last so many of them; otherwise all (an encoder's
+    states).  Query heads that are neighbours share a head of the cache.  `scale` is ``1 / sqrt(element)``
+    by default.  `longest` is the most queries a sequence has, if the caller knows (it chooses a
+    kernel and changes no result beyond rounding).  A page outside the cache (-1) is not seen; a query that sees nothing, and a
+    token of no sequence, get zeros.  With `lse`: also the log of the sum of e^score, float32
+    (token, query head).  The head size is a multiple of 16, at most 256, with a scale for the head or
+    for a multiple of 32 elements.  No gradient goes through it."""
+    if _entered:
+        _order((q, *codes, *scales, pages, lengths, offsets), (out,))
+    return _ext.attend(q, tuple(codes), tuple(scales), pages, lengths, offsets, longest, causal, window, scale, lse, out)
+
+
 # ---- routing -----------------------------------------------------------------------
 def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Optional[torch.Tensor] = None,
           groups: int = 1, top_groups: int = 1, group_score: str = "max", renormalize: bool = False,
@@ -247,6 +269,88 @@ class _Route(torch.autograd.Function):
         if _entered:
             _order((logits, experts, grad_weights))
         return _ext.route_grad(logits, experts, grad_weights, *ctx.how), None, None, None
+
+
+# ---- rows sorted by expert -------------------------------------------------------------
+class Order(NamedTuple):
+    places: torch.Tensor   # int32 (token, choice): the row of each choice, -1 where it has none
+    sources: torch.Tensor  # int32 [row]: token * choices + choice of each row, -1 where there is none
+    offsets: torch.Tensor  # int32 [expert + 1]: where each expert's rows begin, and behind the last one's
+    counts: torch.Tensor   # int32 [expert]: how many rows are of a choice
+
+
+def order(experts: torch.Tensor, count: int, *, align: int = 1) -> Order:
+    """Sort the choices of ``route`` (int32 or int64 (token, choice)) by expert, of which there
+    are `count`: an expert's rows are neighbours, in the order of their tokens, and
+    begin on a multiple of `align`.  A choice outside ``[0, count)`` (-1: masked, or an
+    expert of another device) has no row.  There are as many rows as any choice could
+    need (``token * choices`` where `align` is 1), so no size depends on the data."""
+    if _entered:
+        _order((experts,))
+    return Order._make(_ext.order(experts, count, align))
+
+
+def dispatch(x: torch.Tensor, order: Order) -> torch.Tensor:
+    """The rows of `x` (token, element) at the places of `order`: (row, element), zeros
+    in rows of no choice.  Its gradient is ``combine`` without weights."""
+    if _entered:
+        _order((x, *order[:2]))
+    got = _ext.dispatch(x, order)
+    return _Dispatch.apply(x, *order) if got is NotImplemented else got
+
+
+class _Dispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, *order):
+        ctx.save_for_backward(*order)
+        return _ext.dispatch(x, order)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        order = ctx.saved_tensors
+        if _entered:
+            _order((grad, *order[:2]))
+        return (_ext.combine(_row(grad), order, None),) + (None,) * 4
+
+
+def combine(y: torch.Tensor, order: Order, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Bring rows (row, element) back to their tokens: the sum over a token's choices of
+    ``weights`` (float32 (token, choice), as from ``route``; default: ones) times the choice's
+    row, in 32 bits; (token, element) in `y`'s dtype.  Choices without a row add nothing."""
+    if _entered:
+        _order((y, *order[:2], weights))
+    got = _ext.combine(y, order, weights)
+    return _Combine.apply(y, weights, *order) if got is NotImplemented else got
+
+
+def combine_grad(grad: torch.Tensor, y: torch.Tensor, order: Order,
+                 weights: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The gradients of ``combine``'s rows and weights from that of its result."""
+    if _entered:
+        _order((grad, y, *order[:2], weights))
+    return _ext.combine_grad(grad, y, order, weights, True, True)
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, *order):
+        # the rows are needed for the gradient of the weights only, and those for that of the rows
+        need_y, need_w = ctx.needs_input_grad[0], weights is not None and ctx.needs_input_grad[1]
+        ctx.save_for_backward(y if need_w else None, weights, *order)
+        ctx.need = need_y, need_w
+        return _ext.combine(y, order, weights)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        y, weights, *order = ctx.saved_tensors
+        order, grad = tuple(order), _row(grad)
+        if _entered:
+            _order((grad, y, weights, *order[:2]))
+        if weights is None:
+            return (_ext.dispatch(grad, order), None) + (None,) * 4
+        return _ext.combine_grad(grad, y, order, weights, *ctx.need) + (None,) * 4
 
 
 # ---- log probabilities ---------------------------------------------------------------
@@ -307,3 +411,25 @@ class _LogProbs(torch.autograd.Function):
             _order((logits, targets, stats, entropy, grad_logprob, grad_entropy))
         return (_ext.logprobs_grad(logits, targets, stats, entropy, grad_logprob, grad_entropy, ctx.temperature,
                                    None),) + (None,) * 4
+
+
+# ---- drafted tokens ------------------------------------------------------------------
+class Verified(NamedTuple):
+    tokens: torch.Tensor    # int64 (sequence, draft + 1): the accepted drafts, the next token, then -1
+    accepted: torch.Tensor  # int64 [sequence]: how many drafts were
+
+
+def verify(logits: torch.Tensor, drafts: torch.Tensor, uniforms: Optional[torch.Tensor] = None, *,
+           probs: Optional[torch.Tensor] = None, temperature: float = 1.0) -> Verified:
+    """Check drafted tokens (int32 or int64 (sequence, draft)) against the target's
+    distributions ``softmax(logits / temperature)``, logits (sequence, draft + 1, token), and draw the
+    next token, so that the tokens are distributed as the target's own.  `uniforms`
+    (float32 (sequence, draft + 1)) are random numbers in [0, 1): one for each draft and one for the
+    next token.  `probs` (sequence, draft, token) is what the drafts were drawn from; without
+    them a draft counts as certain (a lookup's).  A negative draft ends a sequence's
+    drafts.  With no drafts this draws a token of each row.  ``temperature=0`` takes the likeliest token,
+    of equal ones the lowest, and needs no `uniforms`.  Counts and tokens are those of 64-bit arithmetic.
+    `logits` and `probs` count as detached."""
+    if _entered:
+        _order((logits, drafts, uniforms, probs))
+    return Verified._make(_ext.verify(logits, drafts, uniforms, probs, temperature))

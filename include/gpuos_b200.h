@@ -388,6 +388,33 @@ int32_t gpuos_cache_write(int32_t n, const gpuos_tensor* x, const gpuos_tensor* 
 int32_t gpuos_cache_read(int32_t n, const gpuos_tensor* slots, const gpuos_tensor* codes,
                          const gpuos_tensor* scales, const gpuos_tensor* out, void* stream);
 
+/* Attention of queries over the cache of gpuos_cache_write, held in 8 bits.  q and
+ * out: f32, f16 or bf16 (token, query head, element), last stride 1, the head size a
+ * multiple of 16, at most 256.  codes and scales: two each (keys, values), GPUOS_I8 or
+ * GPUOS_E4M3, a scale for the whole head or for a multiple of 32 elements (strides of 0 share a
+ * scale among rows, as one a page and head).  The query heads are a multiple of the cache's:
+ * neighbours share one.  pages: i32 or i64 (sequence, page): which page of the cache holds positions
+ * [p * page, (p + 1) * page) of a sequence; lengths: i32 or i64 [sequence], how many positions
+ * it has (at most what the table holds, fewer than 2^31).  offsets: i32 or i64 [sequence + 1],
+ * rising: tokens [offsets[s], offsets[s + 1]) are sequence s's queries, the last of its
+ * positions; NULL: one query each.  With GPUOS_ATTEND_CAUSAL a query sees the positions up
+ * to its own, and of them the last `window` where that is not 0; else all.  A position
+ * whose page is outside the cache (-1) is not seen.  With s = scale * <q, key>:
+ * out = sum of e^(s - lse) value, lse (f32 (token, query head), or NULL) = log of the sum of e^s; a query
+ * that sees nothing, and a token of no sequence, get zeros and -inf.  A NaN code counts as 0.
+ * longest: no sequence has more queries than this, as far as speed goes (it chooses a kernel).
+ * workspace: gpuos_attend_workspace bytes on a 16-byte boundary (q, the keys' codes and
+ * scales, pages and longest as in the call), for this call alone until it has run. */
+#define GPUOS_ATTEND_CAUSAL 1
+int64_t gpuos_attend_workspace(const gpuos_tensor* q, const gpuos_tensor* codes,
+                               const gpuos_tensor* scales, const gpuos_tensor* pages,
+                               int64_t longest);
+int32_t gpuos_attend(const gpuos_tensor* q, const gpuos_tensor* codes, const gpuos_tensor* scales,
+                     const gpuos_tensor* pages, const gpuos_tensor* lengths,
+                     const gpuos_tensor* offsets, const gpuos_tensor* out, const gpuos_tensor* lse,
+                     void* workspace, int64_t workspace_bytes, int64_t longest, int64_t window,
+                     float scale, int32_t flags, void* stream);
+
 /* Route tokens to experts.  logits: f32, f16 or bf16 (token, expert), last
  * stride 1, at most 1024 experts.  Scores s are the softmax or the sigmoid of a
  * row, keys are s + bias (bias: f32 [expert] or NULL; without one, and with one
@@ -442,6 +469,68 @@ int32_t gpuos_logprobs_grad(const gpuos_tensor* logits, const gpuos_tensor* targ
                             const gpuos_tensor* stats, const gpuos_tensor* entropy,
                             const gpuos_tensor* grad_logprob, const gpuos_tensor* grad_entropy,
                             const gpuos_tensor* grad_logits, float temperature, void* stream);
+
+/* Sort the choices of tokens by expert.  experts: i32 or i64 (token, k), k at
+ * most 64: choice t * k + j is the j-th of token t; an expert outside [0, count) (-1:
+ * masked, or on another device) has no row.  count, at most 1024, is counts'
+ * size.  The rows of an expert are neighbours, in the order of their choices, and
+ * begin on a multiple of `align` (at most 65536).  All outputs are i32 and contiguous: places (token,
+ * k), the row of each choice or -1; sources [row], the choice of each row or -1
+ * where there is none; offsets [count + 1], where each expert's rows begin, and behind
+ * the last one's; counts [count], how many choices each has.  sources has at least
+ * gpuos_order_rows(token * k, count, align) rows, which any choice fits in. */
+int64_t gpuos_order_rows(int64_t choices, int64_t count, int64_t align);
+int32_t gpuos_order(const gpuos_tensor* experts, int32_t align, const gpuos_tensor* places,
+                    const gpuos_tensor* sources, const gpuos_tensor* offsets,
+                    const gpuos_tensor* counts, void* stream);
+
+/* Copy token rows to their places: rows[places[t][j]] = x[t], zeros in the rows of
+ * no choice.  x: f32, f16 or bf16 (token, element), last stride 1; rows: the same
+ * dtype, (row of sources, element), contiguous.  places and sources as from
+ * gpuos_order; a place outside the rows counts as -1, a place named twice holds one of
+ * the two. */
+int32_t gpuos_dispatch(const gpuos_tensor* x, const gpuos_tensor* places,
+                       const gpuos_tensor* sources, const gpuos_tensor* rows, void* stream);
+
+/* Bring the experts' results back: out[t] = sum over j of weights[t][j] *
+ * y[places[t][j]], in 32 bits in the order of j, rounded once; choices without a
+ * row add nothing.  y: f32, f16 or bf16 (row of sources, element), last stride 1;
+ * out: the same dtype, (token, element), contiguous; weights: f32 (token, k), or
+ * NULL for ones, which is gpuos_dispatch's gradient. */
+int32_t gpuos_combine(const gpuos_tensor* y, const gpuos_tensor* places,
+                      const gpuos_tensor* sources, const gpuos_tensor* weights,
+                      const gpuos_tensor* out, void* stream);
+
+/* The gradients of gpuos_combine from grad, that of out: grad_y[places[t][j]] =
+ * weights[t][j] * grad[t], zeros in the rows of no choice (grad's dtype,
+ * contiguous), and grad_weights[t][j] = <grad[t], y[places[t][j]]> (f32, 0 for a
+ * choice without a row).  One of the two may be NULL; y is needed for grad_weights only. */
+int32_t gpuos_combine_grad(const gpuos_tensor* grad, const gpuos_tensor* y,
+                           const gpuos_tensor* places, const gpuos_tensor* sources,
+                           const gpuos_tensor* weights, const gpuos_tensor* grad_y,
+                           const gpuos_tensor* grad_weights, void* stream);
+
+/* Check drafted tokens against the target's probabilities from given random
+ * numbers, and draw the next token.  logits: f32, f16 or bf16 (sequence, n + 1, token),
+ * n at most 63, fewer than 2^24 tokens, last stride 1: row i is the target's after i
+ * drafts.  drafts: i32 or i64 (sequence, n); a draft outside the row (-1: padding) ends the
+ * sequence's drafts.  uniforms: f32 (sequence, n + 1) in [0, 1).  probs: f32, f16 or
+ * bf16 (sequence, n, token), last stride 1: what each draft was drawn from; NULL:
+ * drafts that were certain.  With p = softmax(logits / temperature) draft i is
+ * accepted where uniforms[i] * q_i(d_i) < p_i(d_i).  At the first one refused the next
+ * token is drawn from max(p - q, 0) (from p where that leaves nothing; where probs is
+ * NULL, p without the draft), with all accepted from p of the row behind them: the
+ * lowest token whose sum of weights up to it exceeds uniforms[n] times all (a number
+ * below 0, and NaN, count as 0, one of 1 and more as the last below 1).  All this as in
+ * 64 bits.  temperature 0: drafts are accepted, and the next token is, the likeliest one (of equal
+ * logits the lowest); uniforms (may be NULL) and probs are not read.  A -inf logit is a masked token;
+ * at a row of -inf, or with NaN or +inf, the draft is refused, and there is no next token
+ * (-1).  tokens (i64 (sequence, n + 1), contiguous): the accepted drafts, the next token, then
+ * -1; accepted (i64 [sequence]): how many were. */
+int32_t gpuos_verify(const gpuos_tensor* logits, const gpuos_tensor* drafts,
+                     const gpuos_tensor* uniforms, const gpuos_tensor* probs,
+                     const gpuos_tensor* tokens, const gpuos_tensor* accepted, double temperature,
+                     void* stream);
 
 #ifdef __cplusplus
 }
