@@ -18,6 +18,9 @@
 //   2. a draft for which that could matter has S_i summed again in 64 bits;
 //   3. the one row that is drawn from is read again (from L2) and summed in 64 bits:
 //      an SM's 64-bit rate is half its 32-bit rate, and it is one row of a sequence.
+// Reading all rows is the bound at many long rows; else the chain of 3 to 5 steps that the cluster
+// takes together, whose exponentials are by a table (10 instructions of 64 bits each, where exp()
+// takes twice as many) and whose sums are kept a lane, so that the token is found without a third pass.
 #include <cooperative_groups.h>
 
 #include "rowops.cuh"
@@ -28,8 +31,9 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr uint32_t kThreads = 512, kWarps = kThreads / 32;
+constexpr uint32_t kThreads = 256, kWarps = kThreads / 32;
 constexpr uint32_t kCluster = 8;
+constexpr uint32_t kKept = 16;             // steps of a warp whose lanes' sums are kept
 constexpr uint32_t kMaxDrafts = 63;
 constexpr uint32_t kMaxTokens = 1u << 24;  // of a row
 constexpr int kPack = 8;                   // elements a lane takes at once
@@ -48,7 +52,7 @@ struct VerifyArgs {
   int64_t* tokens;      // (sequence, n + 1)
   int64_t* accepted;
   uint32_t n, cols;
-  double inv_t;
+  double k64;           // 64 log2(e) / t
   float k2;             // log2(e) / t
   int draft_wide, greedy, q_type;
 };
@@ -113,12 +117,19 @@ __device__ __forceinline__ void join(Stat& a, const Stat& b, float k2) {
   a.key = max(a.key, b.key);
 }
 
+// (the sum in units of e^(maximum / t) of one maximum)
 __device__ __forceinline__ Stat join_warp(Stat v, float k2) {
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v.m));
+  v.s *= ex2(fmaxf((v.m - m) * k2, -1e4f));
+  v.m = m;
 #pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    const Stat o{__shfl_xor_sync(~0u, v.m, d), __shfl_xor_sync(~0u, v.s, d), __shfl_xor_sync(~0u, v.key, d)};
-    join(v, o, k2);
-  }
+  for (int d = 16; d; d >>= 1) v.s += __shfl_xor_sync(~0u, v.s, d);
+  return v;
+}
+__device__ __forceinline__ unsigned long long max_warp(unsigned long long v) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v = max(v, __shfl_xor_sync(~0u, v, d));
   return v;
 }
 
@@ -131,22 +142,43 @@ __device__ __forceinline__ double sum_warp(double v) {
 
 struct Shared {
   Stat part[kMaxDrafts + 1][kWarps];
-  Stat mine[kMaxDrafts + 1];   // of this CTA, read by the others
+  Stat mine[kMaxDrafts + 1];      // of this CTA, read by the others
   Stat all[kMaxDrafts + 1];
   double warp[kWarps];
-  double sum[2];               // of this CTA, read by the others (two, taken in turn)
+  double sum[2];                  // of this CTA, read by the others (two, taken in turn)
+  double power[64];               // 2^(i / 64)
+  double kept[kWarps][kKept][32];
 };
 
+// e^(d / t) for d <= 0, in 64 bits: with d 64 log2(e) / t = 64 k + j + r, |r| <= 1/2 (Tang's table-driven
+// reduction), 2^k 2^(j / 64) e^y, y = r ln 2 / 64, whose series ends at y^5 / 120 (the next term is below 4e-17).
+__device__ __forceinline__ double power_of(double d, double k64, const double* table) {
+  const double x = fmax(d * k64, -64.0 * 1020.0);  // (2^-1020 stays a normal number; it changes no sum)
+  constexpr double kRound = 6755399441055744.0;    // 1.5 * 2^52: the sum's low bits are the nearest integer
+  const double n = x + kRound;
+  const int i = __double2loint(n);
+  const double y = (x - (n - kRound)) * (0.69314718055994530942 / 64.0);
+  double p = fma(y, 1.0 / 120.0, 1.0 / 24.0);
+  p = fma(y, p, 1.0 / 6.0);
+  p = fma(y, p, 0.5);
+  p = fma(y, p, 1.0);
+  const double t = table[i & 63];
+  p = fma(y * p, t, t);
+  return __hiloint2double(__double2hiint(p) + ((i >> 6) << 20), __double2loint(p));
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 3)
 gpuos_verify_kernel(const __grid_constant__ VerifyArgs a) {
-  __shared__ Shared sh;
+  extern __shared__ __align__(16) uint8_t room[];
+  Shared& sh = *reinterpret_cast<Shared*>(room);
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t rank = cluster.block_rank(), parts = cluster.num_blocks();
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t seq = blockIdx.x / parts;
   const T* x0 = static_cast<const T*>(a.x) + seq * a.xs;
   const uint32_t rows = a.n + 1;
+  if (threadIdx.x < 64) sh.power[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
 
   // the packs of a row that this warp takes, neighbours
   auto share = [&](const Row<T>& r, uint32_t& lo, uint32_t& hi) {
@@ -204,8 +236,12 @@ gpuos_verify_kernel(const __grid_constant__ VerifyArgs a) {
         }
       st.s += sum.x + sum.y;
     }
-    if (a.greedy) st.s = odd ? NAN : 0.f;
-    st = join_warp(st, a.greedy ? 0.f : a.k2);
+    if (a.greedy) {
+      st.key = max_warp(st.key);
+      st.s = __any_sync(~0u, odd) ? NAN : 0.f;
+    } else {
+      st = join_warp(st, a.k2);
+    }
     if (lane == 0) sh.part[i][warp] = st;
   }
   __syncthreads();
@@ -224,30 +260,37 @@ gpuos_verify_kernel(const __grid_constant__ VerifyArgs a) {
 
   // From here on all threads of the cluster take the same way.
   uint32_t turn = 0;
-  // the sum over the cluster of what the warps have, and what lies before this warp
-  auto sum_all = [&](double v, double& before) {
+  // the sum over the cluster of what the warps have; where this warp's share begins and ends in it (an end
+  // is exactly the next one's beginning)
+  auto sum_all = [&](double v, double& begin, double& end) {
     if (lane == 0) sh.warp[warp] = v;
     __syncthreads();
-    double mine = 0.0, ahead = 0.0;
+    double mine = 0.0, ahead = 0.0, until = 0.0;
+#pragma unroll
     for (uint32_t w = 0; w < kWarps; ++w) {
       if (w == warp) ahead = mine;
       mine += sh.warp[w];
+      if (w == warp) until = mine;
     }
     if (threadIdx.x == 0) sh.sum[turn & 1] = mine;
     cluster.sync();
-    double total = 0.0;
-    before = 0.0;
-    for (uint32_t c = 0; c < parts; ++c) {
+    const double part = lane < parts ? *cluster.map_shared_rank(&sh.sum[turn & 1], lane) : 0.0;
+    double total = 0.0, before = 0.0;
+#pragma unroll
+    for (uint32_t c = 0; c < kCluster; ++c) {
       if (c == rank) before = total;
-      total += *cluster.map_shared_rank(&sh.sum[turn & 1], c);
+      total += __shfl_sync(~0u, part, c);
     }
-    // a warp's range ends exactly where the next one's begins
-    before += ahead;
+    begin = before + ahead;
+    end = before + until;
     ++turn;
-    __syncthreads();
     return total;
   };
-  auto weight = [&](float v, float m) { return exp(((double)v - m) * a.inv_t); };
+  auto weight = [&](float v, float m) {
+    // a masked token, and one whose weight would leave 64 bits, has none
+    const double w = power_of((double)v - m, a.k64, sh.power);
+    return (double)(v - m) * a.k64 >= -64.0 * 1020.0 ? w : 0.0;
+  };
   auto whole_sum = [&](uint32_t i) {
     const Row<T> row(x0 + i * a.xr, a.cols);
     uint32_t lo, hi;
@@ -260,7 +303,7 @@ gpuos_verify_kernel(const __grid_constant__ VerifyArgs a) {
 #pragma unroll
       for (int c = 0; c < kPack; ++c) s += weight(v[c], m);
     }
-    return sum_all(sum_warp(s), unused);
+    return sum_all(sum_warp(s), unused, unused);
   };
   auto draft = [&](uint32_t i) { return load_index(a.drafts, a.draft_wide, seq * a.ds + i * a.di); };
   auto valid = [&](uint32_t i) {
@@ -281,7 +324,7 @@ gpuos_verify_kernel(const __grid_constant__ VerifyArgs a) {
     if (a.greedy) {
       refused = d != (uint32_t)~(uint32_t)sh.all[at].key;
     } else {
-      const double w = weight(to_f(x0[at * a.xr + d]), sh.all[at].m);
+      const double w = exp(((double)to_f(x0[at * a.xr + d]) - sh.all[at].m) * (a.k64 / (64.0 * 1.44269504088896340736)));
       const double q = a.q ? (double)prob(a.q, a.q_type, seq * a.qs + at * a.qr + d) : 1.0;
       const double uq = (double)__ldg(a.u + seq * a.us + at * a.ui) * q;
       double bound = uq * sh.all[at].s;
@@ -313,32 +356,40 @@ gpuos_verify_kernel(const __grid_constant__ VerifyArgs a) {
   const double total_w = refused && a.q ? whole_sum(at) : 0.0;
   bool less = refused;
   auto weights = [&](uint32_t p, double (&r)[kPack]) {
-    float v[kPack];
-    row.load(p, v);
+    float v[kPack], q[kPack];
     const int64_t e = row.first(p);
+    if (less && a.q) {
+#pragma unroll
+      for (int c = 0; c < kPack; ++c)
+        q[c] = e + c >= 0 && e + c < a.cols ? prob(a.q, a.q_type, seq * a.qs + at * a.qr + e + c) : 0.f;
+    }
+    row.load(p, v);
 #pragma unroll
     for (int c = 0; c < kPack; ++c) {
       r[c] = weight(v[c], m);
       if (!less) continue;
       if (!a.q) {
         if (e + c == gone) r[c] = 0.0;
-      } else if (r[c] > 0.0) {
-        const double rest = r[c] - (double)prob(a.q, a.q_type, seq * a.qs + at * a.qr + e + c) * total_w;
+      } else {
+        const double rest = r[c] - (double)q[c] * total_w;
         r[c] = rest > 0.0 ? rest : 0.0;  // (a NaN leaves nothing)
       }
     }
   };
-  double before, own, total;
+  const bool kept = hi - lo <= 32 * kKept;
+  double begin, end, total;
   for (;;) {
     double s = 0.0;
-    for (uint32_t p = lo + lane; p < hi; p += 32) {
-      double r[kPack];
+    uint32_t k = 0;
+    for (uint32_t p = lo + lane; p < hi; p += 32, ++k) {
+      double r[kPack], one = 0.0;
       weights(p, r);
 #pragma unroll
-      for (int c = 0; c < kPack; ++c) s += r[c];
+      for (int c = 0; c < kPack; ++c) one += r[c];
+      if (kept) sh.kept[warp][k][lane] = one;
+      s += one;
     }
-    own = sum_warp(s);
-    total = sum_all(own, before);
+    total = sum_all(sum_warp(s), begin, end);
     if (total > 0.0 || !less) break;
     less = false;
   }
@@ -346,60 +397,60 @@ gpuos_verify_kernel(const __grid_constant__ VerifyArgs a) {
   u = u > 0.0 ? u : 0.0;
   double goal = u * total;
   if (!(goal < total)) goal = __longlong_as_double(__double_as_longlong(total) - 1);
-  // the warp that the goal lies in: this one's end is the next one's beginning
-  __shared__ double starts[kWarps];
-  if (lane == 0) starts[warp] = before;
-  __syncthreads();
-  double end = total;
-  if (warp + 1 < kWarps) {
-    end = starts[warp + 1];
-  } else if (rank + 1 < parts) {
-    double sum = 0.0;
-    for (uint32_t c = 0; c <= rank; ++c) sum += *cluster.map_shared_rank(&sh.sum[(turn - 1) & 1], c);
-    end = sum;
-  }
-  if (before <= goal && goal < end) {
-    double run = before;
+  if (begin <= goal && goal < end) {  // one warp of the cluster
+    double run = begin;
     int64_t found = -1, last = -1;
-    for (uint32_t p0 = lo; p0 < hi && found < 0; p0 += 32) {
+    uint32_t k = 0;
+    for (uint32_t p0 = lo; p0 < hi && found < 0; p0 += 32, ++k) {
       const uint32_t p = p0 + lane;
       double r[kPack], s = 0.0;
-      const bool in = p < hi;
-      if (in) weights(p, r);
+      if (p < hi) {
+        if (kept) {
+          s = sh.kept[warp][k][lane];
+        } else {
+          weights(p, r);
 #pragma unroll
-      for (int c = 0; c < kPack; ++c) {
-        if (!in) r[c] = 0.0;
-        s += r[c];
+          for (int c = 0; c < kPack; ++c) s += r[c];
+        }
       }
       double sum = s;
+#pragma unroll
       for (uint32_t d = 1; d < 32; d <<= 1) {
         const double o = __shfl_up_sync(~0u, sum, d);
         if (lane >= d) sum += o;
       }
-      // the first lane whose sum passes the goal; its elements one by one
-      const uint32_t past = __ballot_sync(~0u, run + sum > goal);
+      // the first lane whose sum passes the goal (else the last with any: the sums of step 3 rounded in another
+      // order); of its elements the first that does, or the last with any weight
+      const uint32_t past = __ballot_sync(~0u, run + sum > goal && s > 0.0);
       const uint32_t some = __ballot_sync(~0u, s > 0.0);
-      const uint32_t who = past ? __ffs(past) - 1 : 32 - __clz(some) - 1;
-      int64_t pick = -1, high = -1;
-      if (past || some) {
-        if (lane == who) {
-          double acc = run + (sum - s);
-          for (int c = 0; c < kPack; ++c) {
-            acc += r[c];
-            if (r[c] > 0.0) {
-              high = row.first(p) + c;
-              if (pick < 0 && acc > goal) pick = high;
-            }
-          }
-        }
-        high = __shfl_sync(~0u, high, who);
-        pick = __shfl_sync(~0u, pick, who);
-        if (high >= 0) last = high;
-        if (past) found = pick >= 0 ? pick : last;
-      }
+      const double ahead = run + (sum - s);
       run += __shfl_sync(~0u, sum, 31);
+      if (!past && (!some || p0 + 32 < hi)) {
+        if (some) last = p0 + 31 - __clz(some);  // (a pack)
+        continue;
+      }
+      const uint32_t who = past ? __ffs(past) - 1 : 31 - __clz(some);
+      found = p0 + who;
+      double acc = __shfl_sync(~0u, ahead, who);
+      weights((uint32_t)found, r);
+      int64_t pick = -1, high = -1;
+#pragma unroll
+      for (int c = 0; c < kPack; ++c) {
+        acc += r[c];
+        if (r[c] > 0.0) high = row.first((uint32_t)found) + c;
+        if (r[c] > 0.0 && pick < 0 && acc > goal) pick = high;
+      }
+      if (lane == 0) out[at] = pick >= 0 ? pick : high;
     }
-    if (lane == 0) out[at] = found >= 0 ? found : last;
+    if (found < 0) {  // the last steps had nothing: the last weight of the warp's share
+      double r[kPack];
+      weights((uint32_t)last, r);
+      int64_t high = -1;
+#pragma unroll
+      for (int c = 0; c < kPack; ++c)
+        if (r[c] > 0.0) high = row.first((uint32_t)last) + c;
+      if (lane == 0) out[at] = high;
+    }
   }
   cluster.sync();  // no CTA leaves while another reads its sums
 }
@@ -463,7 +514,7 @@ extern "C" int32_t gpuos_verify(const gpuos_tensor* logits, const gpuos_tensor* 
       a.u = static_cast<const float*>(uniforms->data);
       a.us = uniforms->strides[0];
       a.ui = uniforms->strides[1];
-      a.inv_t = 1.0 / temperature;
+      a.k64 = 64.0 * 1.44269504088896340736 / temperature;
       a.k2 = (float)(1.44269504088896340736 / temperature);
     }
     if (probs && rows > 1 && !greedy) {
@@ -477,15 +528,16 @@ extern "C" int32_t gpuos_verify(const gpuos_tensor* logits, const gpuos_tensor* 
     a.n = (uint32_t)rows - 1;
     a.cols = (uint32_t)v;
     a.greedy = greedy;
-    // CTAs of a sequence: each with a pack for every thread at least; of very many sequences fewer, but
-    // for rows so long that a thread's sums in 32 bits would lose their bound
+    // CTAs of a sequence: as few as keep their lanes' sums (and the bound on sums in 32 bits); of few sequences
+    // more, with a pack for every thread at least
     uint32_t parts = 1;
     while (parts < kCluster && (uint64_t)parts * kThreads * kPack < (uint64_t)v &&
-           ((uint64_t)b * parts < 8u * (uint32_t)sm_count() || v > (1 << 20)))
+           ((uint64_t)b * parts < 3u * (uint32_t)sm_count() || (uint64_t)parts * kWarps * kKept * 32 * kPack < (uint64_t)v + kPack))
       parts *= 2;
     cudaLaunchConfig_t c{};
     c.gridDim = dim3((uint32_t)b * parts);
     c.blockDim = dim3(kThreads);
+    c.dynamicSmemBytes = sizeof(Shared);
     c.stream = static_cast<cudaStream_t>(stream);
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -493,9 +545,12 @@ extern "C" int32_t gpuos_verify(const gpuos_tensor* logits, const gpuos_tensor* 
     c.attrs = at;
     c.numAttrs = 1;
     const VerifyArgs args = a;
-    cuda_ok(logits->dtype == GPUOS_F32   ? cudaLaunchKernelEx(&c, gpuos_verify_kernel<float>, args)
-            : logits->dtype == GPUOS_F16 ? cudaLaunchKernelEx(&c, gpuos_verify_kernel<__half>, args)
-                                         : cudaLaunchKernelEx(&c, gpuos_verify_kernel<__nv_bfloat16>, args),
-            "launch");
+    auto go = [&](auto* kernel) {
+      cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared)), "shared memory");
+      cuda_ok(cudaLaunchKernelEx(&c, kernel, args), "launch");
+    };
+    if (logits->dtype == GPUOS_F32) go(gpuos_verify_kernel<float>);
+    else if (logits->dtype == GPUOS_F16) go(gpuos_verify_kernel<__half>);
+    else go(gpuos_verify_kernel<__nv_bfloat16>);
   });
 }
