@@ -71,7 +71,7 @@ def build_lib(force=False, verbose=False) -> Path:
         src = CSRC / f"{name}.cu"
         deps = [src, CSRC / "rowops.cuh", CSRC / "rowops.h", abi]
         if name.startswith("attend"):
-            deps += [CSRC / "attend.h", CSRC / "attend.cuh"]
+            deps += [CSRC / "attend.h", CSRC / "attend.cuh", CSRC / "attend_wide.cuh"]
         steps.append((BUILD / f"{name}.o", [*nvcc, "-c", src], deps))
     jcubin = BUILD / "jit_kernel.cubin"
     jblob = BUILD / "jit_blob.cpp"

@@ -84,7 +84,7 @@ extern "C" int32_t gpuos_attend(const gpuos_tensor* q, const gpuos_tensor* codes
     need(page >= 1, "pages must have rows");
     need(page < kMostPositions && pages->sizes[1] < kMostPositions && page * pages->sizes[1] < kMostPositions,
          "a sequence has fewer than 2^31 positions");
-    need(n < (1ll << 30) && tokens < kMostPositions / hq, "the call is too large");
+    need(pool < kMostPositions && n < (1ll << 30) && tokens < kMostPositions / hq, "the call is too large");
     if (offsets) {
       check_tensor(offsets, 1, "offsets");
       need(is_index(offsets->dtype), "offsets must be int32 or int64");
@@ -181,7 +181,16 @@ extern "C" int32_t gpuos_attend(const gpuos_tensor* q, const gpuos_tensor* codes
       a.partial = reinterpret_cast<float*>(a.split + s.grid);
     }
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (codes->dtype == GPUOS_I8) launch<kInt8>(s.plan, a, st);
-    else launch<kE4M3>(s.plan, a, st);
+    const bool int8 = codes->dtype == GPUOS_I8;
+    a.few = kAll;
+    if (!s.plan.general && s.plan.padded <= 128 && a.vec == 16 && std::min(longest, tokens) * a.each > kWideFrom) {
+      a.few = kWideFrom;
+      const int64_t most = (tokens * a.each / kWideRows + n) * hk;  // blocks of all sequences
+      need(most < (1ll << 31), "the call is too large");
+      a.wide_grid = (uint32_t)most;
+      a.out_vec = rows_aligned(*out, 8);
+      int8 ? launch_wide<kInt8>(a, st) : launch_wide<kE4M3>(a, st);
+    }
+    int8 ? launch<kInt8>(s.plan, a, st) : launch<kE4M3>(s.plan, a, st);
   });
 }

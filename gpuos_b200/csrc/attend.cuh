@@ -90,7 +90,7 @@ struct Item {
 template <uint32_t RB>
 __device__ __forceinline__ int64_t blocks(const Args& a, const Sequence& s) {
   const int64_t rows = s.n * a.each;
-  return a.few && rows > a.few ? 0 : (rows + RB - 1) / RB;
+  return rows > a.few ? 0 : (rows + RB - 1) / RB;
 }
 template <uint32_t RB>
 __device__ __forceinline__ Range block_range(const Args& a, const Sequence& s, int64_t b) {

@@ -12,6 +12,7 @@ constexpr uint32_t kWarps = 4, kThreads = 32 * kWarps;
 constexpr uint32_t kLeast = 4;       // units of a CTA, at least
 constexpr uint32_t kWhole = 8;       // units up to which an item is not split
 constexpr uint32_t kMaxHead = 256;
+constexpr uint32_t kWideRows = 256;  // of a block of a prompt
 
 // A slice of the cache.
 struct Held {
@@ -44,7 +45,9 @@ struct Args {
   uint32_t head, groups;   // elements; scales of a head
   uint32_t group;          // elements of a scale
   uint32_t grid;           // CTAs over which the work is spread
-  uint32_t few;            // 0, or: sequences of more rows than this are another kernel's
+  uint32_t few;            // sequences of more rows than this are the kernel's for prompts, the others the one's for few rows
+  uint32_t wide_grid;      // blocks of the former there may be
+  int out_vec;             // out can be written 16 bytes at once
   int64_t window;          // 0: none
   float scale2;            // scale * log2(e)
   FastDiv page, each_div;
@@ -163,6 +166,10 @@ inline Plan plan(uint32_t head, uint32_t groups, bool split, int64_t rows) {
   return p;
 }
 template <int F> void launch(const Plan& p, const Args& a, cudaStream_t stream);
+template <int F> void launch_wide(const Args& a, cudaStream_t stream);
+
+constexpr uint32_t kAll = ~0u;        // `few` where there is no other kernel
+constexpr uint32_t kWideFrom = 128;   // rows of a sequence above which it is a prompt
 
 }  // namespace attend
 }  // namespace rowops
