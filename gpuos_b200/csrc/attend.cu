@@ -183,11 +183,12 @@ extern "C" int32_t gpuos_attend(const gpuos_tensor* q, const gpuos_tensor* codes
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool int8 = codes->dtype == GPUOS_I8;
     a.few = kAll;
-    if (!s.plan.general && s.plan.padded <= 128 && a.vec == 16 && std::min(longest, tokens) * a.each > kWideFrom) {
+    if (groups == 1 && q->dtype != GPUOS_F32 && s.plan.padded <= 128 && a.vec == 16 && std::min(longest, tokens) * a.each > kWideFrom) {
       a.few = kWideFrom;
       const int64_t most = (tokens * a.each / kWideRows + n) * hk;  // blocks of all sequences
       need(most < (1ll << 31), "the call is too large");
       a.wide_grid = (uint32_t)most;
+      a.q_vec = rows_aligned(*q, 8);
       a.out_vec = rows_aligned(*out, 8);
       int8 ? launch_wide<kInt8>(a, st) : launch_wide<kE4M3>(a, st);
     }

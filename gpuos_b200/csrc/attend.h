@@ -47,7 +47,7 @@ struct Args {
   uint32_t grid;           // CTAs over which the work is spread
   uint32_t few;            // sequences of more rows than this are the kernel's for prompts, the others the one's for few rows
   uint32_t wide_grid;      // blocks of the former there may be
-  int out_vec;             // out can be written 16 bytes at once
+  int q_vec, out_vec;      // rows of q and out lie on 16 bytes
   int64_t window;          // 0: none
   float scale2;            // scale * log2(e)
   FastDiv page, each_div;
