@@ -2,14 +2,15 @@
 //
 // A CTA takes 256 rows (queries x query heads of one key head) as two tiles of 128
 // and walks over their positions 128 at a time:
-//   S = Q K^T (accumulators in TMEM)  ->  P = 2^(S kappa - M) nu  ->  O += P V (TMEM)
-// Four warps dequantise: codes become 16-bit floats exactly, once for both tiles,
+//   S = Q K^T (accumulators in TMEM)  ->  P = 2^(S kappa - M)  ->  O += P (nu V) (TMEM)
+// Seven warps dequantise: codes become 16-bit floats exactly, once for both tiles,
 // and go into shared memory as the tensor cores read them.  Four warps for each tile
-// take S from TMEM, a row a thread, put P in its place as 16-bit floats (in two parts for
-// 16-bit floats of 11 bits), and one of their threads issues the tile's products.  While one tile's weights
-// are computed the tensor cores work on the other's.  The reference M of a row follows its maximum and the
-// largest scale of V seen (as a power of two), and both O and the sum of weights are in its units; it is
-// raised, and O rescaled, only when a weight could pass 2^14.
+// take S from TMEM, a row a thread, and put P in its place as 16-bit floats (in two parts for
+// 16-bit floats of 11 bits); a thread issues the products.  While one tile's weights
+// are computed the tensor cores work on the other's.  The scales of V, relative to a power of two, go into V for
+// bf16 (three roundings of 2^-12 on average each, an eighth of the result's), into P in its two parts for fp16.
+// The reference M of a row follows its maximum.  A step takes the last one's, and only where the weights' sum then
+// says that one may be too large, or where the row does not see all positions, the maximum is looked for (and O rescaled).
 // The bound are the products: 4 * 128 operations a (row, position) of a head of 128;
 // beside it, an SM has 16 exponentials a cycle, 1024 cycles a tile and step, as many as the
 // two products take, and shared memory feeds Q, K and V to the tensor cores in three quarters of that time.
@@ -21,7 +22,8 @@ namespace rowops {
 namespace attend {
 namespace {
 
-constexpr uint32_t kWideTile = 128, kWideThreads = 384;  // 8 warps of weights, 4 of codes
+constexpr uint32_t kWideTile = 128, kWideThreads = 512;  // 8 warps of weights, 7 of codes, one that issues products
+constexpr uint32_t kCodeWarps = 7;
 constexpr uint32_t kRings = 4;  // of scales: the weights' warps read them after the products that K fed
 
 template <int DT>
@@ -33,10 +35,12 @@ struct Wide {
 };
 
 struct WideShared {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], done[2], where_full;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], done, where_full;
   uint32_t tmem;
-  int dead;
-  uint32_t valid[kRings][4];
+  int dead, top, uniform;  // top: the largest exponent in the block's q
+  uint32_t valid[kRings][4], odd[kRings][4];  // positions with a page; whose scale of V is not finite
+  float most[2][4];      // of a step: the largest scale of V, a warp's positions each
+  float unit[kRings];    // of a step: what V is relative to
   alignas(16) float kappa[kRings][kWideTile];
   alignas(16) float nu[kRings][kWideTile];
   int64_t where[2][2][kWideTile];  // of a step: where each position's codes are in K and in V, -1: nowhere
@@ -62,10 +66,11 @@ __device__ __forceinline__ bool await(uint64_t* b, uint32_t parity, volatile int
   uint64_t since = 0;
   for (uint32_t i = 0;; ++i) {
     uint32_t ok;
-    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-                 : "=r"(ok) : "r"(shared_at(b)), "r"(parity) : "memory");
+    // (asleep for 20 us at most: polls would take their part of shared memory's rate)
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(ok) : "r"(shared_at(b)), "r"(parity), "r"(20000) : "memory");
     if (ok) return true;
-    if ((i & 63) == 63) {
+    if ((i & 15) == 15) {
       if (*dead) return false;
       const uint64_t t = now_ns();
       if (!since) since = t;
@@ -88,16 +93,19 @@ __device__ __forceinline__ uint64_t descriptor(uint32_t at, uint32_t leading, ui
 __host__ __device__ constexpr uint32_t instruction(uint32_t n, bool b_turned) {
   return (1u << 4) | ((uint32_t)b_turned << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
 }
-__device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint32_t what, bool add) {
-  asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a),
-               "l"(b), "r"(what), "r"((uint32_t)add) : "memory");
+// Issued by one thread of a warp whose threads all come here with the same operands: those then stay in uniform
+// registers (with operands of a single thread a product took 170 cycles to issue, and 64 to run).
+__device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint32_t what, uint32_t add) {
+  asm volatile("{ .reg .pred p, q; elect.sync _|q, 0xffffffff; setp.ne.b32 p, %4, 0; "
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(what), "r"(add) : "memory");
 }
-__device__ __forceinline__ void product_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t what, bool add) {
-  asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a),
-               "l"(b), "r"(what), "r"((uint32_t)add) : "memory");
+__device__ __forceinline__ void product_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t what, uint32_t add) {
+  asm volatile("{ .reg .pred p, q; elect.sync _|q, 0xffffffff; setp.ne.b32 p, %4, 0; "
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(what), "r"(add) : "memory");
 }
 __device__ __forceinline__ void commit(uint64_t* b) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_at(b)) : "memory");
+  asm volatile("{ .reg .pred q; elect.sync _|q, 0xffffffff; "
+               "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(shared_at(b)) : "memory");
 }
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -152,9 +160,8 @@ __device__ __forceinline__ void load_query(const Args& a, int64_t at, float (&v)
   }
 }
 
-// Row r of q times a power of two (the result undoes it), as 16-bit floats in a tile.
-template <int DT>
-__device__ __forceinline__ float stage_query(const Args& a, uint8_t* tile, uint32_t r, bool has, int64_t base) {
+// The exponent of a row's largest element (-127: zeros and what is smaller; 128: an infinity).
+__device__ __forceinline__ int query_exponent(const Args& a, bool has, int64_t base) {
   float most = 0.f, v[8];
   if (has)
 #pragma unroll 4
@@ -163,23 +170,35 @@ __device__ __forceinline__ float stage_query(const Args& a, uint8_t* tile, uint3
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[i]));
     }
-  int shift = 14 - (int)((__float_as_uint(most) >> 23) - 127);
-  if (!(most > 0.f)) shift = 0;
-  const int first = min(max(shift, -126), 126);
-  const float up = __uint_as_float((uint32_t)(first + 127) << 23), more = __uint_as_float((uint32_t)(shift - first + 127) << 23);
-  const float by = a.scale2 < 0.f ? -more : more;
+  return (int)(__float_as_uint(most) >> 23) - 127;
+}
+
+// Powers of two beyond the normal numbers, as two factors.
+struct Power {
+  float a, b;
+  __device__ explicit Power(int e) {
+    const int first = min(max(e, -126), 126);
+    a = __uint_as_float((uint32_t)(first + 127) << 23);
+    b = __uint_as_float((uint32_t)(min(max(e - first, -126), 126) + 127) << 23);
+  }
+};
+
+// Row r of q times 2^shift, as 16-bit floats in a tile.
+template <int DT>
+__device__ __forceinline__ void stage_query(const Args& a, uint8_t* tile, uint32_t r, bool has, int64_t base, int shift) {
+  const Power up(shift);
+  const float by = a.scale2 < 0.f ? -up.b : up.b;
+  float v[8];
 #pragma unroll 4
   for (uint32_t x = 0; x < DT / 8; ++x) {
     uint32_t w[4] = {0, 0, 0, 0};
     if (has && x * 8 < a.head) {
       load_query(a, base + x * 8, v);
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) w[i] = pack16(make_float2(v[2 * i] * up * by, v[2 * i + 1] * up * by));
+      for (uint32_t i = 0; i < 4; ++i) w[i] = pack16(make_float2(v[2 * i] * up.a * by, v[2 * i + 1] * up.a * by));
     }
     *reinterpret_cast<uint4*>(tile + (x >> 3) * Wide<DT>::block + r * 128 + (((x & 7) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  // (a scale of 0 as one that makes no difference: a masked score of -inf stays one)
-  return fmaxf(fabsf(a.scale2) / up / more, 1e-38f);
 }
 
 __device__ __forceinline__ int64_t wide_blocks(const Args& a, const Sequence& s) {
@@ -203,7 +222,7 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
     int64_t n = 0;
     for (uint32_t s = s0; s < s1; ++s) n += wide_blocks(a, sequence(a, s)) * a.k_heads;
     sh.units[tid + 1] = n;
-    if (tid == 0) sh.units[0] = 0, sh.seq = a.sequences, sh.dead = 0;
+    if (tid == 0) sh.units[0] = 0, sh.seq = a.sequences, sh.dead = 0, sh.top = -127, sh.uniform = 1;
     __syncthreads();
     if (warp == 0) {
       int64_t run = 0;
@@ -243,38 +262,52 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      barrier_init(&sh.k_full[i], 128);
-      barrier_init(&sh.v_full[i], 128);
-      barrier_init(&sh.k_empty[i], 2);
-      barrier_init(&sh.v_empty[i], 2);
+      barrier_init(&sh.k_full[i], 32 * kCodeWarps);
+      barrier_init(&sh.v_full[i], 32 * kCodeWarps);
+      barrier_init(&sh.k_empty[i], 1);
+      barrier_init(&sh.v_empty[i], 1);
       barrier_init(&sh.s_full[i], 1);
       barrier_init(&sh.p_full[i], 128);
-      barrier_init(&sh.done[i], 1);
+      
     }
-    barrier_init(&sh.where_full, 128);
+    barrier_init(&sh.done, 1);
+    barrier_init(&sh.where_full, 32 * kCodeWarps);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) {
+  if (warp == 15) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(shared_at(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  // the weights' warps bring the block's rows of q
-  float scale = 0.f;
+  // The weights' warps bring the block's rows of q, times one power of two where the rows' largest elements are within
+  // 2^10 of one another (16-bit floats then reach 2^-19 of each, 2^-29 of the largest score), else each its own.
+  float scale = 1.f;
   int64_t lo = 1, hi = 0, token = 0;
   uint32_t q_head = 0;
   const uint32_t t = warp >> 2;  // the tile of a weights' warp
   const int64_t row = row_base + tid;
+  const bool has_row = warp < 8 && row < row_all;
+  int exponent = -127;
+  if (has_row) {
+    const uint32_t query = a.each_div.div((uint32_t)row);
+    token = s.first + query;
+    q_head = head * a.each + (uint32_t)row - query * a.each;
+    const int64_t last = last_seen(a, s, query);
+    lo = first_seen(a, last);
+    hi = last + 1;
+    exponent = query_exponent(a, true, token * a.qt + q_head * a.qh);
+    atomicMax(&sh.top, exponent);
+  }
+  __syncthreads();
+  if (has_row && exponent > -127 && exponent < sh.top - 10) sh.uniform = 0;
+  __syncthreads();
+  const bool uniform = sh.uniform;
   if (warp < 8) {
-    const bool has = row < row_all;
-    if (has) {
-      const uint32_t query = a.each_div.div((uint32_t)row);
-      token = s.first + query;
-      q_head = head * a.each + (uint32_t)row - query * a.each;
-      const int64_t last = last_seen(a, s, query);
-      lo = first_seen(a, last);
-      hi = last + 1;
+    const int shift = uniform ? (sh.top > -127 ? 14 - sh.top : 0) : exponent > -127 ? 14 - exponent : 0;
+    stage_query<DT>(a, smem + W::q + t * W::tile, tid & 127, has_row, token * a.qt + q_head * a.qh, shift);
+    if (!uniform) {
+      const Power down(-shift);
+      scale = fmaxf(fabsf(a.scale2) * down.a * down.b, 1e-38f);  // (a score of -inf stays one)
     }
-    scale = stage_query<DT>(a, smem + W::q + t * W::tile, tid & 127, has, token * a.qt + q_head * a.qh);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   before_sync();
@@ -282,26 +315,32 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
   after_sync();
   const uint32_t tmem = sh.tmem, t_s = tmem + t * 128, t_o = tmem + 256 + t * DT;
 
+  // (256 * 184 + 256 * 72 registers: the 512 * 128 of the launch)
   if (warp >= 8) {
+   asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+   if (warp < 8 + kCodeWarps) {
     // ---- codes: a thread finds a position; then 8 (heads up to 64: 4) threads load one, 16 bytes each
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     const uint32_t j = tid - 256;
-    constexpr uint32_t X = DT / 16;                           // 16-byte pieces of a position
-    constexpr uint32_t PASS = 128 / X, N = kWideTile / PASS;  // positions at once, and how often
+    constexpr uint32_t X = DT / 16;                                        // 16-byte pieces of a position
+    constexpr uint32_t PASS = 32 * kCodeWarps / X, N = (kWideTile + PASS - 1) / PASS;  // positions at once, and how often
+    static_assert(PASS % 4 == 0);
     const uint32_t piece = j % X, own = j / X;
     const bool in = piece * 16 < a.head;
     const int64_t table = sh.seq * a.ps;
     const uint8_t* const k_codes = a.k.codes + head * a.k.ch + piece * 16;
     const uint8_t* const v_codes = a.v.codes + head * a.v.ch + piece * 16;
+    const Power down(uniform && sh.top > -127 ? sh.top - 14 : 0);
+    const float by = uniform ? fabsf(a.scale2) * down.a : 1.f;
     auto page_at = [&](uint32_t step) -> int32_t {  // of this thread's position; -1: not seen
       const int64_t p = range.lo + (int64_t)step * kWideTile + j;
-      if (p >= range.hi) return -1;
+      if (j >= kWideTile || p >= range.hi) return -1;
       const int64_t g = load_index(a.pages, a.page_wide, table + a.page.div((uint32_t)p) * a.pp);
       return g >= 0 && g < a.pool ? (int32_t)g : -1;
     };
     float kappa = 0.f, nu = 0.f;
-    uint32_t valid = 0;
+    uint32_t valid = 0, odd = 0;
     auto find = [&](uint32_t step, int32_t page) {
+      if (warp >= 12) return arrive(&sh.where_full);  // (it has read what was there)
       const uint32_t p = (uint32_t)(range.lo + (int64_t)step * kWideTile + j), at = p - a.page.div(p) * a.page.d;
       const bool has = page >= 0;
       sh.where[step & 1][0][j] = has ? page * a.k.cp + at * a.k.cr : -1;
@@ -309,27 +348,51 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
       kappa = has ? __ldg(a.k.scales + page * a.k.sp + at * a.k.sr + head * a.k.sh) : 0.f;
       nu = has ? __ldg(a.v.scales + page * a.v.sp + at * a.v.sr + head * a.v.sh) : 0.f;
       valid = __ballot_sync(~0u, has);
+      // a scale that is not finite makes NaN of the rows that see it, and must not touch others: it is not multiplied
+      const bool fine = fabsf(nu) < INFINITY;
+      odd = __ballot_sync(~0u, !fine);
+      if (!fine) nu = 0.f;
+      const float high = warp_max(nu);
+      if (lane == 0) sh.most[step & 1][warp - 8] = high;
       arrive(&sh.where_full);
+    };
+    // V is brought in relative to a power of two that is raised when a scale passes it by 2^2
+    float unit = 0.f;
+    auto raise = [&](uint32_t step) {
+      const float* const w = sh.most[step & 1];
+      const float most = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
+      if (most > 4.f * unit)
+        unit = fmaxf(__uint_as_float(min((__float_as_uint(most) & 0x7f800000u) + 0x00800000u, 0x7e800000u)), 0x1p-90f);
     };
     auto load = [&](const uint8_t* codes, uint32_t step, uint32_t which, uint4 (&r)[N]) {
 #pragma unroll
       for (uint32_t i = 0; i < N; ++i) {
-        const int64_t at = sh.where[step & 1][which][i * PASS + own];
+        const uint32_t p = i * PASS + own;
+        const int64_t at = N * PASS == kWideTile || p < kWideTile ? sh.where[step & 1][which][p] : -1;
         r[i] = at >= 0 && in ? __ldg(reinterpret_cast<const uint4*>(codes + at)) : make_uint4(0, 0, 0, 0);
       }
     };
     // (the two halves of 8 threads in turn: no two of them in a bank)
     const uint32_t flip = piece >> 2;
-    uint32_t put0 = (piece >> 2) * W::block + own * 128 + (((2 * (piece & 3) + flip) ^ (own & 7)) << 4);
-    uint32_t put1 = (piece >> 2) * W::block + own * 128 + (((2 * (piece & 3) + 1 - flip) ^ (own & 7)) << 4);
-    auto put = [&](uint8_t* tile, const uint4 (&r)[N]) {
+    const uint32_t put0 = (piece >> 2) * W::block + own * 128 + (((2 * (piece & 3) + flip) ^ (own & 7)) << 4);
+    const uint32_t put1 = (piece >> 2) * W::block + own * 128 + (((2 * (piece & 3) + 1 - flip) ^ (own & 7)) << 4);
+    auto put = [&](uint8_t* tile, const uint4 (&r)[N], [[maybe_unused]] const float* by_scale) {
 #pragma unroll
       for (uint32_t i = 0; i < N; ++i) {
-        // (PASS is a multiple of 8: the swizzle is the same for all of a thread's positions)
+        if (N * PASS != kWideTile && i * PASS + own >= kWideTile) break;
+        const uint32_t turn = (i * PASS & 4) << 4;  // of the swizzle, from a thread's first position to this one
         const uint32_t w0 = raw<F>(flip ? r[i].z : r[i].x), w1 = raw<F>(flip ? r[i].w : r[i].y);
         const uint32_t w2 = raw<F>(flip ? r[i].x : r[i].z), w3 = raw<F>(flip ? r[i].y : r[i].w);
-        *reinterpret_cast<uint4*>(tile + put0 + i * PASS * 128) = make_uint4(pair_low<F>(w0), pair_high<F>(w0), pair_low<F>(w1), pair_high<F>(w1));
-        *reinterpret_cast<uint4*>(tile + put1 + i * PASS * 128) = make_uint4(pair_low<F>(w2), pair_high<F>(w2), pair_low<F>(w3), pair_high<F>(w3));
+        uint4 x = make_uint4(pair_low<F>(w0), pair_high<F>(w0), pair_low<F>(w1), pair_high<F>(w1));
+        uint4 y = make_uint4(pair_low<F>(w2), pair_high<F>(w2), pair_low<F>(w3), pair_high<F>(w3));
+        if (!SPLIT && by_scale) {
+          const __half2 h = __float2half2_rn(by_scale[i * PASS + own]);
+          __half2* const xs[2] = {reinterpret_cast<__half2*>(&x), reinterpret_cast<__half2*>(&y)};
+#pragma unroll
+          for (uint32_t k = 0; k < 8; ++k) xs[k >> 2][k & 3] = __hmul2(xs[k >> 2][k & 3], h);
+        }
+        *reinterpret_cast<uint4*>(tile + (put0 ^ turn) + i * PASS * 128) = x;
+        *reinterpret_cast<uint4*>(tile + (put1 ^ turn) + i * PASS * 128) = y;
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     };
@@ -340,202 +403,268 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
       find(0, page_at(0));
       page = steps > 1 ? page_at(1) : -1;
       ok = await(&sh.where_full, 0, &sh.dead);
-      if (ok) load(k_codes, 0, 0, rk);
+      if (ok) {
+        raise(0);
+        load(k_codes, 0, 0, rk);
+      }
     }
     for (uint32_t i = 0; ok && i < steps; ++i) {
       const uint32_t st = i & 1, ring = i % kRings;
       load(v_codes, i, 1, rv);
       if (i >= 2 && !await(&sh.k_empty[st], (i / 2 - 1) & 1, &sh.dead)) break;
-      put(smem + W::k + st * W::tile, rk);
-      sh.kappa[ring][j] = kappa;
-      sh.nu[ring][j] = nu;
-      if (lane == 0) sh.valid[ring][warp - 8] = valid;
+      put(smem + W::k + st * W::tile, rk, nullptr);
+      if (warp < 12) {
+        sh.kappa[ring][j] = kappa * by * down.b;
+        sh.nu[ring][j] = unit > 0.f ? nu * __uint_as_float(0x7f000000u - __float_as_uint(unit)) : 0.f;
+        if (lane == 0) sh.valid[ring][warp - 8] = valid, sh.odd[ring][warp - 8] = odd;
+        if (tid == 256) sh.unit[ring] = unit;
+      }
       arrive(&sh.k_full[st]);
       if (i + 1 < steps) {
         __syncwarp();
         find(i + 1, page);
         page = i + 2 < steps ? page_at(i + 2) : -1;
-        if (!await(&sh.where_full, (i + 1) & 1, &sh.dead)) break;
+        if (!await(&sh.where_full, (i + 1) & 1, &sh.dead)) break;  // (and this step's scales are there)
+        raise(i + 1);
         load(k_codes, i + 1, 0, rk);
+      } else if (!await(&sh.k_full[st], (i / 2) & 1, &sh.dead)) {
+        break;
       }
       if (i >= 2 && !await(&sh.v_empty[st], (i / 2 - 1) & 1, &sh.dead)) break;
-      put(smem + W::v + st * W::tile, rv);
+      put(smem + W::v + st * W::tile, rv, sh.nu[ring]);
       arrive(&sh.v_full[st]);
     }
-  } else {
-    // ---- weights: a row a thread
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    const uint32_t lanes = (warp & 3) << 21;  // (32 lanes a warp, in the upper half of an address)
-    const bool issuer = (tid & 127) == 0;
-    constexpr uint32_t to_s = instruction(kWideTile, false), to_o = instruction(DT, true);
-    auto scores = [&](uint32_t st) {
-      const uint32_t q = shared_at(smem + W::q + t * W::tile), k = shared_at(smem + W::k + st * W::tile);
+   } else {
+    // ---- products: a warp of its own issues them, since it waits while the tensor cores are busy
+    if (steps) {
+      constexpr uint32_t to_s = instruction(kWideTile, false), to_o = instruction(DT, true);
+      const uint32_t at = shared_at(smem);
+      const uint64_t q0 = descriptor(at + W::q, 16, 1024), k0 = descriptor(at + W::k, 16, 1024), v0 = descriptor(at + W::v, W::block, 1024);
+      auto scores = [&](uint32_t tile, uint32_t st) {
+        const uint64_t q = q0 + tile * (W::tile >> 4), k = k0 + st * (W::tile >> 4);
 #pragma unroll
-      for (uint32_t e = 0; e < DT / 16; ++e) {
-        const uint32_t by = (e >> 2) * W::block + (e & 3) * 32;
-        product(t_s, descriptor(q + by, 16, 1024), descriptor(k + by, 16, 1024), to_s, e > 0);
-      }
-      commit(&sh.s_full[t]);
-      commit(&sh.k_empty[st]);
-    };
-    auto values = [&](uint32_t st, bool add) {
-      const uint32_t v = shared_at(smem + W::v + st * W::tile);
+        for (uint32_t e = 0; e < DT / 16; ++e) {
+          const uint32_t b = ((e >> 2) * W::block + (e & 3) * 32) >> 4;
+          product(tmem + tile * 128, q + b, k + b, to_s, e > 0);
+        }
+        commit(&sh.s_full[tile]);
+      };
+      auto values = [&](uint32_t tile, uint32_t st, bool add) {
+        const uint64_t v = v0 + st * (W::tile >> 4);
+        const uint32_t p = tmem + tile * 128, o = tmem + 256 + tile * DT;
 #pragma unroll
-      for (uint32_t e = 0; e < kWideTile / 16; ++e)
-        product_from_tmem(t_o, t_s + e * 8, descriptor(v + e * 2048, W::block, 1024), to_o, add || e > 0);
-      if constexpr (SPLIT) {
+        for (uint32_t e = 0; e < kWideTile / 16; ++e) product_from_tmem(o, p + e * 8, v + e * 128, to_o, e > 0 || add);
+        if constexpr (SPLIT) {
 #pragma unroll
-        for (uint32_t e = 0; e < kWideTile / 16; ++e)
-          product_from_tmem(t_o, t_s + 64 + e * 8, descriptor(v + e * 2048, W::block, 1024), to_o, true);
-      }
-      commit(&sh.v_empty[st]);
-    };
-    float m = -INFINITY, ref = 0.f, unit = 0.f, sum = 0.f;  // the row's maximum; what weights are relative to
-    bool ok = true;
-    if (issuer && steps) {
-      ok = await(&sh.k_full[0], 0, &sh.dead);
+          for (uint32_t e = 0; e < kWideTile / 16; ++e) product_from_tmem(o, p + 64 + e * 8, v + e * 128, to_o, 1);
+        }
+      };
+      bool ok = __all_sync(~0u, await(&sh.k_full[0], 0, &sh.dead));
       if (ok) {
         after_sync();
-        scores(0);
+        scores(0, 0);
+        scores(1, 0);
+        commit(&sh.k_empty[0]);
       }
+      for (uint32_t i = 0; ok && i < steps; ++i) {
+        const uint32_t st = i & 1, next = st ^ 1;
+        ok = __all_sync(~0u, await(&sh.v_full[st], (i / 2) & 1, &sh.dead));
+#pragma unroll
+        for (uint32_t tile = 0; tile < 2; ++tile) {
+          ok = ok && __all_sync(~0u, await(&sh.p_full[tile], i & 1, &sh.dead));
+          if (!ok) break;
+          after_sync();
+          values(tile, st, i > 0);
+          if (tile == 1) commit(&sh.v_empty[st]);
+          if (i + 1 == steps) continue;
+          if (tile == 0) ok = __all_sync(~0u, await(&sh.k_full[next], ((i + 1) / 2) & 1, &sh.dead));
+          if (!ok) break;
+          after_sync();
+          scores(tile, next);
+          if (tile == 1) commit(&sh.k_empty[next]);
+        }
+      }
+      commit(&sh.done);
+      // (what was issued has to end before TMEM is given back, on a way out too)
+      int alone = 0;
+      await(&sh.done, 0, &alone);
     }
     __syncwarp();
-    // a step's weights; those of positions that the row does not see are 0
-    auto step = [&](auto plain, uint32_t i, int from, int to) {
-      constexpr bool PLAIN = decltype(plain)::value;
+   }
+  } else {
+    // ---- weights: a row a thread
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    const uint32_t lanes = (warp & 3) << 21;  // (32 lanes a warp, in the upper half of an address)
+    float m = -INFINITY, ref = 0.f, unit = 0.f, sum = 0.f;  // the row's maximum; what weights and O are relative to
+    bool ok = true;
+    // (room above for later maxima; for the lower parts, room below)
+    constexpr int kUp = SPLIT ? 4 : 0, kSlack = SPLIT ? 2 : 8;
+    // two weights times their scales, as 16-bit floats, and what those leave
+    auto pair = [&](float2 y, uint32_t& w, uint32_t& low) {
+      w = pack16(y);
+      if constexpr (SPLIT) {
+        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        low = pack16(make_float2(y.x - h.x, y.y - h.y));
+      }
+    };
+    // A step that the rows see all of: its weights in the units of the last one; whether they may be kept.
+    auto quick = [&](uint32_t i, bool sure) {
       const uint32_t ring = i % kRings;
       const float* const kappa = sh.kappa[ring];
       const float* const nu = sh.nu[ring];
-      float r[128];
-#pragma unroll
-      for (uint32_t c = 0; c < 4; ++c) tmem_load(t_s + lanes + c * 32, r, c * 32);
-      float most = fmaxf(fmaxf(nu[lane], nu[lane + 32]), fmaxf(nu[lane + 64], nu[lane + 96]));
-      most = warp_max(most);
-      await_loads();
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (uint32_t c = 0; c < 4; ++c) {
-        uint32_t bits = ~0u;
-        if constexpr (!PLAIN) {
-          const int l = min(max(from - (int)c * 32, 0), 32), h = min(max(to - (int)c * 32, 0), 32);
-          bits = (h >= 32 ? ~0u : (1u << h) - 1) & ~(l >= 32 ? ~0u : (1u << l) - 1) & sh.valid[ring][c];
-        }
-#pragma unroll
-        for (uint32_t e = 0; e < 32; e += 4) {
-          const float4 k4 = *reinterpret_cast<const float4*>(kappa + c * 32 + e);
-          float2 u = mul2(make_float2(r[c * 32 + e], r[c * 32 + e + 1]), make_float2(k4.x, k4.y));
-          float2 v = mul2(make_float2(r[c * 32 + e + 2], r[c * 32 + e + 3]), make_float2(k4.z, k4.w));
-          if constexpr (!PLAIN) {
-            u.x = bits >> e & 1 ? u.x : -INFINITY;
-            u.y = bits >> e & 2 ? u.y : -INFINITY;
-            v.x = bits >> e & 4 ? v.x : -INFINITY;
-            v.y = bits >> e & 8 ? v.y : -INFINITY;
-          }
-          r[c * 32 + e] = u.x;
-          r[c * 32 + e + 1] = u.y;
-          r[c * 32 + e + 2] = v.x;
-          r[c * 32 + e + 3] = v.y;
-          top[c] = fmaxf(fmaxf(top[c], u.x), u.y);
-          top[c] = fmaxf(fmaxf(top[c], v.x), v.y);
-        }
-      }
-      float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-      if (high > -INFINITY) high *= scale;
-      // weights are at most 2^14: 2^8 at the reference, 2^4 from scores above the maximum, 2^2 from scales above their unit
-      const bool larger = most > 4.f * unit;
-      if (__any_sync(~0u, high > m + 4.f || larger)) {
-        if (larger) unit = fmaxf(__uint_as_float(min((__float_as_uint(most) & 0x7f800000u) + 0x00800000u, 0x7e800000u)), 0x1p-90f);
-        const float before = ref;
-        const bool none = m == -INFINITY;
-        m = fmaxf(m, high);
-        // (log2 of a power of two)
-        ref = (m > -INFINITY ? m : 0.f) + (unit > 0.f ? (float)((int)(__float_as_uint(unit) >> 23) - 127) : 0.f) - 8.f;
-        const float f = none ? 0.f : ex2(before - ref);
-        if (i) {
-          sum *= f;
-#pragma unroll 1
-          for (uint32_t c = 0; c < DT / 16; ++c) {
-            float o[16];
-            tmem_load16(t_o + lanes + c * 16, o);
-            await_loads();
-#pragma unroll
-            for (uint32_t e = 0; e < 16; ++e) o[e] *= f;
-            tmem_store16(t_o + lanes + c * 16, *reinterpret_cast<const uint32_t (*)[16]>(&o));
-          }
-        }
-      }
+      float r[2][32];
+      uint32_t w[64];
+      [[maybe_unused]] uint32_t low[SPLIT ? 64 : 1];
+      if (sh.unit[ring] != unit && !sure) return false;
+      tmem_load(t_s + lanes, r[0]);
       float2 add[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
       for (uint32_t c = 0; c < 4; ++c) {
-        uint32_t w[16];
-        [[maybe_unused]] uint32_t low[SPLIT ? 16 : 1];
+        await_loads();
+        if (c < 3) tmem_load(t_s + lanes + (c + 1) * 32, r[(c + 1) & 1]);
+        const float (&x)[32] = r[c & 1];
 #pragma unroll
         for (uint32_t e = 0; e < 32; e += 4) {
-          const float4 n4 = *reinterpret_cast<const float4*>(nu + c * 32 + e);
-          float2 u = fma2(make_float2(r[c * 32 + e], r[c * 32 + e + 1]), both(scale), both(-ref));
-          float2 v = fma2(make_float2(r[c * 32 + e + 2], r[c * 32 + e + 3]), both(scale), both(-ref));
+          const float4 k4 = *reinterpret_cast<const float4*>(kappa + c * 32 + e);
+          float2 u = fma2(make_float2(x[e], x[e + 1]), make_float2(k4.x, k4.y), both(-ref));
+          float2 v = fma2(make_float2(x[e + 2], x[e + 3]), make_float2(k4.z, k4.w), both(-ref));
           u = make_float2(ex2(u.x), ex2(u.y));
           v = make_float2(ex2(v.x), ex2(v.y));
           add[0] = add2(add[0], u);
           add[1] = add2(add[1], v);
-          float2 y = mul2(u, make_float2(n4.x, n4.y)), z = mul2(v, make_float2(n4.z, n4.w));
-          if constexpr (!PLAIN) {  // (no weight, whatever the scale is)
-            y.x = u.x == 0.f ? 0.f : y.x;
-            y.y = u.y == 0.f ? 0.f : y.y;
-            z.x = v.x == 0.f ? 0.f : z.x;
-            z.y = v.y == 0.f ? 0.f : z.y;
-          }
-          w[e / 2] = pack16(y);
-          w[e / 2 + 1] = pack16(z);
           if constexpr (SPLIT) {
-            const float2 y1 = __half22float2(*reinterpret_cast<const __half2*>(&w[e / 2])), z1 = __half22float2(*reinterpret_cast<const __half2*>(&w[e / 2 + 1]));
-            low[e / 2] = pack16(make_float2(y.x - y1.x, y.y - y1.y));
-            low[e / 2 + 1] = pack16(make_float2(z.x - z1.x, z.y - z1.y));
+            const float4 n4 = *reinterpret_cast<const float4*>(nu + c * 32 + e);
+            u = mul2(u, make_float2(n4.x, n4.y));
+            v = mul2(v, make_float2(n4.z, n4.w));
           }
+          pair(u, w[c * 16 + e / 2], low[SPLIT ? c * 16 + e / 2 : 0]);
+          pair(v, w[c * 16 + e / 2 + 1], low[SPLIT ? c * 16 + e / 2 + 1 : 0]);
         }
-        tmem_store16(t_s + lanes + c * 16, w);
-        if constexpr (SPLIT) tmem_store16(t_s + 64 + lanes + c * 16, low);
       }
       add[0] = add2(add[0], add[1]);
-      sum += add[0].x + add[0].y;
+      const float more = add[0].x + add[0].y;
+      // no weight is larger than their sum (their scales, relative to the unit, are 4 at most)
+      if (__any_sync(~0u, !(more <= (SPLIT ? 8192.f : 32768.f))) && !sure) return false;
+#pragma unroll
+      for (uint32_t c = 0; c < 4; ++c) {
+        tmem_store16(t_s + lanes + c * 16, *reinterpret_cast<const uint32_t (*)[16]>(&w[c * 16]));
+        if constexpr (SPLIT) tmem_store16(t_s + 64 + lanes + c * 16, *reinterpret_cast<const uint32_t (*)[16]>(&low[c * 16]));
+      }
+      sum += more;
+      return true;
+    };
+    // O and the sum of weights in units of a higher maximum, or of another unit of V.
+    auto rescale = [&](uint32_t i, float high) {
+      const float before = ref, unit_now = sh.unit[i % kRings];
+      const bool none = m == -INFINITY;
+      m = fmaxf(m, high);
+      ref = (m > -INFINITY ? m : 0.f) - (float)kUp;
+      float f = none ? 0.f : ex2(before - ref);
+      sum *= f;
+      f *= unit_now > 0.f ? unit / unit_now : 0.f;
+      unit = unit_now;
+      if (i == 0) return;
+      float r[32];
+#pragma unroll 1
+      for (uint32_t c = 0; c < DT / 32; ++c) {
+        tmem_load(t_o + lanes + c * 32, r);
+        await_loads();
+#pragma unroll
+        for (uint32_t e = 0; e < 32; e += 2) *reinterpret_cast<float2*>(&r[e]) = mul2(*reinterpret_cast<float2*>(&r[e]), both(f));
+        tmem_store16(t_o + lanes + c * 32, *reinterpret_cast<const uint32_t (*)[16]>(&r[0]));
+        tmem_store16(t_o + lanes + c * 32 + 16, *reinterpret_cast<const uint32_t (*)[16]>(&r[16]));
+      }
+    };
+    auto raise = [&](uint32_t i) {
+      const float* const kappa = sh.kappa[i % kRings];
+      float r[32], high = -INFINITY;
+#pragma unroll 1
+      for (uint32_t c = 0; c < 4; ++c) {
+        tmem_load(t_s + lanes + c * 32, r);
+        await_loads();
+#pragma unroll
+        for (uint32_t e = 0; e < 32; e += 4) {
+          const float4 k4 = *reinterpret_cast<const float4*>(kappa + c * 32 + e);
+          const float2 u = mul2(make_float2(r[e], r[e + 1]), make_float2(k4.x, k4.y)), v = mul2(make_float2(r[e + 2], r[e + 3]), make_float2(k4.z, k4.w));
+          high = fmaxf(fmaxf(high, u.x), u.y);
+          high = fmaxf(fmaxf(high, v.x), v.y);
+        }
+      }
+      rescale(i, high);
+    };
+    // A step of which positions [from, to) are seen.  Seldom run, so small.
+    auto careful = [&](uint32_t i, int from, int to) {
+      const uint32_t ring = i % kRings;
+      const float* const kappa = sh.kappa[ring];
+      [[maybe_unused]] const float* const nu = sh.nu[ring];
+      auto seen_of = [&](uint32_t c) {
+        const int l = min(max(from - (int)c * 32, 0), 32), h = min(max(to - (int)c * 32, 0), 32);
+        return (h >= 32 ? ~0u : (1u << h) - 1) & ~(l >= 32 ? ~0u : (1u << l) - 1) & sh.valid[ring][c];
+      };
+      float r[32], high = -INFINITY;
+#pragma unroll 1
+      for (uint32_t c = 0; c < 4; ++c) {
+        tmem_load(t_s + lanes + c * 32, r);
+        const uint32_t bits = seen_of(c);
+        await_loads();
+#pragma unroll
+        for (uint32_t e = 0; e < 32; ++e) high = fmaxf(high, bits >> e & 1 ? r[e] * kappa[c * 32 + e] : -INFINITY);
+      }
+      if (high > -INFINITY) high *= scale;
+      // weights are at most 2^kUp at the maximum and 2^kSlack more from scores above it
+      if (__any_sync(~0u, high > m + (float)kSlack || sh.unit[ring] != unit)) rescale(i, high);
+      // (the lower parts take the place of the last scores, once those have been read)
+      [[maybe_unused]] uint32_t low[SPLIT ? 64 : 1];
+#pragma unroll(SPLIT ? 4 : 1)
+      for (uint32_t c = 0; c < 4; ++c) {
+        uint32_t w[16];
+        tmem_load(t_s + lanes + c * 32, r);
+        const uint32_t bits = seen_of(c);
+        if (bits & sh.odd[ring][c]) sum = NAN;
+        await_loads();
+#pragma unroll
+        for (uint32_t e = 0; e < 32; e += 2) {
+          float u = ex2(fmaf(r[e] * kappa[c * 32 + e], scale, -ref)), v = ex2(fmaf(r[e + 1] * kappa[c * 32 + e + 1], scale, -ref));
+          u = bits >> e & 1 ? u : 0.f;
+          v = bits >> e & 2 ? v : 0.f;
+          sum += u + v;
+          if constexpr (SPLIT) {
+            u *= nu[c * 32 + e];
+            v *= nu[c * 32 + e + 1];
+          }
+          pair(make_float2(u, v), w[e / 2], low[SPLIT ? c * 16 + e / 2 : 0]);
+        }
+        // (in the place of scores that have been read)
+        tmem_store16(t_s + lanes + c * 16, w);
+      }
+      if constexpr (SPLIT) {
+#pragma unroll
+        for (uint32_t c = 0; c < 4; ++c) tmem_store16(t_s + 64 + lanes + c * 16, *reinterpret_cast<const uint32_t (*)[16]>(&low[c * 16]));
+      }
     };
     for (uint32_t i = 0; i < steps; ++i) {
-      ok = ok && await(&sh.k_full[i & 1], (i / 2) & 1, &sh.dead) && await(&sh.s_full[t], i & 1, &sh.dead);
+      ok = await(&sh.k_full[i & 1], (i / 2) & 1, &sh.dead) && await(&sh.s_full[t], i & 1, &sh.dead);
       if (!__all_sync(~0u, ok)) break;
       after_sync();
       const int64_t p0 = range.lo + (int64_t)i * kWideTile;
-      const int from = (int)max(min(lo - p0, (int64_t)kWideTile), (int64_t)0), to = (int)max(min(hi - p0, (int64_t)kWideTile), (int64_t)0);
       const uint32_t* const v = sh.valid[i % kRings];
-      if (__all_sync(~0u, (v[0] & v[1] & v[2] & v[3]) == ~0u && from == 0 && to == (int)kWideTile)) step(std::true_type{}, i, 0, 0);
-      else step(std::false_type{}, i, from, to);
+      const uint32_t* const x = sh.odd[i % kRings];
+      const bool plain = (v[0] & v[1] & v[2] & v[3]) == ~0u && !(x[0] | x[1] | x[2] | x[3]) && lo <= p0 && hi >= p0 + kWideTile;
+      if (!(uniform && __all_sync(~0u, plain))) {
+        careful(i, (int)max(min(lo - p0, (int64_t)kWideTile), (int64_t)0), (int)max(min(hi - p0, (int64_t)kWideTile), (int64_t)0));
+      } else if (i == 0 || !quick(i, false)) {
+        raise(i);
+        quick(i, true);
+      }
       await_stores();
       before_sync();
       arrive(&sh.p_full[t]);
-      if (issuer) {
-        ok = await(&sh.p_full[t], i & 1, &sh.dead) && await(&sh.v_full[i & 1], (i / 2) & 1, &sh.dead);
-        if (ok) {
-          after_sync();
-          values(i & 1, i > 0);
-          if (i + 1 < steps) {
-            ok = await(&sh.k_full[(i + 1) & 1], ((i + 1) / 2) & 1, &sh.dead);
-            if (ok) {
-              after_sync();
-              scores((i + 1) & 1);
-            }
-          }
-        }
-      }
-      __syncwarp();
     }
-    if (issuer && steps) commit(&sh.done[t]);
-    __syncwarp();
-    // (what was issued has to end before TMEM is given back, on a way out too)
-    int alone = 0;
-    if (steps) ok = await(&sh.done[t], 0, &alone) && ok;
+    if (steps) ok = await(&sh.done, 0, &sh.dead) && ok;
     // ---- the block's rows of the result
     if (!__all_sync(~0u, ok)) sum = NAN;  // given up: shows in the results
     after_sync();
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const float inv = sum == 0.f ? 0.f : unit / sum;
 #pragma unroll
     for (uint32_t c = 0; c < DT / 32; ++c) {
       float r[32];
@@ -570,7 +699,7 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
     before_sync();
   }
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 15) {
     after_sync();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }

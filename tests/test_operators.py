@@ -698,8 +698,9 @@ def check_attend(got, q, cache, queries, lse=None, first=0, **how):
     # a score: d products summed by tensor cores, 2^-23 a step of 16 and of what they add, and 6 roundings of its scales
     # and of the exponential's argument, the exponential 2^-22; it moves a weight and the sum of weights by as much
     score = 2 * ((d / 16 + 8) * 2.0 ** -23 * terms + 2.0 ** -22)
-    # a weight in 16-bit floats: half a step (2^-11), of the split ones 2^-22; the sums over the positions
-    weight = 2.0 ** -11 if q.dtype is BF else 2.0 ** -21
+    # bf16: a weight, a value's scale and their product are 16-bit floats, half a step (2^-11) each; else weights of two
+    # parts, 2^-22; the sums over the positions
+    weight = 3 * 2.0 ** -11 if q.dtype is BF else 2.0 ** -21
     tol = rounding(q.dtype, want) + size * (weight + score[..., None] + (longest / 16 + 64) * 2.0 ** -23)
     err = (got.cpu().double() - want).abs()
     assert bool((err <= tol + 1e-30).all()), (err / (tol + 1e-30)).max()
