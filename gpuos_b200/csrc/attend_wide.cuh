@@ -315,9 +315,9 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
   after_sync();
   const uint32_t tmem = sh.tmem, t_s = tmem + t * 128, t_o = tmem + 256 + t * DT;
 
-  // (256 * 184 + 256 * 72 registers: the 512 * 128 of the launch)
+  // (256 * 168 + 256 * 88 registers: the 512 * 128 of the launch)
   if (warp >= 8) {
-   asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+   asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
    if (warp < 8 + kCodeWarps) {
     // ---- codes: a thread finds a position; then 8 (heads up to 64: 4) threads load one, 16 bytes each
     const uint32_t j = tid - 256;
@@ -331,30 +331,41 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
     const uint8_t* const v_codes = a.v.codes + head * a.v.ch + piece * 16;
     const Power down(uniform && sh.top > -127 ? sh.top - 14 : 0);
     const float by = uniform ? fabsf(a.scale2) * down.a : 1.f;
-    auto page_at = [&](uint32_t step) -> int32_t {  // of this thread's position; -1: not seen
+    // A position's page is read two steps ahead, its scales one (nothing waits for them).
+    auto page_at = [&](uint32_t step) -> int64_t {  // as the table has it; -1 behind the range
       const int64_t p = range.lo + (int64_t)step * kWideTile + j;
-      if (j >= kWideTile || p >= range.hi) return -1;
-      const int64_t g = load_index(a.pages, a.page_wide, table + a.page.div((uint32_t)p) * a.pp);
-      return g >= 0 && g < a.pool ? (int32_t)g : -1;
+      if (warp >= 12 || p >= range.hi) return -1;
+      return load_index(a.pages, a.page_wide, table + a.page.div((uint32_t)p) * a.pp);
     };
-    float kappa = 0.f, nu = 0.f;
+    float kappa = 0.f, nu = 0.f;       // of the step that is put next
+    float kappa1 = 0.f, nu1 = 0.f;     // of the one behind it
     uint32_t valid = 0, odd = 0;
-    auto find = [&](uint32_t step, int32_t page) {
-      if (warp >= 12) return arrive(&sh.where_full);  // (it has read what was there)
+    int64_t k_at = -1, v_at = -1, page2 = -1;
+    auto ahead = [&](uint32_t step, int64_t page) {  // places of a step's codes, and its scales
+      k_at = v_at = -1;
+      kappa1 = nu1 = 0.f;
+      if (warp >= 12 || page < 0 || page >= a.pool) return;
       const uint32_t p = (uint32_t)(range.lo + (int64_t)step * kWideTile + j), at = p - a.page.div(p) * a.page.d;
-      const bool has = page >= 0;
-      sh.where[step & 1][0][j] = has ? page * a.k.cp + at * a.k.cr : -1;
-      sh.where[step & 1][1][j] = has ? page * a.v.cp + at * a.v.cr : -1;
-      kappa = has ? __ldg(a.k.scales + page * a.k.sp + at * a.k.sr + head * a.k.sh) : 0.f;
-      nu = has ? __ldg(a.v.scales + page * a.v.sp + at * a.v.sr + head * a.v.sh) : 0.f;
-      valid = __ballot_sync(~0u, has);
-      // a scale that is not finite makes NaN of the rows that see it, and must not touch others: it is not multiplied
-      const bool fine = fabsf(nu) < INFINITY;
-      odd = __ballot_sync(~0u, !fine);
-      if (!fine) nu = 0.f;
-      const float high = warp_max(nu);
-      if (lane == 0) sh.most[step & 1][warp - 8] = high;
-      arrive(&sh.where_full);
+      k_at = page * a.k.cp + at * a.k.cr;
+      v_at = page * a.v.cp + at * a.v.cr;
+      kappa1 = __ldg(a.k.scales + page * a.k.sp + at * a.k.sr + head * a.k.sh);
+      nu1 = __ldg(a.v.scales + page * a.v.sp + at * a.v.sr + head * a.v.sh);
+    };
+    auto find = [&](uint32_t step) {
+      if (warp < 12) {
+        sh.where[step & 1][0][j] = k_at;
+        sh.where[step & 1][1][j] = v_at;
+        kappa = kappa1;
+        nu = nu1;
+        valid = __ballot_sync(~0u, k_at >= 0);
+        // a scale that is not finite makes NaN of the rows that see it, and must not touch others: it is not multiplied
+        const bool fine = fabsf(nu) < INFINITY;
+        odd = __ballot_sync(~0u, !fine);
+        if (!fine) nu = 0.f;
+        const float high = warp_max(nu);
+        if (lane == 0) sh.most[step & 1][warp - 8] = high;
+      }
+      arrive(&sh.where_full);  // (who finds nothing has read what was there)
     };
     // V is brought in relative to a power of two that is raised when a scale passes it by 2^2
     float unit = 0.f;
@@ -398,10 +409,11 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
     };
     uint4 rk[N], rv[N];
     bool ok = true;
-    int32_t page = -1;
     if (steps) {
-      find(0, page_at(0));
-      page = steps > 1 ? page_at(1) : -1;
+      ahead(0, page_at(0));
+      find(0);
+      ahead(1, page_at(1));
+      page2 = page_at(2);
       ok = await(&sh.where_full, 0, &sh.dead);
       if (ok) {
         raise(0);
@@ -422,8 +434,9 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
       arrive(&sh.k_full[st]);
       if (i + 1 < steps) {
         __syncwarp();
-        find(i + 1, page);
-        page = i + 2 < steps ? page_at(i + 2) : -1;
+        find(i + 1);
+        ahead(i + 2, page2);
+        page2 = page_at(i + 3);
         if (!await(&sh.where_full, (i + 1) & 1, &sh.dead)) break;  // (and this step's scales are there)
         raise(i + 1);
         load(k_codes, i + 1, 0, rk);
@@ -493,7 +506,7 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
    }
   } else {
     // ---- weights: a row a thread
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const uint32_t lanes = (warp & 3) << 21;  // (32 lanes a warp, in the upper half of an address)
     float m = -INFINITY, ref = 0.f, unit = 0.f, sum = 0.f;  // the row's maximum; what weights and O are relative to
     bool ok = true;
@@ -512,33 +525,34 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
       const uint32_t ring = i % kRings;
       const float* const kappa = sh.kappa[ring];
       const float* const nu = sh.nu[ring];
-      float r[2][32];
+      // 16 scores at a time while the next ones are on their way (32 at a time left no registers for their scales ahead)
+      float r[2][16];
       uint32_t w[64];
       [[maybe_unused]] uint32_t low[SPLIT ? 64 : 1];
       if (sh.unit[ring] != unit && !sure) return false;
-      tmem_load(t_s + lanes, r[0]);
+      tmem_load16(t_s + lanes, r[0]);
       float2 add[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
-      for (uint32_t c = 0; c < 4; ++c) {
-        await_loads();
-        if (c < 3) tmem_load(t_s + lanes + (c + 1) * 32, r[(c + 1) & 1]);
-        const float (&x)[32] = r[c & 1];
+      for (uint32_t c = 0; c < 8; ++c) {
+        float4 k4[4];
 #pragma unroll
-        for (uint32_t e = 0; e < 32; e += 4) {
-          const float4 k4 = *reinterpret_cast<const float4*>(kappa + c * 32 + e);
-          float2 u = fma2(make_float2(x[e], x[e + 1]), make_float2(k4.x, k4.y), both(-ref));
-          float2 v = fma2(make_float2(x[e + 2], x[e + 3]), make_float2(k4.z, k4.w), both(-ref));
-          u = make_float2(ex2(u.x), ex2(u.y));
-          v = make_float2(ex2(v.x), ex2(v.y));
-          add[0] = add2(add[0], u);
-          add[1] = add2(add[1], v);
-          if constexpr (SPLIT) {
-            const float4 n4 = *reinterpret_cast<const float4*>(nu + c * 32 + e);
-            u = mul2(u, make_float2(n4.x, n4.y));
-            v = mul2(v, make_float2(n4.z, n4.w));
-          }
-          pair(u, w[c * 16 + e / 2], low[SPLIT ? c * 16 + e / 2 : 0]);
-          pair(v, w[c * 16 + e / 2 + 1], low[SPLIT ? c * 16 + e / 2 + 1 : 0]);
+        for (uint32_t e = 0; e < 4; ++e) k4[e] = *reinterpret_cast<const float4*>(kappa + c * 16 + e * 4);
+        await_loads();
+        if (c < 7) tmem_load16(t_s + lanes + (c + 1) * 16, r[(c + 1) & 1]);
+        const float (&x)[16] = r[c & 1];
+        float2 y[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+          y[2 * e] = fma2(make_float2(x[4 * e], x[4 * e + 1]), make_float2(k4[e].x, k4[e].y), both(-ref));
+          y[2 * e + 1] = fma2(make_float2(x[4 * e + 2], x[4 * e + 3]), make_float2(k4[e].z, k4[e].w), both(-ref));
+        }
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) y[e] = make_float2(ex2(y[e].x), ex2(y[e].y));
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+          add[e & 1] = add2(add[e & 1], y[e]);
+          if constexpr (SPLIT) y[e] = mul2(y[e], *reinterpret_cast<const float2*>(nu + c * 16 + e * 2));
+          pair(y[e], w[c * 8 + e], low[SPLIT ? c * 8 + e : 0]);
         }
       }
       add[0] = add2(add[0], add[1]);
