@@ -24,7 +24,9 @@ namespace {
 
 constexpr uint32_t kWideTile = 128, kWideThreads = 512;  // 8 warps of weights, 7 of codes, one that issues products
 constexpr uint32_t kCodeWarps = 7;
-constexpr uint32_t kRings = 4;  // of scales: the weights' warps read them after the products that K fed
+// Of scales: the weights' warps read them after the products that K fed.  (They may be a step behind the warps of codes but
+// not four, so that a phase cannot pass unseen; of the two stages of K it could.)
+constexpr uint32_t kRings = 4;
 
 template <int DT>
 struct Wide {
@@ -35,7 +37,7 @@ struct Wide {
 };
 
 struct WideShared {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], done, where_full;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], scales_full[kRings], done, where_full;
   uint32_t tmem;
   int dead, top, uniform;  // top: the largest exponent in the block's q
   uint32_t valid[kRings][4], odd[kRings][4];  // positions with a page; whose scale of V is not finite
@@ -270,6 +272,7 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
       barrier_init(&sh.p_full[i], 128);
       
     }
+    for (uint32_t i = 0; i < kRings; ++i) barrier_init(&sh.scales_full[i], 128);
     barrier_init(&sh.done, 1);
     barrier_init(&sh.where_full, 32 * kCodeWarps);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -430,6 +433,7 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
         sh.nu[ring][j] = unit > 0.f ? nu * __uint_as_float(0x7f000000u - __float_as_uint(unit)) : 0.f;
         if (lane == 0) sh.valid[ring][warp - 8] = valid, sh.odd[ring][warp - 8] = odd;
         if (tid == 256) sh.unit[ring] = unit;
+        arrive(&sh.scales_full[ring]);
       }
       arrive(&sh.k_full[st]);
       if (i + 1 < steps) {
@@ -657,7 +661,7 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
       }
     };
     for (uint32_t i = 0; i < steps; ++i) {
-      ok = await(&sh.k_full[i & 1], (i / 2) & 1, &sh.dead) && await(&sh.s_full[t], i & 1, &sh.dead);
+      ok = await(&sh.scales_full[i % kRings], (i / kRings) & 1, &sh.dead) && await(&sh.s_full[t], i & 1, &sh.dead);
       if (!__all_sync(~0u, ok)) break;
       after_sync();
       const int64_t p0 = range.lo + (int64_t)i * kWideTile;
