@@ -146,6 +146,8 @@ extern "C" int32_t gpuos_attend(const gpuos_tensor* q, const gpuos_tensor* codes
       h.sg = scales[i].strides[3];
       while (a.vec > 1 && !rows_aligned(codes[i], a.vec)) a.vec = a.vec == 16 ? 4 : 1;
     }
+    a.alike = 1;
+    for (int d = 0; d < 3; ++d) a.alike &= codes[0].strides[d] == codes[1].strides[d];
     a.pages = pages->data;
     a.ps = pages->strides[0];
     a.pp = pages->strides[1];

@@ -35,7 +35,8 @@ constexpr float kSmallestUnit = 0x1p-100f;
 template <int DT, int NT, bool GEN>
 struct Layout {
   static constexpr uint32_t rows = 8 * NT;
-  static constexpr uint32_t stages = GEN ? 2 : 3;
+  static constexpr uint32_t per_sm = ctas(DT, NT);
+  static constexpr uint32_t stages = GEN || per_sm == 3 ? 2 : 3;
   static constexpr uint32_t scales = GEN ? DT / 32 : 1;                 // of a row, room for
   static constexpr uint32_t codes = kTile * DT;                         // bytes, of K or V
   static constexpr uint32_t stage = 2 * codes + 2 * kTile * scales * 4 + 16;
@@ -126,7 +127,7 @@ __device__ __forceinline__ Item find(const Args& a, uint32_t seq, const Sequence
 }
 
 template <int F, int DT, int NT, bool GEN>
-__global__ void __launch_bounds__(kThreads, DT == 256 ? 1 : 2)
+__global__ void __launch_bounds__(kThreads, ctas(DT, NT))
 gpuos_attend_kernel(const __grid_constant__ Args a) {
   using L = Layout<DT, NT, GEN>;
   constexpr uint32_t RB = L::rows, kStages = L::stages;
@@ -148,6 +149,7 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
   uint8_t* const sq = smem + kWarps * L::ring;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
 
+  asm volatile("griddepcontrol.launch_dependents;");
   // tokens of no sequence get zeros
   if (a.offsets) {
     const int64_t end = min(max(load_index(a.offsets, a.offset_wide, (int64_t)a.sequences * a.os), (int64_t)0), (int64_t)a.tokens);
@@ -255,13 +257,14 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
         const bool has = page >= 0;
         const int64_t k_at = has ? page * a.k.cp + row * a.k.cr + it.head * a.k.ch : 0;
         const int64_t v_at = has ? page * a.v.cp + row * a.v.cr + it.head * a.v.ch : 0;
+        const uint32_t valid = __ballot_sync(~0u, has);
         constexpr uint32_t X = DT / 16;
         if (a.vec == 16) {
 #pragma unroll
           for (uint32_t r0 = 0; r0 < X; ++r0) {
             const uint32_t r = r0 * (32 / X) + lane / X, x = lane % X;
-            const int64_t ko = __shfl_sync(~0u, k_at, r), vo = __shfl_sync(~0u, v_at, r);
-            const bool in = __shfl_sync(~0u, has, r) && x * 16 < a.head;
+            const int64_t ko = __shfl_sync(~0u, k_at, r), vo = a.alike ? ko : __shfl_sync(~0u, v_at, r);
+            const bool in = (valid >> r & 1) && x * 16 < a.head;
             const uint32_t at = place<DT>(r, x);
             copy16(to + at, a.k.codes + ko + (in ? x * 16 : 0), in);
             copy16(to + L::codes + at, a.v.codes + vo + (in ? x * 16 : 0), in);
@@ -270,7 +273,7 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
           uint8_t* const stage = ring + (i % kStages) * L::stage;
           for (uint32_t r = 0; r < kTile; ++r) {
             const int64_t ko = __shfl_sync(~0u, k_at, r), vo = __shfl_sync(~0u, v_at, r);
-            const bool in = __shfl_sync(~0u, has, r);
+            const bool in = valid >> r & 1;
             for (uint32_t e = lane * 4; e < DT; e += 128) {
               const uint32_t at = place<DT>(r, e >> 4) + (e & 15);
               if (a.vec == 4) {
@@ -293,7 +296,6 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
           copy4(sc + (gr * kTile + lane) * 4, a.k.scales + ks + gr * a.k.sg, has);
           copy4(sc + ((L::scales + gr) * kTile + lane) * 4, a.v.scales + vs + gr * a.v.sg, has);
         }
-        const uint32_t valid = __ballot_sync(~0u, has);
         if (lane == 0) *reinterpret_cast<uint32_t*>(ring + (i % kStages) * L::stage + 2 * L::codes + 2 * kTile * L::scales * 4) = valid;
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -659,36 +661,42 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
   if (tid == 0 && a.split) a.split[blockIdx.x] = goes_on;
 }
 
-// Joins the parts of split items, in the order of the CTAs that made them.
+// Joins the parts of split items, in the order of the CTAs that made them; a warp takes a row.  (Launched while the
+// other kernel runs, so that its start is not waited for: it waits here.)
 template <uint32_t RB>
-__global__ void __launch_bounds__(kThreads) gpuos_attend_join_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(256) gpuos_attend_join_kernel(const __grid_constant__ Args a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 it = a.split[blockIdx.x];
   if (it.w == 0) return;
   const Sequence s = sequence(a, (uint32_t)it.x);
-  const uint32_t row0 = (uint32_t)it.z * RB;
+  const uint32_t row0 = (uint32_t)it.z * RB, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rows = (uint32_t)min((int64_t)RB, s.n * a.each - row0);
   const uint32_t stride = a.head + 2;
-  for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
+  for (uint32_t r = warp; r < rows; r += 8) {
     auto part = [&](int i) { return a.partial + (((size_t)blockIdx.x + i) * 2 + (i == 0)) * RB * stride + r * stride; };
     float top = -INFINITY;
-    for (int i = 0; i <= it.w; ++i) top = fmaxf(top, part(i)[a.head]);
+    for (int i = lane; i <= it.w; i += 32) top = fmaxf(top, part(i)[a.head]);
+    top = warp_max(top);
+    float sum = 0.f, x[kMaxHead / 32];
+#pragma unroll
+    for (uint32_t k = 0; k < kMaxHead / 32; ++k) x[k] = 0.f;
+#pragma unroll 4
+    for (int i = 0; i <= it.w; ++i) {
+      const float* const p = part(i);
+      const float m = p[a.head], f = m == -INFINITY ? 0.f : ex2(m - top);
+      if (f == 0.f) continue;  // (nothing seen, or nothing of weight)
+      sum += f * p[a.head + 1];
+#pragma unroll
+      for (uint32_t k = 0; k < kMaxHead / 32; ++k)
+        if (k * 32 + lane < a.head) x[k] += f * p[k * 32 + lane];
+    }
     const uint32_t query = a.each_div.div(row0 + r), h = it.y * a.each + row0 + r - query * a.each;
     const int64_t t = s.first + query;
-    float sum = 0.f;
-    for (int i = 0; i <= it.w; ++i) {
-      const float m = part(i)[a.head];
-      if (m != -INFINITY) sum += ex2(m - top) * part(i)[a.head + 1];
-    }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    for (uint32_t e = threadIdx.x; e < a.head; e += kThreads) {
-      float x = 0.f;
-      for (int i = 0; i <= it.w; ++i) {
-        const float m = part(i)[a.head];
-        if (m != -INFINITY) x += ex2(m - top) * part(i)[e];
-      }
-      store_real(a.out, a.type, t * a.ot + h * a.oh + e, x * inv);
-    }
-    if (a.lse && threadIdx.x == 0) a.lse[t * a.lt + h * a.lh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718056f;
+#pragma unroll
+    for (uint32_t k = 0; k < kMaxHead / 32; ++k)
+      if (k * 32 + lane < a.head) store_real(a.out, a.type, t * a.ot + h * a.oh + k * 32 + lane, x[k] * inv);
+    if (a.lse && lane == 0) a.lse[t * a.lt + h * a.lh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718056f;
   }
 }
 
@@ -698,7 +706,17 @@ void start(const Args& a, cudaStream_t stream) {
   void (*const kernel)(const Args) = gpuos_attend_kernel<F, DT, NT, GEN>;
   cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::total), "shared memory");
   run(kernel, dim3(a.grid), kThreads, L::total, stream, a);
-  if (a.split) run(gpuos_attend_join_kernel<L::rows>, dim3(a.grid, 8), kThreads, 0, stream, a);
+  if (!a.split) return;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(a.grid);
+  c.blockDim = dim3(256);
+  c.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = at;
+  c.numAttrs = 1;
+  cuda_ok(cudaLaunchKernelEx(&c, gpuos_attend_join_kernel<L::rows>, a), "launch");
 }
 
 template <int F, int DT>

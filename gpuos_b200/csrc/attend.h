@@ -53,6 +53,7 @@ struct Args {
   FastDiv page, each_div;
   int causal, type;        // type: of q and out
   int page_wide, length_wide, offset_wide;
+  int alike;               // keys and values have the same strides
   int vec;                 // bytes of codes loaded at once: 16, 4 or 1
   int split_q, split_p;    // 16-bit parts of q and p: one, or two
 };
@@ -150,6 +151,10 @@ __device__ __forceinline__ void store_real(void* p, int type, int64_t i, float v
   else static_cast<__nv_bfloat16*>(p)[i] = from_f<__nv_bfloat16>(v);
 }
 
+// CTAs of an SM: three leave 168 registers a thread, enough for 8 rows.  (64 sequences of 8000 e4m3 positions, 8 rows: AAA us
+// with three and two stages of codes, 217 with two and three.)
+__host__ __device__ constexpr uint32_t ctas(uint32_t padded, uint32_t tiles) { return padded == 256 ? 1 : tiles == 1 ? 3 : 2; }
+
 // Launches of one format (attend_int8.cu, attend_e4m3.cu).  `rows`: of a block.
 struct Plan {
   uint32_t tiles;   // of 8 rows
@@ -162,7 +167,7 @@ inline Plan plan(uint32_t head, uint32_t groups, bool split, int64_t rows) {
   p.padded = head <= 64 ? 64 : head <= 128 ? 128 : 256;
   p.general = groups > 1 || split;
   p.tiles = p.general ? 2 : rows <= 8 ? 1 : p.padded == 256 ? 2 : 4;
-  p.per_sm = p.padded == 256 ? 1 : 2;
+  p.per_sm = ctas(p.padded, p.general ? 2 : p.tiles);
   return p;
 }
 template <int F> void launch(const Plan& p, const Args& a, cudaStream_t stream);
