@@ -147,7 +147,7 @@ extern "C" int32_t gpuos_attend(const gpuos_tensor* q, const gpuos_tensor* codes
       while (a.vec > 1 && !rows_aligned(codes[i], a.vec)) a.vec = a.vec == 16 ? 4 : 1;
     }
     a.alike = 1;
-    for (int d = 0; d < 3; ++d) a.alike &= codes[0].strides[d] == codes[1].strides[d];
+    for (int d = 0; d < 3; ++d) a.alike &= codes[0].strides[d] == codes[1].strides[d] && scales[0].strides[d] == scales[1].strides[d];
     a.pages = pages->data;
     a.ps = pages->strides[0];
     a.pp = pages->strides[1];

@@ -231,9 +231,9 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
       continue;
     }
     const Item it = find<RB>(a, seq, s, unit);
-    const int64_t take = min(it.units - it.from, todo);
+    const uint32_t take = (uint32_t)min(it.units - it.from, todo);
     const Range range = block_range<RB>(a, s, it.block);
-    const int64_t begin = range.lo + it.from * kUnit + warp * kTile;
+    const uint32_t begin = (uint32_t)(range.lo + it.from * kUnit) + warp * kTile, stop = (uint32_t)range.hi;  // (below 2^31 + 2^8)
     const uint32_t row0 = (uint32_t)(it.block * RB), row_count = (uint32_t)min((int64_t)RB, s.n * a.each - row0);
     // positions that every row sees
     const int64_t all_hi = last_seen(a, s, a.each_div.div(row0)) + 1;
@@ -241,62 +241,70 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
 
     // ---- loads: 32 positions of this warp into a stage
     const int64_t table = it.seq * a.ps;
-    auto page_at = [&](int64_t j) -> int64_t {  // of position j; -1 where there is none
-      if (j >= range.hi) return -1;
-      const int64_t p = load_index(a.pages, a.page_wide, table + a.page.div((uint32_t)j) * a.pp);
-      return p >= 0 && p < a.pool ? p : -1;
+    const uint8_t* const k_codes = a.k.codes + it.head * a.k.ch;
+    const uint8_t* const v_codes = a.v.codes + it.head * a.v.ch;
+    const float* const k_scales = a.k.scales + it.head * a.k.sh;
+    const float* const v_scales = a.v.scales + it.head * a.v.sh;
+    auto page_at = [&](uint32_t j) -> int32_t {  // of position j; -1 where there is none
+      if (j >= stop) return -1;
+      const int64_t p = load_index(a.pages, a.page_wide, table + a.page.div(j) * a.pp);
+      return p >= 0 && p < a.pool ? (int32_t)p : -1;
     };
-    int64_t next_page = page_at(begin + lane);
-    auto issue = [&](int64_t i) {  // unit i of the share
+    int32_t next_page = page_at(begin + lane);
+    uint32_t fill = 0;                          // the stage that is filled next
+    auto issue = [&](uint32_t i) {  // unit i of the share
       if (i < take) {
-        const uint32_t to = ring_at + (uint32_t)(i % kStages) * L::stage;
-        const int64_t j = begin + i * kUnit + lane;
-        const int64_t page = next_page;
+        const uint32_t to = ring_at + fill;
+        const uint32_t j = begin + i * kUnit + lane;
+        const int32_t page = next_page;
         if (i + 1 < take) next_page = page_at(j + kUnit);
-        const uint32_t row = (uint32_t)j - a.page.div((uint32_t)j) * a.page.d;
+        const uint32_t row = j - a.page.div(j) * a.page.d;
         const bool has = page >= 0;
-        const int64_t k_at = has ? page * a.k.cp + row * a.k.cr + it.head * a.k.ch : 0;
-        const int64_t v_at = has ? page * a.v.cp + row * a.v.cr + it.head * a.v.ch : 0;
+        const int64_t k_at = has ? page * a.k.cp + row * a.k.cr : 0;
+        const int64_t v_at = a.alike ? k_at : has ? page * a.v.cp + row * a.v.cr : 0;
         const uint32_t valid = __ballot_sync(~0u, has);
         constexpr uint32_t X = DT / 16;
         if (a.vec == 16) {
+          const uint32_t x = lane % X;
+          const bool inside = x * 16 < a.head;
 #pragma unroll
           for (uint32_t r0 = 0; r0 < X; ++r0) {
-            const uint32_t r = r0 * (32 / X) + lane / X, x = lane % X;
+            const uint32_t r = r0 * (32 / X) + lane / X;
             const int64_t ko = __shfl_sync(~0u, k_at, r), vo = a.alike ? ko : __shfl_sync(~0u, v_at, r);
-            const bool in = (valid >> r & 1) && x * 16 < a.head;
+            const bool in = (valid >> r & 1) && inside;
             const uint32_t at = place<DT>(r, x);
-            copy16(to + at, a.k.codes + ko + (in ? x * 16 : 0), in);
-            copy16(to + L::codes + at, a.v.codes + vo + (in ? x * 16 : 0), in);
+            copy16(to + at, k_codes + ko + (inside ? x * 16 : 0), in);
+            copy16(to + L::codes + at, v_codes + vo + (inside ? x * 16 : 0), in);
           }
         } else {
-          uint8_t* const stage = ring + (i % kStages) * L::stage;
+          uint8_t* const stage = ring + fill;
           for (uint32_t r = 0; r < kTile; ++r) {
             const int64_t ko = __shfl_sync(~0u, k_at, r), vo = __shfl_sync(~0u, v_at, r);
             const bool in = valid >> r & 1;
             for (uint32_t e = lane * 4; e < DT; e += 128) {
               const uint32_t at = place<DT>(r, e >> 4) + (e & 15);
               if (a.vec == 4) {
-                copy4(to + at, a.k.codes + ko + (in && e < a.head ? e : 0), in && e < a.head);
-                copy4(to + L::codes + at, a.v.codes + vo + (in && e < a.head ? e : 0), in && e < a.head);
+                copy4(to + at, k_codes + ko + (in && e < a.head ? e : 0), in && e < a.head);
+                copy4(to + L::codes + at, v_codes + vo + (in && e < a.head ? e : 0), in && e < a.head);
               } else {
 #pragma unroll
                 for (uint32_t b = 0; b < 4; ++b) {
-                  stage[at + b] = in && e < a.head ? a.k.codes[ko + e + b] : 0;
-                  stage[L::codes + at + b] = in && e < a.head ? a.v.codes[vo + e + b] : 0;
+                  stage[at + b] = in && e < a.head ? k_codes[ko + e + b] : 0;
+                  stage[L::codes + at + b] = in && e < a.head ? v_codes[vo + e + b] : 0;
                 }
               }
             }
           }
         }
         const uint32_t sc = to + 2 * L::codes;
-        const int64_t ks = has ? page * a.k.sp + row * a.k.sr + it.head * a.k.sh : 0;
-        const int64_t vs = has ? page * a.v.sp + row * a.v.sr + it.head * a.v.sh : 0;
+        const int64_t ks = has ? page * a.k.sp + row * a.k.sr : 0;
+        const int64_t vs = a.alike ? ks : has ? page * a.v.sp + row * a.v.sr : 0;
         for (uint32_t gr = 0; gr < (GEN ? a.groups : 1); ++gr) {
-          copy4(sc + (gr * kTile + lane) * 4, a.k.scales + ks + gr * a.k.sg, has);
-          copy4(sc + ((L::scales + gr) * kTile + lane) * 4, a.v.scales + vs + gr * a.v.sg, has);
+          copy4(sc + (gr * kTile + lane) * 4, k_scales + ks + gr * a.k.sg, has);
+          copy4(sc + ((L::scales + gr) * kTile + lane) * 4, v_scales + vs + gr * a.v.sg, has);
         }
-        if (lane == 0) *reinterpret_cast<uint32_t*>(ring + (i % kStages) * L::stage + 2 * L::codes + 2 * kTile * L::scales * 4) = valid;
+        if (lane == 0) *reinterpret_cast<uint32_t*>(ring + fill + 2 * L::codes + 2 * kTile * L::scales * 4) = valid;
+        fill = fill + L::stage == kStages * L::stage ? 0 : fill + L::stage;
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -364,12 +372,14 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) m[t][0] = m[t][1] = -INFINITY, l[t][0] = l[t][1] = 0.f;
 
-    for (int64_t i = 0; i < take; ++i) {
+    uint32_t drain = 0;  // the stage that is read next
+    for (uint32_t i = 0; i < take; ++i) {
       __syncwarp();  // the stage that is filled next has been read by all
       issue(i + kStages - 1);
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
       __syncwarp();
-      const uint8_t* const stage = ring + (i % kStages) * L::stage;
+      const uint8_t* const stage = ring + drain;
+      drain = drain + L::stage == kStages * L::stage ? 0 : drain + L::stage;
       const float* const kappa = reinterpret_cast<const float*>(stage + 2 * L::codes);
       const float* const nu = kappa + L::scales * kTile;
       const uint32_t valid = *reinterpret_cast<const uint32_t*>(nu + L::scales * kTile);
