@@ -694,11 +694,10 @@ __global__ void __launch_bounds__(256) gpuos_attend_join_kernel(const __grid_con
     for (int i = 0; i <= it.w; ++i) {
       const float* const p = part(i);
       const float m = p[a.head], f = m == -INFINITY ? 0.f : ex2(m - top);
-      if (f == 0.f) continue;  // (nothing seen, or nothing of weight)
       sum += f * p[a.head + 1];
 #pragma unroll
-      for (uint32_t k = 0; k < kMaxHead / 32; ++k)
-        if (k * 32 + lane < a.head) x[k] += f * p[k * 32 + lane];
+      for (uint32_t k = 0; k < kMaxHead / 32; ++k)  // (a part of no weight adds nothing, whatever it holds)
+        if (k * 32 < a.head) x[k] += k * 32 + lane < a.head && f != 0.f ? f * p[k * 32 + lane] : 0.f;
     }
     const uint32_t query = a.each_div.div(row0 + r), h = it.y * a.each + row0 + r - query * a.each;
     const int64_t t = s.first + query;

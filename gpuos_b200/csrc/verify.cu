@@ -37,7 +37,8 @@ constexpr uint32_t kKept = 16;             // steps of a warp whose lanes' sums 
 constexpr uint32_t kMaxDrafts = 63;
 constexpr uint32_t kMaxTokens = 1u << 24;  // of a row
 constexpr int kPack = 8;                   // elements a lane takes at once
-constexpr int kFlight = 4;                 // packs a lane has in flight
+// Packs a lane has in flight: 128 bytes.  (32 x 8 x 128257 bf16 with probabilities: 65 us with half of that.)
+template <typename T> constexpr int kFlight = 16 / sizeof(T);
 constexpr float kLowest = -3.402823466e38f;
 
 struct VerifyArgs {
@@ -63,6 +64,11 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
+template <typename T>
+struct alignas(16) Elements {
+  T v[kPack];
+};
+
 // A row as packs of 8 elements that start on 16 bytes (of 16-bit elements; 32 of 32-bit ones): the first and the last
 // may lie partly outside the row.
 template <typename T>
@@ -74,20 +80,22 @@ struct Row {
   __device__ uint32_t packs() const { return (cols + shift + kPack - 1) / kPack; }
   // the 8 elements from `first()` of pack p on; -inf outside the row
   __device__ int64_t first(uint32_t p) const { return (int64_t)p * kPack - shift; }
-  __device__ void load(uint32_t p, float (&v)[kPack]) const {
+  __device__ void load(uint32_t p, Elements<T>& v) const {
     const int64_t e = first(p);
     if (e >= 0 && e + kPack <= cols) {
       constexpr int W = 16 / sizeof(T);
 #pragma unroll
-      for (int k = 0; k < kPack; k += W) {
-        const Pack<T, W> q = load_pack<T, W, false>(x + e + k);
-#pragma unroll
-        for (int i = 0; i < W; ++i) v[k + i] = to_f(q.v[i]);
-      }
+      for (int k = 0; k < kPack; k += W) *reinterpret_cast<Pack<T, W>*>(&v.v[k]) = load_pack<T, W, false>(x + e + k);
     } else {
 #pragma unroll
-      for (int i = 0; i < kPack; ++i) v[i] = e + i >= 0 && e + i < cols ? to_f(x[e + i]) : -INFINITY;
+      for (int i = 0; i < kPack; ++i) v.v[i] = e + i >= 0 && e + i < cols ? x[e + i] : from_f<T>(-INFINITY);
     }
+  }
+  __device__ void load(uint32_t p, float (&v)[kPack]) const {
+    Elements<T> q;
+    load(p, q);
+#pragma unroll
+    for (int i = 0; i < kPack; ++i) v[i] = to_f(q.v[i]);
   }
 };
 
@@ -131,6 +139,22 @@ __device__ __forceinline__ unsigned long long max_warp(unsigned long long v) {
 #pragma unroll
   for (int d = 16; d; d >>= 1) v = max(v, __shfl_xor_sync(~0u, v, d));
   return v;
+}
+
+// The largest of 8 elements (16-bit ones two at a time; a NaN does not count).
+template <typename T>
+__device__ __forceinline__ float largest(const Elements<T>& x) {
+  if constexpr (sizeof(T) == 2) {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    const T2* h = reinterpret_cast<const T2*>(&x);
+    const T2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(to_f(m.x), to_f(m.y));
+  } else {
+    float m = x.v[0];
+#pragma unroll
+    for (int i = 1; i < kPack; ++i) m = fmaxf(m, x.v[i]);
+    return m;
+  }
 }
 
 // Sums over a warp, the same in all lanes.
@@ -194,30 +218,29 @@ gpuos_verify_kernel(const __grid_constant__ VerifyArgs a) {
     share(row, lo, hi);
     Stat st{a.greedy ? -INFINITY : kLowest, 0.f, 0};
     bool odd = false;  // greedy: NaN or +inf seen
-    for (uint32_t p = lo + lane; p < hi; p += 32 * kFlight) {
-      float v[kFlight][kPack];
+    constexpr int U = kFlight<T>;
+    for (uint32_t p = lo + lane; p < hi; p += 32 * U) {
+      Elements<T> v[U];
 #pragma unroll
-      for (int f = 0; f < kFlight; ++f) {
+      for (int f = 0; f < U; ++f) {
         if (p + 32 * f < hi) {
           row.load(p + 32 * f, v[f]);
         } else {
 #pragma unroll
-          for (int c = 0; c < kPack; ++c) v[f][c] = -INFINITY;
+          for (int c = 0; c < kPack; ++c) v[f].v[c] = from_f<T>(-INFINITY);
         }
       }
       float m = st.m;
 #pragma unroll
-      for (int f = 0; f < kFlight; ++f)
-#pragma unroll
-        for (int c = 0; c < kPack; ++c) m = fmaxf(m, v[f][c]);
+      for (int f = 0; f < U; ++f) m = fmaxf(m, largest(v[f]));
       if (a.greedy) {
 #pragma unroll
-        for (int f = 0; f < kFlight; ++f)
+        for (int f = 0; f < U; ++f)
 #pragma unroll
           for (int c = 0; c < kPack; ++c) {
-            odd |= !(v[f][c] < INFINITY);
-            if (v[f][c] == m && m > st.m)
-              st.key = max(st.key, key_of(m, (uint32_t)(row.first(p + 32 * f) + c)));
+            const float x = to_f(v[f].v[c]);
+            odd |= !(x < INFINITY);
+            if (x == m && m > st.m) st.key = max(st.key, key_of(m, (uint32_t)(row.first(p + 32 * f) + c)));
           }
         if (m > st.m) st.m = m;
         continue;
@@ -226,15 +249,16 @@ gpuos_verify_kernel(const __grid_constant__ VerifyArgs a) {
         st.s *= ex2(fmaxf((st.m - m) * a.k2, -1e4f));
         st.m = m;
       }
-      float2 sum = {0.f, 0.f};
+      float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
-      for (int f = 0; f < kFlight; ++f)
+      for (int f = 0; f < U; ++f)
 #pragma unroll
         for (int c = 0; c < kPack; c += 2) {
-          const float2 y = mul2(add2(make_float2(v[f][c], v[f][c + 1]), both(-m)), both(a.k2));
-          sum = add2(sum, make_float2(ex2(y.x), ex2(y.y)));
+          const float2 y = mul2(add2(make_float2(to_f(v[f].v[c]), to_f(v[f].v[c + 1])), both(-m)), both(a.k2));
+          sum[f & 1] = add2(sum[f & 1], make_float2(ex2(y.x), ex2(y.y)));
         }
-      st.s += sum.x + sum.y;
+      sum[0] = add2(sum[0], sum[1]);
+      st.s += sum[0].x + sum[0].y;
     }
     if (a.greedy) {
       st.key = max_warp(st.key);
