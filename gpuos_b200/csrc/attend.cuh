@@ -671,10 +671,11 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
   if (tid == 0 && a.split) a.split[blockIdx.x] = goes_on;
 }
 
-// Joins the parts of split items, in the order of the CTAs that made them; a warp takes a row.  (Launched while the
-// other kernel runs, so that its start is not waited for: it waits here.)
+// Joins the parts of split items: a CTA takes a row of every 8, its warps parts of it, and all sums are in a fixed order.
+// (Launched while the other kernel runs, so that its start is not waited for: it waits here.)
 template <uint32_t RB>
 __global__ void __launch_bounds__(256) gpuos_attend_join_kernel(const __grid_constant__ Args a) {
+  __shared__ float sums[8][kMaxHead + 2];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 it = a.split[blockIdx.x];
   if (it.w == 0) return;
@@ -682,7 +683,7 @@ __global__ void __launch_bounds__(256) gpuos_attend_join_kernel(const __grid_con
   const uint32_t row0 = (uint32_t)it.z * RB, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rows = (uint32_t)min((int64_t)RB, s.n * a.each - row0);
   const uint32_t stride = a.head + 2;
-  for (uint32_t r = warp; r < rows; r += 8) {
+  for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
     auto part = [&](int i) { return a.partial + (((size_t)blockIdx.x + i) * 2 + (i == 0)) * RB * stride + r * stride; };
     float top = -INFINITY;
     for (int i = lane; i <= it.w; i += 32) top = fmaxf(top, part(i)[a.head]);
@@ -690,22 +691,33 @@ __global__ void __launch_bounds__(256) gpuos_attend_join_kernel(const __grid_con
     float sum = 0.f, x[kMaxHead / 32];
 #pragma unroll
     for (uint32_t k = 0; k < kMaxHead / 32; ++k) x[k] = 0.f;
-#pragma unroll 4
-    for (int i = 0; i <= it.w; ++i) {
+    for (int i = warp; i <= it.w; i += 8) {
       const float* const p = part(i);
       const float m = p[a.head], f = m == -INFINITY ? 0.f : ex2(m - top);
+      float y[kMaxHead / 32];
+#pragma unroll
+      for (uint32_t k = 0; k < kMaxHead / 32; ++k) y[k] = k * 32 + lane < a.head ? p[k * 32 + lane] : 0.f;
       sum += f * p[a.head + 1];
 #pragma unroll
-      for (uint32_t k = 0; k < kMaxHead / 32; ++k)  // (a part of no weight adds nothing, whatever it holds)
-        if (k * 32 < a.head) x[k] += k * 32 + lane < a.head && f != 0.f ? f * p[k * 32 + lane] : 0.f;
+      for (uint32_t k = 0; k < kMaxHead / 32; ++k) x[k] += f == 0.f ? 0.f : f * y[k];  // (no weight, whatever it holds)
     }
-    const uint32_t query = a.each_div.div(row0 + r), h = it.y * a.each + row0 + r - query * a.each;
-    const int64_t t = s.first + query;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-    for (uint32_t k = 0; k < kMaxHead / 32; ++k)
-      if (k * 32 + lane < a.head) store_real(a.out, a.type, t * a.ot + h * a.oh + k * 32 + lane, x[k] * inv);
-    if (a.lse && lane == 0) a.lse[t * a.lt + h * a.lh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718056f;
+    for (uint32_t k = 0; k < kMaxHead / 32; ++k) sums[warp][k * 32 + lane] = x[k];
+    if (lane == 0) sums[warp][kMaxHead] = sum;
+    __syncthreads();
+    sum = 0.f;
+#pragma unroll
+    for (uint32_t w = 0; w < 8; ++w) sum += sums[w][kMaxHead];
+    const uint32_t query = a.each_div.div(row0 + r), h = it.y * a.each + row0 + r - query * a.each, e = threadIdx.x;
+    const int64_t t = s.first + query;
+    if (e < a.head) {
+      float y = 0.f;
+#pragma unroll
+      for (uint32_t w = 0; w < 8; ++w) y += sums[w][e];
+      store_real(a.out, a.type, t * a.ot + h * a.oh + e, sum == 0.f ? 0.f : y / sum);
+    }
+    if (a.lse && e == 0) a.lse[t * a.lt + h * a.lh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718056f;
+    __syncthreads();
   }
 }
 
@@ -717,7 +729,7 @@ void start(const Args& a, cudaStream_t stream) {
   run(kernel, dim3(a.grid), kThreads, L::total, stream, a);
   if (!a.split) return;
   cudaLaunchConfig_t c{};
-  c.gridDim = dim3(a.grid);
+  c.gridDim = dim3(a.grid, 8);
   c.blockDim = dim3(256);
   c.stream = stream;
   cudaLaunchAttribute at[1];

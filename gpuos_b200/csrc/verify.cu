@@ -53,6 +53,7 @@ struct VerifyArgs {
   int64_t* tokens;      // (sequence, n + 1)
   int64_t* accepted;
   uint32_t n, cols;
+  uint32_t groups;      // of a CTA's warps, a row each at a time: 1, 2, 4 or 8
   double k64;           // 64 log2(e) / t
   float k2;             // log2(e) / t
   int draft_wide, greedy, q_type;
@@ -211,11 +212,12 @@ gpuos_verify_kernel(const __grid_constant__ VerifyArgs a) {
     hi = min(lo + each, packs);
   };
 
-  // 1. maxima and sums of all rows
-  for (uint32_t i = 0; i < rows; ++i) {
+  // 1. maxima and sums of all rows; short ones several at a time, a group of the CTA's warps each (a.groups of them)
+  const uint32_t of_row = kWarps / a.groups;  // warps
+  for (uint32_t i = warp / of_row; i < rows; i += a.groups) {
     const Row<T> row(x0 + i * a.xr, a.cols);
-    uint32_t lo, hi;
-    share(row, lo, hi);
+    const uint32_t packs = row.packs(), each = (packs + parts * of_row - 1) / (parts * of_row);
+    const uint32_t lo = min((rank * of_row + warp % of_row) * each, packs), hi = min(lo + each, packs);
     Stat st{a.greedy ? -INFINITY : kLowest, 0.f, 0};
     bool odd = false;  // greedy: NaN or +inf seen
     constexpr int U = kFlight<T>;
@@ -266,12 +268,12 @@ gpuos_verify_kernel(const __grid_constant__ VerifyArgs a) {
     } else {
       st = join_warp(st, a.k2);
     }
-    if (lane == 0) sh.part[i][warp] = st;
+    if (lane == 0) sh.part[i][warp % of_row] = st;
   }
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < rows; i += kThreads) {
     Stat st = sh.part[i][0];
-    for (uint32_t w = 1; w < kWarps; ++w) join(st, sh.part[i][w], a.greedy ? 0.f : a.k2);
+    for (uint32_t w = 1; w < of_row; ++w) join(st, sh.part[i][w], a.greedy ? 0.f : a.k2);
     sh.mine[i] = st;
   }
   cluster.sync();
@@ -352,7 +354,7 @@ gpuos_verify_kernel(const __grid_constant__ VerifyArgs a) {
       const double q = a.q ? (double)prob(a.q, a.q_type, seq * a.qs + at * a.qr + d) : 1.0;
       const double uq = (double)__ldg(a.u + seq * a.us + at * a.ui) * q;
       double bound = uq * sh.all[at].s;
-      // the sum's error: at most 16 + 128 additions in a thread, 29 joins of 6 roundings each (2^-24 is one), and of the
+      // the sum's error: at most 16 + 160 additions in a thread, 29 joins of 6 roundings each (2^-24 is one), and of the
       // exponents' arguments 1.8 roundings times the sum of w |log2 w| / S, at most log2 of the tokens: below 2^-15
       if (fabs(bound - w) <= 0x1p-14 * w && w > 0.0) bound = uq * whole_sum(at);
       refused = !(bound < w);
@@ -558,6 +560,10 @@ extern "C" int32_t gpuos_verify(const gpuos_tensor* logits, const gpuos_tensor* 
     while (parts < kCluster && (uint64_t)parts * kThreads * kPack < (uint64_t)v &&
            ((uint64_t)b * parts < 3u * (uint32_t)sm_count() || (uint64_t)parts * kWarps * kKept * 32 * kPack < (uint64_t)v + kPack))
       parts *= 2;
+    // so many that a warp's share of a row fills what it has in flight
+    const uint32_t flight = 32 * (logits->dtype == GPUOS_F32 ? kFlight<float> : kFlight<__half>) * kPack;
+    a.groups = 1;
+    while (a.groups < kWarps && a.groups < rows && 2 * a.groups * (uint64_t)v <= (uint64_t)flight * parts * kWarps) a.groups *= 2;
     cudaLaunchConfig_t c{};
     c.gridDim = dim3((uint32_t)b * parts);
     c.blockDim = dim3(kThreads);
