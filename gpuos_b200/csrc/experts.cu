@@ -23,7 +23,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr uint32_t kMaxExperts = 1024, kMaxChoices = 64;
-constexpr uint32_t kCounts = 8192;    // 32-bit counters a CTA of the sort holds (32 KB)
+constexpr uint32_t kCounts = 7168;    // 32-bit counters a CTA of the sort holds (28 KB)
 constexpr uint32_t kSortCluster = 8;
 constexpr uint32_t kAhead = 8;        // steps of 32 choices that a warp loads at once
 
@@ -58,6 +58,7 @@ gpuos_order_kernel(const __grid_constant__ OrderArgs a) {
   extern __shared__ uint32_t counters[];  // [warps][count]
   __shared__ uint32_t total[kMaxExperts];   // of this CTA, read by the others
   __shared__ uint32_t amount[kMaxExperts];  // of all
+  __shared__ uint32_t ahead[kMaxExperts];   // of the CTAs before this one; then where this one's rows begin
   __shared__ uint32_t first[kMaxExperts + 1], group[32];
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t rank = cluster.block_rank(), parts = cluster.num_blocks();
@@ -112,7 +113,7 @@ gpuos_order_kernel(const __grid_constant__ OrderArgs a) {
     }
     if (lane == 31) group[g] = sum;
     if (e < a.count) {
-      for (uint32_t w = 0; w < a.warps; ++w) counters[w * a.count + e] += before;
+      ahead[e] = before;
       amount[e] = all;
       first[e] = sum - padded;
     }
@@ -131,6 +132,7 @@ gpuos_order_kernel(const __grid_constant__ OrderArgs a) {
   __syncthreads();
   for (uint32_t e = threadIdx.x; e < a.count; e += threads) {
     first[e] += group[e >> 5];
+    ahead[e] += first[e];
     if (rank == 0) {
       a.offsets[e] = (int32_t)first[e];
       a.counts[e] = (int32_t)amount[e];
@@ -148,7 +150,7 @@ gpuos_order_kernel(const __grid_constant__ OrderArgs a) {
       if (i0 + 32 * s >= hi) break;
       const uint32_t same = __match_any_sync(~0u, e[s]);
       uint32_t at = 0;
-      if (e[s] >= 0) at = first[e[s]] + mine[e[s]] + __popc(same & below);
+      if (e[s] >= 0) at = ahead[e[s]] + mine[e[s]] + __popc(same & below);
       __syncwarp();
       if (e[s] >= 0 && !(same & below)) mine[e[s]] += __popc(same);
       __syncwarp();

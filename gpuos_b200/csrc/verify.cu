@@ -354,7 +354,7 @@ gpuos_verify_kernel(const __grid_constant__ VerifyArgs a) {
       const double q = a.q ? (double)prob(a.q, a.q_type, seq * a.qs + at * a.qr + d) : 1.0;
       const double uq = (double)__ldg(a.u + seq * a.us + at * a.ui) * q;
       double bound = uq * sh.all[at].s;
-      // the sum's error: at most 16 + 160 additions in a thread, 29 joins of 6 roundings each (2^-24 is one), and of the
+      // the sum's error: at most 8 + 256 additions in a thread, 29 joins of 6 roundings each (2^-24 is one), and of the
       // exponents' arguments 1.8 roundings times the sum of w |log2 w| / S, at most log2 of the tokens: below 2^-15
       if (fabs(bound - w) <= 0x1p-14 * w && w > 0.0) bound = uq * whole_sum(at);
       refused = !(bound < w);
