@@ -187,7 +187,8 @@ extern "C" int32_t gpuos_attend(const gpuos_tensor* q, const gpuos_tensor* codes
     a.few = kAll;
     if (groups == 1 && q->dtype != GPUOS_F32 && s.plan.padded <= 128 && a.vec == 16 && std::min(longest, tokens) * a.each > kWideFrom) {
       a.few = kWideFrom;
-      const int64_t most = (tokens * a.each / kWideRows + n) * hk;  // blocks of all sequences
+      // blocks of all sequences with more rows than kWideFrom
+      const int64_t most = std::min(tokens * a.each / kWideRows + n, tokens * a.each / kWideFrom) * hk;
       need(most < (1ll << 31), "the call is too large");
       a.wide_grid = (uint32_t)most;
       a.q_vec = rows_aligned(*q, 8);

@@ -493,9 +493,12 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
           }
       }
       // the scales of V relative to a power of two, which is raised when they pass it by 2^kSlackV
-      float most = nu[lane];
-      if constexpr (GEN)
-        for (uint32_t gr = 1; gr < a.groups; ++gr) most = fmaxf(most, nu[gr * kTile + lane]);
+      // (one that is not finite is left out: it may belong to a position that a row does not see)
+      float most = 0.f;
+      for (uint32_t gr = 0; gr < (GEN ? a.groups : 1); ++gr) {
+        const float x = fabsf(nu[gr * kTile + lane]);
+        most = fmaxf(most, x < INFINITY ? x : 0.f);
+      }
       most = warp_max(most);
       if (most > (float)(1 << kSlackV) * unit_v) {
         const float up = fmaxf(__uint_as_float(min((__float_as_uint(most) & 0x7f800000u) + 0x00800000u, 0x7e800000u)), kSmallestUnit);
@@ -725,7 +728,8 @@ template <int F, int DT, int NT, bool GEN>
 void start(const Args& a, cudaStream_t stream) {
   using L = Layout<DT, NT, GEN>;
   void (*const kernel)(const Args) = gpuos_attend_kernel<F, DT, NT, GEN>;
-  cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::total), "shared memory");
+  static SharedMemory room;
+  room.grant(reinterpret_cast<const void*>(kernel), L::total);
   run(kernel, dim3(a.grid), kThreads, L::total, stream, a);
   if (!a.split) return;
   cudaLaunchConfig_t c{};

@@ -1,6 +1,8 @@
 // What the attention's kernels share: the parameter block, and how the work of a
 // call is cut into units, items and the CTAs' shares of them.
 #pragma once
+#include <atomic>
+
 #include "rowops.cuh"
 
 namespace gpuos {
@@ -154,6 +156,19 @@ __device__ __forceinline__ void store_real(void* p, int type, int64_t i, float v
 // CTAs of an SM: three leave 168 registers a thread, enough for 8 rows.  (64 sequences of 8000 e4m3 positions, 8 rows: AAA us
 // with three and two stages of codes, 217 with two and three.)
 __host__ __device__ constexpr uint32_t ctas(uint32_t padded, uint32_t tiles) { return padded == 256 ? 1 : tiles == 1 ? 3 : 2; }
+
+// A kernel's shared memory beyond 48 KB, asked for once a device.
+struct SharedMemory {
+  std::atomic<bool> has[64] = {};
+  void grant(const void* kernel, size_t bytes) {
+    int dev = -1;
+    cuda_ok(cudaGetDevice(&dev), "cudaGetDevice");
+    if (dev < 0 || dev >= 64) invalid("device index out of range");
+    if (has[dev].load(std::memory_order_relaxed)) return;
+    cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "shared memory");
+    has[dev].store(true, std::memory_order_relaxed);
+  }
+};
 
 // Launches of one format (attend_int8.cu, attend_e4m3.cu).  `rows`: of a block.
 struct Plan {

@@ -365,7 +365,7 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
         const bool fine = fabsf(nu) < INFINITY;
         odd = __ballot_sync(~0u, !fine);
         if (!fine) nu = 0.f;
-        const float high = warp_max(nu);
+        const float high = warp_max(fabsf(nu));
         if (lane == 0) sh.most[step & 1][warp - 8] = high;
       }
       arrive(&sh.where_full);  // (who finds nothing has read what was there)
@@ -726,7 +726,8 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
 template <int F, int DT, bool SPLIT>
 void start_wide(const Args& a, cudaStream_t stream) {
   void (*const kernel)(const Args) = gpuos_attend_wide_kernel<F, DT, SPLIT>;
-  cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Wide<DT>::total), "shared memory");
+  static SharedMemory room;
+  room.grant(reinterpret_cast<const void*>(kernel), Wide<DT>::total);
   run(kernel, dim3(a.wide_grid), kWideThreads, Wide<DT>::total, stream, a);
 }
 

@@ -576,7 +576,7 @@ extern "C" int32_t gpuos_verify(const gpuos_tensor* logits, const gpuos_tensor* 
     c.numAttrs = 1;
     const VerifyArgs args = a;
     auto go = [&](auto* kernel) {
-      cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared)), "shared memory");
+      static_assert(sizeof(Shared) <= 48 << 10);
       cuda_ok(cudaLaunchKernelEx(&c, kernel, args), "launch");
     };
     if (logits->dtype == GPUOS_F32) go(gpuos_verify_kernel<float>);

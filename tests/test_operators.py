@@ -751,6 +751,86 @@ def test_attend_queries(dtype, fmt, d, groups, hq, hk, causal, window):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("d,hq,hk,page", [(64, 4, 1, 16), (16, 8, 2, 5), (48, 3, 3, 64), (80, 8, 1, 16), (128, 2, 2, 100), (112, 6, 2, 256)])
+@pytest.mark.parametrize("window,causal,holes", [(None, True, False), (70, True, True), (None, False, False)])
+def test_attend_prompts(dtype, fmt, d, hq, hk, page, window, causal, holes):
+    """Blocks of 256 rows: heads that do not fill them, lengths and blocks that end anywhere, pages that are not there."""
+    g = gen(d + hq + page)
+    lengths, queries = [400, 1, 300, 131, 700], [400, 1, 129, 140, 65]
+    cache = Cache(g, lengths, hk, d, page, fmt, holes=holes)
+    q = randn(g, sum(queries), hq, d, dtype=dtype, by=2.0)
+    out, lse = attend(q, cache, queries, max(queries), causal=causal, window=window)
+    check_attend(out, q, cache, queries, lse, causal=causal, window=window)
+    few, _ = attend(q, cache, queries, 1, causal=causal, window=window)  # the other kernel
+    check_attend(few, q, cache, queries, causal=causal, window=window)
+    # rows that do not lie on 16 bytes, and results between others
+    wide = torch.zeros(sum(queries), hq, d + 3, dtype=dtype, device=DEV)
+    wide[..., 1: d + 1] = q.to(DEV)
+    codes, scales = cache.on()
+    room = torch.full((sum(queries), hq, d + 5), 7.0, dtype=dtype, device=DEV)
+    off = torch.tensor([0] + queries).cumsum(0).to(DEV)
+    R.attend(wide[..., 1: d + 1], codes, scales, cache.pages.to(DEV), torch.tensor(lengths).to(DEV), offsets=off, causal=causal,
+             window=window, out=room[..., 2: d + 2])
+    assert torch.equal(room[..., 2: d + 2], out) and bool((room[..., :2] == 7).all()) and bool((room[..., d + 2:] == 7).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_prompts_odd_numbers(dtype, d):
+    """Scores that rise along the positions, queries far apart, scales that are not finite where some do not look."""
+    g = gen(d)
+    cache = Cache(g, [900], 1, d, 16, "int8")
+    queries = [400]
+    q = randn(g, 400, 2, d, dtype=dtype)
+    # keys like one query, more and more so, and scales of values that rise: maxima are raised again and again
+    j = torch.arange(900)
+    at = (cache.pages[0, j // 16], j % 16)
+    base = torch.randint(-100, 101, (d,), generator=g).to(torch.int8)
+    cache.codes[0][at[0], at[1], 0] = base
+    cache.scales[0][at[0], at[1], 0, 0] = (j.float() + 1) / 900 * 0.08
+    cache.scales[1][at[0], at[1], 0, 0] = torch.exp2(j.float() / 60 - 10)
+    q[::3] = (base.float() / 60).to(dtype)
+    q[1::3] = (-base.float() / 60).to(dtype)
+
+    def again():
+        cache.values = [torch.where(s.isnan(), 0.0, c.double() * s.double()) for c, s in zip(cache.codes, cache.scales)]
+
+    again()
+    out, lse = attend(q, cache, queries)
+    check_attend(out, q, cache, queries, lse)
+    assert float((lse[399, 0] - lse[0, 0]).abs()) > 1  # (it does rise)
+    # queries of other sizes, zeros among them, and one with NaN
+    q2 = q.clone()
+    q2[5] = 0
+    q2[6] = (q2[6].float() * 2.0 ** -12).to(dtype)
+    q2[7, 0] = (q2[7, 0].float() * 8).to(dtype)
+    out, lse = attend(q2, cache, queries)
+    check_attend(out, q2, cache, queries, lse)
+    q3 = q2.clone()
+    q3[9, 1, 3] = float("nan")
+    q3[11, 0, 0] = float("inf")
+    odd, _ = attend(q3, cache, queries)
+    keep = torch.ones(400, 2, dtype=torch.bool)
+    keep[9, 1] = keep[11, 0] = False
+    assert not odd[~keep.to(DEV)].isfinite().all(-1).any()
+    check_attend(torch.where(keep[..., None].to(DEV), odd, out), q2, cache, queries)
+    # the last positions' scales are not finite: earlier queries do not see them
+    for i, bad in ((1, float("nan")), (1, float("inf")), (0, float("nan"))):
+        before = cache.scales[i].clone()
+        cache.scales[i][at[0][880:], at[1][880:]] = bad
+        for longest in (None, 1):
+            odd, _ = attend(q2, cache, queries, longest)
+            odd = odd.clone()
+            assert not odd[399].isfinite().all()
+            odd[380:] = out[380:]  # (query 380 is position 880)
+            check_attend(odd, q2, cache, queries)
+        cache.scales[i] = before
+
+
+@gpu
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("lengths,queries,hq,hk,d", [([20000], [1], 4, 1, 128), ([9000, 3, 15001], [1, 1, 1], 8, 2, 64), ([5000, 7000], [5, 3], 8, 2, 128), ([6000], [4], 2, 2, 256), ([3000, 4000, 1200], [40, 200, 1], 4, 2, 128)])
 def test_attend_long(fmt, lengths, queries, hq, hk, d):
