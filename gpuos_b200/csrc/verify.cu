@@ -555,10 +555,10 @@ extern "C" int32_t gpuos_verify(const gpuos_tensor* logits, const gpuos_tensor* 
     a.cols = (uint32_t)v;
     a.greedy = greedy;
     // CTAs of a sequence: as few as keep their lanes' sums (and the bound on sums in 32 bits); of few sequences
-    // more, with a pack for every thread at least
+    // more, with a pack for every thread at least, as long as all run at once (64 x 50257 fp32 drawn: 19 us, 25 with twice as many)
     uint32_t parts = 1;
     while (parts < kCluster && (uint64_t)parts * kThreads * kPack < (uint64_t)v &&
-           ((uint64_t)b * parts < 3u * (uint32_t)sm_count() || (uint64_t)parts * kWarps * kKept * 32 * kPack < (uint64_t)v + kPack))
+           (2 * (uint64_t)b * parts <= 3u * (uint32_t)sm_count() || (uint64_t)parts * kWarps * kKept * 32 * kPack < (uint64_t)v + kPack))
       parts *= 2;
     // so many that a warp's share of a row fills what it has in flight
     const uint32_t flight = 32 * (logits->dtype == GPUOS_F32 ? kFlight<float> : kFlight<__half>) * kPack;
