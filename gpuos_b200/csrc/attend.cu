@@ -25,7 +25,7 @@ Shape shape(int64_t sequences, int64_t longest, int64_t q_heads, int64_t k_heads
   const int64_t rows = 8 * s.plan.tiles;
   const int64_t blocks = (longest * each + rows - 1) / rows, units = std::max<int64_t>((capacity + kUnit - 1) / kUnit, 1);
   // (as 64-bit products: at most 2^31 of each)
-  const double most = (double)sequences * (double)k_heads * (double)std::max<int64_t>(blocks, 1) * (double)units / kLeast + 1.0;
+  const double most = (double)sequences * (double)k_heads * (double)std::max<int64_t>(blocks, 1) * (double)units;
   s.grid = (uint32_t)std::min<double>(most, (double)sm_count() * s.plan.per_sm);
   s.join = units > kWhole;
   s.bytes = s.join ? (int64_t)s.grid * (16 + 2 * rows * (head + 2) * 4) : 0;

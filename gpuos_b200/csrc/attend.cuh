@@ -189,7 +189,7 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
     __syncthreads();
   }
   const int64_t all = thread_units[kThreads];
-  const int64_t per = max((all + a.grid - 1) / a.grid, (int64_t)kLeast);
+  const int64_t per = max((all + a.grid - 1) / a.grid, (int64_t)1);
   if (blockIdx.x * per >= all) {
     if (tid == 0 && a.split) a.split[blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
@@ -310,42 +310,48 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
     };
     for (uint32_t i = 0; i + 1 < kStages; ++i) issue(i);
 
-    // ---- the block's rows of q: a warp takes a row
-    for (uint32_t r = warp; r < RB; r += kWarps) {
-      constexpr uint32_t E = DT / 32;
-      float v[E];
-      float most = 0.f;
-      int64_t base = 0;
-      uint32_t query = 0;
-      if (r < row_count) {
-        query = a.each_div.div(row0 + r);
-        base = (s.first + query) * a.qt + (int64_t)(it.head * a.each + row0 + r - query * a.each) * a.qh;
+    // ---- the block's rows of q: a warp takes every fourth row, all of them loaded before the first is looked at
+    {
+      constexpr uint32_t E = DT / 32, MINE = RB / kWarps;
+      float v[MINE][E];
+      uint32_t query[MINE];
+#pragma unroll
+      for (uint32_t k = 0; k < MINE; ++k) {
+        const uint32_t r = warp + k * kWarps;
+        query[k] = r < row_count ? a.each_div.div(row0 + r) : 0;
+        const int64_t base = (s.first + query[k]) * a.qt + (int64_t)(it.head * a.each + row0 + r - query[k] * a.each) * a.qh;
+#pragma unroll
+        for (uint32_t i = 0; i < E; ++i) {
+          const uint32_t e = i * 32 + lane;
+          v[k][i] = r < row_count && e < a.head ? load_real(a.q, a.type, base + e) : 0.f;
+        }
       }
 #pragma unroll
-      for (uint32_t i = 0; i < E; ++i) {
-        const uint32_t e = i * 32 + lane;
-        v[i] = r < row_count && e < a.head ? load_real(a.q, a.type, base + e) : 0.f;
-        most = fmaxf(most, fabsf(v[i]));
-      }
-      most = warp_max(most);
-      // times a power of two that puts the largest into [2^14, 2^15): 16-bit floats reach 2^-29 of it
-      int shift = 14 - (int)((__float_as_uint(most) >> 23) - 127);
-      if (!(most > 0.f)) shift = 0;
-      const float up = __uint_as_float((uint32_t)(min(max(shift, -126), 126) + 127) << 23);  // (in two steps for the smallest)
-      const float more = __uint_as_float((uint32_t)(shift - min(max(shift, -126), 126) + 127) << 23);
+      for (uint32_t k = 0; k < MINE; ++k) {
+        const uint32_t r = warp + k * kWarps;
+        float most = 0.f;
 #pragma unroll
-      for (uint32_t i = 0; i < E; ++i) {
-        const uint32_t e = i * 32 + lane;
-        const float y = v[i] * up * more;
-        const __half hi = __float2half_rn(y);
-        *reinterpret_cast<__half*>(sq + r * L::q_row + e * 2) = hi;
-        if (GEN) *reinterpret_cast<__half*>(sq + (RB + r) * L::q_row + e * 2) = __float2half_rn(a.split_q ? y - __half2float(hi) : 0.f);
-      }
-      if (lane == 0) {
-        row_scale[r] = a.scale2 / up / more;
-        const int64_t last = last_seen(a, s, query);
-        row_lo[r] = r < row_count ? first_seen(a, last) : 1;
-        row_hi[r] = r < row_count ? last + 1 : 0;
+        for (uint32_t i = 0; i < E; ++i) most = fmaxf(most, fabsf(v[k][i]));
+        most = warp_max(most);
+        // times a power of two that puts the largest into [2^14, 2^15): 16-bit floats reach 2^-29 of it
+        int shift = 14 - (int)((__float_as_uint(most) >> 23) - 127);
+        if (!(most > 0.f)) shift = 0;
+        const float up = __uint_as_float((uint32_t)(min(max(shift, -126), 126) + 127) << 23);  // (in two steps for the smallest)
+        const float more = __uint_as_float((uint32_t)(shift - min(max(shift, -126), 126) + 127) << 23);
+#pragma unroll
+        for (uint32_t i = 0; i < E; ++i) {
+          const uint32_t e = i * 32 + lane;
+          const float y = v[k][i] * up * more;
+          const __half hi = __float2half_rn(y);
+          *reinterpret_cast<__half*>(sq + r * L::q_row + e * 2) = hi;
+          if (GEN) *reinterpret_cast<__half*>(sq + (RB + r) * L::q_row + e * 2) = __float2half_rn(a.split_q ? y - __half2float(hi) : 0.f);
+        }
+        if (lane == 0) {
+          row_scale[r] = a.scale2 / up / more;
+          const int64_t last = last_seen(a, s, query[k]);
+          row_lo[r] = r < row_count ? first_seen(a, last) : 1;
+          row_hi[r] = r < row_count ? last + 1 : 0;
+        }
       }
     }
     __syncthreads();

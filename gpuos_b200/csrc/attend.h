@@ -11,7 +11,6 @@ namespace attend {
 
 constexpr uint32_t kUnit = 128;      // positions a CTA takes at once, 32 a warp
 constexpr uint32_t kWarps = 4, kThreads = 32 * kWarps;
-constexpr uint32_t kLeast = 4;       // units of a CTA, at least
 constexpr uint32_t kWhole = 8;       // units up to which an item is not split
 constexpr uint32_t kMaxHead = 256;
 constexpr uint32_t kWideRows = 256;  // of a block of a prompt
