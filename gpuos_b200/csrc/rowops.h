@@ -1,5 +1,6 @@
 // What the row operators' entry points share: argument checks, errors and
-// launch set-up.  The operators (rotary.cu, cache.cu, route.cu, logprobs.cu)
+// launch set-up.  The operators (rotary.cu, cache.cu, attend.cu, route.cu,
+// experts.cu, logprobs.cu, verify.cu)
 // run at once on the caller's stream, as gpuos_reduce_rows_noalloc does: they
 // allocate nothing, keep nothing between calls and need no executor.
 #pragma once

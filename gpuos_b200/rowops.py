@@ -1,9 +1,11 @@
 """Row operators of a language model's step, beside the executor's elementwise
-requests and reductions: rotary positions, a quantised cache, routing to
-experts, and log probabilities of given tokens.
+requests and reductions: rotary positions, a quantised cache and attention over
+it, routing to experts and the sorting of their rows, log probabilities of given
+tokens, and the verification of drafted ones.
 
-Each call runs one kernel at once on torch's current stream of its tensors'
-device; it allocates its outputs (where `out` gives none) and nothing else, so it
+Each call runs one kernel (attention up to three) at once on torch's current stream of its tensors'
+device; it allocates its outputs (where `out` gives none), attention over long
+sequences a workspace that lives for the call, and nothing else, so it
 may be captured into a CUDA graph.  As with an op of torch's own, requests
 submitted to an executor are seen once they are flushed; inside a
 ``scheduler_context``, pending requests on the call's tensors are flushed first.
@@ -11,10 +13,10 @@ Tensors are CUDA tensors of one device.  A call that breaks a rule raises
 ``ValueError`` (``TypeError`` for a dtype, ``RuntimeError`` for a device) and
 launches nothing.
 
-``rotary``, ``route`` and ``logprobs`` take part in autograd; their gradients
+``rotary``, ``route``, ``dispatch``, ``combine`` and ``logprobs`` take part in autograd; their gradients
 are also there as calls of their own (``rotary(..., inverse=True)``,
-``route_grad``, ``logprobs_grad``), for steps that are captured or keep no graph.
-In forward mode ``rotary`` carries tangents; ``route`` and ``logprobs`` raise.
+``route_grad``, ``combine`` and ``dispatch`` of one another, ``combine_grad``, ``logprobs_grad``), for steps that are captured or keep no graph.
+In forward mode ``rotary`` carries tangents; the others raise.
 A given `out` and a written cache count as changed in place: a backward pass that saved
 one of them raises, as after an in-place op of torch's.
 include/gpuos_b200.h states each operator's formula and its edge cases.

@@ -339,8 +339,8 @@ int32_t gpuos_reduce_rows_noalloc(int32_t variant, const void* x, int32_t x_dtyp
 /* ---- row operators of a language model's step ------------------------------
  * No counterpart in the reference.  They stand beside gpuos_reduce_rows_noalloc:
  * each runs at once on `stream` (a cudaStream_t of the current device; NULL =
- * the legacy stream), needs no executor, allocates nothing and keeps nothing
- * between calls, so calls may overlap, run on several streams and be captured
+ * the legacy stream), needs no executor, allocates nothing (gpuos_attend is given
+ * a workspace) and keeps nothing between calls, so calls may overlap, run on several streams and be captured
  * into CUDA graphs.  Requests queued on an executor are not seen before they are
  * flushed.  Strides are in elements and not negative; an output must not
  * overlap itself, an input (but for the in-place forms below) or another
