@@ -101,10 +101,10 @@ SIGNATURES = {
                          [ctypes.c_float, _VP]),
     "gpuos_logprobs": (ctypes.c_int32, [P(Tensor)] * 7 + [ctypes.c_float, _VP]),
     "gpuos_logprobs_grad": (ctypes.c_int32, [P(Tensor)] * 7 + [ctypes.c_float, _VP]),
-    "gpuos_attend_workspace": (ctypes.c_int64, [P(Tensor)] * 4 + [ctypes.c_int64]),
+    "gpuos_attend_workspace": (ctypes.c_int32, [P(Tensor)] * 4 + [ctypes.c_int64, P(ctypes.c_int64)]),
     "gpuos_attend": (ctypes.c_int32, [P(Tensor)] * 8 + [_VP, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                                         ctypes.c_float, ctypes.c_int32, _VP]),
-    "gpuos_order_rows": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64]),
+    "gpuos_order_rows": (ctypes.c_int32, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, P(ctypes.c_int64)]),
     "gpuos_order": (ctypes.c_int32, [P(Tensor), ctypes.c_int32] + [P(Tensor)] * 4 + [_VP]),
     "gpuos_dispatch": (ctypes.c_int32, [P(Tensor)] * 4 + [_VP]),
     "gpuos_combine": (ctypes.c_int32, [P(Tensor)] * 5 + [_VP]),

@@ -43,16 +43,19 @@ void check_held(const gpuos_tensor& c, const gpuos_tensor& s, const char* name) 
 
 }  // namespace
 
-extern "C" int64_t gpuos_attend_workspace(const gpuos_tensor* q, const gpuos_tensor* codes, const gpuos_tensor* scales,
-                                          const gpuos_tensor* pages, int64_t longest) {
-  if (!q || !codes || !scales || !pages || q->ndim != 3 || codes->ndim != 4 || scales->ndim != 4 || pages->ndim != 2) return 0;
-  const int64_t hk = codes->sizes[2], capacity = pages->sizes[1] * codes->sizes[1];
-  if (hk < 1 || q->sizes[1] < hk || q->sizes[1] % hk || capacity < 0 || longest < 1 || longest >= kMostPositions) return 0;
-  int64_t bytes = 0;
-  const int32_t rc = entry("gpuos_attend_workspace", [&] {
-    bytes = shape(pages->sizes[0], longest, q->sizes[1], hk, q->sizes[2], scales->sizes[3], q->dtype, capacity).bytes;
+extern "C" int32_t gpuos_attend_workspace(const gpuos_tensor* q, const gpuos_tensor* codes, const gpuos_tensor* scales,
+                                          const gpuos_tensor* pages, int64_t longest, int64_t* bytes) {
+  return entry("gpuos_attend_workspace", [&] {
+    need(q && codes && scales && pages && bytes, "an argument is NULL");
+    need(q->ndim == 3 && codes->ndim == 4 && scales->ndim == 4 && pages->ndim == 2, "q must have 3 dims, codes and scales 4, pages 2");
+    const int64_t hk = codes->sizes[2], page = codes->sizes[1];
+    need(hk >= 1 && q->sizes[1] >= hk && q->sizes[1] % hk == 0, "the query heads must be a multiple of the cache's");
+    need(page >= 0 && page < kMostPositions && pages->sizes[1] >= 0 && pages->sizes[1] < kMostPositions && page * pages->sizes[1] < kMostPositions,
+         "a sequence has fewer than 2^31 positions");
+    need(longest >= 1 && longest < kMostPositions, "longest must be at least 1");
+    const int64_t most = std::min(longest, std::max<int64_t>(q->sizes[0], 1));
+    *bytes = shape(pages->sizes[0], most, q->sizes[1], hk, q->sizes[2], scales->sizes[3], q->dtype, page * pages->sizes[1]).bytes;
   });
-  return rc == GPUOS_OK ? bytes : 0;
 }
 
 extern "C" int32_t gpuos_attend(const gpuos_tensor* q, const gpuos_tensor* codes, const gpuos_tensor* scales,

@@ -413,9 +413,14 @@ void launch_grad(const MoveArgs& a, int bytes, dim3 grid, cudaStream_t stream) {
 
 using namespace gpuos::rowops;
 
-extern "C" int64_t gpuos_order_rows(int64_t choices, int64_t count, int64_t align) {
-  if (choices < 0 || count < 1 || align < 1 || align > 65536 || choices > (1ll << 40)) return -1;
-  return (choices + std::min(count, choices) * (align - 1)) / align * align;
+extern "C" int32_t gpuos_order_rows(int64_t choices, int64_t count, int64_t align, int64_t* rows) {
+  return entry("gpuos_order_rows", [&] {
+    need(rows != nullptr, "rows is NULL");
+    need(choices >= 0 && choices < (1ll << 31), "too many choices");
+    need(count >= 1 && count <= kMaxExperts, "between 1 and 1024 experts");
+    need(align >= 1 && align <= 65536, "align must be in [1, 65536]");
+    *rows = (choices + std::min(count, choices) * (align - 1)) / align * align;
+  });
 }
 
 extern "C" int32_t gpuos_order(const gpuos_tensor* experts, int32_t align, const gpuos_tensor* places,
@@ -434,7 +439,8 @@ extern "C" int32_t gpuos_order(const gpuos_tensor* experts, int32_t align, const
     need(align >= 1 && align <= 65536, "align must be in [1, 65536]");
     need(offsets->sizes[0] == count + 1, "offsets must have one more element than counts");
     need((count == 1 || counts->strides[0] == 1) && offsets->strides[0] == 1, "offsets and counts must be contiguous");
-    need(sources->sizes[0] >= gpuos_order_rows(n, count, align), "sources is too small: gpuos_order_rows says how many rows there can be");
+    need(sources->sizes[0] >= (n + std::min(count, n) * (align - 1)) / align * align,
+         "sources is too small: gpuos_order_rows says how many rows there can be");
     const gpuos_tensor* outs[4] = {places, sources, offsets, counts};
     for (int i = 0; i < 4; ++i) {
       no_overlap(*outs[i], *experts, "outputs must not overlap experts");

@@ -359,7 +359,8 @@ PyObject* attend(PyObject* const* a, Py_ssize_t n) {
     lse = at.make({x.size(0), x.size(1)}, at::kFloat);
     l = at.in(lse, "lse");
   }
-  const int64_t bytes = gpuos_attend_workspace(&q, &c[0], &s[0], &pages, std::min(longest, std::max<int64_t>(x.size(0), 1)));
+  int64_t bytes = 0;
+  done(gpuos_attend_workspace(&q, &c[0], &s[0], &pages, longest, &bytes));
   if (bytes) work = at.make({bytes}, at::kByte);
   done(gpuos_attend(&q, c, s, &pages, &lengths, ragged ? &offsets : nullptr, &o, lse.defined() ? &l : nullptr,
                     bytes ? const_cast<void*>(work.const_data_ptr()) : nullptr, bytes, longest, window, (float)scale,
@@ -473,8 +474,8 @@ PyObject* order(PyObject* const* a, Py_ssize_t n) {
   two_dims(x, "experts");
   const int32_t count = small(a[1], "count"), align = small(a[2], "align");
   if (count < 1 || count > 1024) throw Raise{PyExc_ValueError, "count must be in [1, 1024]"};
-  const int64_t rows = gpuos_order_rows(x.numel(), count, align);
-  if (rows < 0) throw Raise{PyExc_ValueError, "align must be in [1, 65536]"};
+  int64_t rows = 0;
+  done(gpuos_order_rows(x.numel(), count, align, &rows));
   const at::Tensor out[4] = {at.make(x.sizes(), at::kInt), at.make({rows}, at::kInt), at.make({count + 1}, at::kInt),
                              at.make({count}, at::kInt)};
   const gpuos_tensor o[4] = {at.in(out[0], "places"), at.in(out[1], "sources"), at.in(out[2], "offsets"), at.in(out[3], "counts")};

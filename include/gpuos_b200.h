@@ -403,12 +403,12 @@ int32_t gpuos_cache_read(int32_t n, const gpuos_tensor* slots, const gpuos_tenso
  * out = sum of e^(s - lse) value, lse (f32 (token, query head), or NULL) = log of the sum of e^s; a query
  * that sees nothing, and a token of no sequence, get zeros and -inf.  A NaN code counts as 0.
  * longest: no sequence has more queries than this, as far as speed goes (it chooses a kernel).
- * workspace: gpuos_attend_workspace bytes on a 16-byte boundary (q, the keys' codes and
+ * workspace: as many bytes as gpuos_attend_workspace says, on a 16-byte boundary (q, the keys' codes and
  * scales, pages and longest as in the call), for this call alone until it has run. */
 #define GPUOS_ATTEND_CAUSAL 1
-int64_t gpuos_attend_workspace(const gpuos_tensor* q, const gpuos_tensor* codes,
+int32_t gpuos_attend_workspace(const gpuos_tensor* q, const gpuos_tensor* codes,
                                const gpuos_tensor* scales, const gpuos_tensor* pages,
-                               int64_t longest);
+                               int64_t longest, int64_t* bytes);
 int32_t gpuos_attend(const gpuos_tensor* q, const gpuos_tensor* codes, const gpuos_tensor* scales,
                      const gpuos_tensor* pages, const gpuos_tensor* lengths,
                      const gpuos_tensor* offsets, const gpuos_tensor* out, const gpuos_tensor* lse,
@@ -478,8 +478,8 @@ int32_t gpuos_logprobs_grad(const gpuos_tensor* logits, const gpuos_tensor* targ
  * k), the row of each choice or -1; sources [row], the choice of each row or -1
  * where there is none; offsets [count + 1], where each expert's rows begin, and behind
  * the last one's; counts [count], how many choices each has.  sources has at least
- * gpuos_order_rows(token * k, count, align) rows, which any choice fits in. */
-int64_t gpuos_order_rows(int64_t choices, int64_t count, int64_t align);
+ * the rows that gpuos_order_rows says for token * k choices, which any of them fit in. */
+int32_t gpuos_order_rows(int64_t choices, int64_t count, int64_t align, int64_t* rows);
 int32_t gpuos_order(const gpuos_tensor* experts, int32_t align, const gpuos_tensor* places,
                     const gpuos_tensor* sources, const gpuos_tensor* offsets,
                     const gpuos_tensor* counts, void* stream);

@@ -58,6 +58,12 @@ def refused(rc, text):
 # ---------------------------------------------------------------------------
 # Refusals (CPU): CPU tensors stand for device memory; nothing is launched.
 # ---------------------------------------------------------------------------
+def rows_of(choices, count, align):
+    n = ctypes.c_int64()
+    assert C.lib().gpuos_order_rows(choices, count, align, n) == C.OK
+    return n.value
+
+
 def c_order(experts, places, sources, offsets, counts, align=1):
     return C.lib().gpuos_order(ref(experts), align, ref(places), ref(sources), ref(offsets), ref(counts), None)
 
@@ -81,11 +87,15 @@ def test_order_refuses():
     refused(c_order(e, p, torch.zeros(24, dtype=i32)[::2], o, c), "contiguous")
     both = torch.zeros(12, dtype=i32)
     refused(c_order(e, both.view(6, 2), both, o, c), "overlap")
-    assert C.lib().gpuos_order_rows(12, 4, 1) == 12
-    assert C.lib().gpuos_order_rows(12, 4, 2) == 16
-    assert C.lib().gpuos_order_rows(3, 100, 16) == 48
-    assert C.lib().gpuos_order_rows(0, 4, 8) == 0
-    assert C.lib().gpuos_order_rows(5, 0, 8) == -1 and C.lib().gpuos_order_rows(5, 4, 0) == -1
+    assert rows_of(12, 4, 1) == 12
+    assert rows_of(12, 4, 2) == 16
+    assert rows_of(3, 100, 16) == 48
+    assert rows_of(0, 4, 8) == 0
+    n = ctypes.c_int64()
+    refused(C.lib().gpuos_order_rows(5, 0, 8, n), "experts")
+    refused(C.lib().gpuos_order_rows(5, 4, 0, n), "align")
+    refused(C.lib().gpuos_order_rows(1 << 31, 4, 1, n), "choices")
+    refused(C.lib().gpuos_order_rows(5, 4, 1, None), "NULL")
 
 
 def test_rows_refuse():
@@ -202,6 +212,11 @@ def test_attend_refuses():
     refused(call(lse=out.view(3, 4, 32)[:, :, 0]), "overlap")
     refused(call(k=k[:, :0], v=v[:, :0], ks=ks[:, :0], vs=vs[:, :0]), "rows")
     refused(call(pages=torch.zeros(3, 1).int().expand(3, 1 << 30)), "2^31")
+    n = ctypes.c_int64()
+    refused(C.lib().gpuos_attend_workspace(ref(q), ref(k), ref(ks), ref(pages), 0, n), "longest")
+    refused(C.lib().gpuos_attend_workspace(ref(q), ref(k), ref(ks), None, 1, n), "NULL")
+    refused(C.lib().gpuos_attend_workspace(ref(q[0]), ref(k), ref(ks), ref(pages), 1, n), "dims")
+    refused(C.lib().gpuos_attend_workspace(ref(q[:, :3]), ref(k), ref(ks), ref(pages), 1, n), "multiple of the cache's")
 
 
 def test_python_refusals():
@@ -221,7 +236,7 @@ def test_python_refusals():
 # ---------------------------------------------------------------------------
 def plain_order(experts, count, align):
     t, k = experts.shape
-    rows = C.lib().gpuos_order_rows(t * k, count, align)
+    rows = rows_of(t * k, count, align)
     places, sources = torch.full((t * k,), -1), torch.full((rows,), -1)
     offsets, counts, at = [], [], 0
     for e in range(count):
