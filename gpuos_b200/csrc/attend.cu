@@ -26,7 +26,7 @@ Shape shape(int64_t sequences, int64_t longest, int64_t q_heads, int64_t k_heads
   const int64_t blocks = (longest * each + rows - 1) / rows, units = std::max<int64_t>((capacity + kUnit - 1) / kUnit, 1);
   // (as 64-bit products: at most 2^31 of each)
   const double most = (double)sequences * (double)k_heads * (double)std::max<int64_t>(blocks, 1) * (double)units;
-  s.grid = (uint32_t)std::min<double>(most, (double)sm_count() * s.plan.per_sm);
+  s.grid = (uint32_t)std::max(std::min(most, (double)sm_count() * s.plan.per_sm), 1.0);  // (tokens of no sequence are written too)
   s.join = units > kWhole;
   s.bytes = s.join ? (int64_t)s.grid * (16 + 2 * rows * (head + 2) * 4) : 0;
   return s;
@@ -188,7 +188,7 @@ extern "C" int32_t gpuos_attend(const gpuos_tensor* q, const gpuos_tensor* codes
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool int8 = codes->dtype == GPUOS_I8;
     a.few = kAll;
-    if (groups == 1 && q->dtype != GPUOS_F32 && s.plan.padded <= 128 && a.vec == 16 && std::min(longest, tokens) * a.each > kWideFrom) {
+    if (n && groups == 1 && q->dtype != GPUOS_F32 && s.plan.padded <= 128 && a.vec == 16 && std::min(longest, tokens) * a.each > kWideFrom) {
       a.few = kWideFrom;
       // blocks of all sequences with more rows than kWideFrom
       const int64_t most = std::min(tokens * a.each / kWideRows + n, tokens * a.each / kWideFrom) * hk;

@@ -950,6 +950,27 @@ def test_attend_odd_numbers():
 
 
 @gpu
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1.0])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attend_scales_and_no_sequences(scale, dtype):
+    g = gen(17)
+    cache = Cache(g, [300, 40], 1, 64, 16, "int8")
+    q = randn(g, 210, 4, 64, dtype=dtype)
+    out, lse = attend(q, cache, [200, 10], scale=scale)
+    check_attend(out, q, cache, [200, 10], lse, scale=scale)
+    out, lse = attend(q[:2], cache, [1, 1], scale=scale)
+    check_attend(out, q[:2], cache, [1, 1], lse, scale=scale)
+    # no sequence at all, and sequences without a table
+    codes, scales = cache.on()
+    none = torch.zeros(0, device=DEV).long()
+    out, lse = R.attend(q.to(DEV), codes, scales, cache.pages[:0].to(DEV), none, offsets=torch.zeros(1, device=DEV).int(), lse=True)
+    assert not out.any() and bool((lse == -math.inf).all())
+    out = R.attend(q[:2].to(DEV), codes, scales, cache.pages[:, :0].to(DEV), torch.tensor([5, 7], device=DEV))
+    assert not out.any()
+    assert R.attend(q[:0].to(DEV), codes, scales, cache.pages[:0].to(DEV), none).shape == (0, 4, 64)
+
+
+@gpu
 def test_attend_past_32_bit_offsets():
     pages, page, heads, d = 17000, 256, 8, 128  # 4.4 GB of codes each
     g = gen(11)
