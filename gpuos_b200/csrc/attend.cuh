@@ -8,7 +8,7 @@
 // rows.  At so few rows memory is the bound, and an SM's share of it is 24 codes a
 // cycle, so what a code costs in instructions counts:
 //   - codes are whole numbers, or e4m3 numbers, that 16-bit floats hold exactly: a
-//     code becomes one in about 1.3 instructions, unscaled.  kappa_j multiplies the
+//     code becomes one in about 1.4 instructions (e4m3 1.7), unscaled.  kappa_j multiplies the
 //     finished product; nu_j goes into the 16-bit weight e^(s_j - m) nu_j;
 //   - the codes are the matrix product's first operand (16 positions, or 16 elements of
 //     the head, a step) and the 8 rows its second one, so that no row of it is idle;
@@ -20,6 +20,8 @@
 // A warp takes 32 positions at a time through a ring of its own (no barrier in the
 // loop).  Items (sequence, key head, block of rows) are laid end to end and the CTAs
 // take equal shares of all units; what is split is joined by a second launch in a fixed order.
+// 2 x 200001 positions of 8 heads of 128, int8: 159 us (5.2 TB/s) and the join; 64 sequences to 8000, e4m3: 196 us
+// (4.2 TB/s): about 1000 instructions for a warp's 32 positions (8 KB) are what is left to bound it.
 #pragma once
 #include "attend.h"
 
