@@ -9,6 +9,9 @@ derived beside each check.
 """
 import ctypes
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -17,6 +20,7 @@ import gpuos_b200.cabi as C
 from gpuos_b200 import rowops as R
 from gpuos_b200 import scheduler as S
 
+ROOT = Path(__file__).resolve().parents[1]
 DEV = "cuda:0"
 gpu = pytest.mark.gpu
 BF, FP, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -1150,6 +1154,43 @@ def test_long_attention_on_two_streams_and_in_two_graphs():
     for i, (q, cache, _, want) in enumerate(jobs):
         check_attend(want, q, cache, [1, 1])
         assert torch.equal(graphs[i][1], want) and all(torch.equal(x, want) for x in got[i])
+
+
+@gpu
+def test_first_calls_inside_a_capture():
+    """Nothing is looked up that a capture forbids: a fresh process captures its first calls, of every kernel for attention."""
+    code = """
+import sys
+import torch
+sys.path[:0] = [%r, %r]
+import test_operators as T
+from gpuos_b200 import rowops as R
+g = T.gen(3)
+cache = T.Cache(g, [1500, 300], 2, 64, 16, "int8")
+codes, scales = cache.on()
+queries = [200, 5]
+q = T.randn(g, sum(queries), 4, 64, dtype=T.BF)
+off = torch.tensor([0] + queries).cumsum(0).to(T.DEV)
+args = (q.to(T.DEV), codes, scales, cache.pages.to(T.DEV), torch.tensor(cache.lengths).to(T.DEV))
+x, u, d = torch.randn(3, 2, 5000, device=T.DEV), torch.rand(3, 2, device=T.DEV), torch.zeros(3, 1, device=T.DEV).long()
+e = torch.randint(0, 700, (300, 4), device=T.DEV)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = R.attend(*args, offsets=off)
+    v = R.verify(x, d, u)
+    order = R.order(e, 700)
+for _ in range(2):
+    graph.replay()
+torch.cuda.synchronize()
+T.check_attend(out, q, cache, queries)
+want = T.plain_verify(x.cpu(), d.cpu(), u.cpu(), None, 1.0)
+assert torch.equal(v.tokens.cpu(), want[0])
+assert all(torch.equal(a.cpu().long(), b) for a, b in zip(order, T.plain_order(e.cpu(), 700, 1)))
+print("as eager")
+""" % (str(ROOT), str(ROOT / "tests"))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "as eager" in r.stdout, r.stderr[-2000:]
 
 
 @gpu
