@@ -673,7 +673,8 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
       const bool plain = (v[0] & v[1] & v[2] & v[3]) == ~0u && !(x[0] | x[1] | x[2] | x[3]) && lo <= p0 && hi >= p0 + kWideTile;
       if (!(uniform && __all_sync(~0u, plain))) {
         careful(i, (int)max(min(lo - p0, (int64_t)kWideTile), (int64_t)0), (int)max(min(hi - p0, (int64_t)kWideTile), (int64_t)0));
-      } else if (i == 0 || !quick(i, false)) {
+      } else if (__any_sync(~0u, m == -INFINITY) || !quick(i, false)) {
+        // (a row that has seen nothing yet, at the start or behind steps before its window or without pages, has no reference)
         raise(i);
         quick(i, true);
       }
