@@ -14,7 +14,7 @@
 //     the head, a step) and the 8 rows its second one, so that no row of it is idle;
 //   - a row's maximum is raised only when a score passes it by 2^4;
 //   - q is held as 16-bit floats times a power of two a row, nu_j relative to a
-//     power of two that follows the largest seen: 16-bit floats then lose nothing of a 16-bit q,
+//     power of two that follows the largest that the row sees: 16-bit floats then lose nothing of a 16-bit q,
 //     and half a step, 2^-11, of a weight down to 2^-22 of the largest: an eighth of what a bf16 result is
 //     rounded by.  32-bit queries take q and weights in two parts (2^-22), 16-bit floats of 11 bits the weights.
 // A warp takes 32 positions at a time through a ring of its own (no barrier in the
@@ -138,13 +138,14 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
   // Weights are at most 2^14: 2^kSlack from scores that pass the row's maximum, 2^kSlackV from scales that pass
   // their unit, and the rest as a factor, so that small weights stay among the normal 16-bit numbers.
   constexpr int kSlack = GEN ? 0 : 4, kSlackV = GEN ? 0 : 2, kUp = 14 - kSlack - kSlackV;
+  constexpr float kMostPer = (float)(1 << kUp) / kSmallestUnit;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t thread_units[kThreads + 1];
   __shared__ uint32_t edge_seq[2];
   __shared__ int64_t edge_unit[2], edge_at[2];
   __shared__ float row_scale[RB];              // of a row's q, times scale * log2(e)
   __shared__ int64_t row_lo[RB], row_hi[RB];   // positions a row sees
-  __shared__ float part_m[kWarps][RB], part_l[kWarps][RB], part_e[kWarps];
+  __shared__ float part_m[kWarps][RB], part_l[kWarps][RB], part_e[kWarps][RB];
 
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   uint8_t* const ring = smem + warp * L::ring;
@@ -376,9 +377,10 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[i][t][k] = 0.f;
-    float m[NT][2], l[NT][2], unit_v = 0.f;  // unit_v: the power of two that nu is relative to
+    // per_v: 2^kUp / the power of two that nu is relative to, a row's own (a scale that a row does not see changes nothing of it)
+    float m[NT][2], l[NT][2], per_v[NT][2];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) m[t][0] = m[t][1] = -INFINITY, l[t][0] = l[t][1] = 0.f;
+    for (int t = 0; t < NT; ++t) m[t][0] = m[t][1] = -INFINITY, l[t][0] = l[t][1] = 0.f, per_v[t][0] = per_v[t][1] = kMostPer;
 
     uint32_t drain = 0;  // the stage that is read next
     for (uint32_t i = 0; i < take; ++i) {
@@ -391,6 +393,14 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
       const float* const kappa = reinterpret_cast<const float*>(stage + 2 * L::codes);
       const float* const nu = kappa + L::scales * kTile;
       const uint32_t valid = *reinterpret_cast<const uint32_t*>(nu + L::scales * kTile);
+
+      // the largest scale of V (one that is not finite is left out: a row gets NaN from it where it sees it)
+      float most = 0.f;
+      for (uint32_t gr = 0; gr < (GEN ? a.groups : 1); ++gr) {
+        const float x = fabsf(nu[gr * kTile + lane]);
+        most = fmaxf(most, x < INFINITY ? x : 0.f);
+      }
+      most = warp_max(most);
 
       // scores of 32 positions (rows g and g + 8 of two products) x NT * 8 rows
       float sc[2][NT][4];
@@ -456,7 +466,11 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
       }
       const int64_t j0 = begin + i * kUnit;
       const bool plain = valid == ~0u && j0 >= all_lo && j0 + kTile <= all_hi;
-      bool higher = false;
+      // the scales of V are relative to a power of two, which is raised when those that the row sees pass it by 2^kSlackV
+      constexpr float kPass = (float)(1 << (kUp + kSlackV));
+      bool higher = false, over = false;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) over |= most * fmaxf(per_v[t][0], per_v[t][1]) > kPass;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float k0 = GEN ? 1.f : kappa[16 * h + g], k1 = GEN ? 1.f : kappa[16 * h + g + 8];
@@ -486,7 +500,8 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
           top[t][k] = fmaxf(fmaxf(sc[0][t][k], sc[0][t][k + 2]), fmaxf(sc[1][t][k], sc[1][t][k + 2]));
           higher |= top[t][k] > m[t][k] + (float)kSlack;  // (from nothing: -inf)
         }
-      if (__any_sync(~0u, higher)) {
+      const bool raise = __any_sync(~0u, higher || over);
+      if (raise) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -500,27 +515,31 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
             for (uint32_t d = 0; d < MT; ++d) o[d][t][k] *= f, o[d][t][k + 2] *= f;
           }
       }
-      // the scales of V relative to a power of two, which is raised when they pass it by 2^kSlackV
-      // (one that is not finite is left out: it may belong to a position that a row does not see)
-      float most = 0.f;
-      for (uint32_t gr = 0; gr < (GEN ? a.groups : 1); ++gr) {
-        const float x = fabsf(nu[gr * kTile + lane]);
-        most = fmaxf(most, x < INFINITY ? x : 0.f);
+      if (raise && __any_sync(~0u, over)) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float own = most;
+            if (!plain) {
+              own = 0.f;
+              for (uint32_t gr = 0; gr < (GEN ? a.groups : 1); ++gr)
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                  const float x = fabsf(nu[gr * kTile + 8 * p + g]);
+                  if (sc[p >> 1][t][(p & 1) * 2 + k] != -INFINITY && x < INFINITY) own = fmaxf(own, x);
+                }
+              for (int d = 4; d < 32; d <<= 1) own = fmaxf(own, __shfl_xor_sync(~0u, own, d));
+            }
+            if (own * per_v[t][k] > kPass) {
+              const float up = fmaxf(__uint_as_float(min((__float_as_uint(own) & 0x7f800000u) + 0x00800000u, 0x7e800000u)), kSmallestUnit);
+              const float per = __uint_as_float(0x7f000000u + (kUp << 23) - __float_as_uint(up)), f = per / per_v[t][k];
+#pragma unroll
+              for (uint32_t d = 0; d < MT; ++d) o[d][t][k] *= f, o[d][t][k + 2] *= f;
+              per_v[t][k] = per;
+            }
+          }
       }
-      most = warp_max(most);
-      if (most > (float)(1 << kSlackV) * unit_v) {
-        const float up = fmaxf(__uint_as_float(min((__float_as_uint(most) & 0x7f800000u) + 0x00800000u, 0x7e800000u)), kSmallestUnit);
-        const float f = unit_v / up;
-#pragma unroll
-        for (uint32_t d = 0; d < MT; ++d)
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) o[d][t][k] *= f;
-        unit_v = up;
-      }
-      // 2^kUp / unit_v
-      const float per_v = unit_v > 0.f ? __uint_as_float(0x7f000000u + (kUp << 23) - __float_as_uint(unit_v)) : 0.f;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -531,6 +550,7 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
             float& x = sc[p >> 1][t][(p & 1) * 2 + k];
             x = ex2(x - from);
             l[t][k] += x;
+            x *= per_v[t][k];
           }
         }
       uint32_t bf[2][NT][2], bl[GEN ? 2 : 1][GEN ? NT : 1][2];
@@ -539,7 +559,7 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            const float w = nu[gr * kTile + 16 * h + 8 * q + g] * per_v;
+            const float w = nu[gr * kTile + 16 * h + 8 * q + g];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
               // (a weight of 0 stays 0 whatever the scale is)
@@ -626,7 +646,7 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
         float x = l[t][k];
         for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(~0u, x, d);
         const uint32_t r = 8 * t + 2 * c + k;
-        if (g == 0) part_m[warp][r] = m[t][k], part_l[warp][r] = x;
+        if (g == 0) part_m[warp][r] = m[t][k], part_l[warp][r] = x, part_e[warp][r] = 1.f / per_v[t][k];
 #pragma unroll
         for (uint32_t d = 0; d < MT; ++d) {
           const uint32_t e = GEN ? (d >> 1) * 32 + g * 4 + (d & 1) * 2
@@ -635,7 +655,6 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
           part[r * DT + e + 1] = o[d][t][k + 2];
         }
       }
-    if (lane == 0) part_e[warp] = unit_v > 0.f ? unit_v * (1.f / (1 << kUp)) : 1.f;
     __syncthreads();
     const bool whole = it.from == 0 && take == it.units;
     float* const slot = a.partial + ((size_t)blockIdx.x * 2 + (it.from == 0)) * RB * (a.head + 2);
@@ -648,7 +667,7 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
       for (uint32_t w = 0; w < kWarps; ++w) {
         f[w] = part_m[w][r] == -INFINITY ? 0.f : ex2(part_m[w][r] - top);
         sum += f[w] * part_l[w][r];
-        f[w] *= part_e[w];
+        f[w] *= part_e[w][r];
       }
       const uint32_t query = a.each_div.div(row0 + r), h = it.head * a.each + row0 + r - query * a.each;
       const int64_t t = s.first + query;

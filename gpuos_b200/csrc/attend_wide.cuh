@@ -9,6 +9,8 @@
 // 16-bit floats of 11 bits); a thread issues the products.  While one tile's weights
 // are computed the tensor cores work on the other's.  The scales of V, relative to a power of two, go into V for
 // bf16 (three roundings of 2^-12 on average each, an eighth of the result's), into P in its two parts for fp16.
+// Of a step that some rows of the block do not see all of, they go into P for both, relative to a power of two that is
+// the row's own: a scale that a row does not see could else leave zeros of those that it does (prompts: 2 % of the time).
 // The reference M of a row follows its maximum.  A step takes the last one's, and only where the weights' sum then
 // says that one may be too large, or where the row does not see all positions, the maximum is looked for (and O rescaled).
 // The bound are the products: 4 * 128 operations a (row, position) of a head of 128;
@@ -44,10 +46,12 @@ struct WideShared {
   uint32_t tmem;
   int dead, top, uniform;  // top: the largest exponent in the block's q
   uint32_t valid[kRings][4], odd[kRings][4];  // positions with a page; whose scale of V is not finite
-  float most[2][4];      // of a step: the largest scale of V, a warp's positions each
-  float unit[kRings];    // of a step: what V is relative to
+  float unit[kRings];    // of a step: what V is relative to; 0: each row's own
   alignas(16) float kappa[kRings][kWideTile];
-  alignas(16) float nu[kRings][kWideTile];
+  alignas(16) float nu[kRings][kWideTile];   // relative to the step's unit (1 where rows have their own)
+  alignas(16) float own[kRings][kWideTile];  // as it is
+  alignas(16) float high[kRings][4];         // the largest that is finite, a warp's positions each
+  uint32_t joint0, joint1;                   // the steps of which all rows see all positions
   int64_t where[2][2][kWideTile];  // of a step: where each position's codes are in K and in V, -1: nowhere
   int64_t units[kWideThreads + 1];
   uint32_t seq;
@@ -188,6 +192,13 @@ struct Power {
   }
 };
 
+// What scales of V are relative to: powers of two.
+constexpr float kLeastUnit = 0x1p-90f;
+__device__ __forceinline__ float unit_above(float most) {
+  return fmaxf(__uint_as_float(min((__float_as_uint(most) & 0x7f800000u) + 0x00800000u, 0x7e800000u)), kLeastUnit);
+}
+__device__ __forceinline__ float inverse(float unit) { return __uint_as_float(0x7f000000u - __float_as_uint(unit)); }
+
 // Row r of q times 2^shift, as 16-bit floats in a tile.
 template <int DT>
 __device__ __forceinline__ void stage_query(const Args& a, uint8_t* tile, uint32_t r, bool has, int64_t base, int shift) {
@@ -262,7 +273,8 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
   const int64_t order = sh.at / a.k_heads;
   const uint32_t head = (uint32_t)(sh.at - order * a.k_heads);
   const int64_t row_base = (wide_blocks(a, s) - 1 - order) * kWideRows, row_all = s.n * a.each;
-  const Range range = seen(a, s, a.each_div.div((uint32_t)row_base), a.each_div.div((uint32_t)(min(row_base + kWideRows, row_all) - 1)));
+  const uint32_t query_a = a.each_div.div((uint32_t)row_base), query_b = a.each_div.div((uint32_t)(min(row_base + kWideRows, row_all) - 1));
+  const Range range = seen(a, s, query_a, query_b);
   const uint32_t steps = (uint32_t)((range.hi - range.lo + kWideTile - 1) / kWideTile);
 
   if (tid == 0) {
@@ -275,6 +287,9 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
       barrier_init(&sh.p_full[i], 128);
       
     }
+    const int64_t lo = first_seen(a, last_seen(a, s, query_b)) - range.lo, hi = last_seen(a, s, query_a) + 1 - range.lo;
+    sh.joint0 = (uint32_t)min((lo + kWideTile - 1) / kWideTile, (int64_t)steps);
+    sh.joint1 = (uint32_t)(max(hi, (int64_t)0) / kWideTile);
     for (uint32_t i = 0; i < kRings; ++i) barrier_init(&sh.scales_full[i], 128);
     barrier_init(&sh.done, 1);
     barrier_init(&sh.where_full, 32 * kCodeWarps);
@@ -343,9 +358,7 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
       if (warp >= 12 || p >= range.hi) return -1;
       return load_index(a.pages, a.page_wide, table + a.page.div((uint32_t)p) * a.pp);
     };
-    float kappa = 0.f, nu = 0.f;       // of the step that is put next
-    float kappa1 = 0.f, nu1 = 0.f;     // of the one behind it
-    uint32_t valid = 0, odd = 0;
+    float kappa1 = 0.f, nu1 = 0.f;
     int64_t k_at = -1, v_at = -1, page2 = -1;
     auto ahead = [&](uint32_t step, int64_t page) {  // places of a step's codes, and its scales
       k_at = v_at = -1;
@@ -357,29 +370,32 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
       kappa1 = __ldg(a.k.scales + page * a.k.sp + at * a.k.sr + head * a.k.sh);
       nu1 = __ldg(a.v.scales + page * a.v.sp + at * a.v.sr + head * a.v.sh);
     };
+    // (a step's scales go where those of four steps before were, which have been read: `find` comes after the scores of two
+    // steps before it were issued, and those wait for the weights of three)
     auto find = [&](uint32_t step) {
       if (warp < 12) {
+        const uint32_t ring = step % kRings;
         sh.where[step & 1][0][j] = k_at;
         sh.where[step & 1][1][j] = v_at;
-        kappa = kappa1;
-        nu = nu1;
-        valid = __ballot_sync(~0u, k_at >= 0);
+        sh.kappa[ring][j] = kappa1 * by * down.b;
+        const uint32_t valid = __ballot_sync(~0u, k_at >= 0);
         // a scale that is not finite makes NaN of the rows that see it, and must not touch others: it is not multiplied
-        const bool fine = fabsf(nu) < INFINITY;
-        odd = __ballot_sync(~0u, !fine);
-        if (!fine) nu = 0.f;
-        const float high = warp_max(fabsf(nu));
-        if (lane == 0) sh.most[step & 1][warp - 8] = high;
+        const bool fine = fabsf(nu1) < INFINITY;
+        const uint32_t odd = __ballot_sync(~0u, !fine);
+        const float nu = fine ? nu1 : 0.f, high = warp_max(fabsf(nu));
+        sh.own[ring][j] = nu;
+        if (lane == 0) sh.valid[ring][warp - 8] = valid, sh.odd[ring][warp - 8] = odd, sh.high[ring][warp - 8] = high;
       }
       arrive(&sh.where_full);  // (who finds nothing has read what was there)
     };
-    // V is brought in relative to a power of two that is raised when a scale passes it by 2^2
-    float unit = 0.f;
+    // Of a step that all rows see, V is brought in relative to a power of two that is raised when a scale passes it by 2^2.
+    // Of the others the scales go into the weights, so that none changes a row that does not see it.
+    float unit = kLeastUnit;
+    auto joint = [&](uint32_t step) { return step >= sh.joint0 && step < sh.joint1; };
     auto raise = [&](uint32_t step) {
-      const float* const w = sh.most[step & 1];
-      const float most = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
-      if (most > 4.f * unit)
-        unit = fmaxf(__uint_as_float(min((__float_as_uint(most) & 0x7f800000u) + 0x00800000u, 0x7e800000u)), 0x1p-90f);
+      const float4 w = *reinterpret_cast<const float4*>(sh.high[step % kRings]);
+      const float most = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w));
+      if (most > 4.f * unit && joint(step)) unit = unit_above(most);
     };
     auto load = [&](const uint8_t* codes, uint32_t step, uint32_t which, uint4 (&r)[N]) {
 #pragma unroll
@@ -432,10 +448,9 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
       if (i >= 2 && !await(&sh.k_empty[st], (i / 2 - 1) & 1, &sh.dead)) break;
       put(smem + W::k + st * W::tile, rk, nullptr);
       if (warp < 12) {
-        sh.kappa[ring][j] = kappa * by * down.b;
-        sh.nu[ring][j] = unit > 0.f ? nu * __uint_as_float(0x7f000000u - __float_as_uint(unit)) : 0.f;
-        if (lane == 0) sh.valid[ring][warp - 8] = valid, sh.odd[ring][warp - 8] = odd;
-        if (tid == 256) sh.unit[ring] = unit;
+        const bool all = joint(i);
+        sh.nu[ring][j] = all ? sh.own[ring][j] * inverse(unit) : 1.f;
+        if (tid == 256) sh.unit[ring] = all ? unit : 0.f;
         arrive(&sh.scales_full[ring]);
       }
       arrive(&sh.k_full[st]);
@@ -515,10 +530,10 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
     // ---- weights: a row a thread
     asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const uint32_t lanes = (warp & 3) << 21;  // (32 lanes a warp, in the upper half of an address)
-    float m = -INFINITY, ref = 0.f, unit = 0.f, sum = 0.f;  // the row's maximum; what weights and O are relative to
+    float m = -INFINITY, ref = 0.f, unit = kLeastUnit, sum = 0.f;  // the row's maximum; what weights and O are relative to
     bool ok = true;
     // (room above for later maxima; for the lower parts, room below)
-    constexpr int kUp = SPLIT ? 4 : 0, kSlack = SPLIT ? 2 : 8;
+    constexpr int kUp = SPLIT ? 4 : 0, kSlack = SPLIT ? 2 : 8, kRoom = 5;
     // two weights times their scales, as 16-bit floats, and what those leave
     auto pair = [&](float2 y, uint32_t& w, uint32_t& low) {
       w = pack16(y);
@@ -536,7 +551,7 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
       float r[2][16];
       uint32_t w[64];
       [[maybe_unused]] uint32_t low[SPLIT ? 64 : 1];
-      if (sh.unit[ring] != unit && !sure) return false;
+      if (__any_sync(~0u, sh.unit[ring] != unit) && !sure) return false;
       tmem_load16(t_s + lanes, r[0]);
       float2 add[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
@@ -575,14 +590,14 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
       return true;
     };
     // O and the sum of weights in units of a higher maximum, or of another unit of V.
-    auto rescale = [&](uint32_t i, float high) {
-      const float before = ref, unit_now = sh.unit[i % kRings];
+    auto rescale = [&](uint32_t i, float high, float unit_now) {
+      const float before = ref;
       const bool none = m == -INFINITY;
       m = fmaxf(m, high);
       ref = (m > -INFINITY ? m : 0.f) - (float)kUp;
       float f = none ? 0.f : ex2(before - ref);
       sum *= f;
-      f *= unit_now > 0.f ? unit / unit_now : 0.f;
+      f *= unit / unit_now;  // (at most 2^60)
       unit = unit_now;
       if (i == 0) return;
       float r[32];
@@ -595,6 +610,11 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
         tmem_store16(t_o + lanes + c * 32, *reinterpret_cast<const uint32_t (*)[16]>(&r[0]));
         tmem_store16(t_o + lanes + c * 32 + 16, *reinterpret_cast<const uint32_t (*)[16]>(&r[16]));
       }
+    };
+    // The unit for a step that all rows see.  (One that is 2^60 below the row's takes nothing that O would keep.)
+    auto joint_unit = [&](uint32_t i) {
+      const float u = sh.unit[i % kRings];
+      return unit > u * 0x1p60f ? unit : u;
     };
     auto raise = [&](uint32_t i) {
       const float* const kappa = sh.kappa[i % kRings];
@@ -611,13 +631,14 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
           high = fmaxf(fmaxf(high, v.x), v.y);
         }
       }
-      rescale(i, high);
+      rescale(i, high, joint_unit(i));
     };
     // A step of which positions [from, to) are seen.  Seldom run, so small.
     auto careful = [&](uint32_t i, int from, int to) {
       const uint32_t ring = i % kRings;
       const float* const kappa = sh.kappa[ring];
-      [[maybe_unused]] const float* const nu = sh.nu[ring];
+      const bool joint = sh.unit[ring] > 0.f;
+      const float* const nu = joint ? sh.nu[ring] : sh.own[ring];
       auto seen_of = [&](uint32_t c) {
         const int l = min(max(from - (int)c * 32, 0), 32), h = min(max(to - (int)c * 32, 0), 32);
         return (h >= 32 ? ~0u : (1u << h) - 1) & ~(l >= 32 ? ~0u : (1u << l) - 1) & sh.valid[ring][c];
@@ -632,8 +653,23 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
         for (uint32_t e = 0; e < 32; ++e) high = fmaxf(high, bits >> e & 1 ? r[e] * kappa[c * 32 + e] : -INFINITY);
       }
       if (high > -INFINITY) high *= scale;
+      // a row's own unit: 2^kRoom below the largest scale it has seen (of those behind it, up to 2^(kRoom + 1) above it)
+      float unit_now = unit;
+      if (joint) {
+        unit_now = joint_unit(i);
+      } else {
+        const float4 w = *reinterpret_cast<const float4*>(sh.high[ring]);
+        if (fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)) > (float)(2 << kRoom) * unit) {
+          float most = 0.f;
+#pragma unroll 1
+          for (uint32_t c = 0; c < 4; ++c)
+            for (uint32_t bits = seen_of(c); bits; bits &= bits - 1) most = fmaxf(most, fabsf(nu[c * 32 + __ffs(bits) - 1]));
+          if (most > (float)(2 << kRoom) * unit) unit_now = unit_above(most) * (1.f / (1 << kRoom));
+        }
+      }
       // weights are at most 2^kUp at the maximum and 2^kSlack more from scores above it
-      if (__any_sync(~0u, high > m + (float)kSlack || sh.unit[ring] != unit)) rescale(i, high);
+      if (__any_sync(~0u, high > m + (float)kSlack || unit_now != unit)) rescale(i, high, unit_now);
+      const float by = joint ? sh.unit[ring] * inverse(unit) : inverse(unit);
       // (the lower parts take the place of the last scores, once those have been read)
       [[maybe_unused]] uint32_t low[SPLIT ? 64 : 1];
 #pragma unroll(SPLIT ? 4 : 1)
@@ -649,10 +685,9 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
           u = bits >> e & 1 ? u : 0.f;
           v = bits >> e & 2 ? v : 0.f;
           sum += u + v;
-          if constexpr (SPLIT) {
-            u *= nu[c * 32 + e];
-            v *= nu[c * 32 + e + 1];
-          }
+          // (where it is not seen a scale may be anything)
+          u = u == 0.f ? 0.f : u * ((SPLIT || !joint ? nu[c * 32 + e] : 1.f) * by);
+          v = v == 0.f ? 0.f : v * ((SPLIT || !joint ? nu[c * 32 + e + 1] : 1.f) * by);
           pair(make_float2(u, v), w[e / 2], low[SPLIT ? c * 16 + e / 2 : 0]);
         }
         // (in the place of scores that have been read)
@@ -671,12 +706,14 @@ gpuos_attend_wide_kernel(const __grid_constant__ Args a) {
       const uint32_t* const v = sh.valid[i % kRings];
       const uint32_t* const x = sh.odd[i % kRings];
       const bool plain = (v[0] & v[1] & v[2] & v[3]) == ~0u && !(x[0] | x[1] | x[2] | x[3]) && lo <= p0 && hi >= p0 + kWideTile;
-      if (!(uniform && __all_sync(~0u, plain))) {
-        careful(i, (int)max(min(lo - p0, (int64_t)kWideTile), (int64_t)0), (int)max(min(hi - p0, (int64_t)kWideTile), (int64_t)0));
+      const int from = (int)max(min(lo - p0, (int64_t)kWideTile), (int64_t)0), to = (int)max(min(hi - p0, (int64_t)kWideTile), (int64_t)0);
+      if (!(uniform && sh.unit[i % kRings] > 0.f && __all_sync(~0u, plain))) {
+        careful(i, from, to);
       } else if (__any_sync(~0u, m == -INFINITY) || !quick(i, false)) {
         // (a row that has seen nothing yet, at the start or behind steps before its window or without pages, has no reference)
         raise(i);
-        quick(i, true);
+        if (__all_sync(~0u, sh.unit[i % kRings] == unit)) quick(i, true);
+        else careful(i, from, to);
       }
       await_stores();
       before_sync();

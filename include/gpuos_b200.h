@@ -402,6 +402,8 @@ int32_t gpuos_cache_read(int32_t n, const gpuos_tensor* slots, const gpuos_tenso
  * whose page is outside the cache (-1) is not seen.  With s = scale * <q, key>:
  * out = sum of e^(s - lse) value, lse (f32 (token, query head), or NULL) = log of the sum of e^s; a query
  * that sees nothing, and a token of no sequence, get zeros and -inf.  A NaN code counts as 0.
+ * The scales of a query's values count relative to the largest that it sees: from 2^14 below that on they lose
+ * bits, as 16-bit floats do.  A position that it does not see changes nothing of its result beyond rounding.
  * longest: no sequence has more queries than this, as far as speed goes (it chooses a kernel).
  * workspace: as many bytes as gpuos_attend_workspace says, on a 16-byte boundary (q, the keys' codes and
  * scales, pages and longest as in the call), for this call alone until it has run. */

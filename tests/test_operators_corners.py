@@ -1,4 +1,4 @@
-"""Attention over the cache where blocks of a prompt meet windows and holes.
+"""Attention over the cache where blocks of a prompt meet windows and holes, and where scales of values lie far apart.
 
 The oracles are those of test_operators.py.  Tolerances count roundings in the same way.
 """
@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_operators import BF, FP, Cache, attend, check_attend, gen, gpu, randn
+from test_operators import BF, DEV, FP, TYPES, Cache, attend, check_attend, gen, gpu, plain_attend, randn
 
 
 # ---------------------------------------------------------------------------
@@ -58,3 +58,61 @@ def test_prompts_whose_first_pages_are_gone(dtype, hq, hk, window, holes):
     q = low_scores(cache, randn(g, 512, hq, 128, dtype=dtype), 40.0)
     out, lse = attend(q, cache, queries, 512, window=window)
     check_attend(out, q, cache, queries, lse, window=window)
+
+
+# ---------------------------------------------------------------------------
+# Scales of values that a query does not see
+# ---------------------------------------------------------------------------
+def mixed(got, other, take):
+    """Rows `take` of `got`, the others of `other`."""
+    return torch.where(take.to(got.device)[:, None, None], got, other.to(got.device))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,groups,hq,hk", [(128, 1, 4, 1), (64, 1, 2, 2), (64, 2, 2, 1), (256, 1, 2, 1)])
+@pytest.mark.parametrize("queries,longest", [(5, None), (40, 1), (400, None)])
+@pytest.mark.parametrize("up", [16, 30, 90])
+def test_scales_of_positions_that_are_not_seen(dtype, d, groups, hq, hk, queries, longest, up):
+    """Scales of values 2^up larger at the last positions, and at some before the windows: queries that do not see them have
+    their results as if they were not there, and those that do are dominated by them."""
+    g = gen(d + queries + up)
+    n, window = 700, 300
+    cache = Cache(g, [n], hk, d, 16, "int8", groups)
+    q = randn(g, queries, hq, d, dtype=dtype)
+    j = torch.arange(n)
+    at = (cache.pages[0, j // 16], j % 16)
+    last = n - queries + torch.arange(queries)
+    for where, how in ((slice(n - queries // 2, n), {}), (slice(0, n - window - queries // 2 + 1), {"window": window})):
+        ordinary, values = cache.scales[1].clone(), cache.values[1]
+        out, _ = attend(q, cache, [queries], longest, **how)
+        cache.scales[1][at[0][where], at[1][where]] *= 2.0 ** up
+        odd, _ = attend(q, cache, [queries], longest, **how)
+        free = last < where.start if "window" not in how else last - window >= where.stop - 1
+        assert 0 < int(free.sum()) < queries
+        check_attend(mixed(odd, out, free), q, cache, [queries], **how)  # (cache.values are the ordinary ones)
+        cache.values[1] = (cache.codes[1].double().unflatten(-1, (groups, -1)) * cache.scales[1].double()[..., None]).flatten(-2)
+        want = plain_attend(q, cache, [queries], **how)[0]
+        if float(want.abs().max()) < torch.finfo(dtype).max:
+            check_attend(mixed(odd, want.to(dtype), ~free), q, cache, [queries], **how)
+        cache.scales[1], cache.values[1] = ordinary, values
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("queries", [6, 300])
+def test_scales_that_fall_by_much(dtype, queries):
+    """The largest scales are seen first, in a window's first positions or by some rows only; small ones follow, and the other
+    way round."""
+    g = gen(queries)
+    n = 900
+    for window, steps in ((None, 0.5), (None, -0.5), (400, 0.1), (400, -0.1), (400, -0.5)):
+        cache = Cache(g, [n], 2, 64, 16, "e4m3")
+        j = torch.arange(n)
+        cache.scales[1][cache.pages[0, j // 16], j % 16] = torch.exp2((j.float() - 450) * steps * 0.2)[:, None, None]
+        cache.values[1] = torch.where(cache.scales[1].isnan(), 0.0, cache.codes[1].double() * cache.scales[1].double())
+        q = randn(g, queries, 4, 64, dtype=dtype)
+        out, lse = attend(q, cache, [queries], window=window)
+        want = plain_attend(q, cache, [queries], window=window)[0]
+        fits = (want.abs() < torch.finfo(dtype).max / 2).all(-1, keepdim=True)  # (the others are not numbers of this type)
+        check_attend(torch.where(fits.to(DEV), out.double(), want.to(DEV)), q, cache, [queries], lse, window=window)
