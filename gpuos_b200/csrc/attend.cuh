@@ -83,49 +83,94 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 }
 __device__ __forceinline__ float2 unpack(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
 
-// Of an item, laid out in units: blocks of a head, heads of a sequence.
-struct Item {
-  uint32_t seq, head;
-  int64_t block;
-  int64_t units, from;  // all of it, and where the search's unit lies
+// Items are laid out in units: blocks of a head, heads of a sequence, sequences.  A CTA's share begins at an edge: a unit
+// of an item (or its end), and the units before it.  Edges are looked for once, by a thread for each, or by all threads
+// where a sequence has many blocks; from there a CTA steps from item to item.
+struct Edge {
+  uint32_t seq, head, block, from;
+  int64_t at;
 };
+constexpr uint32_t kFewBlocks = 64;  // that a thread walks over by itself: 100 cycles each, where a step of all takes some 500
 
 template <uint32_t RB>
-__device__ __forceinline__ int64_t blocks(const Args& a, const Sequence& s) {
+__device__ __forceinline__ uint32_t blocks(const Args& a, const Sequence& s) {
   const int64_t rows = s.n * a.each;
-  return rows > a.few ? 0 : (rows + RB - 1) / RB;
+  return rows > a.few ? 0 : (uint32_t)((rows + RB - 1) / RB);
 }
 template <uint32_t RB>
-__device__ __forceinline__ Range block_range(const Args& a, const Sequence& s, int64_t b) {
-  const int64_t last = min((b + 1) * RB, s.n * a.each) - 1;
-  return seen(a, s, a.each_div.div((uint32_t)(b * RB)), a.each_div.div((uint32_t)last));
+__device__ __forceinline__ Range block_range(const Args& a, const Sequence& s, uint32_t b) {
+  const int64_t first = (int64_t)b * RB, last = min(first + RB, s.n * a.each) - 1;
+  return seen(a, s, a.each_div.div((uint32_t)first), a.each_div.div((uint32_t)last));
 }
-__device__ __forceinline__ int64_t units_of(const Range& r) { return max((r.hi - r.lo + kUnit - 1) / kUnit, (int64_t)1); }
+__device__ __forceinline__ uint32_t units_of(const Range& r) { return max((uint32_t)((r.hi - r.lo + kUnit - 1) / kUnit), 1u); }
 
 // Units of a head of a sequence.
 template <uint32_t RB>
 __device__ __forceinline__ int64_t head_units(const Args& a, const Sequence& s) {
-  const int64_t n = blocks<RB>(a, s);
+  const uint32_t n = blocks<RB>(a, s);
   int64_t u = 0;
-  for (int64_t b = 0; b < n; ++b) u += units_of(block_range<RB>(a, s, b));
+  for (uint32_t b = 0; b < n; ++b) u += units_of(block_range<RB>(a, s, b));
+  return u;
+}
+// The same by all threads together.
+template <uint32_t RB>
+__device__ __noinline__ int64_t head_units_together(const Args& a, const Sequence& s, int64_t (&sums)[kWarps]) {
+  const uint32_t n = blocks<RB>(a, s);
+  int64_t u = 0;
+  for (uint32_t b = threadIdx.x; b < n; b += kThreads) u += units_of(block_range<RB>(a, s, b));
+  for (int d = 16; d; d >>= 1) u += __shfl_xor_sync(~0u, u, d);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = u;
+  __syncthreads();
+  u = 0;
+  for (uint32_t w = 0; w < kWarps; ++w) u += sums[w];
   return u;
 }
 
-// The item that unit `u` of sequence s lies in.
+// The edge at unit u, block `b` of which it is unit `from` of `units`.  Short items stay whole: it is moved to their end.
+__device__ __forceinline__ Edge edge_in(uint32_t seq, uint32_t head, uint32_t b, uint32_t from, uint32_t units, int64_t u) {
+  const uint32_t to = from && units <= kWhole ? units : from;
+  return Edge{seq, head, b, to, u + to - from};
+}
+// The edge at unit u, in sequence s whose first unit is `at`.
 template <uint32_t RB>
-__device__ __forceinline__ Item find(const Args& a, uint32_t seq, const Sequence& s, int64_t u) {
-  Item it;
-  it.seq = seq;
-  const int64_t per_head = head_units<RB>(a, s);
-  it.head = (uint32_t)(u / per_head);
-  u -= it.head * per_head;
-  for (it.block = 0;; ++it.block) {
-    it.units = units_of(block_range<RB>(a, s, it.block));
-    if (u < it.units) break;
-    u -= it.units;
+__device__ __forceinline__ Edge find(const Args& a, uint32_t seq, const Sequence& s, int64_t per_head, int64_t u, int64_t at) {
+  const uint32_t head = (uint32_t)((u - at) / per_head);
+  int64_t rest = u - at - head * per_head;
+  for (uint32_t b = 0;; ++b) {
+    const uint32_t units = units_of(block_range<RB>(a, s, b));
+    if (rest < units) return edge_in(seq, head, b, (uint32_t)rest, units, u);
+    rest -= units;
   }
-  it.from = u;
-  return it;
+}
+// The same by all threads together: one of them finds it.
+template <uint32_t RB>
+__device__ __noinline__ void find_together(const Args& a, uint32_t seq, const Sequence& s, int64_t per_head, int64_t u, int64_t at,
+                                           int64_t (&sums)[kWarps], Edge& to) {
+  const uint32_t n = blocks<RB>(a, s), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t head = (uint32_t)((u - at) / per_head);
+  int64_t rest = u - at - head * per_head;
+  for (uint32_t b0 = 0; b0 < n; b0 += kThreads) {
+    const uint32_t b = b0 + threadIdx.x, units = b < n ? units_of(block_range<RB>(a, s, b)) : 0;
+    int64_t until = units;
+    for (uint32_t d = 1; d < 32; d <<= 1) {
+      const int64_t o = __shfl_up_sync(~0u, until, d);
+      if (lane >= d) until += o;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = until;
+    __syncthreads();
+    int64_t total = 0;
+    for (uint32_t w = 0; w < kWarps; ++w) {
+      if (w == warp) until += total;
+      total += sums[w];
+    }
+    if (rest < total) {
+      if (until - units <= rest && rest < until) to = edge_in(seq, head, b, (uint32_t)(rest - (until - units)), units, u);
+      return;
+    }
+    rest -= total;
+  }
 }
 
 template <int F, int DT, int NT, bool GEN>
@@ -141,8 +186,9 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
   constexpr float kMostPer = (float)(1 << kUp) / kSmallestUnit;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t thread_units[kThreads + 1];
-  __shared__ uint32_t edge_seq[2];
-  __shared__ int64_t edge_unit[2], edge_at[2];
+  __shared__ Edge edge[2];
+  __shared__ int64_t sums[kWarps];
+  __shared__ uint32_t turn;
   __shared__ float row_scale[RB];              // of a row's q, times scale * log2(e)
   __shared__ int64_t row_lo[RB], row_hi[RB];   // positions a row sees
   __shared__ float part_m[kWarps][RB], part_l[kWarps][RB], part_e[kWarps][RB];
@@ -170,9 +216,29 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
   // ---- this CTA's share: where unit blockIdx.x * per begins, and the next CTA's
   const uint32_t per_thread = (a.sequences + kThreads - 1) / kThreads;
   const uint32_t s0 = min(tid * per_thread, a.sequences), s1 = min(s0 + per_thread, a.sequences);
+  bool large = false;  // whether a sequence has many blocks
   {
     int64_t u = 0;
-    for (uint32_t s = s0; s < s1; ++s) u += a.k_heads * head_units<RB>(a, sequence(a, s));
+    for (uint32_t s = s0; s < s1; ++s) {
+      const Sequence q = sequence(a, s);
+      if (blocks<RB>(a, q) > kFewBlocks) large = true;
+      else u += a.k_heads * head_units<RB>(a, q);
+    }
+    large = __syncthreads_or(large);
+    if (large) {
+      uint32_t s = s0;  // the next of this thread's that has
+      for (;;) {
+        while (s < s1 && blocks<RB>(a, sequence(a, s)) <= kFewBlocks) ++s;
+        if (tid == 0) turn = ~0u;
+        __syncthreads();
+        if (s < s1) atomicMin(&turn, s);
+        __syncthreads();
+        const uint32_t now = turn;
+        if (now == ~0u) break;
+        const int64_t n = head_units_together<RB>(a, sequence(a, now), sums);
+        if (s < s1 && s == now) u += a.k_heads * n, ++s;  // (another's first is where this thread's end)
+      }
+    }
     int64_t sum = u;
     for (uint32_t d = 1; d < 32; d <<= 1) {
       const int64_t o = __shfl_up_sync(~0u, sum, d);
@@ -185,10 +251,6 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
     __syncthreads();
     thread_units[tid + 1] = sum + ahead;
     if (tid == 0) thread_units[0] = 0;
-    if (tid < 2) {
-      edge_seq[tid] = a.sequences;
-      edge_unit[tid] = 0;
-    }
     __syncthreads();
   }
   const int64_t all = thread_units[kThreads];
@@ -198,46 +260,74 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
     return;
   }
   for (int i = 0; i < 2; ++i) {
-    int64_t u = (blockIdx.x + i) * per;
+    const int64_t u = (blockIdx.x + i) * per;
     if (u >= all) {
-      if (tid == 0) edge_at[i] = all;
-    } else if (thread_units[tid] <= u && u < thread_units[tid + 1]) {
-      int64_t at = thread_units[tid];
-      for (uint32_t s = s0; s < s1; ++s) {
+      if (tid == 0) edge[i].at = all;
+      continue;
+    }
+    const bool here = thread_units[tid] <= u && u < thread_units[tid + 1];
+    if (!large) {
+      if (here) {
+        int64_t at = thread_units[tid];
+        for (uint32_t s = s0; s < s1; ++s) {
+          const Sequence q = sequence(a, s);
+          const int64_t n = head_units<RB>(a, q);
+          if (u < at + a.k_heads * n) {
+            edge[i] = find<RB>(a, s, q, n, u, at);
+            break;
+          }
+          at += a.k_heads * n;
+        }
+      }
+    } else {
+      __syncthreads();  // (`turn` has been read)
+      if (here) turn = tid;
+      __syncthreads();
+      int64_t at = thread_units[turn];
+      for (uint32_t s = turn * per_thread; s < a.sequences; ++s) {
         const Sequence q = sequence(a, s);
-        const int64_t n = a.k_heads * head_units<RB>(a, q);
-        if (u < at + n) {
-          const Item it = find<RB>(a, s, q, u - at);
-          if (it.from && it.units <= kWhole) u += it.units - it.from;  // short items stay whole
-          edge_seq[i] = s;
-          edge_unit[i] = u - at;  // (may be n: the next sequence's first)
-          edge_at[i] = u;
+        const int64_t n = head_units_together<RB>(a, q, sums);
+        if (u < at + a.k_heads * n) {
+          find_together<RB>(a, s, q, n, u, at, sums, edge[i]);
           break;
         }
-        at += n;
+        at += a.k_heads * n;
       }
     }
   }
   __syncthreads();
-  int64_t todo = edge_at[1] - edge_at[0];
-  uint32_t seq = edge_seq[0];
-  int64_t unit = edge_unit[0];
+  int64_t todo = edge[1].at - edge[0].at;
+  Edge it = edge[0];  // (`at` is not kept up)
+  Sequence s{};
+  uint32_t count = 0;  // blocks of the sequence
+  if (todo > 0) {
+    s = sequence(a, it.seq);
+    count = blocks<RB>(a, s);
+  }
   int4 goes_on = make_int4(0, 0, 0, 0);
 
   while (todo > 0) {
     // ---- the item, and how much of it is this CTA's
-    Sequence s = sequence(a, seq);
-    int64_t n = blocks<RB>(a, s) ? a.k_heads * head_units<RB>(a, s) : 0;
-    if (unit >= n) {
-      unit -= n;
-      ++seq;
+    const Range range = block_range<RB>(a, s, it.block);
+    const uint32_t units = units_of(range);
+    if (it.from == units) {  // on to the next one, which there is
+      it.from = 0;
+      if (++it.block == count) {
+        it.block = 0;
+        if (++it.head == a.k_heads) {
+          it.head = 0;
+          for (count = 0; count == 0 && ++it.seq < a.sequences;) {
+            s = sequence(a, it.seq);
+            count = blocks<RB>(a, s);
+          }
+          if (count == 0) break;  // (only if lengths or offsets have changed meanwhile)
+        }
+      }
       continue;
     }
-    const Item it = find<RB>(a, seq, s, unit);
-    const uint32_t take = (uint32_t)min(it.units - it.from, todo);
-    const Range range = block_range<RB>(a, s, it.block);
+    const uint32_t take = (uint32_t)min((int64_t)(units - it.from), todo);
     const uint32_t begin = (uint32_t)(range.lo + it.from * kUnit) + warp * kTile, stop = (uint32_t)range.hi;  // (below 2^31 + 2^8)
-    const uint32_t row0 = (uint32_t)(it.block * RB), row_count = (uint32_t)min((int64_t)RB, s.n * a.each - row0);
+    const uint32_t row0 = it.block * RB, row_count = (uint32_t)min((int64_t)RB, s.n * a.each - row0);
     // positions that every row sees
     const int64_t all_hi = last_seen(a, s, a.each_div.div(row0)) + 1;
     const int64_t all_lo = first_seen(a, last_seen(a, s, a.each_div.div(row0 + row_count - 1)));
@@ -656,7 +746,7 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
         }
       }
     __syncthreads();
-    const bool whole = it.from == 0 && take == it.units;
+    const bool whole = it.from == 0 && take == units;
     float* const slot = a.partial + ((size_t)blockIdx.x * 2 + (it.from == 0)) * RB * (a.head + 2);
     for (uint32_t r = warp; r < row_count; r += kWarps) {
       float top = part_m[0][r];
@@ -691,12 +781,12 @@ gpuos_attend_kernel(const __grid_constant__ Args a) {
     }
     if (it.from == 0 && !whole) {
       // the CTAs behind this one go on with it, a share each
-      const int64_t rest = it.units - take;
+      const int64_t rest = units - take;
       goes_on = make_int4((int)it.seq, (int)it.head, (int)it.block, (int)((rest + per - 1) / per));
     }
     __syncthreads();
     todo -= take;
-    unit += take;
+    it.from += take;
   }
   if (tid == 0 && a.split) a.split[blockIdx.x] = goes_on;
 }

@@ -1,4 +1,5 @@
-"""Attention over the cache where blocks of a prompt meet windows and holes, and where scales of values lie far apart.
+"""Attention over the cache where blocks of a prompt meet windows and holes, where scales of values lie far apart, and where
+prompts are many blocks of few rows.
 
 The oracles are those of test_operators.py.  Tolerances count roundings in the same way.
 """
@@ -7,7 +8,8 @@ import math
 import pytest
 import torch
 
-from test_operators import BF, DEV, FP, TYPES, Cache, attend, check_attend, gen, gpu, plain_attend, randn
+from gpuos_b200 import rowops as R
+from test_operators import BF, DEV, F32, FP, TYPES, Cache, attend, check_attend, gen, gpu, plain_attend, randn
 
 
 # ---------------------------------------------------------------------------
@@ -116,3 +118,45 @@ def test_scales_that_fall_by_much(dtype, queries):
         want = plain_attend(q, cache, [queries], window=window)[0]
         fits = (want.abs() < torch.finfo(dtype).max / 2).all(-1, keepdim=True)  # (the others are not numbers of this type)
         check_attend(torch.where(fits.to(DEV), out.double(), want.to(DEV)), q, cache, [queries], lse, window=window)
+
+
+# ---------------------------------------------------------------------------
+# Prompts that are taken few rows at a time: many blocks of a sequence, shared out over the GPU
+# ---------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype,d,groups", [(F32, 64, 1), (BF, 64, 2), (FP, 256, 1), (BF, 256, 1)])
+@pytest.mark.parametrize("hq,hk", [(16, 1), (6, 2)])
+@pytest.mark.parametrize("queries", [[600, 700, 0, 300, 1], [1, 0, 520], [0, 1, 1, 640, 0, 0, 650, 5, 500], [1] * 130 + [400, 450] + [2] * 150])
+@pytest.mark.parametrize("window", [None, 90])
+def test_prompts_of_few_rows(dtype, d, groups, hq, hk, queries, window):
+    """Sequences of many blocks beside one another, and beside single tokens and none."""
+    g = gen(len(queries) + d)
+    lengths = [n + int(torch.randint(0, 200 if len(queries) < 100 else 20, (1,), generator=g)) for n in queries]
+    cache = Cache(g, lengths, hk, d, 64, "int8", groups)
+    q = randn(g, sum(queries), hq, d, dtype=dtype)
+    out, lse = attend(q, cache, queries, max(queries), window=window)
+    check_attend(out, q, cache, queries, lse, window=window)
+
+
+@gpu
+def test_prompts_of_few_rows_cost_what_their_products_do():
+    """2048 queries of 16 heads are 2048 blocks of 16 rows: finding each must not walk over the others.  Against 64 queries behind
+    4096 positions, a (query, position) took 30 times as long where it did."""
+
+    def per_product(queries, length):
+        g = torch.Generator(device=DEV).manual_seed(1)
+        codes = tuple(torch.randint(-127, 128, (length // 64, 64, 2, 128), generator=g, device=DEV, dtype=torch.int8) for _ in range(2))
+        scales = tuple(torch.rand(length // 64, 64, 2, 1, generator=g, device=DEV) * 0.05 for _ in range(2))
+        q = torch.randn(queries, 32, 128, generator=g, device=DEV)
+        pages, n = torch.arange(length // 64, device=DEV)[None], torch.tensor([length], device=DEV)
+        offsets, times = torch.tensor([0, queries], device=DEV), []
+        for _ in range(4):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            R.attend(q, codes, scales, pages, n, offsets=offsets, longest=queries)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times) / (queries * (length - queries / 2))
+
+    assert per_product(2048, 2048) < 6 * per_product(64, 4096 + 64)
