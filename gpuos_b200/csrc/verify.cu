@@ -14,7 +14,7 @@
 // which gives tokens as the target alone would.  t = 0 takes the likeliest token instead.
 // Counts and tokens are those of 64-bit arithmetic.  A cluster takes a sequence, so
 // that nothing but its tokens leaves it:
-//   1. every row is read once for m_i and S_i in 32 bits, whose error is below 2^-15;
+//   1. every row is read once for m_i and S_i in 32 bits, whose error is below 2^-13;
 //   2. a draft for which that could matter has S_i summed again in 64 bits;
 //   3. the one row that is drawn from is read again (from L2) and summed in 64 bits:
 //      an SM's 64-bit rate is half its 32-bit rate, and it is one row of a sequence.
@@ -356,9 +356,11 @@ gpuos_verify_kernel(const __grid_constant__ VerifyArgs a) {
       const double q = a.q ? (double)prob(a.q, a.q_type, seq * a.qs + at * a.qr + d) : 1.0;
       const double uq = (double)__ldg(a.u + seq * a.us + at * a.ui) * q;
       double bound = uq * sh.all[at].s;
-      // the sum's error: at most 8 + 256 additions in a thread, 29 joins of 6 roundings each (2^-24 is one), and of the
-      // exponents' arguments 1.8 roundings times the sum of w |log2 w| / S, at most log2 of the tokens: below 2^-15
-      if (fabs(bound - w) <= 0x1p-14 * w && w > 0.0) bound = uq * whole_sum(at);
+      // the sum's error, in roundings (2^-24): at most 8 + 256 additions in a thread, whose maximum may rise as often as it
+      // takes packs, 256 times, of 5 each (an exponential of 2^-22 and a product), 29 joins of 6, an exponential of 4, and of the
+      // exponents' arguments 1.8 times the sum of w |log2 w| / S, at most log2 of the tokens (those of the rises add up to one
+      // argument): 1770 together, below 2^-13
+      if (fabs(bound - w) <= 0x1p-12 * w && w > 0.0) bound = uq * whole_sum(at);
       refused = !(bound < w);
     }
     if (refused) break;

@@ -1,5 +1,5 @@
 """Attention over the cache where blocks of a prompt meet windows and holes, where scales of values lie far apart, and where
-prompts are many blocks of few rows.
+prompts are many blocks of few rows; verification of rows whose maximum rises all along.
 
 The oracles are those of test_operators.py.  Tolerances count roundings in the same way.
 """
@@ -160,3 +160,19 @@ def test_prompts_of_few_rows_cost_what_their_products_do():
         return min(times) / (queries * (length - queries / 2))
 
     assert per_product(2048, 2048) < 6 * per_product(64, 4096 + 64)
+
+
+# ---------------------------------------------------------------------------
+# Verification of rows whose maximum rises all along
+# ---------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("v,rise", [((1 << 24) - 1, 0.4), ((1 << 24) - 1, 6.0), (1 << 22, 1.0), (300001, 3.0)])
+def test_verify_rising_rows(v, rise):
+    """A thread's sum is brought to a new maximum at each of its steps, up to 256 times; random numbers next to p."""
+    x = torch.stack((torch.linspace(0, rise, v), torch.zeros(v)))[None]
+    drafts = torch.tensor([[v - 1 - v // 3]])
+    p = x[0, 0].double().softmax(-1)[drafts[0, 0]]
+    for by in (-2.0 ** -12, -2.0 ** -14, -2.0 ** -16, -2.0 ** -20, 2.0 ** -20, 2.0 ** -16, 2.0 ** -14, 2.0 ** -12):
+        u = torch.tensor([[float(p * (1 + by)), 0.5]])
+        got = R.verify(x.to(DEV), drafts.to(DEV), u.to(DEV))
+        assert int(got.accepted) == int(u[0, 0].double() < p)
