@@ -100,7 +100,7 @@ extern "C" int32_t gpuos_attend(const gpuos_tensor* q, const gpuos_tensor* codes
     need((flags & ~GPUOS_ATTEND_CAUSAL) == 0, "unknown flag");
     const bool causal = flags & GPUOS_ATTEND_CAUSAL;
     need(causal || window == 0, "a window needs causal order");
-    need(scale == scale && scale <= 3.4e38f && scale >= -3.4e38f, "scale must be finite");
+    need(scale <= 2e38f && scale >= -2e38f, "scale must be in [-2e38, 2e38]");  // (times log2(e) it stays a 32-bit number)
     check_tensor(out, 3, "out");
     need(out->dtype == q->dtype, "q and out must have one dtype");
     same_sizes(*out, *q, "out must have the sizes of q");

@@ -399,7 +399,7 @@ int32_t gpuos_cache_read(int32_t n, const gpuos_tensor* slots, const gpuos_tenso
  * rising: tokens [offsets[s], offsets[s + 1]) are sequence s's queries, the last of its
  * positions; NULL: one query each.  With GPUOS_ATTEND_CAUSAL a query sees the positions up
  * to its own, and of them the last `window` where that is not 0; else all.  A position
- * whose page is outside the cache (-1) is not seen.  With s = scale * <q, key>:
+ * whose page is outside the cache (-1) is not seen.  With s = scale * <q, key>, |scale| at most 2e38:
  * out = sum of e^(s - lse) value, lse (f32 (token, query head), or NULL) = log of the sum of e^s; a query
  * that sees nothing, and a token of no sequence, get zeros and -inf.  A NaN code counts as 0.
  * The scales of a query's values count relative to the largest that it sees: from 2^14 below that on they lose

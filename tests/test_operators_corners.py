@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from gpuos_b200 import rowops as R
-from test_operators import BF, DEV, F32, FP, TYPES, Cache, attend, check_attend, gen, gpu, plain_attend, randn
+from test_operators import BF, DEV, F32, FP, TYPES, Cache, attend, c_attend, check_attend, gen, gpu, plain_attend, randn, refused
 
 
 # ---------------------------------------------------------------------------
@@ -176,3 +176,14 @@ def test_verify_rising_rows(v, rise):
         u = torch.tensor([[float(p * (1 + by)), 0.5]])
         got = R.verify(x.to(DEV), drafts.to(DEV), u.to(DEV))
         assert int(got.accepted) == int(u[0, 0].double() < p)
+
+
+# ---------------------------------------------------------------------------
+# Refusals (CPU)
+# ---------------------------------------------------------------------------
+def test_attend_refuses_scales_that_leave_32_bits():
+    """Times log2(e) they would be infinite: 2.36e38 is the last that is not."""
+    q, pages, lengths = torch.zeros(1, 2, 32), torch.zeros(1, 1).int(), torch.zeros(1).int()
+    k, v, ks, vs = *(torch.zeros(1, 4, 1, 32, dtype=torch.int8) for _ in range(2)), *(torch.zeros(1, 4, 1, 1) for _ in range(2))
+    for scale in (3e38, -3e38, 2.4e38, math.inf, -math.inf, math.nan):
+        refused(c_attend(q, k, v, ks, vs, pages, lengths, None, torch.zeros(1, 2, 32), scale=scale), "scale")
