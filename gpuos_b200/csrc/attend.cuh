@@ -20,8 +20,11 @@
 // A warp takes 32 positions at a time through a ring of its own (no barrier in the
 // loop).  Items (sequence, key head, block of rows) are laid end to end and the CTAs
 // take equal shares of all units; what is split is joined by a second launch in a fixed order.
-// 2 x 200001 positions of 8 heads of 128, int8: 159 us (5.2 TB/s) and the join; 64 sequences to 8000, e4m3: 196 us
-// (4.2 TB/s): about 1000 instructions for a warp's 32 positions (8 KB) are what is left to bound it.
+// 200001 and 150001 positions of 8 heads of 128, int8 (739 MB): 178 us a call (4.15 TB/s), some 10 of them the join;
+// 64 sequences to 8000, e4m3 (816 MB): 210 to 215 us (3.85 TB/s).  A warp's 32 positions (8 KB) are about 1000
+// instructions, at half of the issue slots: those, and that a warp's loads wait for its pages, are what is left.
+// Prompts on this kernel (32-bit queries, heads above 128, scales of part of the head), 16 rows a block: 2048 queries of 32
+// heads over 8 of 128, fp32: 1.0 ms, over 2: 1.35 ms, bf16 with scales of 32: 1.3 ms; the tensor cores' rate would allow 20 us.
 #pragma once
 #include "attend.h"
 

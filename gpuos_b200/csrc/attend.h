@@ -11,7 +11,9 @@ namespace attend {
 
 constexpr uint32_t kUnit = 128;      // positions a CTA takes at once, 32 a warp
 constexpr uint32_t kWarps = 4, kThreads = 32 * kWarps;
-constexpr uint32_t kWhole = 8;       // units up to which an item is not split
+// Units up to which an item is not split.  (1 sequence of 300, 700, 1000 positions, 32 heads over 8: 14.4, 19.4, 23.0 us with 8;
+// 15.1, 15.0, 15.0 with 3.  16 sequences: 18.2, 21.6, 25.8 and 18.5, 20.0, 26.4.)
+constexpr uint32_t kWhole = 8;
 constexpr uint32_t kMaxHead = 256;
 constexpr uint32_t kWideRows = 256;  // of a block of a prompt
 
@@ -188,7 +190,10 @@ template <int F> void launch(const Plan& p, const Args& a, cudaStream_t stream);
 template <int F> void launch_wide(const Args& a, cudaStream_t stream);
 
 constexpr uint32_t kAll = ~0u;        // `few` where there is no other kernel
-constexpr uint32_t kWideFrom = 128;   // rows of a sequence above which it is a prompt
+// Rows of a key head of a sequence above which it is a prompt.  (16 sequences, 8 key heads of 128, 1000 and 8000 positions:
+// 96 rows take 93 and 344 us by few rows, 67 and 368 as prompts; 128: 95 and 439, 60 and 311; 132 as prompts 58 and 378.  1
+// sequence of 8000, which fills 8 CTAs as a prompt: 132 rows 296 us, 75 by few rows; from 512 on prompts are as fast.)
+constexpr uint32_t kWideFrom = 128;
 
 }  // namespace attend
 }  // namespace rowops

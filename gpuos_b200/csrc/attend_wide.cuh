@@ -16,9 +16,10 @@
 // The bound are the products: 4 * 128 operations a (row, position) of a head of 128;
 // beside it, an SM has 16 exponentials a cycle, 1024 cycles a tile and step, as many as the
 // two products take, and shared memory feeds Q, K and V to the tensor cores in three quarters of that time.
-// Measured: 2 prompts of up to 4096 queries behind up to 8192 positions, 32 heads of 128 over 8, bf16 from int8: 980 us,
-// 0.39 of the products' rate: a step takes 6000 cycles of the dequantising warps, whose chain of loads, conversions and
+// Measured: 2 prompts of up to 4096 queries behind up to 8192 positions, 32 heads of 128 over 8, bf16 from int8: 1007 us,
+// 0.37 of the products' rate: a step takes 6000 cycles of the dequantising warps, whose chain of loads, conversions and
 // stores is what bounds it, where the products take 2048 and the weights 2500.
+// The warps of codes have 88 registers; what does not fit is spilled (180 bytes a thread for heads of 128 in bf16, 530 in fp16).
 #pragma once
 #include "attend.h"
 

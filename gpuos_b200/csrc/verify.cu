@@ -21,8 +21,8 @@
 // Reading all rows is the bound at many long rows; else the chain of 3 to 5 steps that the cluster
 // takes together, whose exponentials are by a table (10 instructions of 64 bits each, where exp()
 // takes twice as many) and whose sums are kept a lane, so that the token is found without a third pass.
-// 32 sequences x 8 rows x 128257 bf16 with probabilities: 60 us (129 with exp() and one CTA an SM), where reading
-// takes 13; 64 x 50257 fp32 drawn: 19; 1 x 5 x 32000: 16.
+// 32 sequences x 8 rows x 128257 bf16 with probabilities: 60 to 69 us (129 with exp() and one CTA an SM), where reading
+// takes 13; 64 x 50257 fp32 drawn: 18; 1 x 5 x 32000: 14.
 #include <cooperative_groups.h>
 
 #include "rowops.cuh"

@@ -405,6 +405,7 @@ int32_t gpuos_cache_read(int32_t n, const gpuos_tensor* slots, const gpuos_tenso
  * The scales of a query's values count relative to the largest that it sees: from 2^14 below that on they lose
  * bits, as 16-bit floats do.  A position that it does not see changes nothing of its result beyond rounding.
  * longest: no sequence has more queries than this, as far as speed goes (it chooses a kernel).
+ * The kernel for prompts waits for parts of itself, two seconds at most: a block that gave up has NaN.
  * workspace: as many bytes as gpuos_attend_workspace says, on a 16-byte boundary (q, the keys' codes and
  * scales, pages and longest as in the call), for this call alone until it has run. */
 #define GPUOS_ATTEND_CAUSAL 1
